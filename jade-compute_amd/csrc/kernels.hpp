@@ -88,6 +88,46 @@ hipError_t rms_norm_f32(hipStream_t stream, const float *x, const float *weight,
 LaunchShape softmax_shape(uint32_t rows, uint32_t cols);
 hipError_t softmax_f32(hipStream_t stream, const float *x, float *out, uint32_t rows, uint32_t cols);
 
+// Rotary positions of `heads` heads per token of x (rotary), or of them and heads2 of
+// x2, each normed first by its weight (qk_norm_rotary; weight null otherwise).
+// `rates`: rotary_rates(), device memory. Layouts [batch, seq, heads, dim]
+// (token major) or [batch, heads, seq, dim].
+struct RotaryArgs {
+    const float *x, *x2, *weight, *weight2, *positions;
+    const double *rates;
+    float *out, *out2;
+    uint32_t batch, seq, heads, heads2, dim, rotary_dim;
+    bool interleaved, inverse, token_major, out_token_major;
+    float epsilon, magnitude;
+};
+LaunchShape rotary_shape(uint32_t tokens, uint32_t heads, uint32_t dim, uint32_t rotary_dim, bool norm);
+hipError_t rotary_f32(hipStream_t stream, const RotaryArgs &args);
+
+// Rows of k and v named by `picks` [batch, picks_count] to the ends of the caches.
+struct CacheAppendArgs {
+    const float *k, *v, *picks, *lengths;
+    float *k_cache, *v_cache, *new_lengths;
+    uint32_t batch, kv_heads, rows, picks_count, capacity, dim;
+    bool token_major;
+};
+LaunchShape cache_append_shape(uint32_t batch, uint32_t kv_heads, uint32_t picks);
+hipError_t cache_append_f32(hipStream_t stream, const CacheAppendArgs &args);
+
+// Attention of `queries` rows per head over keys of `lengths` [batch], with grouped
+// heads, and over the drafted rows of a tree (`nodes` of them, else 0).
+struct RaggedShape {
+    uint32_t batch, heads, kv_heads, queries, keys, nodes, dim;
+    bool token_major;
+};
+struct RaggedBuffers {
+    const float *q, *k, *v, *lengths, *k_draft, *v_draft, *parents;
+    float *out;
+};
+LaunchShape attention_ragged_shape(const RaggedShape &shape);
+size_t attention_ragged_workspace_bytes(const RaggedShape &shape);
+hipError_t attention_ragged_f32(hipStream_t stream, const RaggedShape &shape, const RaggedBuffers &buffers,
+                                float *workspace);
+
 // Streaming elementwise kernels.
 LaunchShape stream_shape(uint32_t len);
 hipError_t swiglu_f32(hipStream_t stream, const float *gate, const float *up, float *out, uint32_t len);

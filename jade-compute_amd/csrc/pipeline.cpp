@@ -12,6 +12,12 @@ using dev::text_of;
 
 namespace {
 
+hipk::RaggedShape ragged_shape(const KernelSpec &s) {
+    const bool tree = s.op == Op::AttentionTree;
+    return {s.batch, s.heads, s.kv_heads, tree ? s.nodes : s.queries, tree ? s.capacity : s.keys, tree ? s.nodes : 0u,
+            s.dim, s.token_major};
+}
+
 hipk::LaunchShape launch_shape(const KernelSpec &s) {
     using namespace hipk;
     switch (s.op) {
@@ -34,6 +40,11 @@ hipk::LaunchShape launch_shape(const KernelSpec &s) {
         case Op::AttentionApply: return attention_apply_shape(s.heads, s.seq, s.dim);
         case Op::RmsNorm: return rms_norm_shape(s.rows, s.cols);
         case Op::Softmax: return softmax_shape(s.rows, s.cols);
+        case Op::Rotary: return rotary_shape(s.batch * s.seq, s.heads, s.dim, s.rotary_dim, false);
+        case Op::QkNormRotary: return rotary_shape(s.batch * s.seq, s.heads + s.kv_heads, s.dim, s.rotary_dim, true);
+        case Op::CacheAppend: return cache_append_shape(s.batch, s.kv_heads, s.picks);
+        case Op::AttentionTree:
+        case Op::AttentionCross: return attention_ragged_shape(ragged_shape(s));
         case Op::GemmMps: break;
     }
     return {nullptr, {0, 0, 0}, {0, 0, 0}, 0};
@@ -62,6 +73,8 @@ size_t workspace_bytes_of(const KernelSpec &spec) {
     if (spec.op == Op::Gemm || spec.op == Op::GemmSimd) return hipk::gemm_f32_workspace_bytes(spec.m, spec.n, spec.k);
     if (spec.op == Op::AttentionOnline)
         return hipk::attention_online_workspace_bytes(spec.heads, spec.seq, spec.dim, spec.causal);
+    if (spec.op == Op::AttentionTree || spec.op == Op::AttentionCross)
+        return hipk::attention_ragged_workspace_bytes(ragged_shape(spec));
     return 0;
 }
 
@@ -119,6 +132,23 @@ hipError_t enqueue(const Pipeline &p, hipStream_t st, void *const *b) {
         case Op::AttentionApply: return attention_apply_f32(st, in(0), in(1), out(2), s.heads, s.seq, s.dim);
         case Op::RmsNorm: return rms_norm_f32(st, in(0), in(1), out(2), s.rows, s.cols, s.epsilon);
         case Op::Softmax: return softmax_f32(st, in(0), out(1), s.rows, s.cols);
+        case Op::Rotary:
+            return rotary_f32(st, {in(0), nullptr, nullptr, nullptr, in(1), p.rates, out(2), nullptr, s.batch, s.seq,
+                                   s.heads, 0, s.dim, s.rotary_dim, s.interleaved, s.inverse, s.token_major,
+                                   s.out_token_major, 0.f, s.magnitude});
+        case Op::QkNormRotary:
+            return rotary_f32(st, {in(0), in(1), in(2), in(3), in(4), p.rates, out(5), out(6), s.batch, s.seq, s.heads,
+                                   s.kv_heads, s.dim, s.rotary_dim, s.interleaved, false, s.token_major,
+                                   s.out_token_major, s.epsilon, s.magnitude});
+        case Op::CacheAppend:
+            return cache_append_f32(st, {in(0), in(1), in(2), in(3), out(4), out(5), out(6), s.batch, s.kv_heads, s.rows,
+                                         s.picks, s.capacity, s.dim, s.token_major});
+        case Op::AttentionTree:
+            return attention_ragged_f32(st, ragged_shape(s), {in(0), in(1), in(2), in(3), in(4), in(5), in(6), out(7)},
+                                        p.workspace);
+        case Op::AttentionCross:
+            return attention_ragged_f32(st, ragged_shape(s),
+                                        {in(0), in(1), in(2), in(3), nullptr, nullptr, nullptr, out(4)}, p.workspace);
         case Op::GemmMps: break;
     }
     return hipErrorInvalidValue;
@@ -131,6 +161,7 @@ PipelineCache::~PipelineCache() {
 
 void PipelineCache::destroy(Pipeline *p) {
     if (p->program) (void)hipFree(p->program);
+    if (p->rates) (void)hipFree(p->rates);
     if (p->workspace) (void)hipFree(p->workspace);
     by_spec_.erase(p->canonical);
     all_.erase(p);
@@ -172,6 +203,14 @@ Pipeline *PipelineCache::obtain(const KernelSpec &spec) {
                         "uploading the expression program");
             session_.drain();
         }
+        if (spec.op == Op::Rotary || spec.op == Op::QkNormRotary) {
+            const std::vector<double> rates = rotary_rates(spec);
+            const size_t bytes = rates.size() * sizeof(double);
+            dev::expect(hipMalloc(&p->rates, bytes), "allocating the rotation's rates");
+            dev::expect(hipMemcpyAsync(p->rates, rates.data(), bytes, hipMemcpyHostToDevice, session_.queue()),
+                        "uploading the rotation's rates");
+            session_.drain();
+        }
         p->workspace_bytes = workspace_bytes_of(spec);
         if (p->workspace_bytes) {
             const hipError_t status = hipMalloc(&p->workspace, p->workspace_bytes);
@@ -184,6 +223,7 @@ Pipeline *PipelineCache::obtain(const KernelSpec &spec) {
         }
     } catch (...) {
         if (p->program) (void)hipFree(p->program);
+        if (p->rates) (void)hipFree(p->rates);
         delete p;
         throw;
     }

@@ -1,6 +1,6 @@
 // Compiled pipelines: a checked KernelSpec bound to one precompiled gfx950
 // kernel, plus the device memory that kernel needs besides its bindings (an
-// Elementwise program, split-K / split-key partials). This replaces the
+// Elementwise program, a rotation's rates, split-K / split-key partials). This replaces the
 // reference's run-time compilation of emitted modules
 // (src/runtime/corex.rs:439-542); identical canonical specs share one cached
 // pipeline, as the reference shares modules by source text (corex.rs:442-460).
@@ -23,6 +23,7 @@ struct Pipeline {
     std::vector<Binding> binds;
     Instr *program = nullptr;    // device copy of an Elementwise program
     uint32_t program_len = 0;
+    double *rates = nullptr;     // device copy of a rotation's rates
     bool copy = false;           // Elementwise whose expression is input0
     float *workspace = nullptr;  // split-K / split-key partials of a small grid
     size_t workspace_bytes = 0;

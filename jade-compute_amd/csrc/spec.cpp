@@ -34,6 +34,11 @@ constexpr OpName kOps[] = {
     {"rms_norm", Op::RmsNorm},
     {"swi_glu", Op::SwiGlu},
     {"softmax", Op::Softmax},
+    {"rotary", Op::Rotary},
+    {"qk_norm_rotary", Op::QkNormRotary},
+    {"attention_tree", Op::AttentionTree},
+    {"cache_append", Op::CacheAppend},
+    {"attention_cross", Op::AttentionCross},
 };
 
 const char *tag_of(Op op) {
@@ -60,6 +65,21 @@ bool get_f32(const Value &obj, const char *key, float &out, std::string &error) 
     if (!v) { error = std::string("missing field `") + key + "`"; return false; }
     if (!json::as_f32(*v, out)) { error = std::string("field `") + key + "` must be a number"; return false; }
     return true;
+}
+
+// A field that may be left out: `out` keeps its default then.
+bool maybe_f32(const Value &obj, const char *key, float &out, std::string &error) {
+    return !obj.find(key) || get_f32(obj, key, out, error);
+}
+bool get_rotation(const Value &obj, KernelSpec &s, std::string &error) {
+    return get_u32(obj, "batch", s.batch, error) && get_u32(obj, "seq", s.seq, error) &&
+           get_u32(obj, "heads", s.heads, error) && get_u32(obj, "dim", s.dim, error) &&
+           get_u32(obj, "rotary_dim", s.rotary_dim, error) && get_bool(obj, "interleaved", s.interleaved, error) &&
+           get_bool(obj, "token_major", s.token_major, error) &&
+           get_bool(obj, "out_token_major", s.out_token_major, error) && get_f32(obj, "base", s.base, error) &&
+           maybe_f32(obj, "factor", s.factor, error) && maybe_f32(obj, "context", s.context, error) &&
+           maybe_f32(obj, "low_turns", s.low_turns, error) && maybe_f32(obj, "high_turns", s.high_turns, error) &&
+           maybe_f32(obj, "magnitude", s.magnitude, error);
 }
 
 bool parse_expr(const Value &v, Expr &out, std::string &error, int depth) {
@@ -127,6 +147,55 @@ bool dim_ok(uint64_t v, std::string &error) {
 bool matrix_ok(uint64_t x, uint64_t y, std::string &error) {
     if (!dim_ok(x, error) || !dim_ok(y, error)) return false;
     if (x * y > kIntMax) { error = "tensor exceeds checked 31-bit indexing"; return false; }
+    return true;
+}
+
+// batch x heads x rows x dim, each at least 1, at most `most` elements.
+bool heads_ok(uint64_t batch, uint64_t heads, uint64_t rows, uint64_t dim, uint64_t most, std::string &error) {
+    // No factor reaches 2^32, so the checks before each product keep it in 64 bits.
+    if (!(batch >= 1 && batch <= kHipMaxHeads)) { error = "batch must be 1..=65535"; return false; }
+    if (!(heads >= 1 && heads <= kHipMaxHeads)) { error = "heads and kv_heads must be 1..=65535"; return false; }
+    if (!(rows >= 1 && rows <= kIntMax)) { error = "dimension must be in 1..=INT_MAX"; return false; }
+    const uint64_t bh = batch * heads;
+    if (bh > most / rows || bh * rows > most / dim) {
+        error = most == kIntMax ? "tensor exceeds checked 31-bit indexing" : "cache exceeds 2^40 elements";
+        return false;
+    }
+    return true;
+}
+bool rotation_ok(const KernelSpec &s, std::string &error) {
+    if (!(s.dim >= 2 && s.dim <= kMaxRotaryDim)) { error = "rotary head dimension must be 2..=512"; return false; }
+    if (!(s.rotary_dim >= 2 && s.rotary_dim <= s.dim && s.rotary_dim % 2 == 0)) {
+        error = "rotary_dim must be even and in 2..=dim";
+        return false;
+    }
+    if (!(std::isfinite(s.base) && s.base > 0.0f)) { error = "base must be finite and positive"; return false; }
+    if (!(std::isfinite(s.factor) && s.factor > 0.0f)) { error = "factor must be finite and positive"; return false; }
+    if (!(std::isfinite(s.magnitude) && s.magnitude > 0.0f)) {
+        error = "magnitude must be finite and positive";
+        return false;
+    }
+    if (!(std::isfinite(s.context) && s.context >= 0.0f)) {
+        error = "context must be finite and not negative";
+        return false;
+    }
+    if (s.context == 0.0f ? s.low_turns != 0.0f || s.high_turns != 0.0f
+                          : !(std::isfinite(s.high_turns) && s.low_turns >= 0.0f && s.low_turns < s.high_turns)) {
+        error = "low_turns and high_turns come with a context, and 0 <= low_turns < high_turns";
+        return false;
+    }
+    return true;
+}
+bool grouped_ok(const KernelSpec &s, std::string &error) {
+    if (!(s.dim >= 1 && s.dim <= 128)) { error = "attention head dimension must be 1..=128"; return false; }
+    if (!(s.kv_heads >= 1 && s.heads % s.kv_heads == 0)) {
+        error = "heads must be a multiple of kv_heads";
+        return false;
+    }
+    return true;
+}
+bool whole_ok(uint32_t v, const char *name, std::string &error) {
+    if (!(v >= 1 && v <= kMaxWhole)) { error = std::string(name) + " must be 1..=16777216"; return false; }
     return true;
 }
 
@@ -234,6 +303,26 @@ bool parse_spec(const std::string &text, KernelSpec &out, std::string &error) {
                    get_f32(root, "epsilon", out.epsilon, error);
         case Op::Softmax:
             return get_u32(root, "rows", out.rows, error) && get_u32(root, "cols", out.cols, error);
+        case Op::Rotary:
+            return get_rotation(root, out, error) && get_bool(root, "inverse", out.inverse, error);
+        case Op::QkNormRotary:
+            return get_rotation(root, out, error) && get_u32(root, "kv_heads", out.kv_heads, error) &&
+                   get_f32(root, "epsilon", out.epsilon, error);
+        case Op::AttentionTree:
+            return get_u32(root, "batch", out.batch, error) && get_u32(root, "heads", out.heads, error) &&
+                   get_u32(root, "kv_heads", out.kv_heads, error) && get_u32(root, "nodes", out.nodes, error) &&
+                   get_u32(root, "capacity", out.capacity, error) && get_u32(root, "dim", out.dim, error) &&
+                   get_bool(root, "token_major", out.token_major, error);
+        case Op::CacheAppend:
+            return get_u32(root, "batch", out.batch, error) && get_u32(root, "kv_heads", out.kv_heads, error) &&
+                   get_u32(root, "rows", out.rows, error) && get_u32(root, "picks", out.picks, error) &&
+                   get_u32(root, "capacity", out.capacity, error) && get_u32(root, "dim", out.dim, error) &&
+                   get_bool(root, "token_major", out.token_major, error);
+        case Op::AttentionCross:
+            return get_u32(root, "batch", out.batch, error) && get_u32(root, "heads", out.heads, error) &&
+                   get_u32(root, "kv_heads", out.kv_heads, error) && get_u32(root, "queries", out.queries, error) &&
+                   get_u32(root, "keys", out.keys, error) && get_u32(root, "dim", out.dim, error) &&
+                   get_bool(root, "token_major", out.token_major, error);
     }
     return false;
 }
@@ -252,11 +341,20 @@ const char *spec_name(const KernelSpec &spec) {
         case Op::RmsNorm: return "rms_norm";
         case Op::SwiGlu: return "swi_glu";
         case Op::Softmax: return "softmax";
+        case Op::Rotary: return "rotary";
+        case Op::QkNormRotary: return "qk_norm_rotary";
+        case Op::AttentionTree: return "attention_tree";
+        case Op::CacheAppend: return "cache_append";
+        case Op::AttentionCross: return "attention_cross";
     }
     return "?";
 }
 
 bool validate(const KernelSpec &s, Rules rules, std::string &error) {
+    if (rules == Rules::Reference && s.op >= Op::Rotary) {
+        error = std::string(tag_of(s.op)) + " is not an operation of the reference";
+        return false;
+    }
     switch (s.op) {
         case Op::Elementwise: {
             if (!dim_ok(s.len, error)) return false;
@@ -310,6 +408,32 @@ bool validate(const KernelSpec &s, Rules rules, std::string &error) {
             return true;
         case Op::Softmax:
             return matrix_ok(s.rows, s.cols, error);
+        case Op::Rotary:
+            return rotation_ok(s, error) && heads_ok(s.batch, s.heads, s.seq, s.dim, kIntMax, error);
+        case Op::QkNormRotary:
+            if (!rotation_ok(s, error) || !heads_ok(s.batch, s.heads, s.seq, s.dim, kIntMax, error) ||
+                !heads_ok(s.batch, s.kv_heads, s.seq, s.dim, kIntMax, error))
+                return false;
+            if (!(std::isfinite(s.epsilon) && s.epsilon > 0.0f)) {
+                error = "epsilon must be finite and positive";
+                return false;
+            }
+            return true;
+        case Op::AttentionTree:
+            if (!(s.nodes >= 1 && s.nodes <= kMaxTreeNodes)) { error = "nodes must be 1..=256"; return false; }
+            return grouped_ok(s, error) && whole_ok(s.capacity, "capacity", error) &&
+                   heads_ok(s.batch, s.heads, s.nodes, s.dim, kIntMax, error) &&
+                   heads_ok(s.batch, s.kv_heads, s.capacity, s.dim, kMaxCacheElements, error);
+        case Op::CacheAppend:
+            if (!(s.dim >= 1 && s.dim <= kMaxRotaryDim)) { error = "head dimension must be 1..=512"; return false; }
+            return whole_ok(s.rows, "rows", error) && whole_ok(s.picks, "picks", error) &&
+                   whole_ok(s.capacity, "capacity", error) && matrix_ok(s.batch, s.picks, error) &&
+                   heads_ok(s.batch, s.kv_heads, s.rows, s.dim, kIntMax, error) &&
+                   heads_ok(s.batch, s.kv_heads, s.capacity, s.dim, kMaxCacheElements, error);
+        case Op::AttentionCross:
+            return grouped_ok(s, error) && whole_ok(s.keys, "keys", error) &&
+                   heads_ok(s.batch, s.heads, s.queries, s.dim, kIntMax, error) &&
+                   heads_ok(s.batch, s.kv_heads, s.keys, s.dim, kMaxCacheElements, error);
     }
     error = "unknown op";
     return false;
@@ -328,6 +452,7 @@ std::vector<Binding> bindings(const KernelSpec &s) {
                                         "input4", "input5", "input6", "input7"};
     const uint64_t hsd = uint64_t(s.heads) * s.seq * s.dim;
     const uint64_t hss = uint64_t(s.heads) * s.seq * s.seq;
+    const uint64_t b = s.batch, d = s.dim, kv = b * s.kv_heads * d;
     switch (s.op) {
         case Op::Elementwise: {
             std::vector<Binding> out;
@@ -359,6 +484,25 @@ std::vector<Binding> bindings(const KernelSpec &s) {
                     {"out", uint64_t(s.rows) * s.cols, true}};
         case Op::Softmax:
             return {{"x", uint64_t(s.rows) * s.cols, false}, {"out", uint64_t(s.rows) * s.cols, true}};
+        case Op::Rotary:
+            return {{"x", b * s.seq * s.heads * d, false}, {"positions", b * s.seq, false},
+                    {"out", b * s.seq * s.heads * d, true}};
+        case Op::QkNormRotary:
+            return {{"q", b * s.seq * s.heads * d, false}, {"k", kv * s.seq, false}, {"q_weight", d, false},
+                    {"k_weight", d, false}, {"positions", b * s.seq, false},
+                    {"q_out", b * s.seq * s.heads * d, true}, {"k_out", kv * s.seq, true}};
+        case Op::AttentionTree:
+            return {{"q", b * s.heads * s.nodes * d, false}, {"k_cache", kv * s.capacity, false},
+                    {"v_cache", kv * s.capacity, false}, {"lengths", b, false}, {"k_draft", kv * s.nodes, false},
+                    {"v_draft", kv * s.nodes, false}, {"parents", b * s.nodes, false},
+                    {"out", b * s.heads * s.nodes * d, true}};
+        case Op::CacheAppend:
+            return {{"k", kv * s.rows, false}, {"v", kv * s.rows, false}, {"picks", b * s.picks, false},
+                    {"lengths", b, false}, {"k_cache", kv * s.capacity, true}, {"v_cache", kv * s.capacity, true},
+                    {"new_lengths", b, true}};
+        case Op::AttentionCross:
+            return {{"q", b * s.heads * s.queries * d, false}, {"k", kv * s.keys, false}, {"v", kv * s.keys, false},
+                    {"lengths", b, false}, {"out", b * s.heads * s.queries * d, true}};
     }
     return {};
 }
@@ -412,8 +556,46 @@ std::string canonical_json(const KernelSpec &s) {
         case Op::AttentionApply: u("heads", s.heads); u("seq", s.seq); u("dim", s.dim); break;
         case Op::RmsNorm: u("rows", s.rows); u("cols", s.cols); f("epsilon", s.epsilon); break;
         case Op::Softmax: u("rows", s.rows); u("cols", s.cols); break;
+        case Op::Rotary:
+        case Op::QkNormRotary:
+            u("batch", s.batch); u("seq", s.seq); u("heads", s.heads);
+            if (s.op == Op::QkNormRotary) u("kv_heads", s.kv_heads);
+            u("dim", s.dim); u("rotary_dim", s.rotary_dim); b("interleaved", s.interleaved);
+            if (s.op == Op::Rotary) b("inverse", s.inverse);
+            b("token_major", s.token_major); b("out_token_major", s.out_token_major);
+            if (s.op == Op::QkNormRotary) f("epsilon", s.epsilon);
+            f("base", s.base); f("factor", s.factor); f("context", s.context); f("low_turns", s.low_turns);
+            f("high_turns", s.high_turns); f("magnitude", s.magnitude);
+            break;
+        case Op::AttentionTree:
+            u("batch", s.batch); u("heads", s.heads); u("kv_heads", s.kv_heads); u("nodes", s.nodes);
+            u("capacity", s.capacity); u("dim", s.dim); b("token_major", s.token_major);
+            break;
+        case Op::CacheAppend:
+            u("batch", s.batch); u("kv_heads", s.kv_heads); u("rows", s.rows); u("picks", s.picks);
+            u("capacity", s.capacity); u("dim", s.dim); b("token_major", s.token_major);
+            break;
+        case Op::AttentionCross:
+            u("batch", s.batch); u("heads", s.heads); u("kv_heads", s.kv_heads); u("queries", s.queries);
+            u("keys", s.keys); u("dim", s.dim); b("token_major", s.token_major);
+            break;
     }
     return out + "}";
+}
+
+std::vector<double> rotary_rates(const KernelSpec &s) {
+    constexpr double kTau = 6.283185307179586476925286766559;
+    std::vector<double> rates;
+    for (uint32_t i = 0; i < s.rotary_dim / 2; ++i) {
+        const double plain = std::pow(double(s.base), -2.0 * i / s.rotary_dim) / kTau;
+        double keep = 0.0;
+        if (s.context > 0.0f) {
+            keep = (s.context * plain - s.low_turns) / (double(s.high_turns) - s.low_turns);
+            keep = keep < 0.0 ? 0.0 : keep > 1.0 ? 1.0 : keep;
+        }
+        rates.push_back(plain * (keep + (1.0 - keep) / s.factor));
+    }
+    return rates;
 }
 
 std::vector<Instr> compile_expression(const Expr &expr) {

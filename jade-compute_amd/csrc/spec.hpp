@@ -27,6 +27,12 @@ enum class Op {
     RmsNorm,
     SwiGlu,
     Softmax,
+    // A decoder's step, which the reference's IR does not have.
+    Rotary,
+    QkNormRotary,
+    AttentionTree,
+    CacheAppend,
+    AttentionCross,
 };
 
 // Expression tree, ir.rs:74-84.
@@ -57,7 +63,16 @@ struct KernelSpec {
     bool tiled = false, causal = false;
     float alpha = 0.0f, epsilon = 0.0f;
     std::shared_ptr<Expr> expression;
+    // The operators of a decoder's step.
+    uint32_t batch = 0, kv_heads = 0, rotary_dim = 0, queries = 0, keys = 0, nodes = 0, capacity = 0, picks = 0;
+    bool interleaved = false, inverse = false, token_major = false, out_token_major = false;
+    float base = 0.0f, factor = 1.0f, context = 0.0f, low_turns = 0.0f, high_turns = 0.0f, magnitude = 1.0f;
 };
+
+constexpr uint32_t kMaxRotaryDim = 512;        // head dim: a head in one wavefront's registers
+constexpr uint32_t kMaxTreeNodes = 256;        // drafted nodes of a sequence
+constexpr uint32_t kMaxWhole = 1u << 24;       // whole numbers are FP32 values: all up to here are exact
+constexpr uint64_t kMaxCacheElements = 1ull << 40;
 
 // ir.rs:146-151. Elements are f32 counts.
 struct Binding {
@@ -94,6 +109,14 @@ bool validate_bindings(const KernelSpec &spec, const uint64_t *lengths, const ui
 
 // Compact serde-shaped JSON (tag first, fields in declaration order).
 std::string canonical_json(const KernelSpec &spec);
+
+// Rotations of pair i per position, in turns (angle / 2 pi) and 64 bits:
+// base^(-2i / rotary_dim) / 2 pi, scaled for long contexts. With no `context`
+// every rate is divided by `factor`. With one, a pair that turns at least
+// `high_turns` times over `context` positions keeps its rate, one that turns
+// at most `low_turns` times has it divided by `factor`, and those between are
+// blended linearly in their turns.
+std::vector<double> rotary_rates(const KernelSpec &spec);
 
 // Postfix lowering of an Elementwise expression (depth-first, left first).
 std::vector<Instr> compile_expression(const Expr &expr);
