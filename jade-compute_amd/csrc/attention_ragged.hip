@@ -34,56 +34,71 @@ typedef float f32x4 __attribute__((ext_vector_type(4)));
 
 constexpr int kThreads = 256, kWaves = 4;
 constexpr int kTile = 64;   // keys per tile
-constexpr uint32_t kWorkers = 512;  // runs: two blocks per CU
+constexpr uint32_t kCus = 256;
 constexpr float kLazyMax = 8.0f;   // log2 units: the running maximum moves only past this
 constexpr uint32_t kRawBuffer = 0x00020000;    // buffer descriptor word 3: raw buffer, 32-bit data format
 constexpr uint32_t kDeadOffset = 0x80000000u;  // past every tile: reads zero
 constexpr float kLog2e = 1.44269504088896340736f;
 constexpr int kWords = int(kMaxTreeNodes) / 64;
 
-// Tiles of one (kv head, row block) of sequence b.
-__device__ inline uint32_t tiles_of(const RaggedArgs &a, uint32_t b, uint32_t draft_tiles) {
-    return (whole_below(a.lengths[b], a.keys) + kTile - 1) / kTile + draft_tiles;
-}
-__device__ inline uint32_t scan_add(uint32_t x, int lane) {
-#pragma unroll
-    for (int step = 1; step < 64; step *= 2) {
-        const uint32_t y = __shfl_up(x, step);
-        if (lane >= step) x += y;
-    }
+__device__ inline uint32_t uniform(uint32_t x) { return __builtin_amdgcn_readfirstlane(x); }
+__device__ inline uint32_t of_lane(uint32_t x, int lane) { return __builtin_amdgcn_readlane(x, lane); }
+
+// Sum over the lanes up to and with this one: within the rows of 16 by shifts, then
+// each row's last lane into the rows after it.
+__device__ inline uint32_t scan_add(uint32_t x) {
+#define JADE_SCAN(control, rows) x += __builtin_amdgcn_update_dpp(0, x, control, rows, 0xf, false)
+    JADE_SCAN(0x111, 0xf);
+    JADE_SCAN(0x112, 0xf);
+    JADE_SCAN(0x114, 0xf);
+    JADE_SCAN(0x118, 0xf);
+    JADE_SCAN(0x142, 0xa);  // row_bcast:15 into rows 1 and 3
+    JADE_SCAN(0x143, 0xc);  // row_bcast:31 into rows 2 and 3
+#undef JADE_SCAN
     return x;
 }
-__device__ inline uint32_t uniform(uint32_t x) { return __builtin_amdgcn_readfirstlane(x); }
 
-// Tiles of all sequences (of one (kv head, row block) each).
-__device__ inline uint32_t all_tiles(const RaggedArgs &a, uint32_t draft_tiles) {
-    const int lane = threadIdx.x & 63;
-    uint32_t sum = 0;
-    for (uint32_t b0 = 0; b0 < a.batch; b0 += 64) {
-        const uint32_t b = b0 + lane;
-        sum += uniform(__shfl(scan_add(b < a.batch ? tiles_of(a, b, draft_tiles) : 0, lane), 63));
+// The tiles of every sequence, of one (kv head, row block) each. A lane has the
+// sequences of its number modulo 64; those of the first 64 stay in registers.
+struct Spread {
+    const RaggedArgs &a;
+    const uint32_t draft_tiles, own, up_to;
+    uint32_t total;
+
+    __device__ uint32_t tiles_at(uint32_t b) const {
+        return b < a.batch ? (whole_below(a.lengths[b], a.keys) + kTile - 1) / kTile + draft_tiles : 0u;
     }
-    return sum;
-}
-// The sequence with tile `t` < all_tiles() and the tiles before it.
-__device__ inline void find_sequence(const RaggedArgs &a, uint32_t draft_tiles, uint32_t t, uint32_t &b,
-                                     uint32_t &before) {
-    const int lane = threadIdx.x & 63;
-    before = 0;
-    for (uint32_t b0 = 0; b0 < a.batch; b0 += 64) {
-        const uint32_t at = b0 + lane;
-        const uint32_t own = at < a.batch ? tiles_of(a, at, draft_tiles) : 0, up_to = scan_add(own, lane);
-        const uint64_t past = __ballot(before + up_to > t);
-        if (past) {
-            const int first = __builtin_ctzll(past);
-            b = b0 + first;
-            before = uniform(before + __shfl(up_to - own, first));
-            return;
+    __device__ explicit Spread(const RaggedArgs &args)
+        : a(args), draft_tiles((a.nodes + kTile - 1) / kTile), own(tiles_at(threadIdx.x & 63)), up_to(scan_add(own)),
+          total(of_lane(up_to, 63)) {
+        for (uint32_t b0 = 64; b0 < a.batch; b0 += 64) total += of_lane(scan_add(tiles_at(b0 + (threadIdx.x & 63))), 63);
+    }
+    // The sequence that tile t < total belongs to, and the tiles before it.
+    __device__ void find(uint32_t t, uint32_t &b, uint32_t &before) const {
+        before = 0;
+        uint32_t sum = up_to, mine = own;
+        for (b = 0;; b += 64, mine = tiles_at(b + (threadIdx.x & 63)), sum = scan_add(mine)) {
+            const uint64_t past = __ballot(before + sum > t);
+            if (past) {
+                const int first = __builtin_ctzll(past);
+                b += first;
+                before += of_lane(sum - mine, first);
+                return;
+            }
+            before += of_lane(sum, 63);
         }
-        before += uniform(__shfl(up_to, 63));
     }
-    b = a.batch;  // not reached
-}
+    // The tiles before sequence b.
+    __device__ uint32_t before(uint32_t b) const {
+        uint32_t sum = 0, last = up_to - own;
+        for (uint32_t b0 = 64; b0 <= b; b0 += 64) {
+            sum += b0 == 64 ? of_lane(up_to, 63) : of_lane(scan_add(tiles_at(b0 - 64 + (threadIdx.x & 63))), 63);
+            const uint32_t mine = tiles_at(b0 + (threadIdx.x & 63));
+            last = scan_add(mine) - mine;
+        }
+        return sum + of_lane(last, int(b & 63));
+    }
+};
 
 __device__ inline bool is_node(float parent, int n) {
     return parent == -1.f || (parent >= 0.f && parent < float(n) && parent == truncf(parent));
@@ -115,25 +130,38 @@ __device__ inline void store_row(const RaggedArgs &a, uint32_t b, uint32_t kv, u
     }
 }
 
-// DP: head dim padded (64, 128); QT: row tiles of 16 per block; VEC: rows of whole
-// float4s, 16-byte aligned.
-template <int DP, int QT, bool VEC>
-__global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2, 2))) void attention_ragged(RaggedArgs a) {
-    constexpr int KJ = DP / 16, NJ = DP / 64, RB = 16 * QT, PITCH = DP + 4;
+// A block's shape: QT row tiles of 16 per wave, RG groups of waves with rows of their
+// own, four waves by keys in each. One row tile keeps its Q in registers, two have
+// it in LDS (the space that the waves' sums take later).
+template <int DP, int QT, int RG>
+struct Shape {
+    static constexpr int kRows = 16 * QT * RG, kThreads = 64 * kWaves * RG, kPitch = DP + 4;
+    static constexpr bool kQInLds = QT > 1;
+};
+
+// DP: head dim padded (64, 128); VEC: rows of whole float4s, 16-byte aligned.
+template <int DP, int QT, int RG, bool VEC>
+__global__ __launch_bounds__(64 * kWaves * RG) __attribute__((amdgpu_waves_per_eu(2, 2))) void
+attention_ragged(RaggedArgs a) {
+    using S = Shape<DP, QT, RG>;
+    constexpr int KJ = DP / 16, NJ = DP / 64, RB = S::kRows, PITCH = S::kPitch;
     __shared__ __attribute__((aligned(16))) float part[kWaves][RB][PITCH];
     __shared__ float2 ml[kWaves][RB];
     __shared__ uint64_t sees[kMaxTreeNodes][kWords];
     __shared__ int above[kMaxTreeNodes];
-    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    float (*const qs)[PITCH] = part[0];  // Q in log2 units, until the sums are joined
+    const int tid = threadIdx.x, lane = tid & 63, waves = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int wave = waves & 3, row0 = (waves >> 2) * 16 * QT;  // this wave's keys of a tile; its rows
     const int m = lane & 15, g = lane >> 4;
-    const uint32_t draft_tiles = (a.nodes + kTile - 1) / kTile, units = a.kv_heads * a.row_blocks;
-    const uint32_t total = all_tiles(a, draft_tiles) * units, chunk = (total + a.runs - 1) / a.runs;
+    const uint32_t units = a.kv_heads * a.row_blocks;
+    const Spread spread(a);
+    const uint32_t total = spread.total * units, chunk = (total + a.runs - 1) / a.runs;
     const uint32_t run = run_of(blockIdx.x, a.runs);
     if (uint64_t(run) * chunk >= total) return;
     uint32_t t = run * chunk;
     const uint32_t t_stop = min(total, t + chunk);
     uint32_t b, before;
-    find_sequence(a, draft_tiles, t / units, b, before);
+    spread.find(t / units, b, before);
 
     const uint32_t row_bytes = a.k_row * 4u;
     uint32_t koff[KJ], voff[NJ][4];
@@ -152,7 +180,7 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2, 2))
 
     while (t < t_stop) {
         const uint32_t len = uniform(whole_below(a.lengths[b], a.keys));
-        const uint32_t cached = (len + kTile - 1) / kTile, tiles = cached + draft_tiles;
+        const uint32_t cached = (len + kTile - 1) / kTile, tiles = cached + spread.draft_tiles;
         if (!tiles) {
             ++b;
             continue;
@@ -161,61 +189,8 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2, 2))
         const uint32_t kv = unit / a.row_blocks, rb = unit - kv * a.row_blocks;
         const uint32_t end = min(tiles, begin + (t_stop - t));
         const bool whole = begin == 0 && end == tiles;
-
-        if (end > cached) {  // the tree: bit n' of row n where node n sees node n'
-            __syncthreads();
-            const int n = tid;
-            int parent = -2;
-            if (n < int(a.nodes)) {
-                const float p = a.parents[size_t(b) * a.nodes + n];
-                parent = is_node(p, n) ? int(p) : -2;
-                above[n] = parent;
-#pragma unroll
-                for (int w = 0; w < kWords; ++w) sees[n][w] = parent != -2 && n / 64 == w ? 1ull << (n & 63) : 0ull;
-            }
-            // Ancestors by doubling: after k steps a node has those up to 2^k above it.
-            for (uint32_t reach = 1; reach < a.nodes; reach *= 2) {
-                __syncthreads();
-                uint64_t more[kWords] = {};
-                int next = parent;
-                if (parent >= 0) {
-#pragma unroll
-                    for (int w = 0; w < kWords; ++w) more[w] = sees[parent][w];
-                    next = above[parent];
-                }
-                __syncthreads();
-                if (parent >= 0) {
-#pragma unroll
-                    for (int w = 0; w < kWords; ++w) sees[n][w] |= more[w];
-                    above[n] = parent = next;
-                }
-            }
-            __syncthreads();
-        }
-
-        // Q^T operand, in log2 units: row m of tile qt, dims 16 j + 4 g + e.
-        f32x4 qf[QT][KJ];
-        int node[QT];
-#pragma unroll
-        for (int qt = 0; qt < QT; ++qt) {
-            const uint32_t r = rb * RB + 16 * qt + m, head = r / a.queries, query = r - head * a.queries;
-            node[qt] = int(query);
-            const bool live = head < a.group;
-            const float *row = a.q + size_t(b) * a.q_batch + (size_t(kv) * a.group + head) * a.q_head + size_t(query) * a.q_row;
-#pragma unroll
-            for (int j = 0; j < KJ; ++j) {
-                const int d = 16 * j + 4 * g;
-                f32x4 x = {0.f, 0.f, 0.f, 0.f};
-                if (VEC) {
-                    if (live && d < a.dim) x = *reinterpret_cast<const f32x4 *>(row + d);
-                } else {
-#pragma unroll
-                    for (int e = 0; e < 4; ++e)
-                        if (live && d + e < a.dim) x[e] = row[d + e];
-                }
-                qf[qt][j] = x * a.qscale;
-            }
-        }
+        float above_me = 0.f;
+        if (end > cached && tid < int(a.nodes)) above_me = a.parents[size_t(b) * a.nodes + tid];
 
         const float *kb = a.k + size_t(b) * a.k_batch + size_t(kv) * a.k_head;
         const float *vb = a.v + size_t(b) * a.k_batch + size_t(kv) * a.k_head;
@@ -252,6 +227,36 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2, 2))
 #pragma unroll
                 for (int i = 0; i < 4; ++i) vf[j][i] = load(from, voff[j][i], 64 * j + 4 * m);
         };
+        // Row r of the block, dims d .. d + 3, in log2 units.
+        auto load_q = [&](int r, int d) {
+            const uint32_t at = rb * RB + r, head = at / a.queries, query = at - head * a.queries;
+            const float *row = a.q + size_t(b) * a.q_batch + (size_t(kv) * a.group + head) * a.q_head + size_t(query) * a.q_row;
+            f32x4 x = {0.f, 0.f, 0.f, 0.f};
+            if (VEC) {
+                if (head < a.group && d < a.dim) x = *reinterpret_cast<const f32x4 *>(row + d);
+            } else {
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    if (head < a.group && d + e < a.dim) x[e] = row[d + e];
+            }
+            return x * a.qscale;
+        };
+        load_k(begin);
+        load_v(begin);
+        // Q^T operand: row m of tile qt, dims 16 j + 4 g + e.
+        f32x4 qf[S::kQInLds ? 1 : KJ];
+        if constexpr (S::kQInLds) {
+            __syncthreads();  // the last unit's sums are read
+            for (int i = tid; i < RB * (DP / 4); i += S::kThreads)
+                *reinterpret_cast<f32x4 *>(&qs[i / (DP / 4)][i % (DP / 4) * 4]) = load_q(i / (DP / 4), i % (DP / 4) * 4);
+            __syncthreads();
+        } else {
+#pragma unroll
+            for (int j = 0; j < KJ; ++j) qf[j] = load_q(row0 + m, 16 * j + 4 * g);
+        }
+        auto q_of = [&](int qt, int j) {
+            return S::kQInLds ? *reinterpret_cast<const f32x4 *>(&qs[row0 + 16 * qt + m][16 * j + 4 * g]) : qf[j];
+        };
 
         f32x4 acc[QT][NJ][4];
         float top[QT], sum[QT];
@@ -264,37 +269,23 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2, 2))
 #pragma unroll
                 for (int e = 0; e < 4; ++e) acc[qt][j][e] = f32x4{0.f, 0.f, 0.f, 0.f};
         }
-        load_k(begin);
-        load_v(begin);
-        for (uint32_t x = begin; x < end; ++x) {
-            f32x4 p[QT];
+        f32x4 p[QT];  // scores, then weights, of keys 16 wave + 4 g + i
+        auto score = [&]() __attribute__((always_inline)) {
 #pragma unroll
             for (int qt = 0; qt < QT; ++qt) p[qt] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-            for (int j = 0; j < KJ; ++j)
+            for (int j = 0; j < KJ; ++j) {
+                f32x4 q[QT];
+#pragma unroll
+                for (int qt = 0; qt < QT; ++qt) q[qt] = q_of(qt, j);
 #pragma unroll
                 for (int e = 0; e < 4; ++e)
 #pragma unroll
                     for (int qt = 0; qt < QT; ++qt)
-                        p[qt] = __builtin_amdgcn_mfma_f32_16x16x4f32(kf[j][e], qf[qt][j][e], p[qt], 0, 0, 0);
-            load_k(x + 1);
-            const bool drafted = x >= cached;
-            const int first = int(drafted ? x - cached : x) * kTile + 16 * wave + 4 * g;  // this lane's key i = 0
-            if (drafted) {
-#pragma unroll
-                for (int qt = 0; qt < QT; ++qt) {
-                    const uint64_t word = node[qt] < int(a.nodes) ? sees[node[qt]][x - cached] : 0;
-#pragma unroll
-                    for (int i = 0; i < 4; ++i)
-                        if (!(word >> ((first + i) & 63) & 1)) p[qt][i] = -INFINITY;
-                }
-            } else if ((x + 1) * kTile > len) {
-#pragma unroll
-                for (int qt = 0; qt < QT; ++qt)
-#pragma unroll
-                    for (int i = 0; i < 4; ++i)
-                        if (first + i >= int(len)) p[qt][i] = -INFINITY;
+                        p[qt] = __builtin_amdgcn_mfma_f32_16x16x4f32(kf[j][e], q[qt][e], p[qt], 0, 0, 0);
             }
+        };
+        auto weigh = [&]() __attribute__((always_inline)) {
 #pragma unroll
             for (int qt = 0; qt < QT; ++qt) {
                 const float most = fmaxf(fmaxf(p[qt].x, p[qt].y), fmaxf(p[qt].z, p[qt].w));
@@ -315,19 +306,8 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2, 2))
                     sum[qt] += p[qt][i];
                 }
             }
-            bool odd = false;  // a drafted value that is not finite: not every row may see it
-            if (drafted) {
-#pragma unroll
-                for (int j = 0; j < NJ; ++j)
-#pragma unroll
-                    for (int i = 0; i < 4; ++i)
-#pragma unroll
-                        for (int e = 0; e < 4; ++e)
-                            if (!(fabsf(vf[j][i][e]) < INFINITY)) {
-                                vf[j][i][e] = 0.f;
-                                odd = true;
-                            }
-            }
+        };
+        auto add = [&]() __attribute__((always_inline)) {
 #pragma unroll
             for (int i = 0; i < 4; ++i)
 #pragma unroll
@@ -338,17 +318,89 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2, 2))
                         for (int qt = 0; qt < QT; ++qt)
                             acc[qt][j][e] =
                                 __builtin_amdgcn_mfma_f32_16x16x4f32(vf[j][i][e], p[qt][i], acc[qt][j][e], 0, 0, 0);
+        };
+        uint32_t x = begin;
+        for (; x < min(end, cached); ++x) {
+            score();
+            load_k(x + 1);
+            if ((x + 1) * kTile > len) {
+                const int first = int(x) * kTile + 16 * wave + 4 * g;
+#pragma unroll
+                for (int qt = 0; qt < QT; ++qt)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        if (first + i >= int(len)) p[qt][i] = -INFINITY;
+            }
+            weigh();
+            add();
             load_v(x + 1);
-            if (drafted && __any(odd)) {
-                for (int key = 0; key < 16; ++key) {
-                    const int at = int(x - cached) * kTile + 16 * wave + key;
-                    if (at >= int(a.nodes)) break;
-                    const float *row = vd + size_t(at) * a.k_row;
+        }
+
+        if (end > cached) {
+            // The tree: bit n' of row n where node n sees node n'. Ancestors by doubling:
+            // after k steps a node has those up to 2^k above it.
+            __syncthreads();
+            const int n = tid;
+            int parent = -2;
+            if (n < int(a.nodes)) {
+                parent = is_node(above_me, n) ? int(above_me) : -2;
+                above[n] = parent;
+#pragma unroll
+                for (int w = 0; w < kWords; ++w) sees[n][w] = parent != -2 && n / 64 == w ? 1ull << (n & 63) : 0ull;
+            }
+            for (uint32_t reach = 1; reach < a.nodes; reach *= 2) {
+                __syncthreads();
+                uint64_t more[kWords] = {};
+                int next = parent;
+                if (parent >= 0) {
+#pragma unroll
+                    for (int w = 0; w < kWords; ++w) more[w] = sees[parent][w];
+                    next = above[parent];
+                }
+                __syncthreads();
+                if (parent >= 0) {
+#pragma unroll
+                    for (int w = 0; w < kWords; ++w) sees[n][w] |= more[w];
+                    above[n] = parent = next;
+                }
+            }
+            __syncthreads();
+            for (; x < end; ++x) {
+                const uint32_t tile = x - cached;
+                const int first = 16 * wave + 4 * g;
+                score();
+                load_k(x + 1);
+                uint64_t seen[QT];
+#pragma unroll
+                for (int qt = 0; qt < QT; ++qt) {
+                    const uint32_t node = (rb * RB + row0 + 16 * qt + m) % a.queries;  // queries == nodes
+                    seen[qt] = sees[node][tile];
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        if (!(seen[qt] >> (first + i) & 1)) p[qt][i] = -INFINITY;
+                }
+                weigh();
+                bool odd = false;  // a drafted value that is not finite: not every row may see it
+#pragma unroll
+                for (int j = 0; j < NJ; ++j)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e)
+                            if (!(fabsf(vf[j][i][e]) < INFINITY)) {
+                                vf[j][i][e] = 0.f;
+                                odd = true;
+                            }
+                add();
+                load_v(x + 1);
+                if (!__any(odd)) continue;
+                for (int key = 16 * wave; key < 16 * wave + 16 && tile * kTile + key < a.nodes; ++key) {
+                    const float *row = vd + size_t(tile * kTile + key) * a.k_row;
 #pragma unroll
                     for (int qt = 0; qt < QT; ++qt) {
-                        const float weight = __shfl(key & 2 ? (key & 1 ? p[qt].w : p[qt].z) : (key & 1 ? p[qt].y : p[qt].x),
-                                                    16 * (key >> 2) + m);
-                        if (node[qt] >= int(a.nodes) || !(sees[node[qt]][at / 64] >> (at & 63) & 1)) continue;
+                        const float mine = key & 2 ? (key & 1 ? p[qt].w : p[qt].z) : (key & 1 ? p[qt].y : p[qt].x);
+                        const float weight = __shfl(mine, 16 * ((key & 15) >> 2) + m);
+                        if (!(seen[qt] >> key & 1)) continue;
 #pragma unroll
                         for (int j = 0; j < NJ; ++j)
 #pragma unroll
@@ -369,18 +421,18 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2, 2))
 #pragma unroll
         for (int qt = 0; qt < QT; ++qt) {
             const float all = across_keys_sum(sum[qt]);
-            if (g == 0) ml[wave][16 * qt + m] = float2{top[qt], all};
+            if (g == 0) ml[wave][row0 + 16 * qt + m] = float2{top[qt], all};
 #pragma unroll
             for (int j = 0; j < NJ; ++j)
 #pragma unroll
                 for (int i = 0; i < 4; ++i)
-                    *reinterpret_cast<f32x4 *>(&part[wave][16 * qt + m][64 * j + 16 * g + 4 * i]) =
+                    *reinterpret_cast<f32x4 *>(&part[wave][row0 + 16 * qt + m][64 * j + 16 * g + 4 * i]) =
                         f32x4{acc[qt][j][0][i], acc[qt][j][1][i], acc[qt][j][2][i], acc[qt][j][3][i]};
         }
         __syncthreads();
         const uint32_t rows = min(uint32_t(RB), a.group * a.queries - rb * RB);
         const size_t slot = 2 * size_t(run) + (begin == 0);
-        for (uint32_t at = tid; at < rows * (DP / 4); at += kThreads) {
+        for (uint32_t at = tid; at < rows * (DP / 4); at += S::kThreads) {
             const uint32_t row = at / (DP / 4), d = at % (DP / 4) * 4;
             float most = -INFINITY;
 #pragma unroll
@@ -410,91 +462,126 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2, 2))
     }
 }
 
-// What the runs left of a (sequence, kv head, row block) cut between them. Block x
-// looks at the cut before run x and joins the unit if that is its first one; block y
-// takes two rows of it. Sequences without keys get their zeros here.
-template <int DP, int QT, bool VEC>
+// What the runs left of a (sequence, kv head, row block) cut between them, and the
+// zeros of sequences without keys. Block y has row y of the units of block x: of
+// unit x itself where there are at most `runs` units, else of the one that the cut
+// before run x is the first of.
+template <int DP, int RB, bool VEC>
 __global__ __launch_bounds__(kThreads) void attention_ragged_join(RaggedArgs a) {
-    constexpr int RB = 16 * QT, LANES = DP / 4, PARTS = kThreads / (2 * LANES);
-    __shared__ __attribute__((aligned(16))) f32x4 sums[PARTS][2 * LANES];
-    __shared__ float weights[PARTS][2 * LANES];
-    const uint32_t draft_tiles = (a.nodes + kTile - 1) / kTile, units = a.kv_heads * a.row_blocks;
-    if (!draft_tiles)
-        for (uint32_t b = blockIdx.x; b < a.batch; b += a.runs) {
-            if (whole_below(a.lengths[b], a.keys)) continue;
-            const size_t n = size_t(a.kv_heads) * a.group * a.queries * a.dim;
-            float *out = a.out + size_t(b) * a.q_batch;
-            for (size_t i = blockIdx.y * kThreads + threadIdx.x; i < n; i += gridDim.y * kThreads) out[i] = 0.f;
-        }
-    const uint32_t total = all_tiles(a, draft_tiles) * units, chunk = (total + a.runs - 1) / a.runs;
-    const uint32_t run = blockIdx.x;
-    if (run == 0 || uint64_t(run) * chunk >= total) return;
-    const uint32_t t = run * chunk;
-    uint32_t b, before;
-    find_sequence(a, draft_tiles, t / units, b, before);
-    const uint32_t tiles = uniform(tiles_of(a, b, draft_tiles)), in = t - before * units, unit = in / tiles;
-    const uint32_t begin = in - unit * tiles, kv = unit / a.row_blocks, rb = unit - kv * a.row_blocks;
-    if (begin == 0 || begin > chunk) return;
-    const uint32_t first = run - 1, last = (t - begin + tiles - 1) / chunk;
-    const uint32_t rows = min(uint32_t(RB), a.group * a.queries - rb * RB);
-    if (2 * blockIdx.y >= rows) return;
-    const int tid = threadIdx.x, at = tid % (2 * LANES), p = tid / (2 * LANES);
-    const uint32_t row = 2 * blockIdx.y + at / LANES, d = at % LANES * 4;
+    constexpr int LANES = DP / 4, PARTS = kThreads / LANES;
+    __shared__ __attribute__((aligned(16))) f32x4 sums[PARTS][LANES];
+    __shared__ float weights[PARTS];
+    const int tid = threadIdx.x, lane = tid % LANES, p = tid / LANES;
+    const uint32_t units = a.kv_heads * a.row_blocks, row = blockIdx.y, d = 4 * lane;
+    const bool by_unit = a.batch * units <= a.runs;
+    const Spread spread(a);
+    const uint32_t chunk = (spread.total * units + a.runs - 1) / a.runs;
+    uint32_t b, unit, start, tiles;
+    if (by_unit) {
+        b = blockIdx.x / units;
+        unit = blockIdx.x - b * units;
+        tiles = uniform(spread.tiles_at(b));
+        start = spread.before(b) * units + unit * tiles;
+    } else {
+        if (!spread.draft_tiles)
+            for (b = blockIdx.x; b < a.batch; b += a.runs) {
+                if (spread.tiles_at(b)) continue;
+                const size_t n = size_t(a.kv_heads) * a.group * a.queries * a.dim;
+                float *out = a.out + size_t(b) * a.q_batch;
+                for (size_t i = blockIdx.y * kThreads + tid; i < n; i += gridDim.y * kThreads) out[i] = 0.f;
+            }
+        const uint64_t cut = uint64_t(blockIdx.x) * chunk;
+        if (cut == 0 || cut >= spread.total * units) return;
+        uint32_t before;
+        spread.find(uint32_t(cut) / units, b, before);
+        tiles = uniform(spread.tiles_at(b));
+        unit = (uint32_t(cut) - before * units) / tiles;
+        start = before * units + unit * tiles;
+        if (start + chunk < cut || start == cut) return;  // not its first cut
+    }
+    const uint32_t kv = unit / a.row_blocks, rb = unit - kv * a.row_blocks;
+    if (row >= min(uint32_t(RB), a.group * a.queries - rb * RB)) return;
+    if (!tiles) {
+        if (p == 0) store_row<VEC>(a, b, kv, rb * RB + row, d, f32x4{0.f, 0.f, 0.f, 0.f}, 1.f);
+        return;
+    }
+    const uint32_t first = start / chunk, last = (start + tiles - 1) / chunk;
+    if (first == last) return;
     const float2 *ml = reinterpret_cast<const float2 *>(a.partial + 2 * size_t(a.runs) * RB * DP);
     // A unit's first run had it last, the others first.
     auto slot = [&](uint32_t r) { return (2 * size_t(r) + (r == first)) * RB + row; };
-    float most = -INFINITY, l = 0.f;
+    float most = -INFINITY;
+    for (uint32_t r = first + lane; r <= last; r += LANES) most = fmaxf(most, ml[slot(r)].x);
+#pragma unroll
+    for (int step = LANES / 2; step > 0; step /= 2) most = fmaxf(most, __shfl_xor(most, step));
+    const float from = most == -INFINITY ? 0.f : most;
+    float l = 0.f;
     f32x4 o = {0.f, 0.f, 0.f, 0.f};
-    if (row < rows) {
-        for (uint32_t r = first; r <= last; ++r) most = fmaxf(most, ml[slot(r)].x);
-        const float from = most == -INFINITY ? 0.f : most;
-        for (uint32_t r = first + p; r <= last; r += PARTS) {
-            const float2 x = ml[slot(r)];
-            const float weight = __builtin_amdgcn_exp2f(x.x - from);
-            l = fmaf(weight, x.y, l);
-            o += weight * *reinterpret_cast<const f32x4 *>(a.partial + slot(r) * DP + d);
-        }
+#pragma unroll 4
+    for (uint32_t r = first + p; r <= last; r += PARTS) {
+        const float2 x = ml[slot(r)];
+        const f32x4 y = *reinterpret_cast<const f32x4 *>(a.partial + slot(r) * DP + d);
+        const float weight = __builtin_amdgcn_exp2f(x.x - from);
+        l = fmaf(weight, x.y, l);
+        o += weight * y;
     }
-    sums[p][at] = o;
-    weights[p][at] = l;
+    sums[p][lane] = o;
+    if (lane == 0) weights[p] = l;
     __syncthreads();
-    if (p || row >= rows) return;
+    if (p) return;
 #pragma unroll
     for (int x = 1; x < PARTS; ++x) {
-        o += sums[x][at];
-        l += weights[x][at];
+        o += sums[x][lane];
+        l += weights[x];
     }
     store_row<VEC>(a, b, kv, rb * RB + row, d, o, l);
 }
 
-struct Plan {
-    uint32_t row_blocks;
-    bool two;  // two row tiles of 16 per block
-};
-Plan plan_of(uint32_t rows) { return {rows <= 16 ? 1u : (rows + 31) / 32, rows > 16}; }
+// Rows per block.
+uint32_t block_rows(uint32_t rows) { return rows <= 16 ? 16 : rows <= 32 ? 32 : 64; }
 
-template <int DP, int QT>
-hipError_t launch(hipStream_t stream, const RaggedArgs &a, bool vec) {
-    const dim3 grid(a.runs), join(a.runs, 8 * QT), block(kThreads);
-    if (vec) {
-        hipLaunchKernelGGL((attention_ragged<DP, QT, true>), grid, block, 0, stream, a);
-        hipLaunchKernelGGL((attention_ragged_join<DP, QT, true>), join, block, 0, stream, a);
-    } else {
-        hipLaunchKernelGGL((attention_ragged<DP, QT, false>), grid, block, 0, stream, a);
-        hipLaunchKernelGGL((attention_ragged_join<DP, QT, false>), join, block, 0, stream, a);
-    }
-    return hipGetLastError();
+uint32_t rows_of(const RaggedShape &s) { return s.heads / s.kv_heads * s.queries; }
+uint32_t row_blocks(const RaggedShape &s) {
+    const uint32_t rb = block_rows(rows_of(s));
+    return (rows_of(s) + rb - 1) / rb;
 }
 
 uint64_t ragged_tiles(const RaggedShape &s) {
     const uint64_t tiles = (uint64_t(s.keys) + kTile - 1) / kTile + (s.nodes + kTile - 1) / kTile;
-    return uint64_t(s.batch) * s.kv_heads * plan_of(s.heads / s.kv_heads * s.queries).row_blocks * tiles;
+    return uint64_t(s.batch) * s.kv_heads * row_blocks(s) * tiles;
 }
 
-// Runs of a launch: kWorkers, or one per tile where there can be no more tiles.
+// Runs of a launch: as many blocks as the chip holds at once (two of four waves or
+// one of eight a CU), or one per tile where there can be no more tiles.
 uint32_t runs_of(const RaggedShape &s) {
     const uint64_t tiles = ragged_tiles(s);
-    return tiles >= kWorkers ? kWorkers : uint32_t((tiles + 7) / 8 * 8);
+    const uint32_t most = block_rows(rows_of(s)) == 64 ? kCus : 2 * kCus;
+    return tiles >= most ? most : uint32_t((tiles + 7) / 8 * 8);
+}
+
+template <int DP, int QT, int RG>
+hipError_t launch(hipStream_t stream, const RaggedArgs &a, bool vec) {
+    using S = Shape<DP, QT, RG>;
+    const uint32_t rows = a.group * a.queries, units = a.batch * a.kv_heads * a.row_blocks;
+    const dim3 grid(a.runs), block(S::kThreads);
+    const dim3 join(units < a.runs ? units : a.runs, rows < S::kRows ? rows : S::kRows);
+    if (vec) {
+        hipLaunchKernelGGL((attention_ragged<DP, QT, RG, true>), grid, block, 0, stream, a);
+        hipLaunchKernelGGL((attention_ragged_join<DP, S::kRows, true>), join, dim3(kThreads), 0, stream, a);
+    } else {
+        hipLaunchKernelGGL((attention_ragged<DP, QT, RG, false>), grid, block, 0, stream, a);
+        hipLaunchKernelGGL((attention_ragged_join<DP, S::kRows, false>), join, dim3(kThreads), 0, stream, a);
+    }
+    return hipGetLastError();
+}
+
+template <int DP>
+hipError_t launch_rows(hipStream_t stream, const RaggedArgs &a, bool vec) {
+    switch (block_rows(a.group * a.queries)) {
+        case 16: return launch<DP, 1, 1>(stream, a, vec);
+        case 32: return launch<DP, 2, 1>(stream, a, vec);
+        default: return launch<DP, 2, 2>(stream, a, vec);
+    }
 }
 
 }  // namespace
@@ -502,17 +589,18 @@ uint32_t runs_of(const RaggedShape &s) {
 LaunchShape attention_ragged_shape(const RaggedShape &s) {
     // Tiles are counted in 32 bits.
     if (ragged_tiles(s) > 0x7fffffffull) return {nullptr, {0, 0, 0}, {0, 0, 0}, 0};
-    const bool two = plan_of(s.heads / s.kv_heads * s.queries).two, wide = s.dim > 64;
-    static const char *const names[2][2] = {{"attention_ragged_d64_r16", "attention_ragged_d64_r32"},
-                                            {"attention_ragged_d128_r16", "attention_ragged_d128_r32"}};
-    const uint32_t rb = two ? 32 : 16, pitch = (wide ? 128 : 64) + 4;
-    return {names[wide][two], {runs_of(s), 1, 1}, {kThreads, 1, 1},
+    const bool wide = s.dim > 64;
+    const uint32_t rb = block_rows(rows_of(s)), pitch = (wide ? 128 : 64) + 4;
+    static const char *const names[2][3] = {
+        {"attention_ragged_d64_r16", "attention_ragged_d64_r32", "attention_ragged_d64_r64"},
+        {"attention_ragged_d128_r16", "attention_ragged_d128_r32", "attention_ragged_d128_r64"}};
+    return {names[wide][rb / 32], {runs_of(s), 1, 1}, {uint32_t(rb == 64 ? 2 * kThreads : kThreads), 1, 1},
             uint32_t(kWaves * rb * (pitch * sizeof(float) + sizeof(float2)) +
                      kMaxTreeNodes * (kWords * sizeof(uint64_t) + sizeof(int)))};
 }
 
 size_t attention_ragged_workspace_bytes(const RaggedShape &s) {
-    const size_t rb = plan_of(s.heads / s.kv_heads * s.queries).two ? 32 : 16, dp = s.dim > 64 ? 128 : 64;
+    const size_t rb = block_rows(rows_of(s)), dp = s.dim > 64 ? 128 : 64;
     return 2 * size_t(runs_of(s)) * rb * (dp + 2) * sizeof(float);
 }
 
@@ -533,16 +621,14 @@ hipError_t attention_ragged_f32(hipStream_t stream, const RaggedShape &s, const 
     a.k_row = uint32_t(s.token_major ? d * s.kv_heads : d);
     a.batch = s.batch; a.kv_heads = s.kv_heads; a.group = s.heads / s.kv_heads; a.queries = s.queries;
     a.keys = s.keys; a.nodes = s.nodes; a.dim = s.dim;
-    const Plan p = plan_of(a.group * s.queries);
-    a.row_blocks = p.row_blocks;
+    a.row_blocks = row_blocks(s);
     a.runs = runs_of(s);
     a.qscale = (1.0f / sqrtf(float(s.dim))) * kLog2e;
     uintptr_t bits = 0;
     for (const float *y : {x.q, x.k, x.v, x.k_draft, x.v_draft, const_cast<const float *>(x.out)})
         bits |= reinterpret_cast<uintptr_t>(y);
     const bool vec = s.dim % 4 == 0 && (bits & 15u) == 0;
-    if (s.dim <= 64) return p.two ? launch<64, 2>(stream, a, vec) : launch<64, 1>(stream, a, vec);
-    return p.two ? launch<128, 2>(stream, a, vec) : launch<128, 1>(stream, a, vec);
+    return s.dim <= 64 ? launch_rows<64>(stream, a, vec) : launch_rows<128>(stream, a, vec);
 }
 
 }  // namespace hipk
