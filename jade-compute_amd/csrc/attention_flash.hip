@@ -35,9 +35,6 @@
 // the operands) and queries past 2^64 in log2 units. With such queries out of
 // the way the bits that a K below 2^-78 loses move no score by more than 2^-38
 // a dim. Weights below 2^-100 of the reference weight keep fewer than 24 bits.
-#include <type_traits>
-#include <utility>
-
 #include "attention_flash.hpp"
 #include "split_bf16.hpp"
 
@@ -68,21 +65,6 @@ __device__ inline float halves_sum(float x) {
     const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
     return __uint_as_float(r[0]) + __uint_as_float(r[1]);
 }
-
-// f(0), f(1), ... f(N - 1) with compile-time arguments: the interleaved
-// schedules below are chosen by the compiler's front end, not by its unroller.
-template <class F, int... I>
-__device__ inline void each(std::integer_sequence<int, I...>, F &&f) {
-    (f(std::integral_constant<int, I>{}), ...);
-}
-template <int N, class F>
-__device__ inline void each(F &&f) {
-    each(std::make_integer_sequence<int, N>{}, f);
-}
-// Event E of ALL, spread evenly over the slots, belongs to slot N of SLOTS
-// when first<N> <= E < first<N + 1>.
-template <int N, int ALL, int SLOTS>
-constexpr int kFirstEvent = N >= SLOTS ? ALL : (N * ALL + SLOTS - 1) / SLOTS;
 
 // (head, query block) of workgroup `id` in a launch over heads x blocks. The
 // hardware hands ids to the XCDs in turn. Each XCD takes kHeadGroup heads at a

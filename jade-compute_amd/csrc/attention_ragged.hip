@@ -22,113 +22,16 @@
 // attention_ragged_join. So neither long sequences nor ragged ones leave CUs idle.
 #include <cmath>
 
-#include "attention_ragged.hpp"
 #include "kernels.hpp"
-#include "whole.hpp"
+#include "ragged_device.hpp"
 
 namespace jade {
 namespace hipk {
 namespace {
 
-typedef float f32x4 __attribute__((ext_vector_type(4)));
+using namespace ragged;
 
-constexpr int kThreads = 256, kWaves = 4;
-constexpr int kTile = 64;   // keys per tile
-constexpr uint32_t kCus = 256;
-constexpr float kLazyMax = 8.0f;   // log2 units: the running maximum moves only past this
-constexpr uint32_t kRawBuffer = 0x00020000;    // buffer descriptor word 3: raw buffer, 32-bit data format
-constexpr uint32_t kDeadOffset = 0x80000000u;  // past every tile: reads zero
-constexpr float kLog2e = 1.44269504088896340736f;
-constexpr int kWords = int(kMaxTreeNodes) / 64;
-
-__device__ inline uint32_t uniform(uint32_t x) { return __builtin_amdgcn_readfirstlane(x); }
-__device__ inline uint32_t of_lane(uint32_t x, int lane) { return __builtin_amdgcn_readlane(x, lane); }
-
-// Sum over the lanes up to and with this one: within the rows of 16 by shifts, then
-// each row's last lane into the rows after it.
-__device__ inline uint32_t scan_add(uint32_t x) {
-#define JADE_SCAN(control, rows) x += __builtin_amdgcn_update_dpp(0, x, control, rows, 0xf, false)
-    JADE_SCAN(0x111, 0xf);
-    JADE_SCAN(0x112, 0xf);
-    JADE_SCAN(0x114, 0xf);
-    JADE_SCAN(0x118, 0xf);
-    JADE_SCAN(0x142, 0xa);  // row_bcast:15 into rows 1 and 3
-    JADE_SCAN(0x143, 0xc);  // row_bcast:31 into rows 2 and 3
-#undef JADE_SCAN
-    return x;
-}
-
-// The tiles of every sequence, of one (kv head, row block) each. A lane has the
-// sequences of its number modulo 64; those of the first 64 stay in registers.
-struct Spread {
-    const RaggedArgs &a;
-    const uint32_t draft_tiles, own, up_to;
-    uint32_t total;
-
-    __device__ uint32_t tiles_at(uint32_t b) const {
-        return b < a.batch ? (whole_below(a.lengths[b], a.keys) + kTile - 1) / kTile + draft_tiles : 0u;
-    }
-    __device__ explicit Spread(const RaggedArgs &args)
-        : a(args), draft_tiles((a.nodes + kTile - 1) / kTile), own(tiles_at(threadIdx.x & 63)), up_to(scan_add(own)),
-          total(of_lane(up_to, 63)) {
-        for (uint32_t b0 = 64; b0 < a.batch; b0 += 64) total += of_lane(scan_add(tiles_at(b0 + (threadIdx.x & 63))), 63);
-    }
-    // The sequence that tile t < total belongs to, and the tiles before it.
-    __device__ void find(uint32_t t, uint32_t &b, uint32_t &before) const {
-        before = 0;
-        uint32_t sum = up_to, mine = own;
-        for (b = 0;; b += 64, mine = tiles_at(b + (threadIdx.x & 63)), sum = scan_add(mine)) {
-            const uint64_t past = __ballot(before + sum > t);
-            if (past) {
-                const int first = __builtin_ctzll(past);
-                b += first;
-                before += of_lane(sum - mine, first);
-                return;
-            }
-            before += of_lane(sum, 63);
-        }
-    }
-    // The tiles before sequence b.
-    __device__ uint32_t before(uint32_t b) const {
-        uint32_t sum = 0, last = up_to - own;
-        for (uint32_t b0 = 64; b0 <= b; b0 += 64) {
-            sum += b0 == 64 ? of_lane(up_to, 63) : of_lane(scan_add(tiles_at(b0 - 64 + (threadIdx.x & 63))), 63);
-            const uint32_t mine = tiles_at(b0 + (threadIdx.x & 63));
-            last = scan_add(mine) - mine;
-        }
-        return sum + of_lane(last, int(b & 63));
-    }
-};
-
-__device__ inline bool is_node(float parent, int n) {
-    return parent == -1.f || (parent >= 0.f && parent < float(n) && parent == truncf(parent));
-}
-
-// Run w of the launch: runs of one XCD are neighbours, so the row blocks of one kv
-// head, which read the same keys, meet in its L2.
-__device__ inline uint32_t run_of(uint32_t id, uint32_t runs) { return id % 8 * (runs / 8) + id / 8; }
-
-__device__ inline float across_keys_max(float x) { return fmaxf(fmaxf(x, __shfl_xor(x, 16)), fmaxf(__shfl_xor(x, 32), __shfl_xor(x, 48))); }
-__device__ inline float across_keys_sum(float x) {
-    x += __shfl_xor(x, 16);
-    return x + __shfl_xor(x, 32);
-}
-
-// Row r of (sequence b, kv head): its sums o of dims d .. d + 3 over its weights' sum.
-template <bool VEC>
-__device__ inline void store_row(const RaggedArgs &a, uint32_t b, uint32_t kv, uint32_t r, uint32_t d, f32x4 o, float l) {
-    const uint32_t head = r / a.queries, query = r - head * a.queries;
-    const bool node = !a.nodes || is_node(a.parents[size_t(b) * a.nodes + query], int(query));
-    o = node ? o * (1.0f / l) : f32x4{0.f, 0.f, 0.f, 0.f};
-    float *out = a.out + size_t(b) * a.q_batch + (size_t(kv) * a.group + head) * a.q_head + size_t(query) * a.q_row;
-    if (VEC) {
-        if (d < a.dim) *reinterpret_cast<f32x4 *>(out + d) = o;
-    } else {
-#pragma unroll
-        for (int e = 0; e < 4; ++e)
-            if (d + e < a.dim) out[d + e] = o[e];
-    }
-}
+constexpr int kTile = 64;  // keys per tile
 
 // A block's shape: QT row tiles of 16 per wave, RG groups of waves with rows of their
 // own, four waves by keys in each. One row tile keeps its Q in registers, two have
@@ -154,7 +57,7 @@ attention_ragged(RaggedArgs a) {
     const int wave = waves & 3, row0 = (waves >> 2) * 16 * QT;  // this wave's keys of a tile; its rows
     const int m = lane & 15, g = lane >> 4;
     const uint32_t units = a.kv_heads * a.row_blocks;
-    const Spread spread(a);
+    const Spread<kTile> spread(a);
     const uint32_t total = spread.total * units, chunk = (total + a.runs - 1) / a.runs;
     const uint32_t run = run_of(blockIdx.x, a.runs);
     if (uint64_t(run) * chunk >= total) return;
@@ -337,82 +240,57 @@ attention_ragged(RaggedArgs a) {
         }
 
         if (end > cached) {
-            // The tree: bit n' of row n where node n sees node n'. Ancestors by doubling:
-            // after k steps a node has those up to 2^k above it.
-            __syncthreads();
-            const int n = tid;
-            int parent = -2;
-            if (n < int(a.nodes)) {
-                parent = is_node(above_me, n) ? int(above_me) : -2;
-                above[n] = parent;
-#pragma unroll
-                for (int w = 0; w < kWords; ++w) sees[n][w] = parent != -2 && n / 64 == w ? 1ull << (n & 63) : 0ull;
-            }
-            for (uint32_t reach = 1; reach < a.nodes; reach *= 2) {
-                __syncthreads();
-                uint64_t more[kWords] = {};
-                int next = parent;
-                if (parent >= 0) {
-#pragma unroll
-                    for (int w = 0; w < kWords; ++w) more[w] = sees[parent][w];
-                    next = above[parent];
-                }
-                __syncthreads();
-                if (parent >= 0) {
-#pragma unroll
-                    for (int w = 0; w < kWords; ++w) sees[n][w] |= more[w];
-                    above[n] = parent = next;
-                }
-            }
-            __syncthreads();
+            see_ancestors(a.nodes, above_me, sees, above);
             for (; x < end; ++x) {
                 const uint32_t tile = x - cached;
                 const int first = 16 * wave + 4 * g;
                 score();
                 load_k(x + 1);
-                uint64_t seen[QT];
 #pragma unroll
                 for (int qt = 0; qt < QT; ++qt) {
                     const uint32_t node = (rb * RB + row0 + 16 * qt + m) % a.queries;  // queries == nodes
-                    seen[qt] = sees[node][tile];
+                    const uint64_t seen = sees[node][tile];
 #pragma unroll
                     for (int i = 0; i < 4; ++i)
-                        if (!(seen[qt] >> (first + i) & 1)) p[qt][i] = -INFINITY;
+                        if (!(seen >> (first + i) & 1)) p[qt][i] = -INFINITY;
                 }
                 weigh();
-                bool odd = false;  // a drafted value that is not finite: not every row may see it
+                bool odd = false;
 #pragma unroll
                 for (int j = 0; j < NJ; ++j)
 #pragma unroll
                     for (int i = 0; i < 4; ++i)
 #pragma unroll
+                        for (int e = 0; e < 4; ++e) odd |= !finite(vf[j][i][e]);
+                if (!__any(odd)) {
+                    add();
+                } else {
+                    // A drafted value that is not finite, which not every row may see: the
+                    // finite ones, then the weight that each row gives to each special one.
+#pragma unroll
+                    for (int j = 0; j < NJ; ++j)
+#pragma unroll
                         for (int e = 0; e < 4; ++e)
-                            if (!(fabsf(vf[j][i][e]) < INFINITY)) {
-                                vf[j][i][e] = 0.f;
-                                odd = true;
-                            }
-                add();
-                load_v(x + 1);
-                if (!__any(odd)) continue;
-                for (int key = 16 * wave; key < 16 * wave + 16 && tile * kTile + key < a.nodes; ++key) {
-                    const float *row = vd + size_t(tile * kTile + key) * a.k_row;
 #pragma unroll
-                    for (int qt = 0; qt < QT; ++qt) {
-                        const float mine = key & 2 ? (key & 1 ? p[qt].w : p[qt].z) : (key & 1 ? p[qt].y : p[qt].x);
-                        const float weight = __shfl(mine, 16 * ((key & 15) >> 2) + m);
-                        if (!(seen[qt] >> key & 1)) continue;
+                            for (int qt = 0; qt < QT; ++qt)
 #pragma unroll
-                        for (int j = 0; j < NJ; ++j)
+                                for (int k = -1; k < 3; ++k) {
+                                    __builtin_amdgcn_sched_barrier(0);  // one at a time: a rare path takes no registers
+                                    f32x4 sums = k < 0 ? acc[qt][j][e] : f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-                            for (int i = 0; i < 4; ++i)
+                                    for (int i = 0; i < 4; ++i) {
+                                        const float v = vf[j][i][e], u = k >= 0 ? is(k, v) : finite(v) ? v : 0.f;
+                                        sums = __builtin_amdgcn_mfma_f32_16x16x4f32(u, p[qt][i], sums, 0, 0, 0);
+                                    }
+                                    if (k < 0)
+                                        acc[qt][j][e] = sums;
+                                    else
 #pragma unroll
-                                for (int e = 0; e < 4; ++e) {
-                                    const int d = 64 * j + 16 * g + 4 * i + e;
-                                    const float v = d < a.dim ? row[d] : 0.f;
-                                    if (!(fabsf(v) < INFINITY)) acc[qt][j][e][i] += weight * v;
+                                        for (int i = 0; i < 4; ++i)
+                                            if (sums[i] > 0.f) acc[qt][j][e][i] += special(k);
                                 }
-                    }
                 }
+                load_v(x + 1);
             }
         }
 
@@ -430,30 +308,7 @@ attention_ragged(RaggedArgs a) {
                         f32x4{acc[qt][j][0][i], acc[qt][j][1][i], acc[qt][j][2][i], acc[qt][j][3][i]};
         }
         __syncthreads();
-        const uint32_t rows = min(uint32_t(RB), a.group * a.queries - rb * RB);
-        const size_t slot = 2 * size_t(run) + (begin == 0);
-        for (uint32_t at = tid; at < rows * (DP / 4); at += S::kThreads) {
-            const uint32_t row = at / (DP / 4), d = at % (DP / 4) * 4;
-            float most = -INFINITY;
-#pragma unroll
-            for (int w = 0; w < kWaves; ++w) most = fmaxf(most, ml[w][row].x);
-            const float from = most == -INFINITY ? 0.f : most;
-            f32x4 o = {0.f, 0.f, 0.f, 0.f};
-            float l = 0.f;
-#pragma unroll
-            for (int w = 0; w < kWaves; ++w) {
-                const float weight = __builtin_amdgcn_exp2f(ml[w][row].x - from);
-                l = fmaf(weight, ml[w][row].y, l);
-                o += weight * *reinterpret_cast<const f32x4 *>(&part[w][row][d]);
-            }
-            if (whole) {
-                store_row<VEC>(a, b, kv, rb * RB + row, d, o, l);
-            } else {
-                *reinterpret_cast<f32x4 *>(a.partial + (slot * RB + row) * DP + d) = o;
-                if (d == 0)
-                    reinterpret_cast<float2 *>(a.partial + 2 * size_t(a.runs) * RB * DP)[slot * RB + row] = float2{most, l};
-            }
-        }
+        finish<DP, RB, S::kThreads, VEC>(a, run, b, kv, rb, whole, begin == 0, part, ml);
         t += end - begin;
         if (t >= (before + tiles) * units) {
             before += tiles;
@@ -466,7 +321,7 @@ attention_ragged(RaggedArgs a) {
 // zeros of sequences without keys. Block y has row y of the units of block x: of
 // unit x itself where there are at most `runs` units, else of the one that the cut
 // before run x is the first of.
-template <int DP, int RB, bool VEC>
+template <int DP, int RB, int TILE, bool VEC>
 __global__ __launch_bounds__(kThreads) void attention_ragged_join(RaggedArgs a) {
     constexpr int LANES = DP / 4, PARTS = kThreads / LANES;
     __shared__ __attribute__((aligned(16))) f32x4 sums[PARTS][LANES];
@@ -474,7 +329,7 @@ __global__ __launch_bounds__(kThreads) void attention_ragged_join(RaggedArgs a) 
     const int tid = threadIdx.x, lane = tid % LANES, p = tid / LANES;
     const uint32_t units = a.kv_heads * a.row_blocks, row = blockIdx.y, d = 4 * lane;
     const bool by_unit = a.batch * units <= a.runs;
-    const Spread spread(a);
+    const Spread<TILE> spread(a);
     const uint32_t chunk = (spread.total * units + a.runs - 1) / a.runs;
     uint32_t b, unit, start, tiles;
     if (by_unit) {
@@ -546,42 +401,51 @@ uint32_t row_blocks(const RaggedShape &s) {
     return (rows_of(s) + rb - 1) / rb;
 }
 
+// More than 16 rows of whole float4s go to the kernel on bf16 parts; the runtime's
+// buffers are all aligned.
+bool on_parts(const RaggedShape &s) { return rows_of(s) > 16 && s.dim % 4 == 0; }
+
 uint64_t ragged_tiles(const RaggedShape &s) {
-    const uint64_t tiles = (uint64_t(s.keys) + kTile - 1) / kTile + (s.nodes + kTile - 1) / kTile;
+    const uint32_t tile = on_parts(s) ? kPartsTile : kTile;
+    const uint64_t tiles = (uint64_t(s.keys) + tile - 1) / tile + (s.nodes + tile - 1) / tile;
     return uint64_t(s.batch) * s.kv_heads * row_blocks(s) * tiles;
 }
 
-// Runs of a launch: as many blocks as the chip holds at once (two of four waves or
-// one of eight a CU), or one per tile where there can be no more tiles.
+// Runs of a launch: as many blocks as the chip holds at once (one a CU of 64 rows or
+// on parts, else two), or one per tile where there can be no more tiles.
 uint32_t runs_of(const RaggedShape &s) {
     const uint64_t tiles = ragged_tiles(s);
-    const uint32_t most = block_rows(rows_of(s)) == 64 ? kCus : 2 * kCus;
+    const uint32_t most = block_rows(rows_of(s)) == 64 || on_parts(s) ? kCus : 2 * kCus;
     return tiles >= most ? most : uint32_t((tiles + 7) / 8 * 8);
 }
 
-template <int DP, int QT, int RG>
-hipError_t launch(hipStream_t stream, const RaggedArgs &a, bool vec) {
-    using S = Shape<DP, QT, RG>;
+template <int DP, int RB, int TILE, bool VEC>
+void launch_join(hipStream_t stream, const RaggedArgs &a) {
     const uint32_t rows = a.group * a.queries, units = a.batch * a.kv_heads * a.row_blocks;
-    const dim3 grid(a.runs), block(S::kThreads);
-    const dim3 join(units < a.runs ? units : a.runs, rows < S::kRows ? rows : S::kRows);
-    if (vec) {
-        hipLaunchKernelGGL((attention_ragged<DP, QT, RG, true>), grid, block, 0, stream, a);
-        hipLaunchKernelGGL((attention_ragged_join<DP, S::kRows, true>), join, dim3(kThreads), 0, stream, a);
-    } else {
-        hipLaunchKernelGGL((attention_ragged<DP, QT, RG, false>), grid, block, 0, stream, a);
-        hipLaunchKernelGGL((attention_ragged_join<DP, S::kRows, false>), join, dim3(kThreads), 0, stream, a);
-    }
-    return hipGetLastError();
+    const dim3 grid(units < a.runs ? units : a.runs, rows < RB ? rows : RB);
+    hipLaunchKernelGGL((attention_ragged_join<DP, RB, TILE, VEC>), grid, dim3(kThreads), 0, stream, a);
 }
 
+template <int DP, int QT, int RG, bool VEC>
+void launch(hipStream_t stream, const RaggedArgs &a) {
+    using S = Shape<DP, QT, RG>;
+    hipLaunchKernelGGL((attention_ragged<DP, QT, RG, VEC>), dim3(a.runs), dim3(S::kThreads), 0, stream, a);
+    launch_join<DP, S::kRows, kTile, VEC>(stream, a);
+}
+
+// `parts`: on bf16 parts; whole rows of float4s otherwise only up to 16 rows.
 template <int DP>
-hipError_t launch_rows(hipStream_t stream, const RaggedArgs &a, bool vec) {
-    switch (block_rows(a.group * a.queries)) {
-        case 16: return launch<DP, 1, 1>(stream, a, vec);
-        case 32: return launch<DP, 2, 1>(stream, a, vec);
-        default: return launch<DP, 2, 2>(stream, a, vec);
+hipError_t launch_rows(hipStream_t stream, const RaggedArgs &a, bool parts) {
+    const uint32_t rb = block_rows(a.group * a.queries);
+    if (parts) {
+        launch_ragged_parts(stream, a, rb);
+        rb == 32 ? launch_join<DP, 32, kPartsTile, true>(stream, a) : launch_join<DP, 64, kPartsTile, true>(stream, a);
+    } else if (rb == 16) {
+        a.dim % 4 == 0 ? launch<DP, 1, 1, true>(stream, a) : launch<DP, 1, 1, false>(stream, a);
+    } else {
+        rb == 32 ? launch<DP, 2, 1, false>(stream, a) : launch<DP, 2, 2, false>(stream, a);
     }
+    return hipGetLastError();
 }
 
 }  // namespace
@@ -591,10 +455,12 @@ LaunchShape attention_ragged_shape(const RaggedShape &s) {
     if (ragged_tiles(s) > 0x7fffffffull) return {nullptr, {0, 0, 0}, {0, 0, 0}, 0};
     const bool wide = s.dim > 64;
     const uint32_t rb = block_rows(rows_of(s)), pitch = (wide ? 128 : 64) + 4;
-    static const char *const names[2][3] = {
-        {"attention_ragged_d64_r16", "attention_ragged_d64_r32", "attention_ragged_d64_r64"},
-        {"attention_ragged_d128_r16", "attention_ragged_d128_r32", "attention_ragged_d128_r64"}};
-    return {names[wide][rb / 32], {runs_of(s), 1, 1}, {uint32_t(rb == 64 ? 2 * kThreads : kThreads), 1, 1},
+    static const char *const names[2][2][3] = {
+        {{"attention_ragged_d64_r16", "attention_ragged_d64_r32", "attention_ragged_d64_r64"},
+         {"attention_ragged_d128_r16", "attention_ragged_d128_r32", "attention_ragged_d128_r64"}},
+        {{nullptr, "attention_ragged_parts_d64_r32", "attention_ragged_parts_d64_r64"},
+         {nullptr, "attention_ragged_parts_d128_r32", "attention_ragged_parts_d128_r64"}}};
+    return {names[on_parts(s)][wide][rb / 32], {runs_of(s), 1, 1}, {uint32_t(rb == 64 && !on_parts(s) ? 2 * kThreads : kThreads), 1, 1},
             uint32_t(kWaves * rb * (pitch * sizeof(float) + sizeof(float2)) +
                      kMaxTreeNodes * (kWords * sizeof(uint64_t) + sizeof(int)))};
 }
@@ -627,8 +493,8 @@ hipError_t attention_ragged_f32(hipStream_t stream, const RaggedShape &s, const 
     uintptr_t bits = 0;
     for (const float *y : {x.q, x.k, x.v, x.k_draft, x.v_draft, const_cast<const float *>(x.out)})
         bits |= reinterpret_cast<uintptr_t>(y);
-    const bool vec = s.dim % 4 == 0 && (bits & 15u) == 0;
-    return s.dim <= 64 ? launch_rows<64>(stream, a, vec) : launch_rows<128>(stream, a, vec);
+    if (s.dim % 4 == 0 && bits & 15u) return hipErrorInvalidValue;  // the runtime's regions are aligned
+    return s.dim <= 64 ? launch_rows<64>(stream, a, on_parts(s)) : launch_rows<128>(stream, a, on_parts(s));
 }
 
 }  // namespace hipk

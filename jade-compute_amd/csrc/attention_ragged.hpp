@@ -22,5 +22,10 @@ struct RaggedArgs {
     float qscale;  // scale * log2(e)
 };
 
+// The kernel on bf16 parts (attention_ragged_parts.hip), with 32 or 64 rows a block and
+// tiles of kPartsTile keys. Needs dim % 4 == 0 and at most 128, 16-byte aligned tensors.
+constexpr uint32_t kPartsTile = 128;
+void launch_ragged_parts(hipStream_t stream, const RaggedArgs &args, uint32_t block_rows);
+
 }  // namespace hipk
 }  // namespace jade

@@ -1,0 +1,485 @@
+// Ragged attention (attention_ragged.hip) of more than 16 rows, of 16-byte rows, on
+// bf16 parts: every FP32 operand is held exactly as three bf16 parts and multiplied
+// as six products of parts with FP32 sums (split_bf16.hpp), on 32x32x16 MFMAs in the
+// transposed form of attention_flash.hip. A wave has all 32 or 64 rows of its block and
+// 32 of a tile's 128 keys. Both products take their dims and keys in the order in which
+// a lane's 16-byte loads of K and V leave them, so K and V go from memory to registers
+// and are split there, by the one wave that multiplies them; LDS has only the parts of
+// Q, which the four waves share.
+//
+// One wave a SIMD, so it overlaps its own work: an MFMA every 32 cycles, and between
+// two of them two of the twelve pieces in which the next eight values of K or V are
+// split; a chunk is loaded again, for the next tile, as soon as it is split. For 64
+// rows and 32 keys of 128 dims that is 192 MFMAs (6144 cycles of a SIMD; FP32 MFMAs
+// take 16384) against some 840 other instructions.
+//
+// V is scaled up before it is split and the outputs are scaled back, Q is scaled up and
+// K down, so every finite V and Q is carried exactly. What the parts do not carry
+// (sums that are not finite, queries past 2^64) a wave notices and does its part of the
+// run again with FP32 MFMAs, as attention_flash.hip does.
+#include "kernels.hpp"
+#include "ragged_device.hpp"
+#include "split_bf16.hpp"
+
+namespace jade {
+namespace hipk {
+namespace {
+
+using namespace ragged;
+using namespace split;
+
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+
+constexpr int kTile = 128;  // keys per tile, 32 for each wave by keys
+constexpr float kMostQ = 0x1p64f * kScaleQ;
+
+__device__ inline float halves_max(float x) {
+    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+__device__ inline float halves_sum(float x) {
+    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+
+// Piece n < 12 of splitting eight values: pairs 0 and 1 in turn, a part at a time, then
+// pairs 2 and 3 (a pair's next part waits for its rest, so two pairs take turns);
+// pair_of(n) says whose. `rest` goes from piece to piece.
+constexpr int pair_of(int n) { return n / 6 * 2 + n % 2; }
+__device__ inline void split_piece(int n, f32x2 x, f32x2 (&rest)[2], uint32_t (&out)[kParts][4]) {
+    const int w = n % 6 / 2;
+    const f32x2 from = w == 0 ? x : rest[n % 2];
+    out[w][pair_of(n)] = pack(from.x, from.y);
+    if (w < 2) rest[n % 2] = rest_of(from, out[w][pair_of(n)]);
+}
+__device__ inline bf16x8 part_of(const uint32_t (&p)[kParts][4], int w) {
+    return __builtin_bit_cast(bf16x8, u32x4{p[w][0], p[w][1], p[w][2], p[w][3]});
+}
+
+template <int DP, int QG>
+struct Shape {
+    static constexpr int kRows = 32 * QG, kBlock = 64 * kWaves, kPitch = DP + 4;
+    static constexpr int kSteps = DP / 16;  // score steps
+    static constexpr int kOut = DP / 32;    // output blocks of 32 dims: dims kOut * r + e
+    // Where K and V of a tile are loaded: each chunk as soon as the last tile's is split,
+    // or, where two row groups leave no registers for all of both, V before the scores
+    // and K before and amid the outputs.
+    static constexpr bool kEarly = QG == 1;
+    static_assert(QG * kSteps * kParts * 1024 <= kWaves * kRows * kPitch * 4, "Q's parts fit the sums' space");
+};
+
+// QG: groups of 32 rows, all of them every wave's.
+template <int DP, int QG>
+__global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(1, 1))) void
+attention_ragged_parts(RaggedArgs a) {
+    using S = Shape<DP, QG>;
+    constexpr int KS = S::kSteps, NB = S::kOut, RB = S::kRows;
+    typedef float vec __attribute__((ext_vector_type(NB)));
+    __shared__ __attribute__((aligned(16))) float part[kWaves][RB][S::kPitch];
+    __shared__ float2 ml[kWaves][RB];
+    __shared__ uint64_t sees[kMaxTreeNodes][kWords];
+    __shared__ int above[kMaxTreeNodes];
+    __shared__ float2 seen_so_far[kWaves][QG][64];  // running maximum and sum of a lane's rows
+    __shared__ int far;  // a query that the parts do not carry
+    char *const qs = reinterpret_cast<char *>(&part[0][0][0]);  // Q's parts until the sums are joined
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int c = lane & 31, h = lane >> 5;
+    const uint32_t units = a.kv_heads * a.row_blocks;
+    const Spread<kTile> spread(a);
+    const uint32_t total = spread.total * units, chunk = (total + a.runs - 1) / a.runs;
+    const uint32_t run = run_of(blockIdx.x, a.runs);
+    if (uint64_t(run) * chunk >= total) return;
+    uint32_t t = run * chunk;
+    const uint32_t t_stop = min(total, t + chunk);
+    uint32_t b, before;
+    spread.find(t / units, b, before);
+
+    const uint32_t row_bytes = a.k_row * 4u;
+    while (t < t_stop) {
+        const uint32_t len = uniform(whole_below(a.lengths[b], a.keys));
+        const uint32_t cached = (len + kTile - 1) / kTile, tiles = cached + spread.draft_tiles;
+        if (!tiles) {
+            ++b;
+            continue;
+        }
+        const uint32_t in = t - before * units, unit = in / tiles, begin = in - unit * tiles;
+        const uint32_t kv = unit / a.row_blocks, rb = unit - kv * a.row_blocks;
+        const uint32_t end = min(tiles, begin + (t_stop - t));
+        const bool whole = begin == 0 && end == tiles;
+        float above_me = 0.f;
+        if (end > cached && tid < int(a.nodes)) above_me = a.parents[size_t(b) * a.nodes + tid];
+
+        const float *kb = a.k + size_t(b) * a.k_batch + size_t(kv) * a.k_head;
+        const float *vb = a.v + size_t(b) * a.k_batch + size_t(kv) * a.k_head;
+        const float *kd = a.kd + size_t(b) * a.d_batch + size_t(kv) * a.d_head;
+        const float *vd = a.vd + size_t(b) * a.d_batch + size_t(kv) * a.d_head;
+        // Tile x of a tensor: its own descriptor (no offset passes 2^31, however long
+        // the cache), which ends with its last key's row; past `end` it holds nothing.
+        auto tile_of = [&](const float *cache, const float *draft, uint32_t x) {
+            const bool drafted = x >= cached;
+            const uint32_t at = drafted ? x - cached : x, left = (drafted ? a.nodes : len) - at * kTile;
+            const float *from = (drafted ? draft : cache) + size_t(at) * kTile * a.k_row;
+            const uint32_t bytes = x < end ? (min(left, uint32_t(kTile)) - 1) * row_bytes + uint32_t(a.dim) * 4u : 0u;
+            return __builtin_amdgcn_make_buffer_rsrc(const_cast<float *>(from), 0, int(bytes), int(kRawBuffer));
+        };
+        f32x4 kf[KS][2];
+        vec vf[2][8];
+        // Offsets are made from the lane's number for each tile: kept, they would be spilled.
+        struct Offsets {
+            uint32_t k, v;
+        };
+        auto offsets = [&]() __attribute__((always_inline)) {
+            uint32_t l = __builtin_amdgcn_mbcnt_hi(~0u, __builtin_amdgcn_mbcnt_lo(~0u, 0u));
+            asm volatile("" : "+v"(l));
+            const uint32_t half = l >> 5, row = l & 31;
+            return Offsets{(32 * wave + row) * row_bytes + 16 * half,
+                           int(NB * row) < a.dim ? (32 * wave + 4 * half) * row_bytes + 4 * NB * row : kDeadOffset};
+        };
+        // Dims of score step s, load x: 8 y + 4 h + 0 .. 3, y = 2 s + x.
+        auto load_k = [&](__amdgpu_buffer_rsrc_t from, uint32_t koff, int s) __attribute__((always_inline)) {
+#pragma unroll
+            for (int x = 0; x < 2; ++x) {
+                const int y = 2 * s + x;
+                const uint32_t at = 8 * y + int(koff >> 2 & 4) < a.dim ? koff + 32u * y : kDeadOffset;
+                kf[s][x] = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(from, int(at), 0, 0));
+            }
+        };
+        // Dims NB c .. + NB - 1 of keys 16 s + 4 h + (u & 3) + 8 (u >> 2).
+        auto load_v = [&](__amdgpu_buffer_rsrc_t from, uint32_t voff, int s, int u) __attribute__((always_inline)) {
+            const uint32_t at = voff + uint32_t(16 * s + (u & 3) + 8 * (u >> 2)) * row_bytes;
+            if constexpr (NB == 4)
+                vf[s][u] = __builtin_bit_cast(vec, __builtin_amdgcn_raw_buffer_load_b128(from, int(at), 0, 0));
+            else
+                vf[s][u] = __builtin_bit_cast(vec, __builtin_amdgcn_raw_buffer_load_b64(from, int(at), 0, 0));
+        };
+        // Row r of the block, dims d .. d + 3, in log2 units.
+        auto load_q = [&](int r, int d) {
+            const uint32_t at = rb * RB + r, head = at / a.queries, query = at - head * a.queries;
+            const float *row = a.q + size_t(b) * a.q_batch + (size_t(kv) * a.group + head) * a.q_head + size_t(query) * a.q_row;
+            f32x4 x = {0.f, 0.f, 0.f, 0.f};
+            if (head < a.group && d < a.dim) x = *reinterpret_cast<const f32x4 *>(row + d);
+            return x * a.qscale;
+        };
+        // The first tile; from here on a chunk is loaded again once it is split.
+        {
+            const auto kfrom = tile_of(kb, kd, begin), vfrom = tile_of(vb, vd, begin);
+            const Offsets at = offsets();
+#pragma unroll
+            for (int s = 0; s < KS; ++s) load_k(kfrom, at.k, s);
+            if (S::kEarly)
+#pragma unroll
+                for (int u = 0; u < 16; ++u) load_v(vfrom, at.v, u >> 3, u & 7);
+        }
+        // Q's parts: for group r, step s, part w and lane, 16 bytes at ((r KS + s) kParts + w) 64 + lane.
+        __syncthreads();  // the last unit's sums are read
+        if (tid == 0) far = 0;
+        __syncthreads();
+        for (int i = tid; i < QG * KS * 64; i += S::kBlock) {
+            const int l = i & 63, s = (i >> 6) % KS, r = (i >> 6) / KS;
+            uint32_t p[kParts][4];
+            f32x2 rest[2];
+            bool past = false;
+#pragma unroll
+            for (int y = 0; y < 2; ++y) {
+                const f32x4 q = load_q(32 * r + (l & 31), 16 * s + 8 * y + 4 * (l >> 5)) * kScaleQ;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) past |= fabsf(q[e]) > kMostQ;
+#pragma unroll
+                for (int n = 0; n < 6; ++n) split_piece(6 * y + n, n % 2 ? f32x2{q.z, q.w} : f32x2{q.x, q.y}, rest, p);
+            }
+            if (past) far = 1;
+#pragma unroll
+            for (int w = 0; w < kParts; ++w)
+                *reinterpret_cast<bf16x8 *>(qs + (((r * KS + s) * kParts + w) * 64 + l) * 16) = part_of(p, w);
+        }
+        if (end > cached)
+            see_ancestors(a.nodes, above_me, sees, above);
+        else
+            __syncthreads();
+
+        f32x16 acc[QG][NB], st[QG];
+        float top[QG], sum[QG];  // of the tile at hand; between tiles in LDS, where nothing spills them
+        float2 (&state)[QG][64] = seen_so_far[wave];
+        auto clear = [&]() __attribute__((always_inline)) {
+#pragma unroll
+            for (int r = 0; r < QG; ++r) {
+                state[r][lane] = float2{-INFINITY, 0.f};
+#pragma unroll
+                for (int e = 0; e < NB; ++e) acc[r][e] = f32x16{};
+            }
+        };
+        clear();
+        // Keys that this wave's rows do not see, of its 32 in tile x.
+        auto mask = [&](uint32_t x) __attribute__((always_inline)) {
+            if (x >= cached) {
+                const uint32_t key = (x - cached) * kTile + 32 * wave;
+#pragma unroll
+                for (int r = 0; r < QG; ++r) {
+                    const uint32_t node = (rb * RB + 32 * r + c) % a.queries;  // queries == nodes
+                    const uint32_t seen = uint32_t(sees[node][key / 64] >> (key & 63)) >> (4 * h);
+#pragma unroll
+                    for (int v = 0; v < 16; ++v)
+                        if (!(seen >> (8 * (v >> 2) + (v & 3)) & 1)) st[r][v] = -INFINITY;
+                }
+            } else if ((x + 1) * kTile > len) {
+                const int first = int(x) * kTile + 32 * wave + 4 * h;
+#pragma unroll
+                for (int r = 0; r < QG; ++r)
+#pragma unroll
+                    for (int v = 0; v < 16; ++v)
+                        if (first + 8 * (v >> 2) + (v & 3) >= int(len)) st[r][v] = -INFINITY;
+            }
+        };
+        // The running maximum of the rows past this tile's scores; what was summed so far
+        // is scaled to it.
+        auto raise = [&]() __attribute__((always_inline)) {
+#pragma unroll
+            for (int r = 0; r < QG; ++r) {
+                top[r] = state[r][lane].x;
+                sum[r] = state[r][lane].y;
+                float most = st[r][0];
+#pragma unroll
+                for (int v = 1; v < 16; ++v) most = fmaxf(most, st[r][v]);
+                if (__any(most > top[r] + kLazyMax)) {
+                    const float reached = fmaxf(top[r], halves_max(most));
+                    const float keep = reached == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(top[r] - reached);
+                    top[r] = reached;
+                    sum[r] *= keep;
+#pragma unroll
+                    for (int e = 0; e < NB; ++e) acc[r][e] *= keep;
+                }
+            }
+        };
+        auto keep_state = [&]() __attribute__((always_inline)) {
+#pragma unroll
+            for (int r = 0; r < QG; ++r) state[r][lane] = float2{top[r], sum[r]};
+        };
+        // Score v of row group r to its weight.
+        auto weigh = [&](int r, int v) __attribute__((always_inline)) {
+            st[r][v] = __builtin_amdgcn_exp2f(st[r][v] - (top[r] == -INFINITY ? 0.f : top[r]));
+            sum[r] += st[r][v];
+        };
+
+        // Two buffers of parts each for K steps, Q steps and V octets (s, e): one is
+        // multiplied while the next is made.
+        uint32_t kp[2][kParts][4], vp[2][kParts][4];
+        bf16x8 q0[2][QG], q12[QG][2];  // a step's last product takes Q's part 0, so that one twice
+        f32x2 rest[2];
+        auto read_q = [&](int s, int w) __attribute__((always_inline)) {
+#pragma unroll
+            for (int r = 0; r < QG; ++r)
+                (w ? q12[r][w - 1] : q0[s & 1][r]) =
+                    *reinterpret_cast<const bf16x8 *>(qs + (((r * KS + s) * kParts + w) * 64 + lane) * 16);
+        };
+        auto split_k = [&](int s, int n) __attribute__((always_inline)) {
+            const f32x4 k = kf[s][n / 6];
+            split_piece(n, (n % 2 ? f32x2{k.z, k.w} : f32x2{k.x, k.y}) * kScaleK, rest, kp[s & 1]);
+        };
+        auto split_v = [&](int o, int n) __attribute__((always_inline)) {  // octet o: keys o / NB, dim o % NB
+            const int u = 2 * pair_of(n);
+            split_piece(n, f32x2{vf[o / NB][u][o % NB], vf[o / NB][u + 1][o % NB]} * kScaleV, rest, vp[o & 1]);
+        };
+#pragma unroll
+        for (int n = 0; n < 12; ++n) split_k(0, n);
+#pragma unroll
+        for (int w = 0; w < kParts; ++w) read_q(0, w);
+
+        for (uint32_t x = begin; x < end; ++x) {
+            const auto kfrom = tile_of(kb, kd, x + 1), vfrom = tile_of(vb, vd, S::kEarly ? x + 1 : x);
+            const Offsets at = offsets();
+            if (S::kEarly)
+                load_k(kfrom, at.k, 0);
+            else
+#pragma unroll
+                for (int u = 0; u < 8; ++u) load_v(vfrom, at.v, 0, u);
+#pragma unroll
+            for (int r = 0; r < QG; ++r) st[r] = f32x16{};
+            // Scores; beside step s the parts of K's and Q's step s + 1, or V's first octet.
+            each<6 * KS * QG>([&](auto nc) __attribute__((always_inline)) {
+                constexpr int i = decltype(nc)::value % (6 * QG), s = decltype(nc)::value / (6 * QG), p = i / QG, r = i % QG;
+                __builtin_amdgcn_sched_barrier(0);
+                st[r] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(
+                    part_of(kp[s & 1], kPartA[p]), kPartB[p] ? q12[r][kPartB[p] - 1] : q0[s & 1][r], st[r], 0, 0, 0);
+                __builtin_amdgcn_sched_barrier(0);
+                each<2 / QG>([&](auto ec) __attribute__((always_inline)) {
+                    constexpr int piece = 2 * i / QG + decltype(ec)::value;
+                    if constexpr (s + 1 < KS)
+                        split_k(s + 1, piece);
+                    else
+                        split_v(0, piece);
+                });
+                if constexpr (s + 1 < KS && r == QG - 1) {
+                    // Each part once its last product is issued (B's parts go 0 2 1 0 1 0).
+                    if constexpr (p == 0) read_q(s + 1, 0);
+                    if constexpr (p == 1) read_q(s + 1, 2);
+                    if constexpr (p == 4) read_q(s + 1, 1);
+                    if constexpr (S::kEarly && p == 5) load_k(kfrom, at.k, s + 1);
+                    if constexpr (!S::kEarly && p == 5)
+#pragma unroll
+                        for (int u = s * 8 / (KS - 1); u < (s + 1) * 8 / (KS - 1); ++u) load_v(vfrom, at.v, 1, u);
+                }
+            });
+            __builtin_amdgcn_sched_barrier(0);
+            mask(x);
+            raise();
+            // Weights and their parts, of keys 0 .. 15 here, of 16 .. 31 beside the first outputs.
+            uint32_t pp[QG][2][kParts][4];
+            f32x2 prest[2];
+            auto split_p = [&](int r, int s, int n) __attribute__((always_inline)) {
+                const int v = 8 * s + 2 * pair_of(n);
+                if (n % 6 < 2) {
+                    weigh(r, v);
+                    weigh(r, v + 1);
+                }
+                split_piece(n, f32x2{st[r][v], st[r][v + 1]}, prest, pp[r][s]);
+            };
+#pragma unroll
+            for (int r = 0; r < QG; ++r)
+#pragma unroll
+                for (int n = 0; n < 12; ++n) split_p(r, 0, n);
+            if (!S::kEarly)
+#pragma unroll
+                for (int k = 0; k < KS / 2; ++k) load_k(kfrom, at.k, k);
+            // Outputs; beside octet o the parts of octet o + 1, or of the next tile's first K step.
+            each<12 * NB * QG>([&](auto nc) __attribute__((always_inline)) {
+                constexpr int n = decltype(nc)::value, i = n % (6 * QG), o = n / (6 * QG), p = i / QG, r = i % QG;
+                constexpr int s = o / NB, e = o % NB;
+                __builtin_amdgcn_sched_barrier(0);
+                acc[r][e] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(part_of(vp[o & 1], kPartA[p]),
+                                                                    part_of(pp[r][s], kPartB[p]), acc[r][e], 0, 0, 0);
+                __builtin_amdgcn_sched_barrier(0);
+                constexpr int lo = kFirstEvent<n, 12 * QG, 6 * NB * QG>, hi = kFirstEvent<n + 1, 12 * QG, 6 * NB * QG>;
+                if constexpr (o < NB)
+                    each<hi - lo>([&](auto ec) __attribute__((always_inline)) {
+                        constexpr int j = lo + decltype(ec)::value;
+                        split_p(j / 12, 1, j % 12);
+                    });
+                if constexpr (n == 6 * NB * QG) keep_state();
+                each<2 / QG>([&](auto ec) __attribute__((always_inline)) {
+                    constexpr int piece = 2 * i / QG + decltype(ec)::value;
+                    if constexpr (o + 1 < 2 * NB)
+                        split_v(o + 1, piece);
+                    else
+                        split_k(0, piece);
+                });
+                if constexpr (r == QG - 1) {
+                    // The last octet of these keys is split: their registers again.
+                    if constexpr (o + 1 < 2 * NB && (o + 1) % NB == NB - 1 && p == 5) {
+                        constexpr int half = (o + 1) / NB;
+                        if constexpr (S::kEarly)
+#pragma unroll
+                            for (int u = 0; u < 8; ++u) load_v(vfrom, at.v, half, u);
+                        else if constexpr (half == 0)
+#pragma unroll
+                            for (int k = KS / 2; k < KS; ++k) load_k(kfrom, at.k, k);
+                    }
+                    if constexpr (o + 1 == 2 * NB && p < kParts) read_q(0, p);
+                }
+            });
+            __builtin_amdgcn_sched_barrier(0);
+        }
+
+        // What the parts do not carry: see the file's head.
+        float unscale = kUnscaleV, odd = 0.f;
+#pragma unroll
+        for (int r = 0; r < QG; ++r) {
+            odd += state[r][lane].y * 0.f;
+#pragma unroll
+            for (int e = 0; e < NB; ++e)
+#pragma unroll
+                for (int v = 0; v < 16; ++v) odd += acc[r][e][v] * 0.f;
+        }
+        if (far || __any(odd != 0.f)) {
+            unscale = 1.f;
+            clear();
+            for (uint32_t x = begin; x < end; ++x) {
+                const bool drafted = x >= cached;
+                const uint32_t tile = drafted ? x - cached : x, keys = drafted ? a.nodes : len;
+                const uint32_t key0 = tile * kTile + 32 * wave;
+                const float *krow = (drafted ? kd : kb) + size_t(key0 + c) * a.k_row;
+                const float *vrow = (drafted ? vd : vb) + size_t(key0) * a.k_row;
+#pragma unroll
+                for (int r = 0; r < QG; ++r) {
+                    st[r] = f32x16{};
+                    for (int d0 = 0; d0 < DP; d0 += 8) {
+                        const int d = d0 + 4 * h;
+                        const f32x4 q = load_q(32 * r + c, d);
+                        f32x4 k = {0.f, 0.f, 0.f, 0.f};
+                        if (d < a.dim && key0 + c < keys) k = *reinterpret_cast<const f32x4 *>(krow + d);
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) st[r] = __builtin_amdgcn_mfma_f32_32x32x2f32(k[e], q[e], st[r], 0, 0, 0);
+                    }
+                }
+                mask(x);
+                raise();
+#pragma unroll
+                for (int r = 0; r < QG; ++r)
+#pragma unroll
+                    for (int v = 0; v < 16; ++v) weigh(r, v);
+                keep_state();
+                // Drafted values that are not finite, which not every row may see: the finite
+                // ones, then the weight that each row gives to each special one.
+                for (int e = 0; e < NB; ++e)
+                    for (int k = -1; k < (drafted ? 3 : 0); ++k)
+#pragma unroll
+                        for (int r = 0; r < QG; ++r) {
+                            f32x16 sums = {};
+#pragma unroll
+                            for (int v = 0; v < 16; ++v) {
+                                const uint32_t key = 8 * (v >> 2) + 4 * h + (v & 3);
+                                const float z = NB * c < a.dim && key0 + key < keys ? vrow[size_t(key) * a.k_row + NB * c + e] : 0.f;
+                                const float y = k >= 0 ? is(k, z) : finite(z) || !drafted ? z : 0.f;
+                                sums = __builtin_amdgcn_mfma_f32_32x32x2f32(y, st[r][v], sums, 0, 0, 0);
+                            }
+#pragma unroll
+                            for (int v = 0; v < 16; ++v) {
+                                const float more = k < 0 ? sums[v] : sums[v] > 0.f ? special(k) : 0.f;
+#pragma unroll
+                                for (int f = 0; f < NB; ++f)
+                                    if (f == e) acc[r][f][v] += more;
+                            }
+                        }
+            }
+        }
+
+        // The four waves' sums joined: dim NB i + e of row c for i = 8 (v >> 2) + 4 h + (v & 3).
+        __syncthreads();
+#pragma unroll
+        for (int r = 0; r < QG; ++r) {
+            const float2 mine = state[r][lane];
+            const float all = halves_sum(mine.y);
+            if (h == 0) ml[wave][32 * r + c] = float2{mine.x, all};
+#pragma unroll
+            for (int v = 0; v < 16; ++v) {
+                vec o;
+#pragma unroll
+                for (int e = 0; e < NB; ++e) o[e] = acc[r][e][v] * unscale;
+                *reinterpret_cast<vec *>(&part[wave][32 * r + c][NB * (8 * (v >> 2) + 4 * h + (v & 3))]) = o;
+            }
+        }
+        __syncthreads();
+        finish<DP, RB, S::kBlock, true>(a, run, b, kv, rb, whole, begin == 0, part, ml);
+        t += end - begin;
+        if (t >= (before + tiles) * units) {
+            before += tiles;
+            ++b;
+        }
+    }
+}
+
+template <int DP, int QG>
+void launch(hipStream_t stream, const RaggedArgs &a) {
+    hipLaunchKernelGGL((attention_ragged_parts<DP, QG>), dim3(a.runs), dim3(Shape<DP, QG>::kBlock), 0, stream, a);
+}
+
+}  // namespace
+
+void launch_ragged_parts(hipStream_t stream, const RaggedArgs &a, uint32_t block_rows) {
+    if (a.dim <= 64)
+        block_rows == 32 ? launch<64, 1>(stream, a) : launch<64, 2>(stream, a);
+    else
+        block_rows == 32 ? launch<128, 1>(stream, a) : launch<128, 2>(stream, a);
+}
+
+}  // namespace hipk
+}  // namespace jade

@@ -1,0 +1,192 @@
+// Device parts shared by the ragged attention kernels: where a run's tiles lie, and
+// how a row's sums become outputs or go to the workspace.
+#pragma once
+
+#include <hip/hip_runtime.h>
+
+#include <cmath>
+#include <cstdint>
+
+#include "attention_ragged.hpp"
+#include "spec.hpp"
+#include "whole.hpp"
+
+namespace jade {
+namespace hipk {
+namespace {
+namespace ragged {
+
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+
+constexpr int kThreads = 256, kWaves = 4;
+constexpr uint32_t kCus = 256;
+constexpr float kLazyMax = 8.0f;   // log2 units: the running maximum moves only past this
+constexpr uint32_t kRawBuffer = 0x00020000;    // buffer descriptor word 3: raw buffer, 32-bit data format
+constexpr uint32_t kDeadOffset = 0x80000000u;  // past every tile: reads zero
+constexpr float kLog2e = 1.44269504088896340736f;
+constexpr int kWords = int(kMaxTreeNodes) / 64;
+
+__device__ inline uint32_t uniform(uint32_t x) { return __builtin_amdgcn_readfirstlane(x); }
+__device__ inline uint32_t of_lane(uint32_t x, int lane) { return __builtin_amdgcn_readlane(x, lane); }
+
+// Sum over the lanes up to and with this one: within the rows of 16 by shifts, then
+// each row's last lane into the rows after it.
+__device__ inline uint32_t scan_add(uint32_t x) {
+#define JADE_SCAN(control, rows) x += __builtin_amdgcn_update_dpp(0, x, control, rows, 0xf, false)
+    JADE_SCAN(0x111, 0xf);
+    JADE_SCAN(0x112, 0xf);
+    JADE_SCAN(0x114, 0xf);
+    JADE_SCAN(0x118, 0xf);
+    JADE_SCAN(0x142, 0xa);  // row_bcast:15 into rows 1 and 3
+    JADE_SCAN(0x143, 0xc);  // row_bcast:31 into rows 2 and 3
+#undef JADE_SCAN
+    return x;
+}
+
+// The tiles of every sequence, of one (kv head, row block) each. A lane has the
+// sequences of its number modulo 64; those of the first 64 stay in registers.
+template <int TILE>
+struct Spread {
+    const RaggedArgs &a;
+    const uint32_t draft_tiles, own, up_to;
+    uint32_t total;
+
+    __device__ uint32_t tiles_at(uint32_t b) const {
+        return b < a.batch ? (whole_below(a.lengths[b], a.keys) + TILE - 1) / TILE + draft_tiles : 0u;
+    }
+    __device__ explicit Spread(const RaggedArgs &args)
+        : a(args), draft_tiles((a.nodes + TILE - 1) / TILE), own(tiles_at(threadIdx.x & 63)), up_to(scan_add(own)),
+          total(of_lane(up_to, 63)) {
+        for (uint32_t b0 = 64; b0 < a.batch; b0 += 64) total += of_lane(scan_add(tiles_at(b0 + (threadIdx.x & 63))), 63);
+    }
+    // The sequence that tile t < total belongs to, and the tiles before it.
+    __device__ void find(uint32_t t, uint32_t &b, uint32_t &before) const {
+        before = 0;
+        uint32_t sum = up_to, mine = own;
+        for (b = 0;; b += 64, mine = tiles_at(b + (threadIdx.x & 63)), sum = scan_add(mine)) {
+            const uint64_t past = __ballot(before + sum > t);
+            if (past) {
+                const int first = __builtin_ctzll(past);
+                b += first;
+                before += of_lane(sum - mine, first);
+                return;
+            }
+            before += of_lane(sum, 63);
+        }
+    }
+    // The tiles before sequence b.
+    __device__ uint32_t before(uint32_t b) const {
+        uint32_t sum = 0, last = up_to - own;
+        for (uint32_t b0 = 64; b0 <= b; b0 += 64) {
+            sum += b0 == 64 ? of_lane(up_to, 63) : of_lane(scan_add(tiles_at(b0 - 64 + (threadIdx.x & 63))), 63);
+            const uint32_t mine = tiles_at(b0 + (threadIdx.x & 63));
+            last = scan_add(mine) - mine;
+        }
+        return sum + of_lane(last, int(b & 63));
+    }
+};
+
+__device__ inline bool is_node(float parent, int n) {
+    return parent == -1.f || (parent >= 0.f && parent < float(n) && parent == truncf(parent));
+}
+
+// Run w of the launch: runs of one XCD are neighbours, so the row blocks of one kv
+// head, which read the same keys, meet in its L2.
+__device__ inline uint32_t run_of(uint32_t id, uint32_t runs) { return id % 8 * (runs / 8) + id / 8; }
+
+__device__ inline float across_keys_max(float x) { return fmaxf(fmaxf(x, __shfl_xor(x, 16)), fmaxf(__shfl_xor(x, 32), __shfl_xor(x, 48))); }
+__device__ inline float across_keys_sum(float x) {
+    x += __shfl_xor(x, 16);
+    return x + __shfl_xor(x, 32);
+}
+
+// Row r of (sequence b, kv head): its sums o of dims d .. d + 3 over its weights' sum.
+template <bool VEC>
+__device__ inline void store_row(const RaggedArgs &a, uint32_t b, uint32_t kv, uint32_t r, uint32_t d, f32x4 o, float l) {
+    const uint32_t head = r / a.queries, query = r - head * a.queries;
+    const bool node = !a.nodes || is_node(a.parents[size_t(b) * a.nodes + query], int(query));
+    o = node ? o * (1.0f / l) : f32x4{0.f, 0.f, 0.f, 0.f};
+    float *out = a.out + size_t(b) * a.q_batch + (size_t(kv) * a.group + head) * a.q_head + size_t(query) * a.q_row;
+    if (VEC) {
+        if (d < a.dim) *reinterpret_cast<f32x4 *>(out + d) = o;
+    } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            if (d + e < a.dim) out[d + e] = o[e];
+    }
+}
+
+// A unit's sums as its four waves by keys left them in LDS, joined: outputs where the
+// run holds the `whole` unit, else sums, maximum and weight to the run's slot (a unit's
+// first run had it last, the others first).
+template <int DP, int RB, int THREADS, bool VEC>
+__device__ inline void finish(const RaggedArgs &a, uint32_t run, uint32_t b, uint32_t kv, uint32_t rb, bool whole,
+                              bool starts, const float (&part)[kWaves][RB][DP + 4], const float2 (&ml)[kWaves][RB]) {
+    const uint32_t rows = min(uint32_t(RB), a.group * a.queries - rb * RB);
+    const size_t slot = 2 * size_t(run) + starts;
+    for (uint32_t at = threadIdx.x; at < rows * (DP / 4); at += THREADS) {
+        const uint32_t row = at / (DP / 4), d = at % (DP / 4) * 4;
+        float most = -INFINITY;
+#pragma unroll
+        for (int w = 0; w < kWaves; ++w) most = fmaxf(most, ml[w][row].x);
+        const float from = most == -INFINITY ? 0.f : most;
+        f32x4 o = {0.f, 0.f, 0.f, 0.f};
+        float l = 0.f;
+#pragma unroll
+        for (int w = 0; w < kWaves; ++w) {
+            const float weight = __builtin_amdgcn_exp2f(ml[w][row].x - from);
+            l = fmaf(weight, ml[w][row].y, l);
+            o += weight * *reinterpret_cast<const f32x4 *>(&part[w][row][d]);
+        }
+        if (whole) {
+            store_row<VEC>(a, b, kv, rb * RB + row, d, o, l);
+        } else {
+            *reinterpret_cast<f32x4 *>(a.partial + (slot * RB + row) * DP + d) = o;
+            if (d == 0)
+                reinterpret_cast<float2 *>(a.partial + 2 * size_t(a.runs) * RB * DP)[slot * RB + row] = float2{most, l};
+        }
+    }
+}
+
+// The tree of sequence b in LDS, by all threads of the block (each with the parent
+// `mine` of slot threadIdx.x): bit n' of row n where node n sees node n'. Ancestors by
+// doubling: after k steps a node has those up to 2^k above it.
+__device__ inline void see_ancestors(uint32_t nodes, float mine, uint64_t (&sees)[kMaxTreeNodes][kWords],
+                                     int (&above)[kMaxTreeNodes]) {
+    __syncthreads();
+    const int n = threadIdx.x;
+    int parent = -2;
+    if (n < int(nodes)) {
+        parent = is_node(mine, n) ? int(mine) : -2;
+        above[n] = parent;
+#pragma unroll
+        for (int w = 0; w < kWords; ++w) sees[n][w] = parent != -2 && n / 64 == w ? 1ull << (n & 63) : 0ull;
+    }
+    for (uint32_t reach = 1; reach < nodes; reach *= 2) {
+        __syncthreads();
+        uint64_t more[kWords] = {};
+        int next = parent;
+        if (parent >= 0) {
+#pragma unroll
+            for (int w = 0; w < kWords; ++w) more[w] = sees[parent][w];
+            next = above[parent];
+        }
+        __syncthreads();
+        if (parent >= 0) {
+#pragma unroll
+            for (int w = 0; w < kWords; ++w) sees[n][w] |= more[w];
+            above[n] = parent = next;
+        }
+    }
+    __syncthreads();
+}
+
+__device__ inline bool finite(float x) { return fabsf(x) < INFINITY; }
+// The three values that a weight of zero does not cancel; is(k, x): x is the k-th.
+__device__ inline float special(int k) { return k == 0 ? INFINITY : k == 1 ? -INFINITY : NAN; }
+__device__ inline float is(int k, float x) { return (k == 2 ? x != x : x == special(k)) ? 1.f : 0.f; }
+
+}  // namespace ragged
+}  // namespace
+}  // namespace hipk
+}  // namespace jade

@@ -15,6 +15,8 @@
 #include <hip/hip_runtime.h>
 
 #include <cstdint>
+#include <type_traits>
+#include <utility>
 
 namespace jade {
 namespace hipk {
@@ -75,6 +77,21 @@ constexpr float kScale = 0x1p16f, kUnscale = 0x1p-32f;
 // 2^103 may overflow. Its Q is scaled up by as much and its K down, so the
 // scores are as they are without.
 constexpr float kScaleV = 0x1p24f, kUnscaleV = 0x1p-24f, kScaleQ = 0x1p24f, kScaleK = 0x1p-24f;
+
+// f(0), f(1), ... f(N - 1) with compile-time arguments: the interleaved
+// schedules below are chosen by the compiler's front end, not by its unroller.
+template <class F, int... I>
+__device__ inline void each(std::integer_sequence<int, I...>, F &&f) {
+    (f(std::integral_constant<int, I>{}), ...);
+}
+template <int N, class F>
+__device__ inline void each(F &&f) {
+    each(std::make_integer_sequence<int, N>{}, f);
+}
+// Event E of ALL, spread evenly over the slots, belongs to slot N of SLOTS
+// when first<N> <= E < first<N + 1>.
+template <int N, int ALL, int SLOTS>
+constexpr int kFirstEvent = N >= SLOTS ? ALL : (N * ALL + SLOTS - 1) / SLOTS;
 
 }  // namespace split
 }  // namespace
