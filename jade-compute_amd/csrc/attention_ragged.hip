@@ -60,11 +60,9 @@ attention_ragged(RaggedArgs a) {
     const Spread<kTile> spread(a);
     const uint32_t total = spread.total * units, chunk = (total + a.runs - 1) / a.runs;
     const uint32_t run = run_of(blockIdx.x, a.runs);
-    if (uint64_t(run) * chunk >= total) return;
-    uint32_t t = run * chunk;
-    const uint32_t t_stop = min(total, t + chunk);
     uint32_t b, before;
-    spread.find(t / units, b, before);
+    const uint32_t t_stop = spread.start(run + 1, chunk, units, b, before);
+    uint32_t t = spread.start(run, chunk, units, b, before);
 
     const uint32_t row_bytes = a.k_row * 4u;
     uint32_t koff[KJ], voff[NJ][4];
@@ -345,12 +343,12 @@ __global__ __launch_bounds__(kThreads) void attention_ragged_join(RaggedArgs a) 
                 float *out = a.out + size_t(b) * a.q_batch;
                 for (size_t i = blockIdx.y * kThreads + tid; i < n; i += gridDim.y * kThreads) out[i] = 0.f;
             }
-        const uint64_t cut = uint64_t(blockIdx.x) * chunk;
-        if (cut == 0 || cut >= spread.total * units) return;
         uint32_t before;
-        spread.find(uint32_t(cut) / units, b, before);
+        const uint32_t cut = spread.start(blockIdx.x, chunk, units, b, before);
+        if (cut == 0 || cut == spread.total * units) return;
         tiles = uniform(spread.tiles_at(b));
-        unit = (uint32_t(cut) - before * units) / tiles;
+        if (!tiles) return;  // at a sequence's start
+        unit = (cut - before * units) / tiles;
         start = before * units + unit * tiles;
         if (start + chunk < cut || start == cut) return;  // not its first cut
     }
@@ -361,7 +359,7 @@ __global__ __launch_bounds__(kThreads) void attention_ragged_join(RaggedArgs a) 
         return;
     }
     const uint32_t first = start / chunk, last = (start + tiles - 1) / chunk;
-    if (first == last) return;
+    if (first == last || spread.rounds(tiles, chunk)) return;
     const float2 *ml = reinterpret_cast<const float2 *>(a.partial + 2 * size_t(a.runs) * RB * DP);
     // A unit's first run had it last, the others first.
     auto slot = [&](uint32_t r) { return (2 * size_t(r) + (r == first)) * RB + row; };

@@ -44,16 +44,27 @@ __device__ inline float halves_sum(float x) {
 
 // Piece n < 12 of splitting eight values: pairs 0 and 1 in turn, a part at a time, then
 // pairs 2 and 3 (a pair's next part waits for its rest, so two pairs take turns);
-// pair_of(n) says whose. `rest` goes from piece to piece.
+// pair_of(n) says whose. `rest` goes from piece to piece. Rests by a shift or a mask and
+// a subtraction: v_dot2_f32_bf16, which does it in one instruction, waits for the matrix
+// cores (four of them after a 32-cycle MFMA: 62 cycles; eight VALU instructions: 42).
 constexpr int pair_of(int n) { return n / 6 * 2 + n % 2; }
 __device__ inline void split_piece(int n, f32x2 x, f32x2 (&rest)[2], uint32_t (&out)[kParts][4]) {
     const int w = n % 6 / 2;
     const f32x2 from = w == 0 ? x : rest[n % 2];
-    out[w][pair_of(n)] = pack(from.x, from.y);
-    if (w < 2) rest[n % 2] = rest_of(from, out[w][pair_of(n)]);
+    const uint32_t p = pack(from.x, from.y);
+    out[w][pair_of(n)] = p;
+    if (w < 2) rest[n % 2] = f32x2{from.x - low_part(p), from.y - high_part(p)};
 }
 __device__ inline bf16x8 part_of(const uint32_t (&p)[kParts][4], int w) {
     return __builtin_bit_cast(bf16x8, u32x4{p[w][0], p[w][1], p[w][2], p[w][3]});
+}
+
+// The lane's number, made anew: what is computed from it is not kept in registers from
+// outside the main loop.
+__device__ inline int lane_now() {
+    int l = __builtin_amdgcn_mbcnt_hi(~0u, __builtin_amdgcn_mbcnt_lo(~0u, 0u));
+    asm volatile("" : "+v"(l));
+    return l;
 }
 
 template <int DP, int QG>
@@ -64,7 +75,8 @@ struct Shape {
     // Where K and V of a tile are loaded: each chunk as soon as the last tile's is split,
     // or, where two row groups leave no registers for all of both, V before the scores
     // and K before and amid the outputs.
-    static constexpr bool kEarly = QG == 1;
+    static constexpr bool kEarly = QG == 1 || DP <= 64;
+    static constexpr int kEarlyK = kEarly ? kSteps : kSteps / 2;
     static_assert(QG * kSteps * kParts * 1024 <= kWaves * kRows * kPitch * 4, "Q's parts fit the sums' space");
 };
 
@@ -83,16 +95,13 @@ attention_ragged_parts(RaggedArgs a) {
     __shared__ int far;  // a query that the parts do not carry
     char *const qs = reinterpret_cast<char *>(&part[0][0][0]);  // Q's parts until the sums are joined
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int c = lane & 31, h = lane >> 5;
     const uint32_t units = a.kv_heads * a.row_blocks;
     const Spread<kTile> spread(a);
     const uint32_t total = spread.total * units, chunk = (total + a.runs - 1) / a.runs;
     const uint32_t run = run_of(blockIdx.x, a.runs);
-    if (uint64_t(run) * chunk >= total) return;
-    uint32_t t = run * chunk;
-    const uint32_t t_stop = min(total, t + chunk);
     uint32_t b, before;
-    spread.find(t / units, b, before);
+    const uint32_t t_stop = spread.start(run + 1, chunk, units, b, before);
+    uint32_t t = spread.start(run, chunk, units, b, before);
 
     const uint32_t row_bytes = a.k_row * 4u;
     while (t < t_stop) {
@@ -124,13 +133,11 @@ attention_ragged_parts(RaggedArgs a) {
         };
         f32x4 kf[KS][2];
         vec vf[2][8];
-        // Offsets are made from the lane's number for each tile: kept, they would be spilled.
         struct Offsets {
             uint32_t k, v;
         };
         auto offsets = [&]() __attribute__((always_inline)) {
-            uint32_t l = __builtin_amdgcn_mbcnt_hi(~0u, __builtin_amdgcn_mbcnt_lo(~0u, 0u));
-            asm volatile("" : "+v"(l));
+            const uint32_t l = lane_now();
             const uint32_t half = l >> 5, row = l & 31;
             return Offsets{(32 * wave + row) * row_bytes + 16 * half,
                            int(NB * row) < a.dim ? (32 * wave + 4 * half) * row_bytes + 4 * NB * row : kDeadOffset};
@@ -211,6 +218,8 @@ attention_ragged_parts(RaggedArgs a) {
         clear();
         // Keys that this wave's rows do not see, of its 32 in tile x.
         auto mask = [&](uint32_t x) __attribute__((always_inline)) {
+            if (x < cached && (x + 1) * kTile <= len) return;
+            const int l = lane_now(), c = l & 31, h = l >> 5;
             if (x >= cached) {
                 const uint32_t key = (x - cached) * kTile + 32 * wave;
 #pragma unroll
@@ -221,7 +230,7 @@ attention_ragged_parts(RaggedArgs a) {
                     for (int v = 0; v < 16; ++v)
                         if (!(seen >> (8 * (v >> 2) + (v & 3)) & 1)) st[r][v] = -INFINITY;
                 }
-            } else if ((x + 1) * kTile > len) {
+            } else {
                 const int first = int(x) * kTile + 32 * wave + 4 * h;
 #pragma unroll
                 for (int r = 0; r < QG; ++r)
@@ -287,9 +296,8 @@ attention_ragged_parts(RaggedArgs a) {
         for (uint32_t x = begin; x < end; ++x) {
             const auto kfrom = tile_of(kb, kd, x + 1), vfrom = tile_of(vb, vd, S::kEarly ? x + 1 : x);
             const Offsets at = offsets();
-            if (S::kEarly)
-                load_k(kfrom, at.k, 0);
-            else
+            load_k(kfrom, at.k, 0);
+            if (!S::kEarly)
 #pragma unroll
                 for (int u = 0; u < 8; ++u) load_v(vfrom, at.v, 0, u);
 #pragma unroll
@@ -313,7 +321,7 @@ attention_ragged_parts(RaggedArgs a) {
                     if constexpr (p == 0) read_q(s + 1, 0);
                     if constexpr (p == 1) read_q(s + 1, 2);
                     if constexpr (p == 4) read_q(s + 1, 1);
-                    if constexpr (S::kEarly && p == 5) load_k(kfrom, at.k, s + 1);
+                    if constexpr (s + 1 < S::kEarlyK && p == 5) load_k(kfrom, at.k, s + 1);
                     if constexpr (!S::kEarly && p == 5)
 #pragma unroll
                         for (int u = s * 8 / (KS - 1); u < (s + 1) * 8 / (KS - 1); ++u) load_v(vfrom, at.v, 1, u);
@@ -337,9 +345,6 @@ attention_ragged_parts(RaggedArgs a) {
             for (int r = 0; r < QG; ++r)
 #pragma unroll
                 for (int n = 0; n < 12; ++n) split_p(r, 0, n);
-            if (!S::kEarly)
-#pragma unroll
-                for (int k = 0; k < KS / 2; ++k) load_k(kfrom, at.k, k);
             // Outputs; beside octet o the parts of octet o + 1, or of the next tile's first K step.
             each<12 * NB * QG>([&](auto nc) __attribute__((always_inline)) {
                 constexpr int n = decltype(nc)::value, i = n % (6 * QG), o = n / (6 * QG), p = i / QG, r = i % QG;
@@ -371,7 +376,7 @@ attention_ragged_parts(RaggedArgs a) {
                             for (int u = 0; u < 8; ++u) load_v(vfrom, at.v, half, u);
                         else if constexpr (half == 0)
 #pragma unroll
-                            for (int k = KS / 2; k < KS; ++k) load_k(kfrom, at.k, k);
+                            for (int k = S::kEarlyK; k < KS; ++k) load_k(kfrom, at.k, k);
                     }
                     if constexpr (o + 1 == 2 * NB && p < kParts) read_q(0, p);
                 }
@@ -392,6 +397,7 @@ attention_ragged_parts(RaggedArgs a) {
         if (far || __any(odd != 0.f)) {
             unscale = 1.f;
             clear();
+            const int l = lane_now(), c = l & 31, h = l >> 5;
             for (uint32_t x = begin; x < end; ++x) {
                 const bool drafted = x >= cached;
                 const uint32_t tile = drafted ? x - cached : x, keys = drafted ? a.nodes : len;
@@ -442,6 +448,7 @@ attention_ragged_parts(RaggedArgs a) {
             }
         }
 
+        const int l = lane_now(), c = l & 31, h = l >> 5;
         // The four waves' sums joined: dim NB i + e of row c for i = 8 (v >> 2) + 4 h + (v & 3).
         __syncthreads();
 #pragma unroll

@@ -74,6 +74,28 @@ struct Spread {
             before += of_lane(sum, 63);
         }
     }
+    // Where run `run` starts: tile run * chunk, but at the nearest end of a (kv head, row
+    // block) where a run has four or more whole ones of that sequence: then none of them
+    // needs joining, and runs with neighbouring row blocks, which read the same keys, do so
+    // at the same time, from their XCD's L2 (4 x 32 heads x 1000 queries x 4096 keys: 1540
+    // us with every run as long as the next, KEPT_US so). `b` and `before` as find() leaves
+    // them; at the last tile's end they say nothing.
+    __device__ uint32_t start(uint32_t run, uint32_t chunk, uint32_t units, uint32_t &b, uint32_t &before) const {
+        const uint64_t at = uint64_t(run) * chunk, end = uint64_t(total) * units;
+        if (at >= end) return uint32_t(end);
+        uint32_t t = uint32_t(at);
+        find(t / units, b, before);
+        const uint32_t tiles = of_lane(tiles_at(b), 0);
+        if (!rounds(tiles, chunk)) return t;
+        const uint32_t over = (t - before * units) % tiles;
+        t = 2 * over < tiles ? t - over : t - over + tiles;
+        if (t == (before + tiles) * units) {
+            before += tiles;
+            ++b;
+        }
+        return t;
+    }
+    __device__ static bool rounds(uint32_t tiles, uint32_t chunk) { return 4 * tiles <= chunk; }
     // The tiles before sequence b.
     __device__ uint32_t before(uint32_t b) const {
         uint32_t sum = 0, last = up_to - own;
@@ -90,8 +112,7 @@ __device__ inline bool is_node(float parent, int n) {
     return parent == -1.f || (parent >= 0.f && parent < float(n) && parent == truncf(parent));
 }
 
-// Run w of the launch: runs of one XCD are neighbours, so the row blocks of one kv
-// head, which read the same keys, meet in its L2.
+// Run of block `id`: the runs of one XCD are neighbours.
 __device__ inline uint32_t run_of(uint32_t id, uint32_t runs) { return id % 8 * (runs / 8) + id / 8; }
 
 __device__ inline float across_keys_max(float x) { return fmaxf(fmaxf(x, __shfl_xor(x, 16)), fmaxf(__shfl_xor(x, 32), __shfl_xor(x, 48))); }
@@ -124,7 +145,9 @@ __device__ inline void finish(const RaggedArgs &a, uint32_t run, uint32_t b, uin
                               bool starts, const float (&part)[kWaves][RB][DP + 4], const float2 (&ml)[kWaves][RB]) {
     const uint32_t rows = min(uint32_t(RB), a.group * a.queries - rb * RB);
     const size_t slot = 2 * size_t(run) + starts;
-    for (uint32_t at = threadIdx.x; at < rows * (DP / 4); at += THREADS) {
+    uint32_t tid = threadIdx.x;
+    asm volatile("" : "+v"(tid));  // nothing below is computed ahead of a caller's main loop
+    for (uint32_t at = tid; at < rows * (DP / 4); at += THREADS) {
         const uint32_t row = at / (DP / 4), d = at % (DP / 4) * 4;
         float most = -INFINITY;
 #pragma unroll
