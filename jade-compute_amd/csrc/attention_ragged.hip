@@ -50,6 +50,7 @@ attention_ragged(RaggedArgs a) {
     constexpr int KJ = DP / 16, NJ = DP / 64, RB = S::kRows, PITCH = S::kPitch;
     __shared__ __attribute__((aligned(16))) float part[kWaves][RB][PITCH];
     __shared__ float2 ml[kWaves][RB];
+    __shared__ RowPlan plans[RB];
     __shared__ uint64_t sees[kMaxTreeNodes][kWords];
     __shared__ int above[kMaxTreeNodes];
     float (*const qs)[PITCH] = part[0];  // Q in log2 units, until the sums are joined
@@ -306,7 +307,7 @@ attention_ragged(RaggedArgs a) {
                         f32x4{acc[qt][j][0][i], acc[qt][j][1][i], acc[qt][j][2][i], acc[qt][j][3][i]};
         }
         __syncthreads();
-        finish<DP, RB, S::kThreads, VEC>(a, run, b, kv, rb, whole, begin == 0, part, ml);
+        finish<DP, RB, S::kThreads, VEC>(a, run, b, kv, rb, whole, begin == 0, part, ml, plans);
         t += end - begin;
         if (t >= (before + tiles) * units) {
             before += tiles;

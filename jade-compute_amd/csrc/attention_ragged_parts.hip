@@ -44,16 +44,17 @@ __device__ inline float halves_sum(float x) {
 
 // Piece n < 12 of splitting eight values: pairs 0 and 1 in turn, a part at a time, then
 // pairs 2 and 3 (a pair's next part waits for its rest, so two pairs take turns);
-// pair_of(n) says whose. `rest` goes from piece to piece. Rests by a shift or a mask and
-// a subtraction: v_dot2_f32_bf16, which does it in one instruction, waits for the matrix
-// cores (four of them after a 32-cycle MFMA: 62 cycles; eight VALU instructions: 42).
+// pair_of(n) says whose. `rest` holds what is left of the two pairs, at first the pairs
+// themselves. Rests by a shift or a mask and a subtraction: v_dot2_f32_bf16, which does
+// it in one instruction, waits for the matrix cores (four of them after a 32-cycle MFMA:
+// 62 cycles; eight VALU instructions: 42).
 constexpr int pair_of(int n) { return n / 6 * 2 + n % 2; }
-__device__ inline void split_piece(int n, f32x2 x, f32x2 (&rest)[2], uint32_t (&out)[kParts][4]) {
+__device__ inline void split_piece(int n, f32x2 (&rest)[2], uint32_t (&out)[kParts][4]) {
     const int w = n % 6 / 2;
-    const f32x2 from = w == 0 ? x : rest[n % 2];
-    const uint32_t p = pack(from.x, from.y);
+    f32x2 &x = rest[n % 2];
+    const uint32_t p = pack(x.x, x.y);
     out[w][pair_of(n)] = p;
-    if (w < 2) rest[n % 2] = f32x2{from.x - low_part(p), from.y - high_part(p)};
+    if (w < 2) x = f32x2{x.x - low_part(p), x.y - high_part(p)};
 }
 __device__ inline bf16x8 part_of(const uint32_t (&p)[kParts][4], int w) {
     return __builtin_bit_cast(bf16x8, u32x4{p[w][0], p[w][1], p[w][2], p[w][3]});
@@ -89,6 +90,7 @@ attention_ragged_parts(RaggedArgs a) {
     typedef float vec __attribute__((ext_vector_type(NB)));
     __shared__ __attribute__((aligned(16))) float part[kWaves][RB][S::kPitch];
     __shared__ float2 ml[kWaves][RB];
+    __shared__ RowPlan plans[RB];
     __shared__ uint64_t sees[kMaxTreeNodes][kWords];
     __shared__ int above[kMaxTreeNodes];
     __shared__ float2 seen_so_far[kWaves][QG][64];  // running maximum and sum of a lane's rows
@@ -159,16 +161,29 @@ attention_ragged_parts(RaggedArgs a) {
             else
                 vf[s][u] = __builtin_bit_cast(vec, __builtin_amdgcn_raw_buffer_load_b64(from, int(at), 0, 0));
         };
-        // Row r of the block, dims d .. d + 3, in log2 units.
-        auto load_q = [&](int r, int d) {
+        // Row r of the block, from its first dim; null past the last row.
+        auto q_row = [&](int r) -> const float * {
             const uint32_t at = rb * RB + r, head = at / a.queries, query = at - head * a.queries;
-            const float *row = a.q + size_t(b) * a.q_batch + (size_t(kv) * a.group + head) * a.q_head + size_t(query) * a.q_row;
-            f32x4 x = {0.f, 0.f, 0.f, 0.f};
-            if (head < a.group && d < a.dim) x = *reinterpret_cast<const f32x4 *>(row + d);
-            return x * a.qscale;
+            if (head >= a.group) return nullptr;
+            return a.q + size_t(b) * a.q_batch + (size_t(kv) * a.group + head) * a.q_head + size_t(query) * a.q_row;
         };
-        // The first tile; from here on a chunk is loaded again once it is split.
+        // Its dims d .. d + 3.
+        auto load_q = [&](const float *row, int d) {
+            return row && d < a.dim ? *reinterpret_cast<const f32x4 *>(row + d) : f32x4{0.f, 0.f, 0.f, 0.f};
+        };
+        // Q first, then the first tile; from there on a chunk is loaded again once it is
+        // split. A wave stages the steps wave + 4 i % KS of row group 4 i / KS.
+        constexpr int kItems = QG * KS / kWaves;
+        f32x4 qraw[kItems][2];
         {
+            const int l = lane_now();
+#pragma unroll
+            for (int i = 0; i < kItems; ++i) {
+                const float *row = q_row(32 * (kWaves * i / KS) + (l & 31));
+#pragma unroll
+                for (int y = 0; y < 2; ++y)
+                    qraw[i][y] = load_q(row, 16 * (wave + kWaves * i % KS) + 8 * y + 4 * (l >> 5));
+            }
             const auto kfrom = tile_of(kb, kd, begin), vfrom = tile_of(vb, vd, begin);
             const Offsets at = offsets();
 #pragma unroll
@@ -181,23 +196,24 @@ attention_ragged_parts(RaggedArgs a) {
         __syncthreads();  // the last unit's sums are read
         if (tid == 0) far = 0;
         __syncthreads();
-        for (int i = tid; i < QG * KS * 64; i += S::kBlock) {
-            const int l = i & 63, s = (i >> 6) % KS, r = (i >> 6) / KS;
+#pragma unroll
+        for (int i = 0; i < kItems; ++i) {
+            const int s = wave + kWaves * i % KS, r = kWaves * i / KS;
             uint32_t p[kParts][4];
-            f32x2 rest[2];
             bool past = false;
 #pragma unroll
             for (int y = 0; y < 2; ++y) {
-                const f32x4 q = load_q(32 * r + (l & 31), 16 * s + 8 * y + 4 * (l >> 5)) * kScaleQ;
+                const f32x4 q = qraw[i][y] * (a.qscale * kScaleQ);
 #pragma unroll
                 for (int e = 0; e < 4; ++e) past |= fabsf(q[e]) > kMostQ;
+                f32x2 rest[2] = {{q.x, q.y}, {q.z, q.w}};
 #pragma unroll
-                for (int n = 0; n < 6; ++n) split_piece(6 * y + n, n % 2 ? f32x2{q.z, q.w} : f32x2{q.x, q.y}, rest, p);
+                for (int n = 0; n < 6; ++n) split_piece(6 * y + n, rest, p);
             }
             if (past) far = 1;
 #pragma unroll
             for (int w = 0; w < kParts; ++w)
-                *reinterpret_cast<bf16x8 *>(qs + (((r * KS + s) * kParts + w) * 64 + l) * 16) = part_of(p, w);
+                *reinterpret_cast<bf16x8 *>(qs + (((r * KS + s) * kParts + w) * 64 + lane) * 16) = part_of(p, w);
         }
         if (end > cached)
             see_ancestors(a.nodes, above_me, sees, above);
@@ -265,8 +281,9 @@ attention_ragged_parts(RaggedArgs a) {
         };
         // Score v of row group r to its weight.
         auto weigh = [&](int r, int v) __attribute__((always_inline)) {
-            st[r][v] = __builtin_amdgcn_exp2f(st[r][v] - (top[r] == -INFINITY ? 0.f : top[r]));
-            sum[r] += st[r][v];
+            const float weight = __builtin_amdgcn_exp2f(st[r][v] - (top[r] == -INFINITY ? 0.f : top[r]));
+            sum[r] += weight;
+            return weight;
         };
 
         // Two buffers of parts each for K steps, Q steps and V octets (s, e): one is
@@ -280,51 +297,55 @@ attention_ragged_parts(RaggedArgs a) {
                 (w ? q12[r][w - 1] : q0[s & 1][r]) =
                     *reinterpret_cast<const bf16x8 *>(qs + (((r * KS + s) * kParts + w) * 64 + lane) * 16);
         };
-        auto split_k = [&](int s, int n) __attribute__((always_inline)) {
-            const f32x4 k = kf[s][n / 6];
-            split_piece(n, (n % 2 ? f32x2{k.z, k.w} : f32x2{k.x, k.y}) * kScaleK, rest, kp[s & 1]);
+        // What is split beside the products of a tile, in order: K's steps 1 .. KS - 1, V's
+        // octets (o: keys 16 (o / NB) .. + 15 of the lane's half, dim o % NB) and the next
+        // tile's K step 0. A pair is scaled beside the last parts of the pair before.
+        auto scaled = [&](int q, int pair) __attribute__((always_inline)) {
+            const int s = (q + 1) % (KS + 2 * NB), o = s - KS;
+            if (s < KS) {
+                const f32x4 k = kf[s][pair / 2];
+                return (pair % 2 ? f32x2{k.z, k.w} : f32x2{k.x, k.y}) * kScaleK;
+            }
+            return f32x2{vf[o / NB][2 * pair][o % NB], vf[o / NB][2 * pair + 1][o % NB]} * kScaleV;
         };
-        auto split_v = [&](int o, int n) __attribute__((always_inline)) {  // octet o: keys o / NB, dim o % NB
-            const int u = 2 * pair_of(n);
-            split_piece(n, f32x2{vf[o / NB][u][o % NB], vf[o / NB][u + 1][o % NB]} * kScaleV, rest, vp[o & 1]);
+        auto split = [&](int q, int n) __attribute__((always_inline)) {
+            const int s = (q + 1) % (KS + 2 * NB), o = s - KS;
+            split_piece(n, rest, s < KS ? kp[s & 1] : vp[o & 1]);
+            if (n % 6 >= 4) rest[n % 2] = n < 6 ? scaled(q, pair_of(n + 2)) : scaled((q + 1) % (KS + 2 * NB), pair_of(n - 10));
         };
 #pragma unroll
-        for (int n = 0; n < 12; ++n) split_k(0, n);
+        for (int n = 0; n < 2; ++n) rest[n] = scaled(KS + 2 * NB - 1, n);
+#pragma unroll
+        for (int n = 0; n < 12; ++n) split(KS + 2 * NB - 1, n);
 #pragma unroll
         for (int w = 0; w < kParts; ++w) read_q(0, w);
+        auto kfrom = tile_of(kb, kd, begin + 1), vfrom = tile_of(vb, vd, S::kEarly ? begin + 1 : begin);
+        Offsets at = offsets();
 
         for (uint32_t x = begin; x < end; ++x) {
-            const auto kfrom = tile_of(kb, kd, x + 1), vfrom = tile_of(vb, vd, S::kEarly ? x + 1 : x);
-            const Offsets at = offsets();
-            load_k(kfrom, at.k, 0);
-            if (!S::kEarly)
-#pragma unroll
-                for (int u = 0; u < 8; ++u) load_v(vfrom, at.v, 0, u);
 #pragma unroll
             for (int r = 0; r < QG; ++r) st[r] = f32x16{};
-            // Scores; beside step s the parts of K's and Q's step s + 1, or V's first octet.
             each<6 * KS * QG>([&](auto nc) __attribute__((always_inline)) {
                 constexpr int i = decltype(nc)::value % (6 * QG), s = decltype(nc)::value / (6 * QG), p = i / QG, r = i % QG;
                 __builtin_amdgcn_sched_barrier(0);
                 st[r] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(
                     part_of(kp[s & 1], kPartA[p]), kPartB[p] ? q12[r][kPartB[p] - 1] : q0[s & 1][r], st[r], 0, 0, 0);
                 __builtin_amdgcn_sched_barrier(0);
-                each<2 / QG>([&](auto ec) __attribute__((always_inline)) {
-                    constexpr int piece = 2 * i / QG + decltype(ec)::value;
-                    if constexpr (s + 1 < KS)
-                        split_k(s + 1, piece);
-                    else
-                        split_v(0, piece);
-                });
+                each<2 / QG>([&](auto ec) __attribute__((always_inline)) { split(s, 2 * i / QG + decltype(ec)::value); });
                 if constexpr (s + 1 < KS && r == QG - 1) {
                     // Each part once its last product is issued (B's parts go 0 2 1 0 1 0).
                     if constexpr (p == 0) read_q(s + 1, 0);
                     if constexpr (p == 1) read_q(s + 1, 2);
                     if constexpr (p == 4) read_q(s + 1, 1);
-                    if constexpr (s + 1 < S::kEarlyK && p == 5) load_k(kfrom, at.k, s + 1);
-                    if constexpr (!S::kEarly && p == 5)
-#pragma unroll
-                        for (int u = s * 8 / (KS - 1); u < (s + 1) * 8 / (KS - 1); ++u) load_v(vfrom, at.v, 1, u);
+                }
+                // Step s's values are split: K's next tile there.
+                if constexpr (p == 0 && r == QG - 1 && s < S::kEarlyK) load_k(kfrom, at.k, s);
+                // V's rows where they are not loaded yet: the first eight early.
+                if constexpr (!S::kEarly && r == QG - 1) {
+                    constexpr int n = 6 * s + p, last = 6 * KS - 6;
+                    if constexpr (n % 2 == 1 && n < 16) load_v(vfrom, at.v, 0, n / 2);
+                    if constexpr (n >= 16 && (n - 16) % ((last - 16) / 8) == 0 && (n - 16) / ((last - 16) / 8) < 8)
+                        load_v(vfrom, at.v, 1, (n - 16) / ((last - 16) / 8));
                 }
             });
             __builtin_amdgcn_sched_barrier(0);
@@ -335,17 +356,13 @@ attention_ragged_parts(RaggedArgs a) {
             f32x2 prest[2];
             auto split_p = [&](int r, int s, int n) __attribute__((always_inline)) {
                 const int v = 8 * s + 2 * pair_of(n);
-                if (n % 6 < 2) {
-                    weigh(r, v);
-                    weigh(r, v + 1);
-                }
-                split_piece(n, f32x2{st[r][v], st[r][v + 1]}, prest, pp[r][s]);
+                if (n % 6 < 2) prest[n % 2] = f32x2{weigh(r, v), weigh(r, v + 1)};
+                split_piece(n, prest, pp[r][s]);
             };
 #pragma unroll
             for (int r = 0; r < QG; ++r)
 #pragma unroll
                 for (int n = 0; n < 12; ++n) split_p(r, 0, n);
-            // Outputs; beside octet o the parts of octet o + 1, or of the next tile's first K step.
             each<12 * NB * QG>([&](auto nc) __attribute__((always_inline)) {
                 constexpr int n = decltype(nc)::value, i = n % (6 * QG), o = n / (6 * QG), p = i / QG, r = i % QG;
                 constexpr int s = o / NB, e = o % NB;
@@ -360,25 +377,22 @@ attention_ragged_parts(RaggedArgs a) {
                         split_p(j / 12, 1, j % 12);
                     });
                 if constexpr (n == 6 * NB * QG) keep_state();
-                each<2 / QG>([&](auto ec) __attribute__((always_inline)) {
-                    constexpr int piece = 2 * i / QG + decltype(ec)::value;
-                    if constexpr (o + 1 < 2 * NB)
-                        split_v(o + 1, piece);
-                    else
-                        split_k(0, piece);
-                });
+                each<2 / QG>([&](auto ec) __attribute__((always_inline)) { split(KS + o, 2 * i / QG + decltype(ec)::value); });
                 if constexpr (r == QG - 1) {
-                    // The last octet of these keys is split: their registers again.
-                    if constexpr (o + 1 < 2 * NB && (o + 1) % NB == NB - 1 && p == 5) {
-                        constexpr int half = (o + 1) / NB;
-                        if constexpr (S::kEarly)
+                    // The last octet of 16 keys is split from octet NB - 2's products on: V's
+                    // next tile there, or K's remaining steps.
+                    constexpr int u = 6 * (o % NB - (NB - 1)) + p;  // slots since
+                    if constexpr (S::kEarly && (u == 0 || u == 1 || u == 2 || u == 3))
 #pragma unroll
-                            for (int u = 0; u < 8; ++u) load_v(vfrom, at.v, half, u);
-                        else if constexpr (half == 0)
-#pragma unroll
-                            for (int k = S::kEarlyK; k < KS; ++k) load_k(kfrom, at.k, k);
-                    }
+                        for (int j = 2 * u; j < 2 * u + 2; ++j) load_v(vfrom, at.v, s, j);
+                    if constexpr (!S::kEarly && s == 0 && u >= 0 && u < KS - S::kEarlyK) load_k(kfrom, at.k, S::kEarlyK + u);
                     if constexpr (o + 1 == 2 * NB && p < kParts) read_q(0, p);
+                    // The tile after the next.
+                    if constexpr (n / QG == 12 * NB - 1) {
+                        kfrom = tile_of(kb, kd, x + 2);
+                        vfrom = tile_of(vb, vd, S::kEarly ? x + 2 : x + 1);
+                        at = offsets();
+                    }
                 }
             });
             __builtin_amdgcn_sched_barrier(0);
@@ -407,9 +421,10 @@ attention_ragged_parts(RaggedArgs a) {
 #pragma unroll
                 for (int r = 0; r < QG; ++r) {
                     st[r] = f32x16{};
+                    const float *qrow = q_row(32 * r + c);
                     for (int d0 = 0; d0 < DP; d0 += 8) {
                         const int d = d0 + 4 * h;
-                        const f32x4 q = load_q(32 * r + c, d);
+                        const f32x4 q = load_q(qrow, d) * a.qscale;
                         f32x4 k = {0.f, 0.f, 0.f, 0.f};
                         if (d < a.dim && key0 + c < keys) k = *reinterpret_cast<const f32x4 *>(krow + d);
 #pragma unroll
@@ -421,7 +436,7 @@ attention_ragged_parts(RaggedArgs a) {
 #pragma unroll
                 for (int r = 0; r < QG; ++r)
 #pragma unroll
-                    for (int v = 0; v < 16; ++v) weigh(r, v);
+                    for (int v = 0; v < 16; ++v) st[r][v] = weigh(r, v);
                 keep_state();
                 // Drafted values that are not finite, which not every row may see: the finite
                 // ones, then the weight that each row gives to each special one.
@@ -465,7 +480,7 @@ attention_ragged_parts(RaggedArgs a) {
             }
         }
         __syncthreads();
-        finish<DP, RB, S::kBlock, true>(a, run, b, kv, rb, whole, begin == 0, part, ml);
+        finish<DP, RB, S::kBlock, true>(a, run, b, kv, rb, whole, begin == 0, part, ml, plans);
         t += end - begin;
         if (t >= (before + tiles) * units) {
             before += tiles;

@@ -137,36 +137,64 @@ __device__ inline void store_row(const RaggedArgs &a, uint32_t b, uint32_t kv, u
     }
 }
 
+// What joining the four waves' sums of a row takes.
+struct RowPlan {
+    f32x4 weights;  // of the waves, with the whole sum's reciprocal where the row is finished
+    float2 top_sum;
+    size_t at;  // its first dim in the outputs, or in the run's slot
+};
 // A unit's sums as its four waves by keys left them in LDS, joined: outputs where the
 // run holds the `whole` unit, else sums, maximum and weight to the run's slot (a unit's
-// first run had it last, the others first).
+// first run had it last, the others first). The block's threads do it together; `plans`
+// is LDS.
 template <int DP, int RB, int THREADS, bool VEC>
 __device__ inline void finish(const RaggedArgs &a, uint32_t run, uint32_t b, uint32_t kv, uint32_t rb, bool whole,
-                              bool starts, const float (&part)[kWaves][RB][DP + 4], const float2 (&ml)[kWaves][RB]) {
+                              bool starts, const float (&part)[kWaves][RB][DP + 4], const float2 (&ml)[kWaves][RB],
+                              RowPlan (&plans)[RB]) {
     const uint32_t rows = min(uint32_t(RB), a.group * a.queries - rb * RB);
-    const size_t slot = 2 * size_t(run) + starts;
     uint32_t tid = threadIdx.x;
     asm volatile("" : "+v"(tid));  // nothing below is computed ahead of a caller's main loop
-    for (uint32_t at = tid; at < rows * (DP / 4); at += THREADS) {
-        const uint32_t row = at / (DP / 4), d = at % (DP / 4) * 4;
+    if (tid < rows) {
         float most = -INFINITY;
 #pragma unroll
-        for (int w = 0; w < kWaves; ++w) most = fmaxf(most, ml[w][row].x);
+        for (int w = 0; w < kWaves; ++w) most = fmaxf(most, ml[w][tid].x);
         const float from = most == -INFINITY ? 0.f : most;
-        f32x4 o = {0.f, 0.f, 0.f, 0.f};
+        RowPlan p;
         float l = 0.f;
 #pragma unroll
         for (int w = 0; w < kWaves; ++w) {
-            const float weight = __builtin_amdgcn_exp2f(ml[w][row].x - from);
-            l = fmaf(weight, ml[w][row].y, l);
-            o += weight * *reinterpret_cast<const f32x4 *>(&part[w][row][d]);
+            p.weights[w] = __builtin_amdgcn_exp2f(ml[w][tid].x - from);
+            l = fmaf(p.weights[w], ml[w][tid].y, l);
         }
+        p.top_sum = float2{most, l};
         if (whole) {
-            store_row<VEC>(a, b, kv, rb * RB + row, d, o, l);
+            const uint32_t r = rb * RB + tid, head = r / a.queries, query = r - head * a.queries;
+            p.at = size_t(b) * a.q_batch + (size_t(kv) * a.group + head) * a.q_head + size_t(query) * a.q_row;
+            p.top_sum.y = a.nodes && !is_node(a.parents[size_t(b) * a.nodes + query], int(query)) ? 0.f : 1.0f / l;
         } else {
-            *reinterpret_cast<f32x4 *>(a.partial + (slot * RB + row) * DP + d) = o;
-            if (d == 0)
-                reinterpret_cast<float2 *>(a.partial + 2 * size_t(a.runs) * RB * DP)[slot * RB + row] = float2{most, l};
+            const size_t slot = (2 * size_t(run) + starts) * RB + tid;
+            p.at = slot * DP;
+            reinterpret_cast<float2 *>(a.partial + 2 * size_t(a.runs) * RB * DP)[slot] = p.top_sum;
+            p.top_sum.y = 1.f;
+        }
+        plans[tid] = p;
+    }
+    __syncthreads();
+    float *const to = whole ? a.out : a.partial;
+    for (uint32_t at = tid; at < rows * (DP / 4); at += THREADS) {
+        const uint32_t row = at / (DP / 4), d = at % (DP / 4) * 4;
+        const RowPlan &p = plans[row];
+        f32x4 o = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int w = 0; w < kWaves; ++w) o += p.weights[w] * *reinterpret_cast<const f32x4 *>(&part[w][row][d]);
+        // A slot without a node is zeros whatever its sums are.
+        o = p.top_sum.y == 0.f ? f32x4{0.f, 0.f, 0.f, 0.f} : o * p.top_sum.y;
+        if (VEC || !whole) {
+            if (!whole || d < uint32_t(a.dim)) *reinterpret_cast<f32x4 *>(to + p.at + d) = o;
+        } else {
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                if (d + e < uint32_t(a.dim)) to[p.at + d + e] = o[e];
         }
     }
 }
