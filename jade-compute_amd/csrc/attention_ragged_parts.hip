@@ -13,10 +13,11 @@
 // rows and 32 keys of 128 dims that is 192 MFMAs (6144 cycles of a SIMD; FP32 MFMAs
 // take 16384) against some 840 other instructions.
 //
-// V is scaled up before it is split and the outputs are scaled back, Q is scaled up and
-// K down, so every finite V and Q is carried exactly. What the parts do not carry
-// (sums that are not finite, queries past 2^64) a wave notices and does its part of the
-// run again with FP32 MFMAs, as attention_flash.hip does.
+// Q is scaled up before it is split (the scores are scaled back where their maximum is
+// taken off), so every finite Q is carried exactly; parts of K below 2^-109 lose bits
+// below 2^-134, which move no score: a query is at most 2^64. What the parts do not carry
+// (sums that are not finite, queries past 2^64, outputs so small that bits of V below
+// 2^-134 count) a wave notices and does its part of the run again with FP32 MFMAs.
 #include "kernels.hpp"
 #include "ragged_device.hpp"
 #include "split_bf16.hpp"
@@ -31,7 +32,10 @@ using namespace split;
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 
 constexpr int kTile = 128;  // keys per tile, 32 for each wave by keys
-constexpr float kMostQ = 0x1p64f * kScaleQ;
+constexpr float kMostQ = 0x1p64f * kScaleQ, kUnscaleS = 1.f / kScaleQ;
+// Sums of V times weights of at least 2^-8 (the lazy maximum) in all: below this an error
+// of 2^-134 a key is more than 2^-40 of them.
+constexpr float kLeastOut = 0x1p-70f;
 
 __device__ inline float halves_max(float x) {
     const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
@@ -77,7 +81,7 @@ struct Shape {
     // or, where two row groups leave no registers for all of both, V before the scores
     // and K before and amid the outputs.
     static constexpr bool kEarly = QG == 1 || DP <= 64;
-    static constexpr int kEarlyK = kEarly ? kSteps : kSteps / 2;
+    static constexpr int kEarlyK = kEarly ? kSteps : 0;
     static_assert(QG * kSteps * kParts * 1024 <= kWaves * kRows * kPitch * 4, "Q's parts fit the sums' space");
 };
 
@@ -137,19 +141,21 @@ attention_ragged_parts(RaggedArgs a) {
         vec vf[2][8];
         struct Offsets {
             uint32_t k, v;
+            int last;  // K's chunks of eight dims that have this lane's four of them
         };
         auto offsets = [&]() __attribute__((always_inline)) {
             const uint32_t l = lane_now();
             const uint32_t half = l >> 5, row = l & 31;
             return Offsets{(32 * wave + row) * row_bytes + 16 * half,
-                           int(NB * row) < a.dim ? (32 * wave + 4 * half) * row_bytes + 4 * NB * row : kDeadOffset};
+                           NB * row < a.dim ? (32 * wave + 4 * half) * row_bytes + 4 * NB * row : kDeadOffset,
+                           int(a.dim / 4 + 1 - half) / 2};
         };
         // Dims of score step s, load x: 8 y + 4 h + 0 .. 3, y = 2 s + x.
-        auto load_k = [&](__amdgpu_buffer_rsrc_t from, uint32_t koff, int s) __attribute__((always_inline)) {
+        auto load_k = [&](__amdgpu_buffer_rsrc_t from, const Offsets &o, int s) __attribute__((always_inline)) {
 #pragma unroll
             for (int x = 0; x < 2; ++x) {
                 const int y = 2 * s + x;
-                const uint32_t at = 8 * y + int(koff >> 2 & 4) < a.dim ? koff + 32u * y : kDeadOffset;
+                const uint32_t at = y < o.last ? o.k + 32u * y : kDeadOffset;
                 kf[s][x] = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(from, int(at), 0, 0));
             }
         };
@@ -187,7 +193,7 @@ attention_ragged_parts(RaggedArgs a) {
             const auto kfrom = tile_of(kb, kd, begin), vfrom = tile_of(vb, vd, begin);
             const Offsets at = offsets();
 #pragma unroll
-            for (int s = 0; s < KS; ++s) load_k(kfrom, at.k, s);
+            for (int s = 0; s < KS; ++s) load_k(kfrom, at, s);
             if (S::kEarly)
 #pragma unroll
                 for (int u = 0; u < 16; ++u) load_v(vfrom, at.v, u >> 3, u & 7);
@@ -257,7 +263,8 @@ attention_ragged_parts(RaggedArgs a) {
         };
         // The running maximum of the rows past this tile's scores; what was summed so far
         // is scaled to it.
-        auto raise = [&]() __attribute__((always_inline)) {
+        // The scores come `unit` times as large as they are.
+        auto raise = [&](float unit) __attribute__((always_inline)) {
 #pragma unroll
             for (int r = 0; r < QG; ++r) {
                 top[r] = state[r][lane].x;
@@ -265,8 +272,8 @@ attention_ragged_parts(RaggedArgs a) {
                 float most = st[r][0];
 #pragma unroll
                 for (int v = 1; v < 16; ++v) most = fmaxf(most, st[r][v]);
-                if (__any(most > top[r] + kLazyMax)) {
-                    const float reached = fmaxf(top[r], halves_max(most));
+                if (__any(most * unit > top[r] + kLazyMax)) {
+                    const float reached = fmaxf(top[r], halves_max(most) * unit);
                     const float keep = reached == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(top[r] - reached);
                     top[r] = reached;
                     sum[r] *= keep;
@@ -280,8 +287,8 @@ attention_ragged_parts(RaggedArgs a) {
             for (int r = 0; r < QG; ++r) state[r][lane] = float2{top[r], sum[r]};
         };
         // Score v of row group r to its weight.
-        auto weigh = [&](int r, int v) __attribute__((always_inline)) {
-            const float weight = __builtin_amdgcn_exp2f(st[r][v] - (top[r] == -INFINITY ? 0.f : top[r]));
+        auto weigh = [&](int r, int v, float unit) __attribute__((always_inline)) {
+            const float weight = __builtin_amdgcn_exp2f(fmaf(st[r][v], unit, top[r] == -INFINITY ? 0.f : -top[r]));
             sum[r] += weight;
             return weight;
         };
@@ -299,22 +306,22 @@ attention_ragged_parts(RaggedArgs a) {
         };
         // What is split beside the products of a tile, in order: K's steps 1 .. KS - 1, V's
         // octets (o: keys 16 (o / NB) .. + 15 of the lane's half, dim o % NB) and the next
-        // tile's K step 0. A pair is scaled beside the last parts of the pair before.
-        auto scaled = [&](int q, int pair) __attribute__((always_inline)) {
+        // tile's K step 0.
+        auto values = [&](int q, int pair) __attribute__((always_inline)) {
             const int s = (q + 1) % (KS + 2 * NB), o = s - KS;
             if (s < KS) {
                 const f32x4 k = kf[s][pair / 2];
-                return (pair % 2 ? f32x2{k.z, k.w} : f32x2{k.x, k.y}) * kScaleK;
+                return pair % 2 ? f32x2{k.z, k.w} : f32x2{k.x, k.y};
             }
-            return f32x2{vf[o / NB][2 * pair][o % NB], vf[o / NB][2 * pair + 1][o % NB]} * kScaleV;
+            return f32x2{vf[o / NB][2 * pair][o % NB], vf[o / NB][2 * pair + 1][o % NB]};
         };
         auto split = [&](int q, int n) __attribute__((always_inline)) {
             const int s = (q + 1) % (KS + 2 * NB), o = s - KS;
             split_piece(n, rest, s < KS ? kp[s & 1] : vp[o & 1]);
-            if (n % 6 >= 4) rest[n % 2] = n < 6 ? scaled(q, pair_of(n + 2)) : scaled((q + 1) % (KS + 2 * NB), pair_of(n - 10));
+            if (n % 6 >= 4) rest[n % 2] = n < 6 ? values(q, pair_of(n + 2)) : values((q + 1) % (KS + 2 * NB), pair_of(n - 10));
         };
 #pragma unroll
-        for (int n = 0; n < 2; ++n) rest[n] = scaled(KS + 2 * NB - 1, n);
+        for (int n = 0; n < 2; ++n) rest[n] = values(KS + 2 * NB - 1, n);
 #pragma unroll
         for (int n = 0; n < 12; ++n) split(KS + 2 * NB - 1, n);
 #pragma unroll
@@ -339,7 +346,7 @@ attention_ragged_parts(RaggedArgs a) {
                     if constexpr (p == 4) read_q(s + 1, 1);
                 }
                 // Step s's values are split: K's next tile there.
-                if constexpr (p == 0 && r == QG - 1 && s < S::kEarlyK) load_k(kfrom, at.k, s);
+                if constexpr (p == 0 && r == QG - 1 && s < S::kEarlyK) load_k(kfrom, at, s);
                 // V's rows where they are not loaded yet: the first eight early.
                 if constexpr (!S::kEarly && r == QG - 1) {
                     constexpr int n = 6 * s + p, last = 6 * KS - 6;
@@ -350,13 +357,13 @@ attention_ragged_parts(RaggedArgs a) {
             });
             __builtin_amdgcn_sched_barrier(0);
             mask(x);
-            raise();
+            raise(kUnscaleS);
             // Weights and their parts, of keys 0 .. 15 here, of 16 .. 31 beside the first outputs.
             uint32_t pp[QG][2][kParts][4];
             f32x2 prest[2];
             auto split_p = [&](int r, int s, int n) __attribute__((always_inline)) {
                 const int v = 8 * s + 2 * pair_of(n);
-                if (n % 6 < 2) prest[n % 2] = f32x2{weigh(r, v), weigh(r, v + 1)};
+                if (n % 6 < 2) prest[n % 2] = f32x2{weigh(r, v, kUnscaleS), weigh(r, v + 1, kUnscaleS)};
                 split_piece(n, prest, pp[r][s]);
             };
 #pragma unroll
@@ -385,7 +392,9 @@ attention_ragged_parts(RaggedArgs a) {
                     if constexpr (S::kEarly && (u == 0 || u == 1 || u == 2 || u == 3))
 #pragma unroll
                         for (int j = 2 * u; j < 2 * u + 2; ++j) load_v(vfrom, at.v, s, j);
-                    if constexpr (!S::kEarly && s == 0 && u >= 0 && u < KS - S::kEarlyK) load_k(kfrom, at.k, S::kEarlyK + u);
+                    constexpr int at0 = 6 * o + p;
+                    if constexpr (!S::kEarly && at0 % 2 == 1 && at0 < KS) load_k(kfrom, at, at0 / 2);
+                    if constexpr (!S::kEarly && s == 0 && u >= 0 && u < KS / 2) load_k(kfrom, at, KS / 2 + u);
                     if constexpr (o + 1 == 2 * NB && p < kParts) read_q(0, p);
                     // The tile after the next.
                     if constexpr (n / QG == 12 * NB - 1) {
@@ -399,17 +408,20 @@ attention_ragged_parts(RaggedArgs a) {
         }
 
         // What the parts do not carry: see the file's head.
-        float unscale = kUnscaleV, odd = 0.f;
+        float odd = 0.f;
+        uint32_t least = ~0u;  // of the first rows' outputs that are not zero: 2 x their bits - 1
 #pragma unroll
         for (int r = 0; r < QG; ++r) {
             odd += state[r][lane].y * 0.f;
 #pragma unroll
             for (int e = 0; e < NB; ++e)
 #pragma unroll
-                for (int v = 0; v < 16; ++v) odd += acc[r][e][v] * 0.f;
+                for (int v = 0; v < 16; ++v) {
+                    odd += acc[r][e][v] * 0.f;
+                    if (r == 0) least = min(least, (__float_as_uint(acc[r][e][v]) << 1) - 1);
+                }
         }
-        if (far || __any(odd != 0.f)) {
-            unscale = 1.f;
+        if (far || __any(odd != 0.f || least < __float_as_uint(kLeastOut) * 2)) {
             clear();
             const int l = lane_now(), c = l & 31, h = l >> 5;
             for (uint32_t x = begin; x < end; ++x) {
@@ -432,11 +444,11 @@ attention_ragged_parts(RaggedArgs a) {
                     }
                 }
                 mask(x);
-                raise();
+                raise(1.f);
 #pragma unroll
                 for (int r = 0; r < QG; ++r)
 #pragma unroll
-                    for (int v = 0; v < 16; ++v) st[r][v] = weigh(r, v);
+                    for (int v = 0; v < 16; ++v) st[r][v] = weigh(r, v, 1.f);
                 keep_state();
                 // Drafted values that are not finite, which not every row may see: the finite
                 // ones, then the weight that each row gives to each special one.
@@ -475,7 +487,7 @@ attention_ragged_parts(RaggedArgs a) {
             for (int v = 0; v < 16; ++v) {
                 vec o;
 #pragma unroll
-                for (int e = 0; e < NB; ++e) o[e] = acc[r][e][v] * unscale;
+                for (int e = 0; e < NB; ++e) o[e] = acc[r][e][v];
                 *reinterpret_cast<vec *>(&part[wave][32 * r + c][NB * (8 * (v >> 2) + 4 * h + (v & 3))]) = o;
             }
         }

@@ -473,3 +473,52 @@ def test_two_kernels_of_one_shape_and_two_contexts(runtime):
     assert (again == got[1]).all()
     for x, y in zip(xs, got):
         within(y, *dec.cross(spec, x["q"], x["k"], x["v"], [2000]))
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("heads", [16, 20, 40])
+@pytest.mark.parametrize("q_scale,k_scale,v_scale", [(1.0, 1.0, 2.0 ** -120), (1.0, 1.0, 2.0 ** -60), (2.0 ** -120, 1.0, 1.0),
+                                                    (1.0, 2.0 ** -120, 1.0), (2.0 ** -80, 2.0 ** 80, 2.0 ** 100),
+                                                    (2.0 ** 70, 2.0 ** -70, 1.0), (1.0, 1.0, 0.0)])
+def test_attention_cross_tiny_and_large_operands(runtime, dim, heads, q_scale, k_scale, v_scale):
+    # Powers of two on the operands are exact: the outputs are those of N(0, 1) operands, scaled. V of 2^-120 has
+    # outputs above 2^-126: nothing is subnormal but single values.
+    rng = np.random.default_rng(31)
+    spec = cross_spec(1, heads, 1, 1, 150, dim)
+    x = cross_inputs(rng, spec, [150])
+    for name, scale in (("q", q_scale), ("k", k_scale), ("v", v_scale)):
+        x[name] = (x[name].astype(np.float64) * scale).astype(np.float32)
+    want, off = dec.cross(spec, x["q"], x["k"], x["v"], [150])
+    # Besides attend()'s bound, an FP32 output may be rounded to a multiple of 2^-149.
+    within(run(runtime, spec, x)["out"], want, off + 2.0 ** -149)
+
+
+@pytest.mark.parametrize("heads", [3, 20, 40])
+@pytest.mark.parametrize("dim", [4, 12, 20, 36, 44, 60, 68, 76, 84, 100, 116, 124, 1, 2, 61, 67, 127])
+@pytest.mark.parametrize("token_major", [False, True])
+def test_attention_cross_head_dims(runtime, heads, dim, token_major):
+    # Every remainder of the loads' 4, 8 and 16 dims, with one, two and three groups of rows.
+    rng = np.random.default_rng(33)
+    spec = cross_spec(1, 2 * heads, 2, 1, 140, dim, token_major)
+    x = cross_inputs(rng, spec, [139])
+    within(run(runtime, spec, x)["out"], *dec.cross(spec, x["q"], x["k"], x["v"], [139]))
+
+
+@pytest.mark.parametrize("heads,dim", [(16, 64), (20, 128), (40, 64), (40, 128), (20, 36)])
+def test_attention_cross_not_finite_among_many_rows(runtime, heads, dim):
+    # One row's query, one key's value: the others' outputs are as without them.
+    rng = np.random.default_rng(32)
+    spec = cross_spec(2, heads, 1, 1, 200, dim)
+    x = cross_inputs(rng, spec, [200, 150])
+    want, off = dec.cross(spec, x["q"], x["k"], x["v"], [200, 150])
+    x["q"][0, 5] = np.nan
+    x["q"][0, 7, 0, 1] = np.inf
+    x["v"][1, 0, 149, 3] = -np.inf
+    x["v"][1, 0, 150:] = np.nan
+    got = run(runtime, spec, x)["out"].reshape(want.shape)
+    others = [h for h in range(heads) if h not in (5, 7)]
+    within(got[0, others], want[0, others], off[0, others])
+    assert np.isnan(got[0, 5]).all()
+    kept = [d for d in range(dim) if d != 3]
+    within(got[1][..., kept], want[1][..., kept], off[1][..., kept])
+    assert np.isneginf(got[1, :, 0, 3]).all()
