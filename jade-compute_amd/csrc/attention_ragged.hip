@@ -317,16 +317,17 @@ attention_ragged(RaggedArgs a) {
 }
 
 // What the runs left of a (sequence, kv head, row block) cut between them, and the
-// zeros of sequences without keys. Block y has row y of the units of block x: of
-// unit x itself where there are at most `runs` units, else of the one that the cut
-// before run x is the first of.
-template <int DP, int RB, int TILE, bool VEC>
+// zeros of sequences without keys. Blocks x go over the units: unit x itself where there
+// are at most `runs` units, else the one that the cut before run x is the first of. DP / 4
+// lanes have a row; ROWS rows of a unit go to a block, each with all of its slots, or
+// (ROWS 1) one, with the slots shared out (a unit of many runs).
+template <int DP, int RB, int TILE, int ROWS, bool VEC>
 __global__ __launch_bounds__(kThreads) void attention_ragged_join(RaggedArgs a) {
-    constexpr int LANES = DP / 4, PARTS = kThreads / LANES;
+    constexpr int LANES = DP / 4, PARTS = kThreads / LANES / ROWS;
     __shared__ __attribute__((aligned(16))) f32x4 sums[PARTS][LANES];
     __shared__ float weights[PARTS];
-    const int tid = threadIdx.x, lane = tid % LANES, p = tid / LANES;
-    const uint32_t units = a.kv_heads * a.row_blocks, row = blockIdx.y, d = 4 * lane;
+    const int tid = threadIdx.x, lane = tid % LANES, p = ROWS == 1 ? tid / LANES : 0;
+    const uint32_t units = a.kv_heads * a.row_blocks, row = blockIdx.y * ROWS + (ROWS == 1 ? 0 : tid / LANES), d = 4 * lane;
     const bool by_unit = a.batch * units <= a.runs;
     const Spread<TILE> spread(a);
     const uint32_t chunk = (spread.total * units + a.runs - 1) / a.runs;
@@ -354,9 +355,9 @@ __global__ __launch_bounds__(kThreads) void attention_ragged_join(RaggedArgs a) 
         if (start + chunk < cut || start == cut) return;  // not its first cut
     }
     const uint32_t kv = unit / a.row_blocks, rb = unit - kv * a.row_blocks;
-    if (row >= min(uint32_t(RB), a.group * a.queries - rb * RB)) return;
+    const bool mine = row < min(uint32_t(RB), a.group * a.queries - rb * RB);
     if (!tiles) {
-        if (p == 0) store_row<VEC>(a, b, kv, rb * RB + row, d, f32x4{0.f, 0.f, 0.f, 0.f}, 1.f);
+        if (p == 0 && mine) store_row<VEC>(a, b, kv, rb * RB + row, d, f32x4{0.f, 0.f, 0.f, 0.f}, 1.f);
         return;
     }
     const uint32_t first = start / chunk, last = (start + tiles - 1) / chunk;
@@ -365,30 +366,35 @@ __global__ __launch_bounds__(kThreads) void attention_ragged_join(RaggedArgs a) 
     // A unit's first run had it last, the others first.
     auto slot = [&](uint32_t r) { return (2 * size_t(r) + (r == first)) * RB + row; };
     float most = -INFINITY;
-    for (uint32_t r = first + lane; r <= last; r += LANES) most = fmaxf(most, ml[slot(r)].x);
+    if (mine)
+        for (uint32_t r = first + lane; r <= last; r += LANES) most = fmaxf(most, ml[slot(r)].x);
 #pragma unroll
     for (int step = LANES / 2; step > 0; step /= 2) most = fmaxf(most, __shfl_xor(most, step));
     const float from = most == -INFINITY ? 0.f : most;
     float l = 0.f;
     f32x4 o = {0.f, 0.f, 0.f, 0.f};
+    if (mine) {
 #pragma unroll 4
-    for (uint32_t r = first + p; r <= last; r += PARTS) {
-        const float2 x = ml[slot(r)];
-        const f32x4 y = *reinterpret_cast<const f32x4 *>(a.partial + slot(r) * DP + d);
-        const float weight = __builtin_amdgcn_exp2f(x.x - from);
-        l = fmaf(weight, x.y, l);
-        o += weight * y;
+        for (uint32_t r = first + p; r <= last; r += PARTS) {
+            const float2 x = ml[slot(r)];
+            const f32x4 y = *reinterpret_cast<const f32x4 *>(a.partial + slot(r) * DP + d);
+            const float weight = __builtin_amdgcn_exp2f(x.x - from);
+            l = fmaf(weight, x.y, l);
+            o += weight * y;
+        }
     }
-    sums[p][lane] = o;
-    if (lane == 0) weights[p] = l;
-    __syncthreads();
-    if (p) return;
+    if constexpr (PARTS > 1) {
+        sums[p][lane] = o;
+        if (lane == 0) weights[p] = l;
+        __syncthreads();
+        if (p) return;
 #pragma unroll
-    for (int x = 1; x < PARTS; ++x) {
-        o += sums[x][lane];
-        l += weights[x];
+        for (int x = 1; x < PARTS; ++x) {
+            o += sums[x][lane];
+            l += weights[x];
+        }
     }
-    store_row<VEC>(a, b, kv, rb * RB + row, d, o, l);
+    if (mine) store_row<VEC>(a, b, kv, rb * RB + row, d, o, l);
 }
 
 // Rows per block.
@@ -420,9 +426,16 @@ uint32_t runs_of(const RaggedShape &s) {
 
 template <int DP, int RB, int TILE, bool VEC>
 void launch_join(hipStream_t stream, const RaggedArgs &a) {
-    const uint32_t rows = a.group * a.queries, units = a.batch * a.kv_heads * a.row_blocks;
-    const dim3 grid(units < a.runs ? units : a.runs, rows < RB ? rows : RB);
-    hipLaunchKernelGGL((attention_ragged_join<DP, RB, TILE, VEC>), grid, dim3(kThreads), 0, stream, a);
+    constexpr uint32_t kRowsOf = kThreads / (DP / 4);  // rows of a block
+    const uint32_t units = a.batch * a.kv_heads * a.row_blocks, all = a.group * a.queries, rows = all < RB ? all : RB;
+    const uint32_t x = units < a.runs ? units : a.runs;
+    // Units of 16 runs or so: their slots are shared out (4 nodes over 131072 keys, 64 runs a
+    // unit: 15 us otherwise, 8 so); else whole rows (64 nodes x 4 sequences: 14 us shared, 6).
+    if (16 * units <= a.runs)
+        hipLaunchKernelGGL((attention_ragged_join<DP, RB, TILE, 1, VEC>), dim3(x, rows), dim3(kThreads), 0, stream, a);
+    else
+        hipLaunchKernelGGL((attention_ragged_join<DP, RB, TILE, kRowsOf, VEC>), dim3(x, (rows + kRowsOf - 1) / kRowsOf),
+                           dim3(kThreads), 0, stream, a);
 }
 
 template <int DP, int QT, int RG, bool VEC>

@@ -110,7 +110,7 @@ struct CacheAppendArgs {
     uint32_t batch, kv_heads, rows, picks_count, capacity, dim;
     bool token_major;
 };
-LaunchShape cache_append_shape(uint32_t batch, uint32_t kv_heads, uint32_t picks);
+LaunchShape cache_append_shape(uint32_t batch, uint32_t kv_heads, uint32_t picks, uint32_t dim, bool token_major);
 hipError_t cache_append_f32(hipStream_t stream, const CacheAppendArgs &args);
 
 // Attention of `queries` rows per head over keys of `lengths` [batch], with grouped

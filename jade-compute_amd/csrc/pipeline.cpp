@@ -42,7 +42,7 @@ hipk::LaunchShape launch_shape(const KernelSpec &s) {
         case Op::Softmax: return softmax_shape(s.rows, s.cols);
         case Op::Rotary: return rotary_shape(s.batch * s.seq, s.heads, s.dim, s.rotary_dim, false);
         case Op::QkNormRotary: return rotary_shape(s.batch * s.seq, s.heads + s.kv_heads, s.dim, s.rotary_dim, true);
-        case Op::CacheAppend: return cache_append_shape(s.batch, s.kv_heads, s.picks);
+        case Op::CacheAppend: return cache_append_shape(s.batch, s.kv_heads, s.picks, s.dim, s.token_major);
         case Op::AttentionTree:
         case Op::AttentionCross: return attention_ragged_shape(ragged_shape(s));
         case Op::GemmMps: break;

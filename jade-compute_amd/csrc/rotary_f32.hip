@@ -56,29 +56,39 @@ __device__ inline Head head_of(const RotaryArgs &a, uint32_t b, uint32_t s, uint
             (second ? a.out2 : a.out) + head_at(a, a.out_token_major, heads, b, s, at)};
 }
 
-// Heads whose rows take whole float4s: LANES lanes (a power of two) share a head,
-// a lane with eight of its dims: four pairs, or eight dims that are not turned.
-// A wave keeps one token's angles and goes over `per_wave` groups of 64 / LANES
-// heads.
-template <int LANES, bool NORM>
+// Rows that take whole vectors of W floats: LANES lanes (a power of two) share a head,
+// a lane with two vectors of it: W pairs, or 2 W dims that are not turned, each vector
+// beside its neighbour lane's. A wave keeps one token's angles and goes over `per_wave`
+// groups of 64 / LANES heads.
+//
+// Bound by memory: 4 x 4096 tokens of 32 heads of 128, interleaved, 537 MB in 92.8 us (5.8
+// TB/s; 110.9 with a lane's two float4s side by side and ordinary loads and stores).
+template <int LANES, int W, bool NORM>
 __global__ __launch_bounds__(kThreads) void rotary_lanes(RotaryArgs a, uint32_t per_wave, uint32_t spans,
                                                          uint32_t items) {
-    const int lane = threadIdx.x & 63, unit = lane % LANES;
-    const uint32_t all = a.heads + a.heads2, turned = a.rotary_dim / 8;
-    const bool mine = uint32_t(unit) < a.dim / 8, turns = uint32_t(unit) < turned;
-    const uint32_t d0 = a.interleaved || !turns ? 8 * unit : 4 * unit;
-    const uint32_t d1 = a.interleaved || !turns ? d0 + 4 : d0 + a.rotary_dim / 2;
+    typedef float vec __attribute__((ext_vector_type(W)));
+    constexpr int kHalf = W > 1 ? W / 2 : 1;
+    const int lane = threadIdx.x & 63;
+    const uint32_t unit = lane % LANES, all = a.heads + a.heads2, turned = a.rotary_dim / (2 * W);
+    const bool mine = unit < a.dim / (2 * W), turns = unit < turned;
+    // Half of the turned dims, or of the others, lies between a lane's two vectors; single
+    // floats of an interleaved pair are neighbours.
+    const bool near = W == 1 && a.interleaved;
+    const uint32_t d0 = turns ? (near ? 2 * unit : W * unit) : a.rotary_dim + W * (unit - turned);
+    const uint32_t d1 = turns && near ? d0 + 1 : d0 + (turns ? a.rotary_dim : a.dim - a.rotary_dim) / 2;
     for (uint32_t item = blockIdx.x * (kThreads / 64) + (threadIdx.x >> 6); item < items;
          item += gridDim.x * (kThreads / 64)) {
         const uint32_t token = item / spans, h0 = item % spans * per_wave * (64 / LANES);
         const uint32_t b = token / a.seq, s = token % a.seq;
-        f32x4 c = {1.f, 1.f, 1.f, 1.f}, sn = {0.f, 0.f, 0.f, 0.f};
+        float c[W], sn[W];
         if (turns) {
             const double position = a.positions[token];
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
+            for (int e = 0; e < W; ++e) {
                 float cosine, sine;
-                turn(position * a.rates[4 * unit + e], cosine, sine);
+                // The lane's pairs: of halves W unit + e, else half of them in each vector.
+                const uint32_t pair = W > 1 && a.interleaved ? kHalf * unit + e % kHalf + e / kHalf * (a.rotary_dim / 4) : W * unit + e;
+                turn(position * a.rates[pair], cosine, sine);
                 c[e] = cosine * a.magnitude;
                 sn[e] = a.inverse ? -sine * a.magnitude : sine * a.magnitude;
             }
@@ -88,41 +98,48 @@ __global__ __launch_bounds__(kThreads) void rotary_lanes(RotaryArgs a, uint32_t 
             const bool live = h < all && mine;
             if (!NORM && !live) continue;
             const Head head = head_of(a, b, s, h < all ? h : 0);
-            f32x4 x0 = {0.f, 0.f, 0.f, 0.f}, x1 = x0;
+            vec x0 = 0.f, x1 = 0.f;
             if (live) {
-                x0 = *reinterpret_cast<const f32x4 *>(head.x + d0);
-                x1 = *reinterpret_cast<const f32x4 *>(head.x + d1);
+                x0 = __builtin_nontemporal_load(reinterpret_cast<const vec *>(head.x + d0));
+                x1 = __builtin_nontemporal_load(reinterpret_cast<const vec *>(head.x + d1));
             }
             if constexpr (NORM) {
                 float sum = 0.f;
 #pragma unroll
-                for (int e = 0; e < 4; ++e) sum = fmaf(x0[e], x0[e], fmaf(x1[e], x1[e], sum));
+                for (int e = 0; e < W; ++e) sum = fmaf(x0[e], x0[e], fmaf(x1[e], x1[e], sum));
 #pragma unroll
                 for (int offset = LANES / 2; offset > 0; offset >>= 1) sum += __shfl_xor(sum, offset);
-                if (!live) continue;
                 const float inv = rsqrtf(sum / float(a.dim) + a.epsilon);
-                x0 = x0 * inv * *reinterpret_cast<const f32x4 *>(head.weight + d0);
-                x1 = x1 * inv * *reinterpret_cast<const f32x4 *>(head.weight + d1);
+                if (!live) continue;
+                x0 = x0 * inv * *reinterpret_cast<const vec *>(head.weight + d0);
+                x1 = x1 * inv * *reinterpret_cast<const vec *>(head.weight + d1);
             }
-            f32x4 y0 = x0, y1 = x1;
+            vec y0 = x0, y1 = x1;
             if (turns) {
-                if (a.interleaved) {
-                    y0 = {x0.x * c.x - x0.y * sn.x, x0.y * c.x + x0.x * sn.x, x0.z * c.y - x0.w * sn.y,
-                          x0.w * c.y + x0.z * sn.y};
-                    y1 = {x1.x * c.z - x1.y * sn.z, x1.y * c.z + x1.x * sn.z, x1.z * c.w - x1.w * sn.w,
-                          x1.w * c.w + x1.z * sn.w};
+                if (W > 1 && a.interleaved) {
+#pragma unroll
+                    for (int e = 0; e < W / 2; ++e) {
+                        y0[2 * e] = x0[2 * e] * c[e] - x0[2 * e + 1] * sn[e];
+                        y0[2 * e + 1] = x0[2 * e + 1] * c[e] + x0[2 * e] * sn[e];
+                        y1[2 * e] = x1[2 * e] * c[W / 2 + e] - x1[2 * e + 1] * sn[W / 2 + e];
+                        y1[2 * e + 1] = x1[2 * e + 1] * c[W / 2 + e] + x1[2 * e] * sn[W / 2 + e];
+                    }
                 } else {
-                    y0 = x0 * c - x1 * sn;
-                    y1 = x1 * c + x0 * sn;
+#pragma unroll
+                    for (int e = 0; e < W; ++e) {
+                        y0[e] = x0[e] * c[e] - x1[e] * sn[e];
+                        y1[e] = x1[e] * c[e] + x0[e] * sn[e];
+                    }
                 }
             }
-            *reinterpret_cast<f32x4 *>(head.out + d0) = y0;
-            *reinterpret_cast<f32x4 *>(head.out + d1) = y1;
+            __builtin_nontemporal_store(y0, reinterpret_cast<vec *>(head.out + d0));
+            __builtin_nontemporal_store(y1, reinterpret_cast<vec *>(head.out + d1));
         }
     }
 }
 
-// Any other head: one wave a head, pairs and single dims in turn.
+// Odd head dims, and even ones too long for the lanes: one wave a head, pairs and single
+// dims in turn.
 template <bool NORM>
 __global__ __launch_bounds__(kThreads) void rotary_any(RotaryArgs a, uint32_t per_wave, uint32_t spans,
                                                        uint32_t items) {
@@ -170,50 +187,68 @@ __global__ __launch_bounds__(kThreads) void rotary_any(RotaryArgs a, uint32_t pe
     }
 }
 
-// Lanes per head of rotary_lanes; 0 for rotary_any: parts of a head that are no
-// multiple of eight dims.
-uint32_t lanes_of(uint32_t dim, uint32_t rotary_dim) {
-    if (dim % 8 || rotary_dim % 8) return 0;
-    uint32_t lanes = 4;
-    while (lanes < dim / 8) lanes *= 2;
-    return lanes;
+// How rotary_lanes takes a head: the widest vectors of which half the turned dims and half
+// the others are whole numbers, and lanes per head; 0 lanes for rotary_any.
+struct Lanes {
+    uint32_t lanes, width;
+};
+Lanes lanes_of(uint32_t dim, uint32_t rotary_dim, bool aligned) {
+    for (uint32_t width = aligned ? 4 : 1; width; width /= 2) {
+        if (dim % (2 * width) || rotary_dim % (2 * width)) continue;
+        const uint32_t units = dim / (2 * width);
+        return {units <= 8 ? 8u : units <= 16 ? 16u : units <= 32 ? 32u : units <= 64 ? 64u : 0u, width};
+    }
+    return {0, 1};
 }
 
 struct Split {
     uint32_t per_wave, spans, items, blocks;  // head groups a wave takes, waves per token, waves, blocks
 };
-// Waves with several groups of heads share their angles, as long as the chip has its
-// waves (2048 of them are one for each SIMD twice).
+// Waves with several groups of heads share their angles, as long as the chip has all the
+// waves it holds (1531 tokens of 24 heads of 80: 10.0 us where 2048 were enough, 9.2 so).
+// The next head loaded ahead of this one's stores: 117.5 -> 115.0 with a norm, but 93 ->
+// 94 without and 90 -> 108 for heads of 66 in single floats; not kept.
+constexpr uint32_t kLeastWaves = 8192;
 Split split_of(uint32_t tokens, uint32_t heads, uint32_t lanes) {
     const uint32_t groups = lanes ? (heads + 64 / lanes - 1) / (64 / lanes) : heads;
     uint32_t per_wave = 1;
-    while (per_wave < 8 && per_wave < groups && uint64_t(tokens) * ((groups + 2 * per_wave - 1) / (2 * per_wave)) >= 2048)
+    while (per_wave < 8 && per_wave < groups && uint64_t(tokens) * ((groups + 2 * per_wave - 1) / (2 * per_wave)) >= kLeastWaves)
         per_wave *= 2;
     const uint32_t spans = (groups + per_wave - 1) / per_wave, items = tokens * spans;
     const uint32_t blocks = (items + kThreads / 64 - 1) / (kThreads / 64);
     return {per_wave, spans, items, blocks < kMaxBlocks ? blocks : kMaxBlocks};
 }
 
-template <bool NORM>
-hipError_t launch(hipStream_t stream, const RotaryArgs &a, bool aligned) {
-    const uint32_t lanes = aligned ? lanes_of(a.dim, a.rotary_dim) : 0;
-    const Split p = split_of(a.batch * a.seq, a.heads + a.heads2, lanes);
+template <int W, bool NORM>
+void launch_lanes(hipStream_t stream, const RotaryArgs &a, uint32_t lanes, Split p) {
     const dim3 grid(p.blocks), block(kThreads);
     switch (lanes) {
-        case 0: hipLaunchKernelGGL((rotary_any<NORM>), grid, block, 0, stream, a, p.per_wave, p.spans, p.items); break;
-        case 4: hipLaunchKernelGGL((rotary_lanes<4, NORM>), grid, block, 0, stream, a, p.per_wave, p.spans, p.items); break;
-        case 8: hipLaunchKernelGGL((rotary_lanes<8, NORM>), grid, block, 0, stream, a, p.per_wave, p.spans, p.items); break;
-        case 16: hipLaunchKernelGGL((rotary_lanes<16, NORM>), grid, block, 0, stream, a, p.per_wave, p.spans, p.items); break;
-        case 32: hipLaunchKernelGGL((rotary_lanes<32, NORM>), grid, block, 0, stream, a, p.per_wave, p.spans, p.items); break;
-        default: hipLaunchKernelGGL((rotary_lanes<64, NORM>), grid, block, 0, stream, a, p.per_wave, p.spans, p.items); break;
+        case 8: hipLaunchKernelGGL((rotary_lanes<8, W, NORM>), grid, block, 0, stream, a, p.per_wave, p.spans, p.items); break;
+        case 16: hipLaunchKernelGGL((rotary_lanes<16, W, NORM>), grid, block, 0, stream, a, p.per_wave, p.spans, p.items); break;
+        case 32: hipLaunchKernelGGL((rotary_lanes<32, W, NORM>), grid, block, 0, stream, a, p.per_wave, p.spans, p.items); break;
+        default: hipLaunchKernelGGL((rotary_lanes<64, W, NORM>), grid, block, 0, stream, a, p.per_wave, p.spans, p.items); break;
     }
+}
+
+template <bool NORM>
+hipError_t launch(hipStream_t stream, const RotaryArgs &a, bool aligned) {
+    const Lanes l = lanes_of(a.dim, a.rotary_dim, aligned);
+    const Split p = split_of(a.batch * a.seq, a.heads + a.heads2, l.lanes);
+    if (!l.lanes)
+        hipLaunchKernelGGL((rotary_any<NORM>), dim3(p.blocks), dim3(kThreads), 0, stream, a, p.per_wave, p.spans, p.items);
+    else if (l.width == 4)
+        launch_lanes<4, NORM>(stream, a, l.lanes, p);
+    else if (l.width == 2)
+        launch_lanes<2, NORM>(stream, a, l.lanes, p);
+    else
+        launch_lanes<1, NORM>(stream, a, l.lanes, p);
     return hipGetLastError();
 }
 
 }  // namespace
 
 LaunchShape rotary_shape(uint32_t tokens, uint32_t heads, uint32_t dim, uint32_t rotary_dim, bool norm) {
-    const uint32_t lanes = lanes_of(dim, rotary_dim);
+    const uint32_t lanes = lanes_of(dim, rotary_dim, true).lanes;
     static const char *const names[2][2] = {{"rotary_any", "rotary_lanes"}, {"qk_norm_rotary_any", "qk_norm_rotary_lanes"}};
     return {names[norm][lanes != 0], {split_of(tokens, heads, lanes).blocks, 1, 1}, {kThreads, 1, 1}, 0};
 }
