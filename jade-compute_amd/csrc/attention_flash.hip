@@ -36,7 +36,9 @@
 // the way the bits that a K below 2^-78 loses move no score by more than 2^-38
 // a dim. Weights below 2^-100 of the reference weight keep fewer than 24 bits.
 #include "attention_flash.hpp"
+#include "attention_ragged.hpp"
 #include "split_bf16.hpp"
+#include "whole.hpp"
 
 namespace jade {
 namespace hipk {
@@ -100,11 +102,16 @@ struct Shape {
 };
 }  // namespace flash
 
-template <int DP, int NW, bool CAUSAL>
+// What a launch over [heads, seq, dim] of itself adds: nothing. With RaggedArgs the
+// rows are a (sequence, kv head)'s heads and queries and the keys another tensor's.
+struct Whole {};
+
+template <int DP, int NW, bool CAUSAL, class More = Whole>
 __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(DP <= 64 || NW == 8 ? 2 : 1, DP <= 64 || NW == 8 ? 2 : 1))) void
 attention_flash(const float *__restrict__ Q, const float *__restrict__ K, const float *__restrict__ V,
-                float *__restrict__ O, int seq, int dim, float qscale) {
+                float *__restrict__ O, int seq, int dim, float qscale, More more) {
     using namespace flash;
+    constexpr bool kRagged = !std::is_same<More, Whole>::value;
     using S = Shape<DP, NW>;
     constexpr int KS = S::kSteps, NB = S::kBlocks, WIDE = S::kWide, CH = S::kChunks, VROWS = 4 * CH;
     __shared__ __attribute__((aligned(1024))) char lds[S::kLdsBytes];
@@ -113,22 +120,45 @@ attention_flash(const float *__restrict__ Q, const float *__restrict__ K, const 
     constexpr int kBQ = 32 * NW;
     int head, qb;
     block_of(int(blockIdx.x) + int(gridDim.x) * int(blockIdx.y), int(gridDim.x), int(gridDim.y), head, qb);
-    const size_t base = size_t(head) * size_t(seq) * size_t(dim);
     const int q0 = qb * kBQ + wave * 32, qi = q0 + c;
-    const int t_end = ((CAUSAL ? min(seq, qb * kBQ + kBQ) : seq) + kKeys - 1) / kKeys;
+    // Ragged: `seq` rows of q and out at qoff (bytes of row qi) from qbase, `keys` rows of k and
+    // v, row_bytes apart, from base.
+    int keys = seq;
+    size_t base, qbase;
+    uint32_t row_bytes = uint32_t(dim) * 4u, qoff = uint32_t(qi) * row_bytes, head_bytes, q_bytes;
+    if constexpr (kRagged) {
+        const uint32_t b = uint32_t(head) / more.kv_heads, kv = uint32_t(head) - b * more.kv_heads;
+        keys = int(__builtin_amdgcn_readfirstlane(whole_below(more.lengths[b], more.keys)));
+        base = size_t(b) * more.k_batch + size_t(kv) * more.k_head;
+        qbase = size_t(b) * more.q_batch + size_t(kv) * more.group * more.q_head;
+        row_bytes = more.k_row * 4u;
+        const uint32_t member = uint32_t(qi) / more.queries, query = uint32_t(qi) - member * more.queries;
+        qoff = uint32_t(member * more.q_head + query * more.q_row) * 4u;
+        q_bytes = uint32_t((more.group - 1) * more.q_head + size_t(more.queries - 1) * more.q_row + dim) * 4u;
+        head_bytes = uint32_t(keys - 1) * row_bytes + uint32_t(dim) * 4u;
+        if (!keys) {  // rows without a key are zeros
+            if (qi < seq)
+                for (int d = 4 * h; d < dim; d += 8)
+                    *reinterpret_cast<f32x4 *>(reinterpret_cast<char *>(O + qbase + d) + qoff) = f32x4{0.f, 0.f, 0.f, 0.f};
+            return;
+        }
+    } else {
+        base = qbase = size_t(head) * size_t(seq) * size_t(dim);
+        head_bytes = q_bytes = uint32_t(seq) * row_bytes;
+    }
+    const int t_end = ((CAUSAL ? min(seq, qb * kBQ + kBQ) : keys) + kKeys - 1) / kKeys;
 
-    const uint32_t head_bytes = uint32_t(seq) * uint32_t(dim) * 4u, row_bytes = uint32_t(dim) * 4u;
     // Q^T operand: step s holds dims 16s + 8h + e of query qi, in log2 units.
     // Rows past seq and dims past dim read zero.
     const __amdgpu_buffer_rsrc_t rq =
-        __builtin_amdgcn_make_buffer_rsrc(const_cast<float *>(Q + base), 0, int(head_bytes), int(kRawBuffer));
+        __builtin_amdgcn_make_buffer_rsrc(const_cast<float *>(Q + qbase), 0, int(q_bytes), int(kRawBuffer));
     f32x4 qraw[KS][2];
 #pragma unroll
     for (int s = 0; s < KS; ++s)
 #pragma unroll
         for (int x = 0; x < 2; ++x) {
             const int d = 16 * s + 8 * h + 4 * x;
-            const uint32_t at = qi < seq && d < dim ? uint32_t(qi) * row_bytes + uint32_t(d) * 4u : kDeadOffset;
+            const uint32_t at = qi < seq && d < dim ? qoff + uint32_t(d) * 4u : kDeadOffset;
             qraw[s][x] = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(rq, int(at), 0, 0));
         }
     bf16x8 qp[KS][kParts];
@@ -263,11 +293,11 @@ attention_flash(const float *__restrict__ Q, const float *__restrict__ K, const 
     f32x16 st;  // scores, then probabilities, of the tile being weighted
     auto mask = [&](int t, f32x16 &s) {
         const int kt = t * kKeys;
-        if (kt + kKeys <= seq && (!CAUSAL || kt + kKeys - 1 <= q0)) return;  // wave-uniform
+        if (kt + kKeys <= keys && (!CAUSAL || kt + kKeys - 1 <= q0)) return;  // wave-uniform
 #pragma unroll
         for (int v = 0; v < 16; ++v) {
             const int key = kt + 8 * (v >> 2) + 4 * h + (v & 3);
-            if (key >= seq || (CAUSAL && key > qi)) s[v] = -INFINITY;
+            if (key >= keys || (CAUSAL && key > qi)) s[v] = -INFINITY;
         }
     };
 
@@ -619,16 +649,17 @@ attention_flash(const float *__restrict__ Q, const float *__restrict__ K, const 
 #pragma unroll
         for (int b = 0; b < NB; ++b) acc[b] = f32x16{};
         const bool mine = qi < seq;
-        const float *qrow = Q + base + size_t(mine ? qi : 0) * dim;
+        const float *qrow = reinterpret_cast<const float *>(reinterpret_cast<const char *>(Q + qbase) + (mine ? qoff : 0u));
+        const size_t pitch = row_bytes / 4u;
         for (int t = 0; t < t_end && live(t); ++t) {
             const int key = t * kKeys + c;
-            const float *krow = K + base + size_t(min(key, seq - 1)) * dim;
+            const float *krow = K + base + size_t(min(key, keys - 1)) * pitch;
             st = f32x16{};
             for (int d0 = 0; d0 < DP; d0 += 8) {
                 const int d = d0 + 4 * h;
                 f32x4 a = {0.f, 0.f, 0.f, 0.f}, b = {0.f, 0.f, 0.f, 0.f};
                 if (d < dim) {
-                    if (key < seq) a = *reinterpret_cast<const f32x4 *>(krow + d);
+                    if (key < keys) a = *reinterpret_cast<const f32x4 *>(krow + d);
                     if (mine) b = *reinterpret_cast<const f32x4 *>(qrow + d);
                 }
 #pragma unroll
@@ -655,11 +686,11 @@ attention_flash(const float *__restrict__ Q, const float *__restrict__ K, const 
 #pragma unroll
             for (int v = 0; v < 16; ++v) {
                 const int k = t * kKeys + 8 * (v >> 2) + 4 * h + (v & 3);
-                const float *vr = V + base + size_t(min(k, seq - 1)) * dim;
+                const float *vr = V + base + size_t(min(k, keys - 1)) * pitch;
 #pragma unroll
                 for (int b = 0; b < NB; ++b) {
                     const int r = 32 * b + c, d = r < DP / 2 ? 2 * r : 2 * r - DP + 1;
-                    const float x = k < seq && d < dim ? vr[d] : 0.f;
+                    const float x = k < keys && d < dim ? vr[d] : 0.f;
                     acc[b] = __builtin_amdgcn_mfma_f32_32x32x2f32(x, st[v], acc[b], 0, 0, 0);
                 }
             }
@@ -669,7 +700,7 @@ attention_flash(const float *__restrict__ Q, const float *__restrict__ K, const 
     row_sum = halves_sum(row_sum);
     if (qi < seq) {
         const float inv = unscale / row_sum;
-        float *orow = O + base + size_t(qi) * dim;
+        float *orow = reinterpret_cast<float *>(reinterpret_cast<char *>(O + qbase) + qoff);
         // LDS row r of V is dim 2r (r < DP / 2) or 2 (r - DP / 2) + 1, and a
         // lane holds rows 32b + 8 (v >> 2) + 4h + (v & 3): r, r + 1 and their
         // odd partners are four adjacent dims.
@@ -693,10 +724,19 @@ hipError_t launch(hipStream_t stream, const FlashArgs &a) {
     const dim3 grid(a.heads, (a.seq + bq - 1) / bq), block(64 * NW);
     if (a.causal)
         hipLaunchKernelGGL((attention_flash<DP, NW, true>), grid, block, 0, stream, a.q, a.k, a.v, a.out, int(a.seq),
-                           int(a.dim), a.qscale);
+                           int(a.dim), a.qscale, Whole{});
     else
         hipLaunchKernelGGL((attention_flash<DP, NW, false>), grid, block, 0, stream, a.q, a.k, a.v, a.out, int(a.seq),
-                           int(a.dim), a.qscale);
+                           int(a.dim), a.qscale, Whole{});
+    return hipGetLastError();
+}
+
+template <int DP, int NW>
+hipError_t launch_ragged(hipStream_t stream, const RaggedArgs &a) {
+    const uint32_t rows = a.group * a.queries;
+    const dim3 grid(a.batch * a.kv_heads, (rows + 32 * NW - 1) / (32 * NW));
+    hipLaunchKernelGGL((attention_flash<DP, NW, false, RaggedArgs>), grid, dim3(64 * NW), 0, stream, a.q, a.k, a.v, a.out,
+                       int(rows), int(a.dim), a.qscale, a);
     return hipGetLastError();
 }
 
@@ -714,6 +754,14 @@ uint32_t attention_flash_lds_bytes(uint32_t dim, int waves) {
     if (dim <= 64) return Shape<64, 4>::kLdsBytes;
     if (waves != 8) return Shape<128, 4>::kLdsBytes;
     return dim <= 96 ? Shape<96, 8>::kLdsBytes : Shape<128, 8>::kLdsBytes;
+}
+
+hipError_t launch_flash_ragged(hipStream_t stream, const RaggedArgs &a) {
+    if (a.dim % 4 != 0 || a.dim > 128) return hipErrorInvalidValue;
+    if (a.dim <= 32) return launch_ragged<32, 4>(stream, a);
+    if (a.dim <= 64) return launch_ragged<64, 4>(stream, a);
+    if (a.dim <= 96) return launch_ragged<96, 8>(stream, a);
+    return launch_ragged<128, 8>(stream, a);
 }
 
 hipError_t launch_attention_flash(hipStream_t stream, const FlashArgs &a) {

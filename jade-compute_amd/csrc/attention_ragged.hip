@@ -22,6 +22,7 @@
 // attention_ragged_join. So neither long sequences nor ragged ones leave CUs idle.
 #include <cmath>
 
+#include "attention_flash.hpp"
 #include "kernels.hpp"
 #include "ragged_device.hpp"
 
@@ -416,6 +417,28 @@ uint64_t ragged_tiles(const RaggedShape &s) {
     return uint64_t(s.batch) * s.kv_heads * row_blocks(s) * tiles;
 }
 
+// Queries of an encoder's states may go to the flash kernel (attention_flash.hip), which
+// splits K and V once for 128 or 256 rows but has one block for them and all their keys.
+// Both are estimated, in us, from what they measured: the flash kernel 8 and, for every 256
+// blocks, 1.7 (dims to 64), 3.6 (to 96) or 4.6 for 32 keys of full blocks, 0.35 of that for
+// empty ones; the kernel on parts 2.8 (to 64) or 5.9 for 128 keys, 8 or 11 for each unit a
+// run begins, and 3 for the join. Measured, flash and parts: 4 x 32 heads (8 of keys) x 1000
+// queries x 4096 keys of 128 1179 and 1385 us; 32 x 16 x 200 x 100 of 128 48 and 129; 32 x
+// 16 x 80 x 128 of 64 21 and 43; 16 x 3000 x 1500 of 128 198 and 220; 4 x 32 x 256 x 2048
+// of 128 256 and 221; 16 x 1500 x 1500 of 64 82 and 71; 4 x 8 x 256 x 1024 of 128 131 and 40.
+bool on_flash(const RaggedShape &s) {
+    const uint64_t d = s.dim, heads = uint64_t(s.batch) * s.kv_heads, rows = rows_of(s), fb = flash_ragged_rows(s.dim);
+    const uint64_t q_span = s.token_major ? d * s.heads * s.queries : d * rows, k_span = (s.token_major ? d * s.kv_heads : d) * s.keys;
+    if (!on_parts(s) || s.nodes || q_span >= 1u << 29 || k_span >= 1u << 29) return false;
+    const uint64_t blocks = heads * ((rows + fb - 1) / fb), units = heads * row_blocks(s);
+    const double full = double(rows) / double((rows + fb - 1) / fb * fb);
+    const double flash = 8.0 + double((blocks + kCus - 1) / kCus) * double((s.keys + 31) / 32) *
+                                   (d <= 64 ? 1.7 : d <= 96 ? 3.6 : 4.6) * (0.35 + 0.65 * full);
+    const double parts = 3.0 + double((ragged_tiles(s) + kCus - 1) / kCus) * (d <= 64 ? 2.8 : 5.9) +
+                         double((units + kCus - 1) / kCus) * (d <= 64 ? 8.0 : 11.0);
+    return flash < parts;
+}
+
 // Runs of a launch: as many blocks as the chip holds at once (one a CU of 64 rows or
 // on parts, else two), or one per tile where there can be no more tiles.
 uint32_t runs_of(const RaggedShape &s) {
@@ -463,6 +486,13 @@ hipError_t launch_rows(hipStream_t stream, const RaggedArgs &a, bool parts) {
 }  // namespace
 
 LaunchShape attention_ragged_shape(const RaggedShape &s) {
+    if (on_flash(s)) {
+        static const char *const names[4] = {"attention_flash_ragged_d32", "attention_flash_ragged_d64",
+                                             "attention_flash_ragged_d96", "attention_flash_ragged_d128"};
+        const uint32_t rb = flash_ragged_rows(s.dim);
+        return {names[(s.dim - 1) / 32], {s.batch * s.kv_heads, (rows_of(s) + rb - 1) / rb, 1}, {2 * rb, 1, 1},
+                attention_flash_lds_bytes(s.dim, int(rb / 32))};
+    }
     // Tiles are counted in 32 bits.
     if (ragged_tiles(s) > 0x7fffffffull) return {nullptr, {0, 0, 0}, {0, 0, 0}, 0};
     const bool wide = s.dim > 64;
@@ -478,12 +508,12 @@ LaunchShape attention_ragged_shape(const RaggedShape &s) {
 }
 
 size_t attention_ragged_workspace_bytes(const RaggedShape &s) {
+    if (on_flash(s)) return 0;
     const size_t rb = block_rows(rows_of(s)), dp = s.dim > 64 ? 128 : 64;
     return 2 * size_t(runs_of(s)) * rb * (dp + 2) * sizeof(float);
 }
 
 hipError_t attention_ragged_f32(hipStream_t stream, const RaggedShape &s, const RaggedBuffers &x, float *workspace) {
-    if (!workspace) return hipErrorInvalidValue;
     RaggedArgs a{};
     a.q = x.q; a.k = x.k; a.v = x.v; a.lengths = x.lengths; a.kd = x.k_draft; a.vd = x.v_draft; a.parents = x.parents;
     a.out = x.out;
@@ -506,6 +536,8 @@ hipError_t attention_ragged_f32(hipStream_t stream, const RaggedShape &s, const 
     for (const float *y : {x.q, x.k, x.v, x.k_draft, x.v_draft, const_cast<const float *>(x.out)})
         bits |= reinterpret_cast<uintptr_t>(y);
     if (s.dim % 4 == 0 && bits & 15u) return hipErrorInvalidValue;  // the runtime's regions are aligned
+    if (on_flash(s)) return launch_flash_ragged(stream, a);
+    if (!workspace) return hipErrorInvalidValue;
     return s.dim <= 64 ? launch_rows<64>(stream, a, on_parts(s)) : launch_rows<128>(stream, a, on_parts(s));
 }
 
