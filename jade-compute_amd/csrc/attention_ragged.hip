@@ -82,7 +82,7 @@ attention_ragged(RaggedArgs a) {
         }
 
     while (t < t_stop) {
-        const uint32_t len = uniform(whole_below(a.lengths[b], a.keys));
+        const uint32_t len = spread.length(b);
         const uint32_t cached = (len + kTile - 1) / kTile, tiles = cached + spread.draft_tiles;
         if (!tiles) {
             ++b;
@@ -326,7 +326,7 @@ template <int DP, int RB, int TILE, int ROWS, bool VEC>
 __global__ __launch_bounds__(kThreads) void attention_ragged_join(RaggedArgs a) {
     constexpr int LANES = DP / 4, PARTS = kThreads / LANES / ROWS;
     __shared__ __attribute__((aligned(16))) f32x4 sums[PARTS][LANES];
-    __shared__ float weights[PARTS];
+    __shared__ float2 weights[PARTS];
     const int tid = threadIdx.x, lane = tid % LANES, p = ROWS == 1 ? tid / LANES : 0;
     const uint32_t units = a.kv_heads * a.row_blocks, row = blockIdx.y * ROWS + (ROWS == 1 ? 0 : tid / LANES), d = 4 * lane;
     const bool by_unit = a.batch * units <= a.runs;
@@ -336,7 +336,7 @@ __global__ __launch_bounds__(kThreads) void attention_ragged_join(RaggedArgs a) 
     if (by_unit) {
         b = blockIdx.x / units;
         unit = blockIdx.x - b * units;
-        tiles = uniform(spread.tiles_at(b));
+        tiles = spread.tiles_at(b);
         start = spread.before(b) * units + unit * tiles;
     } else {
         if (!spread.draft_tiles)
@@ -349,7 +349,7 @@ __global__ __launch_bounds__(kThreads) void attention_ragged_join(RaggedArgs a) 
         uint32_t before;
         const uint32_t cut = spread.start(blockIdx.x, chunk, units, b, before);
         if (cut == 0 || cut == spread.total * units) return;
-        tiles = uniform(spread.tiles_at(b));
+        tiles = spread.tiles_at(b);
         if (!tiles) return;  // at a sequence's start
         unit = (cut - before * units) / tiles;
         start = before * units + unit * tiles;
@@ -366,34 +366,29 @@ __global__ __launch_bounds__(kThreads) void attention_ragged_join(RaggedArgs a) 
     const float2 *ml = reinterpret_cast<const float2 *>(a.partial + 2 * size_t(a.runs) * RB * DP);
     // A unit's first run had it last, the others first.
     auto slot = [&](uint32_t r) { return (2 * size_t(r) + (r == first)) * RB + row; };
-    float most = -INFINITY;
-    if (mine)
-        for (uint32_t r = first + lane; r <= last; r += LANES) most = fmaxf(most, ml[slot(r)].x);
-#pragma unroll
-    for (int step = LANES / 2; step > 0; step /= 2) most = fmaxf(most, __shfl_xor(most, step));
-    const float from = most == -INFINITY ? 0.f : most;
-    float l = 0.f;
+    float most = -INFINITY, l = 0.f;
     f32x4 o = {0.f, 0.f, 0.f, 0.f};
+    auto join = [&](float top, float sum, f32x4 outs) {
+        const float next = fmaxf(most, top), from = next == -INFINITY ? 0.f : next;
+        const float old = __builtin_amdgcn_exp2f(most - from), weight = __builtin_amdgcn_exp2f(top - from);
+        most = next;
+        l = l * old + sum * weight;
+        o = o * old + outs * weight;
+    };
     if (mine) {
 #pragma unroll 4
         for (uint32_t r = first + p; r <= last; r += PARTS) {
             const float2 x = ml[slot(r)];
-            const f32x4 y = *reinterpret_cast<const f32x4 *>(a.partial + slot(r) * DP + d);
-            const float weight = __builtin_amdgcn_exp2f(x.x - from);
-            l = fmaf(weight, x.y, l);
-            o += weight * y;
+            join(x.x, x.y, *reinterpret_cast<const f32x4 *>(a.partial + slot(r) * DP + d));
         }
     }
     if constexpr (PARTS > 1) {
         sums[p][lane] = o;
-        if (lane == 0) weights[p] = l;
+        if (lane == 0) weights[p] = float2{most, l};
         __syncthreads();
         if (p) return;
 #pragma unroll
-        for (int x = 1; x < PARTS; ++x) {
-            o += sums[x][lane];
-            l += weights[x];
-        }
+        for (int x = 1; x < PARTS; ++x) join(weights[x].x, weights[x].y, sums[x][lane]);
     }
     if (mine) store_row<VEC>(a, b, kv, rb * RB + row, d, o, l);
 }

@@ -111,7 +111,7 @@ attention_ragged_parts(RaggedArgs a) {
 
     const uint32_t row_bytes = a.k_row * 4u;
     while (t < t_stop) {
-        const uint32_t len = uniform(whole_below(a.lengths[b], a.keys));
+        const uint32_t len = spread.length(b);
         const uint32_t cached = (len + kTile - 1) / kTile, tiles = cached + spread.draft_tiles;
         if (!tiles) {
             ++b;

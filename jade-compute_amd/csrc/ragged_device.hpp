@@ -44,26 +44,36 @@ __device__ inline uint32_t scan_add(uint32_t x) {
 }
 
 // The tiles of every sequence, of one (kv head, row block) each. A lane has the
-// sequences of its number modulo 64; those of the first 64 stay in registers.
+// sequences of its number modulo 64; those of the first 64 stay in registers, so that
+// one load of the lengths is all that the first loads of keys wait for.
 template <int TILE>
 struct Spread {
     const RaggedArgs &a;
-    const uint32_t draft_tiles, own, up_to;
+    const uint32_t draft_tiles, len, own, up_to;  // of sequence (lane): length, tiles, tiles up to it
     uint32_t total;
 
-    __device__ uint32_t tiles_at(uint32_t b) const {
-        return b < a.batch ? (whole_below(a.lengths[b], a.keys) + TILE - 1) / TILE + draft_tiles : 0u;
+    __device__ uint32_t load_length(uint32_t b) const { return b < a.batch ? whole_below(a.lengths[b], a.keys) : 0u; }
+    __device__ uint32_t tiles_of(uint32_t b, uint32_t length) const {
+        return b < a.batch ? (length + TILE - 1) / TILE + draft_tiles : 0u;
     }
+    // Of one sequence, for the whole wave.
+    __device__ uint32_t length(uint32_t b) const { return b < 64 ? of_lane(len, int(b)) : uniform(load_length(b)); }
+    __device__ uint32_t tiles_at(uint32_t b) const { return tiles_of(b, length(b)); }
     __device__ explicit Spread(const RaggedArgs &args)
-        : a(args), draft_tiles((a.nodes + TILE - 1) / TILE), own(tiles_at(threadIdx.x & 63)), up_to(scan_add(own)),
-          total(of_lane(up_to, 63)) {
-        for (uint32_t b0 = 64; b0 < a.batch; b0 += 64) total += of_lane(scan_add(tiles_at(b0 + (threadIdx.x & 63))), 63);
+        : a(args), draft_tiles((a.nodes + TILE - 1) / TILE), len(load_length(threadIdx.x & 63)),
+          own(tiles_of(threadIdx.x & 63, len)), up_to(scan_add(own)), total(of_lane(up_to, 63)) {
+        for (uint32_t b0 = 64; b0 < a.batch; b0 += 64) total += of_lane(scan_add(lane_tiles(b0)), 63);
+    }
+    // This lane's tiles among the sequences from b0 on.
+    __device__ uint32_t lane_tiles(uint32_t b0) const {
+        const uint32_t b = b0 + (threadIdx.x & 63);
+        return tiles_of(b, load_length(b));
     }
     // The sequence that tile t < total belongs to, and the tiles before it.
     __device__ void find(uint32_t t, uint32_t &b, uint32_t &before) const {
         before = 0;
         uint32_t sum = up_to, mine = own;
-        for (b = 0;; b += 64, mine = tiles_at(b + (threadIdx.x & 63)), sum = scan_add(mine)) {
+        for (b = 0;; b += 64, mine = lane_tiles(b), sum = scan_add(mine)) {
             const uint64_t past = __ballot(before + sum > t);
             if (past) {
                 const int first = __builtin_ctzll(past);
@@ -78,14 +88,14 @@ struct Spread {
     // block) where a run has four or more whole ones of that sequence: then none of them
     // needs joining, and runs with neighbouring row blocks, which read the same keys, do so
     // at the same time, from their XCD's L2 (4 x 32 heads x 1000 queries x 4096 keys: 1540
-    // us with every run as long as the next, KEPT_US so). `b` and `before` as find() leaves
+    // us with every run as long as the next, 1503 so). `b` and `before` as find() leaves
     // them; at the last tile's end they say nothing.
     __device__ uint32_t start(uint32_t run, uint32_t chunk, uint32_t units, uint32_t &b, uint32_t &before) const {
         const uint64_t at = uint64_t(run) * chunk, end = uint64_t(total) * units;
         if (at >= end) return uint32_t(end);
         uint32_t t = uint32_t(at);
         find(t / units, b, before);
-        const uint32_t tiles = of_lane(tiles_at(b), 0);
+        const uint32_t tiles = tiles_at(b);
         if (!rounds(tiles, chunk)) return t;
         const uint32_t over = (t - before * units) % tiles;
         t = 2 * over < tiles ? t - over : t - over + tiles;
@@ -100,8 +110,8 @@ struct Spread {
     __device__ uint32_t before(uint32_t b) const {
         uint32_t sum = 0, last = up_to - own;
         for (uint32_t b0 = 64; b0 <= b; b0 += 64) {
-            sum += b0 == 64 ? of_lane(up_to, 63) : of_lane(scan_add(tiles_at(b0 - 64 + (threadIdx.x & 63))), 63);
-            const uint32_t mine = tiles_at(b0 + (threadIdx.x & 63));
+            sum += b0 == 64 ? of_lane(up_to, 63) : of_lane(scan_add(lane_tiles(b0 - 64)), 63);
+            const uint32_t mine = lane_tiles(b0);
             last = scan_add(mine) - mine;
         }
         return sum + of_lane(last, int(b & 63));
