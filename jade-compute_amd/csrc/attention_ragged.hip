@@ -402,9 +402,11 @@ uint32_t row_blocks(const RaggedShape &s) {
     return (rows_of(s) + rb - 1) / rb;
 }
 
-// More than 16 rows of whole float4s go to the kernel on bf16 parts; the runtime's
-// buffers are all aligned.
-bool on_parts(const RaggedShape &s) { return rows_of(s) > 16 && s.dim % 4 == 0; }
+// More than 16 rows of whole float4s go to the kernel on bf16 parts (the runtime's buffers
+// are all aligned), where a tile of 128 keys spans less than 2 GiB.
+bool on_parts(const RaggedShape &s) {
+    return rows_of(s) > 16 && s.dim % 4 == 0 && (!s.token_major || uint64_t(s.kv_heads) * s.dim < 1u << 22);
+}
 
 uint64_t ragged_tiles(const RaggedShape &s) {
     const uint32_t tile = on_parts(s) ? kPartsTile : kTile;
@@ -423,8 +425,9 @@ uint64_t ragged_tiles(const RaggedShape &s) {
 // of 128 256 and 221; 16 x 1500 x 1500 of 64 82 and 71; 4 x 8 x 256 x 1024 of 128 131 and 40.
 bool on_flash(const RaggedShape &s) {
     const uint64_t d = s.dim, heads = uint64_t(s.batch) * s.kv_heads, rows = rows_of(s), fb = flash_ragged_rows(s.dim);
-    const uint64_t q_span = s.token_major ? d * s.heads * s.queries : d * rows, k_span = (s.token_major ? d * s.kv_heads : d) * s.keys;
-    if (!on_parts(s) || s.nodes || q_span >= 1u << 29 || k_span >= 1u << 29) return false;
+    const uint64_t q_span = s.token_major ? d * s.heads * s.queries : d * rows, k_span = (s.token_major ? d * s.kv_heads : d) * (s.keys + 128ull);
+    // Offsets of a head's rows in 31 bits, tiles past the last one in 32; grid.y.
+    if (!on_parts(s) || s.nodes || q_span >= 1u << 29 || k_span >= 1u << 29 || (rows + fb - 1) / fb > 65535) return false;
     const uint64_t blocks = heads * ((rows + fb - 1) / fb), units = heads * row_blocks(s);
     const double full = double(rows) / double((rows + fb - 1) / fb * fb);
     const double flash = 8.0 + double((blocks + kCus - 1) / kCus) * double((s.keys + 31) / 32) *

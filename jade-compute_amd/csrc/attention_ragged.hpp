@@ -23,7 +23,8 @@ struct RaggedArgs {
 };
 
 // The kernel on bf16 parts (attention_ragged_parts.hip), with 32 or 64 rows a block and
-// tiles of kPartsTile keys. Needs dim % 4 == 0 and at most 128, 16-byte aligned tensors.
+// tiles of kPartsTile keys. Needs dim % 4 == 0 and at most 128, 16-byte aligned tensors and
+// k_row < 2^22.
 constexpr uint32_t kPartsTile = 128;
 void launch_ragged_parts(hipStream_t stream, const RaggedArgs &args, uint32_t block_rows);
 

@@ -104,6 +104,21 @@ def test_work_past_32_bits_of_tiles_has_no_kernel():
     assert not d["hip_supported"] and d["launch"] is None
 
 
+def test_rows_too_far_apart_for_a_kernels_offsets_take_another():
+    def kernel(**more):
+        return jade_hip.spec_describe(dict(CROSS, batch=1, heads=65535, kv_heads=65535, queries=17, keys=5, **more))["launch"]["kernel"]
+
+    # 128 keys, 65535 heads of 128 apart, span more than 2 GiB.
+    assert kernel(dim=128, token_major=True) == "attention_ragged_d128_r32"
+    assert kernel(dim=128, token_major=False) == "attention_flash_ragged_d128"
+    # 2^29 elements of one head's queries.
+    far = jade_hip.spec_describe(dict(CROSS, batch=1, heads=1, kv_heads=1, queries=2 ** 23, keys=1000, dim=64))
+    assert far["launch"]["kernel"] == "attention_ragged_parts_d64_r64"
+    # More row blocks than a grid's second dimension.
+    many = jade_hip.spec_describe(dict(CROSS, batch=1, heads=1, kv_heads=1, queries=2 ** 24, keys=1000, dim=4))
+    assert many["launch"]["kernel"] == "attention_ragged_parts_d64_r64"
+
+
 def test_caches_pass_31_bits():
     d = jade_hip.spec_describe(dict(TREE, batch=64, heads=8, kv_heads=8, capacity=131072, dim=128))
     assert d["bindings"][1]["elements"] == 64 * 8 * 131072 * 128 > 2 ** 31 and d["hip_supported"]

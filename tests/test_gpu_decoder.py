@@ -504,6 +504,75 @@ def test_attention_cross_head_dims(runtime, heads, dim, token_major):
     within(run(runtime, spec, x)["out"], *dec.cross(spec, x["q"], x["k"], x["v"], [139]))
 
 
+# (batch, heads, kv_heads, queries, keys, dim) of each kernel, more sequences than a wave scans at once among them.
+KERNELS = {"attention_ragged_d64_r16": (70, 4, 2, 3, 90, 40), "attention_ragged_d128_r16": (3, 2, 1, 8, 200, 100),
+           "attention_ragged_d64_r32": (3, 6, 2, 9, 150, 31), "attention_ragged_d64_r64": (70, 1, 1, 40, 70, 63),
+           "attention_ragged_d128_r32": (3, 1, 1, 30, 150, 101), "attention_ragged_d128_r64": (3, 2, 1, 35, 130, 127),
+           "attention_ragged_parts_d64_r32": (3, 2, 1, 12, 500, 64), "attention_ragged_parts_d64_r64": (3, 2, 1, 40, 500, 60),
+           "attention_ragged_parts_d128_r32": (3, 5, 1, 6, 400, 128), "attention_ragged_parts_d128_r64": (3, 2, 1, 33, 300, 84),
+           "attention_flash_ragged_d32": (90, 8, 4, 20, 40, 24), "attention_flash_ragged_d64": (90, 4, 4, 33, 70, 60),
+           "attention_flash_ragged_d96": (70, 10, 5, 17, 33, 84), "attention_flash_ragged_d128": (66, 8, 4, 50, 35, 116)}
+
+
+@pytest.mark.parametrize("kernel", KERNELS)
+@pytest.mark.parametrize("token_major", [False, True])
+def test_every_kernel_of_attention_cross(runtime, kernel, token_major):
+    spec = cross_spec(*KERNELS[kernel], token_major)
+    assert jade_hip.spec_describe(spec)["launch"]["kernel"] == kernel
+    rng = np.random.default_rng(40)
+    lengths = [spec["keys"], 0, 1, 32, 33][:spec["batch"]] + [int(n) for n in rng.integers(0, spec["keys"] + 1, spec["batch"])]
+    lengths = lengths[:spec["batch"]]
+    x = cross_inputs(rng, spec, lengths)
+    clean = {n: x[n].copy() for n in "kv"}
+    for b, n in enumerate(lengths):  # what lies past a length is never looked at
+        dec.by_token(x["k"], token_major)[b, n:] = np.inf
+        dec.by_token(x["v"], token_major)[b, n:] = np.nan
+    # Some of the sequences against 64 bits; all of them against a launch of each alone would say the same.
+    some = [0, 1, 2, spec["batch"] - 1]
+    got = run(runtime, spec, x, repeats=2)["out"].reshape(x["q"].shape)
+    part = dict(spec, batch=len(some))
+    want, off = dec.cross(part, x["q"][some], clean["k"][some], clean["v"][some], [lengths[b] for b in some])
+    within(got[some], want, off)
+    assert np.isfinite(got).all()
+    empty = [b for b in range(spec["batch"]) if lengths[b] == 0]
+    assert (got[empty] == 0).all() and len(empty) >= 1
+
+
+@pytest.mark.parametrize("kernel", [k for k in KERNELS if "flash" in k or "parts" in k])
+def test_what_the_parts_do_not_carry(runtime, kernel):
+    # Queries past 2^64, infinities and NaN among q, k and v: rows that do not meet them are as without them.
+    spec = cross_spec(*KERNELS[kernel])
+    rng = np.random.default_rng(41)
+    lengths = [spec["keys"]] * spec["batch"]
+    x = cross_inputs(rng, spec, lengths)
+    x["q"][0, 0, 0] *= np.float32(2.0 ** 70)
+    x["k"][0, 0] *= np.float32(2.0 ** -70)
+    want, off = dec.cross(dict(spec, batch=3), x["q"][:3], x["k"][:3], x["v"][:3], lengths)
+    x["q"][1, 0, 1, 2] = np.nan
+    x["k"][2, 0, 7, 1] = np.nan  # seen by all rows of the group
+    got = run(runtime, spec, x)["out"].reshape(x["q"].shape)
+    within(got[0], want[0], off[0])
+    assert np.isnan(got[1, 0, 1]).all()
+    rows = [n for n in range(spec["queries"]) if n != 1]
+    within(got[1, 0, rows], want[1, 0, rows], off[1, 0, rows])
+    group = spec["heads"] // spec["kv_heads"]
+    assert np.isnan(got[2, :group]).all()
+    within(got[2, group:], want[2, group:], off[2, group:]) if group < spec["heads"] else None
+
+
+@pytest.mark.parametrize("nodes,dim", [(9, 64), (40, 128), (17, 30)])
+def test_attention_tree_many_sequences(runtime, nodes, dim):
+    rng = np.random.default_rng(42)
+    spec = tree_spec(80, 2, 2, nodes, 50, dim)
+    lengths = rng.integers(0, 51, 80)
+    x = tree_inputs(rng, spec, lengths)
+    got = run(runtime, spec, x)["out"].reshape(x["q"].shape)
+    some = [0, 63, 64, 79]
+    part = {n: v[some] for n, v in x.items()}
+    want, off = tree_want(dict(spec, batch=4), part)
+    within(got[some], want, off)
+
+
 @pytest.mark.parametrize("heads,dim", [(16, 64), (20, 128), (40, 64), (40, 128), (20, 36)])
 def test_attention_cross_not_finite_among_many_rows(runtime, heads, dim):
     # One row's query, one key's value: the others' outputs are as without them.
