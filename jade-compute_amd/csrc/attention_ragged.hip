@@ -308,7 +308,7 @@ attention_ragged(RaggedArgs a) {
                         f32x4{acc[qt][j][0][i], acc[qt][j][1][i], acc[qt][j][2][i], acc[qt][j][3][i]};
         }
         __syncthreads();
-        finish<DP, RB, S::kThreads, VEC>(a, run, b, kv, rb, whole, begin == 0, part, ml, plans);
+        finish<DP, RB, S::kThreads, VEC>(a, run, b, kv, rb, whole, begin == 0, part, ml, plans, sees, 0.f);
         t += end - begin;
         if (t >= (before + tiles) * units) {
             before += tiles;

@@ -17,7 +17,8 @@
 // taken off), so every finite Q is carried exactly; parts of K below 2^-109 lose bits
 // below 2^-134, which move no score: a query is at most 2^64. What the parts do not carry
 // (sums that are not finite, queries past 2^64, outputs so small that bits of V below
-// 2^-134 count) a wave notices and does its part of the run again with FP32 MFMAs.
+// 2^-134 count) the block notices when it joins its sums, and does them again with FP32
+// MFMAs.
 #include "kernels.hpp"
 #include "ragged_device.hpp"
 #include "split_bf16.hpp"
@@ -407,21 +408,29 @@ attention_ragged_parts(RaggedArgs a) {
             __builtin_amdgcn_sched_barrier(0);
         }
 
-        // What the parts do not carry: see the file's head.
-        float odd = 0.f;
-        uint32_t least = ~0u;  // of the first rows' outputs that are not zero: 2 x their bits - 1
+        // The sums of a wave to LDS: dim NB i + e of row c for i = 8 (v >> 2) + 4 h + (v & 3).
+        auto hand_over = [&]() __attribute__((always_inline)) {
+            const int l = lane_now(), c = l & 31, h = l >> 5;
+            __syncthreads();
 #pragma unroll
-        for (int r = 0; r < QG; ++r) {
-            odd += state[r][lane].y * 0.f;
-#pragma unroll
-            for (int e = 0; e < NB; ++e)
+            for (int r = 0; r < QG; ++r) {
+                const float2 mine = state[r][lane];
+                const float all = halves_sum(mine.y);
+                if (h == 0) ml[wave][32 * r + c] = float2{mine.x, all};
 #pragma unroll
                 for (int v = 0; v < 16; ++v) {
-                    odd += acc[r][e][v] * 0.f;
-                    if (r == 0) least = min(least, (__float_as_uint(acc[r][e][v]) << 1) - 1);
+                    vec o;
+#pragma unroll
+                    for (int e = 0; e < NB; ++e) o[e] = acc[r][e][v];
+                    *reinterpret_cast<vec *>(&part[wave][32 * r + c][NB * (8 * (v >> 2) + 4 * h + (v & 3))]) = o;
                 }
-        }
-        if (far || __any(odd != 0.f || least < __float_as_uint(kLeastOut) * 2)) {
+            }
+            __syncthreads();
+        };
+        hand_over();
+        if (finish<DP, RB, S::kBlock, true>(a, run, b, kv, rb, whole, begin == 0, part, ml, plans, sees, kLeastOut)) far = 1;
+        __syncthreads();
+        if (far) {  // what the parts do not carry: see the file's head
             clear();
             const int l = lane_now(), c = l & 31, h = l >> 5;
             for (uint32_t x = begin; x < end; ++x) {
@@ -473,26 +482,9 @@ attention_ragged_parts(RaggedArgs a) {
                             }
                         }
             }
+            hand_over();
+            finish<DP, RB, S::kBlock, true>(a, run, b, kv, rb, whole, begin == 0, part, ml, plans, sees, kLeastOut);
         }
-
-        const int l = lane_now(), c = l & 31, h = l >> 5;
-        // The four waves' sums joined: dim NB i + e of row c for i = 8 (v >> 2) + 4 h + (v & 3).
-        __syncthreads();
-#pragma unroll
-        for (int r = 0; r < QG; ++r) {
-            const float2 mine = state[r][lane];
-            const float all = halves_sum(mine.y);
-            if (h == 0) ml[wave][32 * r + c] = float2{mine.x, all};
-#pragma unroll
-            for (int v = 0; v < 16; ++v) {
-                vec o;
-#pragma unroll
-                for (int e = 0; e < NB; ++e) o[e] = acc[r][e][v];
-                *reinterpret_cast<vec *>(&part[wave][32 * r + c][NB * (8 * (v >> 2) + 4 * h + (v & 3))]) = o;
-            }
-        }
-        __syncthreads();
-        finish<DP, RB, S::kBlock, true>(a, run, b, kv, rb, whole, begin == 0, part, ml, plans);
         t += end - begin;
         if (t >= (before + tiles) * units) {
             before += tiles;
