@@ -20,6 +20,13 @@
 // per block. A run that holds a whole (sequence, kv head, row block) writes its
 // outputs; one that holds part of it leaves sums and maximum in the workspace for
 // attention_ragged_join. So neither long sequences nor ragged ones leave CUs idle.
+//
+// This kernel takes up to 16 rows and is bound by reading K and V: 4 nodes x 32 heads (8 of
+// keys) over 131072 keys of 128, 1.07 GB in 187 us, 5.7 TB/s; 16 x 24 heads of one query
+// over at most 1531 keys of 80, 59 us, 4.9 TB/s; one query over 1024 keys 8.7 us, which is
+// two launches and loads that wait for one another (lengths, Q, K, the partial sums). More
+// rows go to the kernel on bf16 parts (attention_ragged_parts.hip): 64 nodes over 4
+// sequences took 169 us with FP32 MFMAs, 64 rows a block, and take 116.
 #include <cmath>
 
 #include "attention_flash.hpp"
@@ -34,29 +41,16 @@ using namespace ragged;
 
 constexpr int kTile = 64;  // keys per tile
 
-// A block's shape: QT row tiles of 16 per wave, RG groups of waves with rows of their
-// own, four waves by keys in each. One row tile keeps its Q in registers, two have
-// it in LDS (the space that the waves' sums take later).
-template <int DP, int QT, int RG>
-struct Shape {
-    static constexpr int kRows = 16 * QT * RG, kThreads = 64 * kWaves * RG, kPitch = DP + 4;
-    static constexpr bool kQInLds = QT > 1;
-};
-
-// DP: head dim padded (64, 128); VEC: rows of whole float4s, 16-byte aligned.
-template <int DP, int QT, int RG, bool VEC>
-__global__ __launch_bounds__(64 * kWaves * RG) __attribute__((amdgpu_waves_per_eu(2, 2))) void
-attention_ragged(RaggedArgs a) {
-    using S = Shape<DP, QT, RG>;
-    constexpr int KJ = DP / 16, NJ = DP / 64, RB = S::kRows, PITCH = S::kPitch;
-    __shared__ __attribute__((aligned(16))) float part[kWaves][RB][PITCH];
+// DP: head dim padded (64, 128).
+template <int DP, bool VEC>
+__global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2, 2))) void attention_ragged(RaggedArgs a) {
+    constexpr int KJ = DP / 16, NJ = DP / 64, RB = 16;
+    __shared__ __attribute__((aligned(16))) float part[kWaves][RB][DP + 4];
     __shared__ float2 ml[kWaves][RB];
     __shared__ RowPlan plans[RB];
     __shared__ uint64_t sees[kMaxTreeNodes][kWords];
     __shared__ int above[kMaxTreeNodes];
-    float (*const qs)[PITCH] = part[0];  // Q in log2 units, until the sums are joined
-    const int tid = threadIdx.x, lane = tid & 63, waves = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int wave = waves & 3, row0 = (waves >> 2) * 16 * QT;  // this wave's keys of a tile; its rows
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int m = lane & 15, g = lane >> 4;
     const uint32_t units = a.kv_heads * a.row_blocks;
     const Spread<kTile> spread(a);
@@ -81,6 +75,7 @@ attention_ragged(RaggedArgs a) {
             voff[j][i] = d < a.dim ? uint32_t(16 * wave + 4 * g + i) * row_bytes + uint32_t(d) * 4u : kDeadOffset;
         }
 
+    uint32_t tree = ~0u;  // the sequence whose tree is in LDS
     while (t < t_stop) {
         const uint32_t len = spread.length(b);
         const uint32_t cached = (len + kTile - 1) / kTile, tiles = cached + spread.draft_tiles;
@@ -93,7 +88,7 @@ attention_ragged(RaggedArgs a) {
         const uint32_t end = min(tiles, begin + (t_stop - t));
         const bool whole = begin == 0 && end == tiles;
         float above_me = 0.f;
-        if (end > cached && tid < int(a.nodes)) above_me = a.parents[size_t(b) * a.nodes + tid];
+        if (end > cached && tree != b && tid < int(a.nodes)) above_me = a.parents[size_t(b) * a.nodes + tid];
 
         const float *kb = a.k + size_t(b) * a.k_batch + size_t(kv) * a.k_head;
         const float *vb = a.v + size_t(b) * a.k_batch + size_t(kv) * a.k_head;
@@ -108,106 +103,71 @@ attention_ragged(RaggedArgs a) {
             const uint32_t bytes = x < end ? (min(left, uint32_t(kTile)) - 1) * row_bytes + uint32_t(a.dim) * 4u : 0u;
             return __builtin_amdgcn_make_buffer_rsrc(const_cast<float *>(from), 0, int(bytes), int(kRawBuffer));
         };
-        auto load = [&](__amdgpu_buffer_rsrc_t from, uint32_t at, int d) {
-            if (VEC) return __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(from, int(at), 0, 0));
-            f32x4 x;
-#pragma unroll
-            for (int e = 0; e < 4; ++e)
-                x[e] = __builtin_bit_cast(
-                    float, __builtin_amdgcn_raw_buffer_load_b32(from, int(d + e < a.dim ? at + 4u * e : kDeadOffset), 0, 0));
-            return x;
+        // A last chunk that is not whole reads into the next row, or nothing past the tile.
+        auto load = [&](__amdgpu_buffer_rsrc_t from, uint32_t at) {
+            return __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(from, int(at), 0, 0));
         };
         f32x4 kf[KJ], vf[NJ][4];
         auto load_k = [&](uint32_t x) {
             const auto from = tile_of(kb, kd, x);
 #pragma unroll
-            for (int j = 0; j < KJ; ++j) kf[j] = load(from, koff[j], 16 * j + 4 * g);
+            for (int j = 0; j < KJ; ++j) kf[j] = load(from, koff[j]);
         };
         auto load_v = [&](uint32_t x) {
             const auto from = tile_of(vb, vd, x);
 #pragma unroll
             for (int j = 0; j < NJ; ++j)
 #pragma unroll
-                for (int i = 0; i < 4; ++i) vf[j][i] = load(from, voff[j][i], 64 * j + 4 * m);
-        };
-        // Row r of the block, dims d .. d + 3, in log2 units.
-        auto load_q = [&](int r, int d) {
-            const uint32_t at = rb * RB + r, head = at / a.queries, query = at - head * a.queries;
-            const float *row = a.q + size_t(b) * a.q_batch + (size_t(kv) * a.group + head) * a.q_head + size_t(query) * a.q_row;
-            f32x4 x = {0.f, 0.f, 0.f, 0.f};
-            if (VEC) {
-                if (head < a.group && d < a.dim) x = *reinterpret_cast<const f32x4 *>(row + d);
-            } else {
-#pragma unroll
-                for (int e = 0; e < 4; ++e)
-                    if (head < a.group && d + e < a.dim) x[e] = row[d + e];
-            }
-            return x * a.qscale;
+                for (int i = 0; i < 4; ++i) vf[j][i] = load(from, voff[j][i]);
         };
         load_k(begin);
         load_v(begin);
-        // Q^T operand: row m of tile qt, dims 16 j + 4 g + e.
-        f32x4 qf[S::kQInLds ? 1 : KJ];
-        if constexpr (S::kQInLds) {
-            __syncthreads();  // the last unit's sums are read
-            for (int i = tid; i < RB * (DP / 4); i += S::kThreads)
-                *reinterpret_cast<f32x4 *>(&qs[i / (DP / 4)][i % (DP / 4) * 4]) = load_q(i / (DP / 4), i % (DP / 4) * 4);
-            __syncthreads();
-        } else {
+        // Q^T operand in log2 units: row m of the block, dims 16 j + 4 g + e.
+        const uint32_t r = rb * RB + m, head = r / a.queries, query = r - head * a.queries;
+        f32x4 qf[KJ];
+        {
+            const float *row = a.q + size_t(b) * a.q_batch + (size_t(kv) * a.group + head) * a.q_head + size_t(query) * a.q_row;
 #pragma unroll
-            for (int j = 0; j < KJ; ++j) qf[j] = load_q(row0 + m, 16 * j + 4 * g);
+            for (int j = 0; j < KJ; ++j) qf[j] = load_dims<VEC>(head < a.group ? row : nullptr, 16 * j + 4 * g, a.dim) * a.qscale;
         }
-        auto q_of = [&](int qt, int j) {
-            return S::kQInLds ? *reinterpret_cast<const f32x4 *>(&qs[row0 + 16 * qt + m][16 * j + 4 * g]) : qf[j];
-        };
 
-        f32x4 acc[QT][NJ][4];
-        float top[QT], sum[QT];
+        f32x4 acc[NJ][4];
+        float top = -INFINITY, sum = 0.f;
 #pragma unroll
-        for (int qt = 0; qt < QT; ++qt) {
-            top[qt] = -INFINITY;
-            sum[qt] = 0.f;
+        for (int j = 0; j < NJ; ++j)
 #pragma unroll
-            for (int j = 0; j < NJ; ++j)
-#pragma unroll
-                for (int e = 0; e < 4; ++e) acc[qt][j][e] = f32x4{0.f, 0.f, 0.f, 0.f};
-        }
-        f32x4 p[QT];  // scores, then weights, of keys 16 wave + 4 g + i
+            for (int e = 0; e < 4; ++e) acc[j][e] = f32x4{0.f, 0.f, 0.f, 0.f};
+        f32x4 p;  // scores, then weights, of keys 16 wave + 4 g + i
         auto score = [&]() __attribute__((always_inline)) {
+            if (!VEC)  // the next row's values may not be finite
 #pragma unroll
-            for (int qt = 0; qt < QT; ++qt) p[qt] = f32x4{0.f, 0.f, 0.f, 0.f};
+                for (int j = 0; j < KJ; ++j)
 #pragma unroll
-            for (int j = 0; j < KJ; ++j) {
-                f32x4 q[QT];
+                    for (int e = 0; e < 4; ++e)
+                        if (16 * j + 4 * g + e >= a.dim) kf[j][e] = 0.f;
+            p = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-                for (int qt = 0; qt < QT; ++qt) q[qt] = q_of(qt, j);
+            for (int j = 0; j < KJ; ++j)
 #pragma unroll
-                for (int e = 0; e < 4; ++e)
-#pragma unroll
-                    for (int qt = 0; qt < QT; ++qt)
-                        p[qt] = __builtin_amdgcn_mfma_f32_16x16x4f32(kf[j][e], q[qt][e], p[qt], 0, 0, 0);
-            }
+                for (int e = 0; e < 4; ++e) p = __builtin_amdgcn_mfma_f32_16x16x4f32(kf[j][e], qf[j][e], p, 0, 0, 0);
         };
         auto weigh = [&]() __attribute__((always_inline)) {
+            const float most = fmaxf(fmaxf(p.x, p.y), fmaxf(p.z, p.w));
+            if (__any(most > top + kLazyMax)) {
+                const float reached = fmaxf(top, across_keys_max(most));
+                const float keep = reached == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(top - reached);
+                top = reached;
+                sum *= keep;
 #pragma unroll
-            for (int qt = 0; qt < QT; ++qt) {
-                const float most = fmaxf(fmaxf(p[qt].x, p[qt].y), fmaxf(p[qt].z, p[qt].w));
-                if (__any(most > top[qt] + kLazyMax)) {
-                    const float reached = fmaxf(top[qt], across_keys_max(most));
-                    const float keep = reached == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(top[qt] - reached);
-                    top[qt] = reached;
-                    sum[qt] *= keep;
+                for (int j = 0; j < NJ; ++j)
 #pragma unroll
-                    for (int j = 0; j < NJ; ++j)
+                    for (int e = 0; e < 4; ++e) acc[j][e] *= keep;
+            }
+            const float from = top == -INFINITY ? 0.f : top;
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) acc[qt][j][e] *= keep;
-                }
-                const float from = top[qt] == -INFINITY ? 0.f : top[qt];
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    p[qt][i] = __builtin_amdgcn_exp2f(p[qt][i] - from);
-                    sum[qt] += p[qt][i];
-                }
+            for (int i = 0; i < 4; ++i) {
+                p[i] = __builtin_amdgcn_exp2f(p[i] - from);
+                sum += p[i];
             }
         };
         auto add = [&]() __attribute__((always_inline)) {
@@ -217,10 +177,7 @@ attention_ragged(RaggedArgs a) {
                 for (int j = 0; j < NJ; ++j)
 #pragma unroll
                     for (int e = 0; e < 4; ++e)
-#pragma unroll
-                        for (int qt = 0; qt < QT; ++qt)
-                            acc[qt][j][e] =
-                                __builtin_amdgcn_mfma_f32_16x16x4f32(vf[j][i][e], p[qt][i], acc[qt][j][e], 0, 0, 0);
+                        acc[j][e] = __builtin_amdgcn_mfma_f32_16x16x4f32(vf[j][i][e], p[i], acc[j][e], 0, 0, 0);
         };
         uint32_t x = begin;
         for (; x < min(end, cached); ++x) {
@@ -229,10 +186,8 @@ attention_ragged(RaggedArgs a) {
             if ((x + 1) * kTile > len) {
                 const int first = int(x) * kTile + 16 * wave + 4 * g;
 #pragma unroll
-                for (int qt = 0; qt < QT; ++qt)
-#pragma unroll
-                    for (int i = 0; i < 4; ++i)
-                        if (first + i >= int(len)) p[qt][i] = -INFINITY;
+                for (int i = 0; i < 4; ++i)
+                    if (first + i >= int(len)) p[i] = -INFINITY;
             }
             weigh();
             add();
@@ -240,20 +195,15 @@ attention_ragged(RaggedArgs a) {
         }
 
         if (end > cached) {
-            see_ancestors(a.nodes, above_me, sees, above);
+            if (tree != b) see_ancestors(a.nodes, above_me, sees, above);
+            tree = b;
             for (; x < end; ++x) {
-                const uint32_t tile = x - cached;
-                const int first = 16 * wave + 4 * g;
                 score();
                 load_k(x + 1);
+                const uint64_t seen = sees[query][x - cached];  // queries == nodes; rows past the last see as others do
 #pragma unroll
-                for (int qt = 0; qt < QT; ++qt) {
-                    const uint32_t node = (rb * RB + row0 + 16 * qt + m) % a.queries;  // queries == nodes
-                    const uint64_t seen = sees[node][tile];
-#pragma unroll
-                    for (int i = 0; i < 4; ++i)
-                        if (!(seen >> (first + i) & 1)) p[qt][i] = -INFINITY;
-                }
+                for (int i = 0; i < 4; ++i)
+                    if (!(seen >> (16 * wave + 4 * g + i) & 1)) p[i] = -INFINITY;
                 weigh();
                 bool odd = false;
 #pragma unroll
@@ -272,43 +222,38 @@ attention_ragged(RaggedArgs a) {
 #pragma unroll
                         for (int e = 0; e < 4; ++e)
 #pragma unroll
-                            for (int qt = 0; qt < QT; ++qt)
+                            for (int k = -1; k < 3; ++k) {
+                                __builtin_amdgcn_sched_barrier(0);  // one at a time: a rare path takes no registers
+                                f32x4 sums = k < 0 ? acc[j][e] : f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-                                for (int k = -1; k < 3; ++k) {
-                                    __builtin_amdgcn_sched_barrier(0);  // one at a time: a rare path takes no registers
-                                    f32x4 sums = k < 0 ? acc[qt][j][e] : f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-                                    for (int i = 0; i < 4; ++i) {
-                                        const float v = vf[j][i][e], u = k >= 0 ? is(k, v) : finite(v) ? v : 0.f;
-                                        sums = __builtin_amdgcn_mfma_f32_16x16x4f32(u, p[qt][i], sums, 0, 0, 0);
-                                    }
-                                    if (k < 0)
-                                        acc[qt][j][e] = sums;
-                                    else
-#pragma unroll
-                                        for (int i = 0; i < 4; ++i)
-                                            if (sums[i] > 0.f) acc[qt][j][e][i] += special(k);
+                                for (int i = 0; i < 4; ++i) {
+                                    const float v = vf[j][i][e], u = k >= 0 ? is(k, v) : finite(v) ? v : 0.f;
+                                    sums = __builtin_amdgcn_mfma_f32_16x16x4f32(u, p[i], sums, 0, 0, 0);
                                 }
+                                if (k < 0)
+                                    acc[j][e] = sums;
+                                else
+#pragma unroll
+                                    for (int i = 0; i < 4; ++i)
+                                        if (sums[i] > 0.f) acc[j][e][i] += special(k);
+                            }
                 }
                 load_v(x + 1);
             }
         }
 
-        // The four waves' sums joined.
+        // The four waves' sums joined: row m, dims 64 j + 16 g + 4 i + e.
         __syncthreads();
+        const float all = across_keys_sum(sum);
+        if (g == 0) ml[wave][m] = float2{top, all};
 #pragma unroll
-        for (int qt = 0; qt < QT; ++qt) {
-            const float all = across_keys_sum(sum[qt]);
-            if (g == 0) ml[wave][row0 + 16 * qt + m] = float2{top[qt], all};
+        for (int j = 0; j < NJ; ++j)
 #pragma unroll
-            for (int j = 0; j < NJ; ++j)
-#pragma unroll
-                for (int i = 0; i < 4; ++i)
-                    *reinterpret_cast<f32x4 *>(&part[wave][row0 + 16 * qt + m][64 * j + 16 * g + 4 * i]) =
-                        f32x4{acc[qt][j][0][i], acc[qt][j][1][i], acc[qt][j][2][i], acc[qt][j][3][i]};
-        }
+            for (int i = 0; i < 4; ++i)
+                *reinterpret_cast<f32x4 *>(&part[wave][m][64 * j + 16 * g + 4 * i]) =
+                    f32x4{acc[j][0][i], acc[j][1][i], acc[j][2][i], acc[j][3][i]};
         __syncthreads();
-        finish<DP, RB, S::kThreads, VEC>(a, run, b, kv, rb, whole, begin == 0, part, ml, plans, sees, 0.f);
+        finish<DP, RB, VEC>(a, run, b, kv, rb, whole, begin == 0, part, ml, plans, sees, 0.f);
         t += end - begin;
         if (t >= (before + tiles) * units) {
             before += tiles;
@@ -393,20 +338,15 @@ __global__ __launch_bounds__(kThreads) void attention_ragged_join(RaggedArgs a) 
     if (mine) store_row<VEC>(a, b, kv, rb * RB + row, d, o, l);
 }
 
-// Rows per block.
-uint32_t block_rows(uint32_t rows) { return rows <= 16 ? 16 : rows <= 32 ? 32 : 64; }
-
 uint32_t rows_of(const RaggedShape &s) { return s.heads / s.kv_heads * s.queries; }
-uint32_t row_blocks(const RaggedShape &s) {
-    const uint32_t rb = block_rows(rows_of(s));
-    return (rows_of(s) + rb - 1) / rb;
-}
 
-// More than 16 rows of whole float4s go to the kernel on bf16 parts (the runtime's buffers
-// are all aligned), where a tile of 128 keys spans less than 2 GiB.
+// More than 16 rows go to the kernel on bf16 parts, where a tile of its 128 keys spans less
+// than 2 GiB.
 bool on_parts(const RaggedShape &s) {
-    return rows_of(s) > 16 && s.dim % 4 == 0 && (!s.token_major || uint64_t(s.kv_heads) * s.dim < 1u << 22);
+    return rows_of(s) > 16 && (!s.token_major || uint64_t(s.kv_heads) * s.dim < 1u << 22);
 }
+uint32_t block_rows(const RaggedShape &s) { return !on_parts(s) ? 16 : rows_of(s) <= 32 ? 32 : 64; }
+uint32_t row_blocks(const RaggedShape &s) { return (rows_of(s) + block_rows(s) - 1) / block_rows(s); }
 
 uint64_t ragged_tiles(const RaggedShape &s) {
     const uint32_t tile = on_parts(s) ? kPartsTile : kTile;
@@ -418,30 +358,33 @@ uint64_t ragged_tiles(const RaggedShape &s) {
 // splits K and V once for 128 or 256 rows but has one block for them and all their keys.
 // Both are estimated, in us, from what they measured: the flash kernel 8 and, for every 256
 // blocks, 1.7 (dims to 64), 3.6 (to 96) or 4.6 for 32 keys of full blocks, 0.35 of that for
-// empty ones; the kernel on parts 2.8 (to 64) or 5.9 for 128 keys, 8 or 11 for each unit a
+// empty ones; the kernel on parts 2.8, 4.1 or 5.9 for 128 keys, 8, 9.5 or 11 for each unit a
 // run begins, and 3 for the join. Measured, flash and parts: 4 x 32 heads (8 of keys) x 1000
 // queries x 4096 keys of 128 1179 and 1385 us; 32 x 16 x 200 x 100 of 128 48 and 129; 32 x
 // 16 x 80 x 128 of 64 21 and 43; 16 x 3000 x 1500 of 128 198 and 220; 4 x 32 x 256 x 2048
-// of 128 256 and 221; 16 x 1500 x 1500 of 64 82 and 71; 4 x 8 x 256 x 1024 of 128 131 and 40.
+// of 128 256 and 221, of 96 212 and 170; 16 x 1500 x 1500 of 64 82 and 71, of 80 154 and 93;
+// 16 x 3000 x 1500 of 96 160 and 178; 4 x 8 x 256 x 1024 of 128 131 and 40.
 bool on_flash(const RaggedShape &s) {
     const uint64_t d = s.dim, heads = uint64_t(s.batch) * s.kv_heads, rows = rows_of(s), fb = flash_ragged_rows(s.dim);
     const uint64_t q_span = s.token_major ? d * s.heads * s.queries : d * rows, k_span = (s.token_major ? d * s.kv_heads : d) * (s.keys + 128ull);
     // Offsets of a head's rows in 31 bits, tiles past the last one in 32; grid.y.
-    if (!on_parts(s) || s.nodes || q_span >= 1u << 29 || k_span >= 1u << 29 || (rows + fb - 1) / fb > 65535) return false;
+    if (!on_parts(s) || s.dim % 4 || s.nodes || q_span >= 1u << 29 || k_span >= 1u << 29 || (rows + fb - 1) / fb > 65535) return false;
     const uint64_t blocks = heads * ((rows + fb - 1) / fb), units = heads * row_blocks(s);
     const double full = double(rows) / double((rows + fb - 1) / fb * fb);
     const double flash = 8.0 + double((blocks + kCus - 1) / kCus) * double((s.keys + 31) / 32) *
                                    (d <= 64 ? 1.7 : d <= 96 ? 3.6 : 4.6) * (0.35 + 0.65 * full);
-    const double parts = 3.0 + double((ragged_tiles(s) + kCus - 1) / kCus) * (d <= 64 ? 2.8 : 5.9) +
-                         double((units + kCus - 1) / kCus) * (d <= 64 ? 8.0 : 11.0);
+    const double parts = 3.0 + double((ragged_tiles(s) + kCus - 1) / kCus) * (d <= 64 ? 2.8 : d <= 96 ? 4.1 : 5.9) +
+                         double((units + kCus - 1) / kCus) * (d <= 64 ? 8.0 : d <= 96 ? 9.5 : 11.0);
     return flash < parts;
 }
 
-// Runs of a launch: as many blocks as the chip holds at once (one a CU of 64 rows or
-// on parts, else two), or one per tile where there can be no more tiles.
+// Runs of a launch: as many blocks as the chip holds at once (one a CU on parts, else two),
+// or one per tile where there can be no more tiles. Three a CU, where the registers allow
+// it (dims to 64): 36 x 20 heads x 1101 keys 61.6 -> 57.0 us, but 8 x 16 x 4096 52.4 -> 55.1
+// and 64 x 8 x 100 11.3 -> 13.3.
 uint32_t runs_of(const RaggedShape &s) {
     const uint64_t tiles = ragged_tiles(s);
-    const uint32_t most = block_rows(rows_of(s)) == 64 || on_parts(s) ? kCus : 2 * kCus;
+    const uint32_t most = on_parts(s) ? kCus : 2 * kCus;
     return tiles >= most ? most : uint32_t((tiles + 7) / 8 * 8);
 }
 
@@ -450,8 +393,9 @@ void launch_join(hipStream_t stream, const RaggedArgs &a) {
     constexpr uint32_t kRowsOf = kThreads / (DP / 4);  // rows of a block
     const uint32_t units = a.batch * a.kv_heads * a.row_blocks, all = a.group * a.queries, rows = all < RB ? all : RB;
     const uint32_t x = units < a.runs ? units : a.runs;
-    // Units of 16 runs or so: their slots are shared out (4 nodes over 131072 keys, 64 runs a
-    // unit: 15 us otherwise, 8 so); else whole rows (64 nodes x 4 sequences: 14 us shared, 6).
+    // Units of 16 runs or more: their slots are shared out (with the attention itself, 4 nodes over 131072
+    // keys, 64 runs a unit: 186 us so, 193 by whole rows); else whole rows (64 nodes x 4 heads
+    // over 4 sequences of 4096 keys: 133 us shared, 122 by rows).
     if (16 * units <= a.runs)
         hipLaunchKernelGGL((attention_ragged_join<DP, RB, TILE, 1, VEC>), dim3(x, rows), dim3(kThreads), 0, stream, a);
     else
@@ -459,26 +403,23 @@ void launch_join(hipStream_t stream, const RaggedArgs &a) {
                            dim3(kThreads), 0, stream, a);
 }
 
-template <int DP, int QT, int RG, bool VEC>
-void launch(hipStream_t stream, const RaggedArgs &a) {
-    using S = Shape<DP, QT, RG>;
-    hipLaunchKernelGGL((attention_ragged<DP, QT, RG, VEC>), dim3(a.runs), dim3(S::kThreads), 0, stream, a);
-    launch_join<DP, S::kRows, kTile, VEC>(stream, a);
-}
-
-// `parts`: on bf16 parts; whole rows of float4s otherwise only up to 16 rows.
-template <int DP>
-hipError_t launch_rows(hipStream_t stream, const RaggedArgs &a, bool parts) {
-    const uint32_t rb = block_rows(a.group * a.queries);
-    if (parts) {
-        launch_ragged_parts(stream, a, rb);
-        rb == 32 ? launch_join<DP, 32, kPartsTile, true>(stream, a) : launch_join<DP, 64, kPartsTile, true>(stream, a);
-    } else if (rb == 16) {
-        a.dim % 4 == 0 ? launch<DP, 1, 1, true>(stream, a) : launch<DP, 1, 1, false>(stream, a);
+template <int DP, bool VEC>
+hipError_t launch_rows(hipStream_t stream, const RaggedArgs &a, uint32_t rb) {
+    if (rb == 16) {
+        hipLaunchKernelGGL((attention_ragged<DP, VEC>), dim3(a.runs), dim3(kThreads), 0, stream, a);
+        launch_join<DP, 16, kTile, VEC>(stream, a);
     } else {
-        rb == 32 ? launch<DP, 2, 1, false>(stream, a) : launch<DP, 2, 2, false>(stream, a);
+        launch_ragged_parts(stream, a, rb);
+        rb == 32 ? launch_join<DP, 32, kPartsTile, VEC>(stream, a) : launch_join<DP, 64, kPartsTile, VEC>(stream, a);
     }
     return hipGetLastError();
+}
+
+uint32_t ragged_lds_bytes(uint32_t dim, uint32_t rb) {
+    if (rb > 16) return ragged_parts_lds_bytes(dim, rb);
+    const uint32_t pitch = (dim <= 64 ? 64 : 128) + 4;
+    return uint32_t(kWaves * rb * (pitch * sizeof(float) + sizeof(float2)) + rb * sizeof(RowPlan) +
+                    kMaxTreeNodes * (kWords * sizeof(uint64_t) + sizeof(int)));
 }
 
 }  // namespace
@@ -493,21 +434,17 @@ LaunchShape attention_ragged_shape(const RaggedShape &s) {
     }
     // Tiles are counted in 32 bits.
     if (ragged_tiles(s) > 0x7fffffffull) return {nullptr, {0, 0, 0}, {0, 0, 0}, 0};
-    const bool wide = s.dim > 64;
-    const uint32_t rb = block_rows(rows_of(s)), pitch = (wide ? 128 : 64) + 4;
-    static const char *const names[2][2][3] = {
-        {{"attention_ragged_d64_r16", "attention_ragged_d64_r32", "attention_ragged_d64_r64"},
-         {"attention_ragged_d128_r16", "attention_ragged_d128_r32", "attention_ragged_d128_r64"}},
-        {{nullptr, "attention_ragged_parts_d64_r32", "attention_ragged_parts_d64_r64"},
-         {nullptr, "attention_ragged_parts_d128_r32", "attention_ragged_parts_d128_r64"}}};
-    return {names[on_parts(s)][wide][rb / 32], {runs_of(s), 1, 1}, {uint32_t(rb == 64 && !on_parts(s) ? 2 * kThreads : kThreads), 1, 1},
-            uint32_t(kWaves * rb * (pitch * sizeof(float) + sizeof(float2)) +
-                     kMaxTreeNodes * (kWords * sizeof(uint64_t) + sizeof(int)))};
+    const uint32_t rb = block_rows(s), wide = s.dim <= 64 ? 0 : s.dim <= 96 ? 1 : 2;
+    static const char *const names[3][3] = {
+        {"attention_ragged_d64", "attention_ragged_parts_d64_r32", "attention_ragged_parts_d64_r64"},
+        {"attention_ragged_d128", "attention_ragged_parts_d96_r32", "attention_ragged_parts_d96_r64"},
+        {"attention_ragged_d128", "attention_ragged_parts_d128_r32", "attention_ragged_parts_d128_r64"}};
+    return {names[wide][rb / 32], {runs_of(s), 1, 1}, {kThreads, 1, 1}, ragged_lds_bytes(s.dim, rb)};
 }
 
 size_t attention_ragged_workspace_bytes(const RaggedShape &s) {
     if (on_flash(s)) return 0;
-    const size_t rb = block_rows(rows_of(s)), dp = s.dim > 64 ? 128 : 64;
+    const size_t rb = block_rows(s), dp = s.dim > 64 ? 128 : 64;
     return 2 * size_t(runs_of(s)) * rb * (dp + 2) * sizeof(float);
 }
 
@@ -536,7 +473,9 @@ hipError_t attention_ragged_f32(hipStream_t stream, const RaggedShape &s, const 
     if (s.dim % 4 == 0 && bits & 15u) return hipErrorInvalidValue;  // the runtime's regions are aligned
     if (on_flash(s)) return launch_flash_ragged(stream, a);
     if (!workspace) return hipErrorInvalidValue;
-    return s.dim <= 64 ? launch_rows<64>(stream, a, on_parts(s)) : launch_rows<128>(stream, a, on_parts(s));
+    const uint32_t rb = block_rows(s);
+    if (s.dim % 4) return s.dim <= 64 ? launch_rows<64, false>(stream, a, rb) : launch_rows<128, false>(stream, a, rb);
+    return s.dim <= 64 ? launch_rows<64, true>(stream, a, rb) : launch_rows<128, true>(stream, a, rb);
 }
 
 }  // namespace hipk

@@ -23,10 +23,11 @@ struct RaggedArgs {
 };
 
 // The kernel on bf16 parts (attention_ragged_parts.hip), with 32 or 64 rows a block and
-// tiles of kPartsTile keys. Needs dim % 4 == 0 and at most 128, 16-byte aligned tensors and
-// k_row < 2^22.
+// tiles of kPartsTile keys. Needs dim at most 128, 16-byte aligned rows where they are
+// whole float4s, and k_row < 2^22.
 constexpr uint32_t kPartsTile = 128;
 void launch_ragged_parts(hipStream_t stream, const RaggedArgs &args, uint32_t block_rows);
+uint32_t ragged_parts_lds_bytes(uint32_t dim, uint32_t block_rows);
 
 }  // namespace hipk
 }  // namespace jade

@@ -1,17 +1,22 @@
-// Ragged attention (attention_ragged.hip) of more than 16 rows, of 16-byte rows, on
-// bf16 parts: every FP32 operand is held exactly as three bf16 parts and multiplied
-// as six products of parts with FP32 sums (split_bf16.hpp), on 32x32x16 MFMAs in the
-// transposed form of attention_flash.hip. A wave has all 32 or 64 rows of its block and
+// Ragged attention (attention_ragged.hip) of more than 16 rows on bf16 parts: every FP32
+// operand is held exactly as three bf16 parts and multiplied as six products of parts with
+// FP32 sums (split_bf16.hpp), on 32x32x16 MFMAs in the transposed form of
+// attention_flash.hip. Head dims are padded to 64, 96 or 128. A wave has all 32 or 64 rows of its block and
 // 32 of a tile's 128 keys. Both products take their dims and keys in the order in which
 // a lane's 16-byte loads of K and V leave them, so K and V go from memory to registers
 // and are split there, by the one wave that multiplies them; LDS has only the parts of
-// Q, which the four waves share.
+// Q, which the four waves share. A last chunk that is not whole reads into the next row (or
+// nothing past the tile): Q's parts are zeros there, and V's dims past the last are dropped.
 //
 // One wave a SIMD, so it overlaps its own work: an MFMA every 32 cycles, and between
 // two of them two of the twelve pieces in which the next eight values of K or V are
 // split; a chunk is loaded again, for the next tile, as soon as it is split. For 64
 // rows and 32 keys of 128 dims that is 192 MFMAs (6144 cycles of a SIMD; FP32 MFMAs
-// take 16384) against some 840 other instructions.
+// take 16384) and 1150 other vector instructions, most of them beside the MFMAs; masks,
+// maxima and the first weights are between the two products and beside none. 64 nodes x 32
+// heads (8 of keys) over 4 sequences of at most 4096 keys of 128: 116 us, 117 TFLOP/s; 13
+// nodes over 8 sequences: 71 us, 3.0 TB/s of K and V. A run's unit costs 8 to 11 us besides
+// its tiles: Q's loads and parts, the first tile's loads, the waves' sums joined.
 //
 // Q is scaled up before it is split (the scores are scaled back where their maximum is
 // taken off), so every finite Q is carried exactly; parts of K below 2^-109 lose bits
@@ -75,20 +80,20 @@ __device__ inline int lane_now() {
 
 template <int DP, int QG>
 struct Shape {
-    static constexpr int kRows = 32 * QG, kBlock = 64 * kWaves, kPitch = DP + 4;
+    static constexpr int kRows = 32 * QG, kPitch = DP + 4;
     static constexpr int kSteps = DP / 16;  // score steps
     static constexpr int kOut = DP / 32;    // output blocks of 32 dims: dims kOut * r + e
     // Where K and V of a tile are loaded: each chunk as soon as the last tile's is split,
     // or, where two row groups leave no registers for all of both, V before the scores
     // and K before and amid the outputs.
-    static constexpr bool kEarly = QG == 1 || DP <= 64;
+    static constexpr bool kEarly = QG == 1 || DP <= 96;
     static constexpr int kEarlyK = kEarly ? kSteps : 0;
     static_assert(QG * kSteps * kParts * 1024 <= kWaves * kRows * kPitch * 4, "Q's parts fit the sums' space");
 };
 
 // QG: groups of 32 rows, all of them every wave's.
-template <int DP, int QG>
-__global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(1, 1))) void
+template <int DP, int QG, bool VEC>
+__global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(1, 1))) void
 attention_ragged_parts(RaggedArgs a) {
     using S = Shape<DP, QG>;
     constexpr int KS = S::kSteps, NB = S::kOut, RB = S::kRows;
@@ -111,6 +116,7 @@ attention_ragged_parts(RaggedArgs a) {
     uint32_t t = spread.start(run, chunk, units, b, before);
 
     const uint32_t row_bytes = a.k_row * 4u;
+    uint32_t tree = ~0u;  // the sequence whose tree is in LDS
     while (t < t_stop) {
         const uint32_t len = spread.length(b);
         const uint32_t cached = (len + kTile - 1) / kTile, tiles = cached + spread.draft_tiles;
@@ -123,7 +129,7 @@ attention_ragged_parts(RaggedArgs a) {
         const uint32_t end = min(tiles, begin + (t_stop - t));
         const bool whole = begin == 0 && end == tiles;
         float above_me = 0.f;
-        if (end > cached && tid < int(a.nodes)) above_me = a.parents[size_t(b) * a.nodes + tid];
+        if (end > cached && tree != b && tid < int(a.nodes)) above_me = a.parents[size_t(b) * a.nodes + tid];
 
         const float *kb = a.k + size_t(b) * a.k_batch + size_t(kv) * a.k_head;
         const float *vb = a.v + size_t(b) * a.k_batch + size_t(kv) * a.k_head;
@@ -149,7 +155,7 @@ attention_ragged_parts(RaggedArgs a) {
             const uint32_t half = l >> 5, row = l & 31;
             return Offsets{(32 * wave + row) * row_bytes + 16 * half,
                            NB * row < a.dim ? (32 * wave + 4 * half) * row_bytes + 4 * NB * row : kDeadOffset,
-                           int(a.dim / 4 + 1 - half) / 2};
+                           int((a.dim + 3) / 4 + 1 - half) / 2};
         };
         // Dims of score step s, load x: 8 y + 4 h + 0 .. 3, y = 2 s + x.
         auto load_k = [&](__amdgpu_buffer_rsrc_t from, const Offsets &o, int s) __attribute__((always_inline)) {
@@ -165,6 +171,8 @@ attention_ragged_parts(RaggedArgs a) {
             const uint32_t at = voff + uint32_t(16 * s + (u & 3) + 8 * (u >> 2)) * row_bytes;
             if constexpr (NB == 4)
                 vf[s][u] = __builtin_bit_cast(vec, __builtin_amdgcn_raw_buffer_load_b128(from, int(at), 0, 0));
+            else if constexpr (NB == 3)
+                vf[s][u] = __builtin_bit_cast(vec, __builtin_amdgcn_raw_buffer_load_b96(from, int(at), 0, 0));
             else
                 vf[s][u] = __builtin_bit_cast(vec, __builtin_amdgcn_raw_buffer_load_b64(from, int(at), 0, 0));
         };
@@ -174,22 +182,19 @@ attention_ragged_parts(RaggedArgs a) {
             if (head >= a.group) return nullptr;
             return a.q + size_t(b) * a.q_batch + (size_t(kv) * a.group + head) * a.q_head + size_t(query) * a.q_row;
         };
-        // Its dims d .. d + 3.
-        auto load_q = [&](const float *row, int d) {
-            return row && d < a.dim ? *reinterpret_cast<const f32x4 *>(row + d) : f32x4{0.f, 0.f, 0.f, 0.f};
-        };
         // Q first, then the first tile; from there on a chunk is loaded again once it is
-        // split. A wave stages the steps wave + 4 i % KS of row group 4 i / KS.
-        constexpr int kItems = QG * KS / kWaves;
+        // split. A wave stages every fourth of the QG * KS (row group, step)s.
+        constexpr int kItems = (QG * KS + kWaves - 1) / kWaves;
         f32x4 qraw[kItems][2];
         {
             const int l = lane_now();
 #pragma unroll
             for (int i = 0; i < kItems; ++i) {
-                const float *row = q_row(32 * (kWaves * i / KS) + (l & 31));
+                const int n = kWaves * i + wave, r = n / KS, s = n % KS;
+                const float *row = r < QG ? q_row(32 * r + (l & 31)) : nullptr;
 #pragma unroll
                 for (int y = 0; y < 2; ++y)
-                    qraw[i][y] = load_q(row, 16 * (wave + kWaves * i % KS) + 8 * y + 4 * (l >> 5));
+                    qraw[i][y] = load_dims<VEC>(row, 16 * s + 8 * y + 4 * (l >> 5), a.dim);
             }
             const auto kfrom = tile_of(kb, kd, begin), vfrom = tile_of(vb, vd, begin);
             const Offsets at = offsets();
@@ -205,7 +210,8 @@ attention_ragged_parts(RaggedArgs a) {
         __syncthreads();
 #pragma unroll
         for (int i = 0; i < kItems; ++i) {
-            const int s = wave + kWaves * i % KS, r = kWaves * i / KS;
+            const int n = kWaves * i + wave, r = n / KS, s = n % KS;
+            if (r >= QG) break;
             uint32_t p[kParts][4];
             bool past = false;
 #pragma unroll
@@ -222,10 +228,12 @@ attention_ragged_parts(RaggedArgs a) {
             for (int w = 0; w < kParts; ++w)
                 *reinterpret_cast<bf16x8 *>(qs + (((r * KS + s) * kParts + w) * 64 + lane) * 16) = part_of(p, w);
         }
-        if (end > cached)
+        if (end > cached && tree != b) {
             see_ancestors(a.nodes, above_me, sees, above);
-        else
+            tree = b;
+        } else {
             __syncthreads();
+        }
 
         f32x16 acc[QG][NB], st[QG];
         float top[QG], sum[QG];  // of the tile at hand; between tiles in LDS, where nothing spills them
@@ -422,13 +430,18 @@ attention_ragged_parts(RaggedArgs a) {
                     vec o;
 #pragma unroll
                     for (int e = 0; e < NB; ++e) o[e] = acc[r][e][v];
-                    *reinterpret_cast<vec *>(&part[wave][32 * r + c][NB * (8 * (v >> 2) + 4 * h + (v & 3))]) = o;
+                    float *const to = &part[wave][32 * r + c][NB * (8 * (v >> 2) + 4 * h + (v & 3))];
+                    if constexpr (NB == 3)  // twelve bytes
+#pragma unroll
+                        for (int e = 0; e < NB; ++e) to[e] = o[e];
+                    else
+                        *reinterpret_cast<vec *>(to) = o;
                 }
             }
             __syncthreads();
         };
         hand_over();
-        if (finish<DP, RB, S::kBlock, true>(a, run, b, kv, rb, whole, begin == 0, part, ml, plans, sees, kLeastOut)) far = 1;
+        if (finish<DP, RB, VEC>(a, run, b, kv, rb, whole, begin == 0, part, ml, plans, sees, kLeastOut)) far = 1;
         __syncthreads();
         if (far) {  // what the parts do not carry: see the file's head
             clear();
@@ -445,9 +458,8 @@ attention_ragged_parts(RaggedArgs a) {
                     const float *qrow = q_row(32 * r + c);
                     for (int d0 = 0; d0 < DP; d0 += 8) {
                         const int d = d0 + 4 * h;
-                        const f32x4 q = load_q(qrow, d) * a.qscale;
-                        f32x4 k = {0.f, 0.f, 0.f, 0.f};
-                        if (d < a.dim && key0 + c < keys) k = *reinterpret_cast<const f32x4 *>(krow + d);
+                        const f32x4 q = load_dims<VEC>(qrow, d, a.dim) * a.qscale;
+                        const f32x4 k = load_dims<VEC>(key0 + c < keys ? krow : nullptr, d, a.dim);
 #pragma unroll
                         for (int e = 0; e < 4; ++e) st[r] = __builtin_amdgcn_mfma_f32_32x32x2f32(k[e], q[e], st[r], 0, 0, 0);
                     }
@@ -469,7 +481,7 @@ attention_ragged_parts(RaggedArgs a) {
 #pragma unroll
                             for (int v = 0; v < 16; ++v) {
                                 const uint32_t key = 8 * (v >> 2) + 4 * h + (v & 3);
-                                const float z = NB * c < a.dim && key0 + key < keys ? vrow[size_t(key) * a.k_row + NB * c + e] : 0.f;
+                                const float z = NB * c + e < a.dim && key0 + key < keys ? vrow[size_t(key) * a.k_row + NB * c + e] : 0.f;
                                 const float y = k >= 0 ? is(k, z) : finite(z) || !drafted ? z : 0.f;
                                 sums = __builtin_amdgcn_mfma_f32_32x32x2f32(y, st[r][v], sums, 0, 0, 0);
                             }
@@ -483,7 +495,7 @@ attention_ragged_parts(RaggedArgs a) {
                         }
             }
             hand_over();
-            finish<DP, RB, S::kBlock, true>(a, run, b, kv, rb, whole, begin == 0, part, ml, plans, sees, kLeastOut);
+            finish<DP, RB, VEC>(a, run, b, kv, rb, whole, begin == 0, part, ml, plans, sees, kLeastOut);
         }
         t += end - begin;
         if (t >= (before + tiles) * units) {
@@ -493,18 +505,32 @@ attention_ragged_parts(RaggedArgs a) {
     }
 }
 
-template <int DP, int QG>
+template <int DP, int QG, bool VEC>
 void launch(hipStream_t stream, const RaggedArgs &a) {
-    hipLaunchKernelGGL((attention_ragged_parts<DP, QG>), dim3(a.runs), dim3(Shape<DP, QG>::kBlock), 0, stream, a);
+    hipLaunchKernelGGL((attention_ragged_parts<DP, QG, VEC>), dim3(a.runs), dim3(kThreads), 0, stream, a);
+}
+
+template <int DP, int QG>
+void launch_rows(hipStream_t stream, const RaggedArgs &a) {
+    a.dim % 4 ? launch<DP, QG, false>(stream, a) : launch<DP, QG, true>(stream, a);
 }
 
 }  // namespace
 
+uint32_t ragged_parts_lds_bytes(uint32_t dim, uint32_t block_rows) {
+    const uint32_t pitch = (dim <= 64 ? 64 : dim <= 96 ? 96 : 128) + 4;
+    return uint32_t(kWaves * block_rows * (pitch * sizeof(float) + sizeof(float2)) + block_rows * sizeof(RowPlan) +
+                    kMaxTreeNodes * (kWords * sizeof(uint64_t) + sizeof(int)) +
+                    kWaves * block_rows / 32 * 64 * sizeof(float2) + sizeof(int));
+}
+
 void launch_ragged_parts(hipStream_t stream, const RaggedArgs &a, uint32_t block_rows) {
     if (a.dim <= 64)
-        block_rows == 32 ? launch<64, 1>(stream, a) : launch<64, 2>(stream, a);
+        block_rows == 32 ? launch_rows<64, 1>(stream, a) : launch_rows<64, 2>(stream, a);
+    else if (a.dim <= 96)
+        block_rows == 32 ? launch_rows<96, 1>(stream, a) : launch_rows<96, 2>(stream, a);
     else
-        block_rows == 32 ? launch<128, 1>(stream, a) : launch<128, 2>(stream, a);
+        block_rows == 32 ? launch_rows<128, 1>(stream, a) : launch_rows<128, 2>(stream, a);
 }
 
 }  // namespace hipk

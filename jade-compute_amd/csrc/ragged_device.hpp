@@ -131,23 +131,46 @@ __device__ inline float across_keys_sum(float x) {
     return x + __shfl_xor(x, 32);
 }
 
+// Dims d .. d + 3 of a row, zeros from `dim` on and for no row. VEC: dim % 4 == 0 and
+// 16-byte rows. Asked at run time its branches cost 1.2 us a launch (8 heads x 1024 keys of
+// 64 dims, one query: 9.9 against 8.7 us).
+template <bool VEC>
+__device__ inline f32x4 load_dims(const float *row, int d, int dim) {
+    f32x4 x = {0.f, 0.f, 0.f, 0.f};
+    if (VEC) {
+        if (row && d < dim) x = *reinterpret_cast<const f32x4 *>(row + d);
+    } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            if (row && d + e < dim) x[e] = row[d + e];
+    }
+    return x;
+}
+template <bool VEC>
+__device__ inline void store_dims(float *row, int d, int dim, f32x4 x) {
+    if (VEC) {
+        if (d < dim) *reinterpret_cast<f32x4 *>(row + d) = x;
+    } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            if (d + e < dim) row[d + e] = x[e];
+    }
+}
 // Row r of (sequence b, kv head): its sums o of dims d .. d + 3 over its weights' sum.
 template <bool VEC>
 __device__ inline void store_row(const RaggedArgs &a, uint32_t b, uint32_t kv, uint32_t r, uint32_t d, f32x4 o, float l) {
     const uint32_t head = r / a.queries, query = r - head * a.queries;
     const bool node = !a.nodes || is_node(a.parents[size_t(b) * a.nodes + query], int(query));
     o = node ? o * (1.0f / l) : f32x4{0.f, 0.f, 0.f, 0.f};
-    float *out = a.out + size_t(b) * a.q_batch + (size_t(kv) * a.group + head) * a.q_head + size_t(query) * a.q_row;
-    if (VEC) {
-        if (d < a.dim) *reinterpret_cast<f32x4 *>(out + d) = o;
-    } else {
-#pragma unroll
-        for (int e = 0; e < 4; ++e)
-            if (d + e < a.dim) out[d + e] = o[e];
-    }
+    float *const row = a.out + size_t(b) * a.q_batch + (size_t(kv) * a.group + head) * a.q_head + size_t(query) * a.q_row;
+    store_dims<VEC>(row, int(d), int(a.dim), o);
 }
 
 __device__ inline bool finite(float x) { return fabsf(x) < INFINITY; }
+
+// Floats of a row in a run's slots.
+template <int DP>
+constexpr int kSlotRow = DP <= 64 ? 64 : 128;
 
 // What joining the four waves' sums of a row takes.
 struct RowPlan {
@@ -160,7 +183,7 @@ struct RowPlan {
 // first run had it last, the others first). The block's threads do it together; `plans`
 // is LDS. True for a thread that met a sum that is not finite, or one that is not zero but
 // below `least`.
-template <int DP, int RB, int THREADS, bool VEC>
+template <int DP, int RB, bool VEC>
 __device__ inline bool finish(const RaggedArgs &a, uint32_t run, uint32_t b, uint32_t kv, uint32_t rb, bool whole,
                               bool starts, const float (&part)[kWaves][RB][DP + 4], const float2 (&ml)[kWaves][RB],
                               RowPlan (&plans)[RB], const uint64_t (&sees)[kMaxTreeNodes][kWords], float least) {
@@ -187,8 +210,8 @@ __device__ inline bool finish(const RaggedArgs &a, uint32_t run, uint32_t b, uin
             p.top_sum.y = a.nodes && !(sees[query][query / 64] >> (query & 63) & 1) ? 0.f : 1.0f / l;
         } else {
             const size_t slot = (2 * size_t(run) + starts) * RB + tid;
-            p.at = slot * DP;
-            reinterpret_cast<float2 *>(a.partial + 2 * size_t(a.runs) * RB * DP)[slot] = p.top_sum;
+            p.at = slot * kSlotRow<DP>;
+            reinterpret_cast<float2 *>(a.partial + 2 * size_t(a.runs) * RB * kSlotRow<DP>)[slot] = p.top_sum;
             p.top_sum.y = 1.f;
         }
         plans[tid] = p;
@@ -196,7 +219,7 @@ __device__ inline bool finish(const RaggedArgs &a, uint32_t run, uint32_t b, uin
     __syncthreads();
     float *const to = whole ? a.out : a.partial;
     bool odd = false;
-    for (uint32_t at = tid; at < rows * (DP / 4); at += THREADS) {
+    for (uint32_t at = tid; at < rows * (DP / 4); at += kThreads) {
         const uint32_t row = at / (DP / 4), d = at % (DP / 4) * 4;
         const RowPlan &p = plans[row];
         f32x4 o = {0.f, 0.f, 0.f, 0.f};
@@ -204,15 +227,14 @@ __device__ inline bool finish(const RaggedArgs &a, uint32_t run, uint32_t b, uin
         for (int w = 0; w < kWaves; ++w) o += p.weights[w] * *reinterpret_cast<const f32x4 *>(&part[w][row][d]);
         if (p.top_sum.y != 0.f && d < uint32_t(a.dim))
 #pragma unroll
-            for (int e = 0; e < 4; ++e) odd |= !finite(o[e]) || (fabsf(o[e]) < least && o[e] != 0.f);
+            for (int e = 0; e < 4; ++e)
+                odd |= (VEC || d + e < uint32_t(a.dim)) && (!finite(o[e]) || (fabsf(o[e]) < least && o[e] != 0.f));
         // A slot without a node is zeros whatever its sums are.
         o = p.top_sum.y == 0.f ? f32x4{0.f, 0.f, 0.f, 0.f} : o * p.top_sum.y;
         if (VEC || !whole) {
             if (!whole || d < uint32_t(a.dim)) *reinterpret_cast<f32x4 *>(to + p.at + d) = o;
         } else {
-#pragma unroll
-            for (int e = 0; e < 4; ++e)
-                if (d + e < uint32_t(a.dim)) to[p.at + d + e] = o[e];
+            store_dims<false>(to + p.at, int(d), int(a.dim), o);
         }
     }
     return odd;
@@ -226,7 +248,7 @@ __device__ inline void see_ancestors(uint32_t nodes, float mine, uint64_t (&sees
     __syncthreads();
     const int n = threadIdx.x;
     int parent = -2;
-    if (nodes <= 64) {  // one wave by itself (4.4 us less a step than by all, with their barriers)
+    if (nodes <= 64) {  // one wave by itself, without barriers (28 nodes: 32.0 us of a launch by all, 29.9 so)
         if (n < 64) {
             if (n < int(nodes)) parent = is_node(mine, n) ? int(mine) : -2;
             uint32_t lo = parent != -2 && n < 32 ? 1u << n : 0u, hi = parent != -2 && n >= 32 ? 1u << (n - 32) : 0u;

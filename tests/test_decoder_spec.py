@@ -109,7 +109,7 @@ def test_rows_too_far_apart_for_a_kernels_offsets_take_another():
         return jade_hip.spec_describe(dict(CROSS, batch=1, heads=65535, kv_heads=65535, queries=17, keys=5, **more))["launch"]["kernel"]
 
     # 128 keys, 65535 heads of 128 apart, span more than 2 GiB.
-    assert kernel(dim=128, token_major=True) == "attention_ragged_d128_r32"
+    assert kernel(dim=128, token_major=True) == "attention_ragged_d128"
     assert kernel(dim=128, token_major=False) == "attention_flash_ragged_d128"
     # 2^29 elements of one head's queries.
     far = jade_hip.spec_describe(dict(CROSS, batch=1, heads=1, kv_heads=1, queries=2 ** 23, keys=1000, dim=64))

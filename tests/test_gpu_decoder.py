@@ -290,7 +290,7 @@ def test_attention_tree_shapes_of_trees(runtime, kind, nodes):
     assert (got.reshape(want.shape)[:, :, absent] == 0).all()
 
 
-@pytest.mark.parametrize("nodes,dim", [(5, 64), (20, 128), (70, 36), (9, 30)])
+@pytest.mark.parametrize("nodes,dim", [(5, 64), (20, 128), (70, 36), (9, 30), (40, 80), (20, 91)])
 def test_attention_tree_non_finite_values_stay_in_their_branch(runtime, nodes, dim):
     # Two chains; the first's last node is infinite and NaN in k, v and q, absent slots and the cache past its
     # length hold NaN. The second chain, and the first's earlier nodes, do not notice.
@@ -475,7 +475,7 @@ def test_two_kernels_of_one_shape_and_two_contexts(runtime):
         within(y, *dec.cross(spec, x["q"], x["k"], x["v"], [2000]))
 
 
-@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("dim", [64, 96, 128])
 @pytest.mark.parametrize("heads", [16, 20, 40])
 @pytest.mark.parametrize("q_scale,k_scale,v_scale", [(1.0, 1.0, 2.0 ** -120), (1.0, 1.0, 2.0 ** -60), (2.0 ** -120, 1.0, 1.0),
                                                     (1.0, 2.0 ** -120, 1.0), (2.0 ** -80, 2.0 ** 80, 2.0 ** 100),
@@ -505,11 +505,10 @@ def test_attention_cross_head_dims(runtime, heads, dim, token_major):
 
 
 # (batch, heads, kv_heads, queries, keys, dim) of each kernel, more sequences than a wave scans at once among them.
-KERNELS = {"attention_ragged_d64_r16": (70, 4, 2, 3, 90, 40), "attention_ragged_d128_r16": (3, 2, 1, 8, 200, 100),
-           "attention_ragged_d64_r32": (3, 6, 2, 9, 150, 31), "attention_ragged_d64_r64": (70, 1, 1, 40, 70, 63),
-           "attention_ragged_d128_r32": (3, 1, 1, 30, 150, 101), "attention_ragged_d128_r64": (3, 2, 1, 35, 130, 127),
-           "attention_ragged_parts_d64_r32": (3, 2, 1, 12, 500, 64), "attention_ragged_parts_d64_r64": (3, 2, 1, 40, 500, 60),
-           "attention_ragged_parts_d128_r32": (3, 5, 1, 6, 400, 128), "attention_ragged_parts_d128_r64": (3, 2, 1, 33, 300, 84),
+KERNELS = {"attention_ragged_d64": (70, 4, 2, 3, 90, 39), "attention_ragged_d128": (3, 2, 1, 8, 200, 101),
+           "attention_ragged_parts_d64_r32": (3, 6, 2, 9, 150, 31), "attention_ragged_parts_d64_r64": (70, 1, 1, 40, 70, 63),
+           "attention_ragged_parts_d96_r32": (3, 4, 1, 8, 390, 80), "attention_ragged_parts_d96_r64": (66, 1, 1, 50, 129, 95),
+           "attention_ragged_parts_d128_r32": (3, 5, 1, 6, 400, 128), "attention_ragged_parts_d128_r64": (3, 2, 1, 35, 130, 127),
            "attention_flash_ragged_d32": (90, 8, 4, 20, 40, 24), "attention_flash_ragged_d64": (90, 4, 4, 33, 70, 60),
            "attention_flash_ragged_d96": (70, 10, 5, 17, 33, 84), "attention_flash_ragged_d128": (66, 8, 4, 50, 35, 116)}
 
@@ -560,6 +559,27 @@ def test_what_the_parts_do_not_carry(runtime, kernel):
     within(got[2, group:], want[2, group:], off[2, group:]) if group < spec["heads"] else None
 
 
+@pytest.mark.parametrize("heads", [4, 20, 40])
+@pytest.mark.parametrize("dim", [1, 30, 61, 67, 68, 80, 127])
+@pytest.mark.parametrize("token_major", [False, True])
+def test_what_lies_behind_a_row_that_is_not_whole_vectors(runtime, heads, dim, token_major):
+    # Infinities and NaN in the other kv head, whose rows begin where a last vector of this one's ends, and (in
+    # another sequence) in this head's next key, which is past the length.
+    rng = np.random.default_rng(43)
+    spec = cross_spec(2, 2 * heads, 2, 1, 140, dim, token_major)
+    x = cross_inputs(rng, spec, [140, 77])
+    want, off = dec.cross(spec, x["q"], x["k"], x["v"], [140, 77])
+    for n, bad in (("k", np.nan), ("v", np.inf)):
+        rows = dec.by_token(x[n], token_major)  # [batch, key, kv head, dim]
+        rows[0, :, 1] = bad
+        rows[1, 77:] = bad
+    got = dec.by_token(run(runtime, spec, x)["out"].reshape(x["q"].shape), token_major)
+    want, off = dec.by_token(want, token_major), dec.by_token(off, token_major)
+    within(got[0, :, :heads], want[0, :, :heads], off[0, :, :heads])
+    assert not np.isfinite(got[0, :, heads:]).any()
+    within(got[1], want[1], off[1])
+
+
 @pytest.mark.parametrize("nodes,dim", [(9, 64), (40, 128), (17, 30)])
 def test_attention_tree_many_sequences(runtime, nodes, dim):
     rng = np.random.default_rng(42)
@@ -573,7 +593,7 @@ def test_attention_tree_many_sequences(runtime, nodes, dim):
     within(got[some], want, off)
 
 
-@pytest.mark.parametrize("heads,dim", [(16, 64), (20, 128), (40, 64), (40, 128), (20, 36)])
+@pytest.mark.parametrize("heads,dim", [(16, 64), (20, 128), (40, 64), (40, 128), (20, 36), (20, 96), (40, 80), (40, 87)])
 def test_attention_cross_not_finite_among_many_rows(runtime, heads, dim):
     # One row's query, one key's value: the others' outputs are as without them.
     rng = np.random.default_rng(32)
