@@ -348,11 +348,12 @@ bool on_parts(const RaggedShape &s) {
 uint32_t block_rows(const RaggedShape &s) { return !on_parts(s) ? 16 : rows_of(s) <= 32 ? 32 : 64; }
 uint32_t row_blocks(const RaggedShape &s) { return (rows_of(s) + block_rows(s) - 1) / block_rows(s); }
 
-uint64_t ragged_tiles(const RaggedShape &s) {
+// Tiles of a (sequence, kv head, row block) of full length, and of a launch of such.
+uint32_t unit_tiles(const RaggedShape &s) {
     const uint32_t tile = on_parts(s) ? kPartsTile : kTile;
-    const uint64_t tiles = (uint64_t(s.keys) + tile - 1) / tile + (s.nodes + tile - 1) / tile;
-    return uint64_t(s.batch) * s.kv_heads * row_blocks(s) * tiles;
+    return (s.keys + tile - 1) / tile + (s.nodes + tile - 1) / tile;
 }
+uint64_t ragged_tiles(const RaggedShape &s) { return uint64_t(s.batch) * s.kv_heads * row_blocks(s) * unit_tiles(s); }
 
 // Queries of an encoder's states may go to the flash kernel (attention_flash.hip), which
 // splits K and V once for 128 or 256 rows but has one block for them and all their keys.
@@ -378,13 +379,18 @@ bool on_flash(const RaggedShape &s) {
     return flash < parts;
 }
 
-// Runs of a launch: as many blocks as the chip holds at once (one a CU on parts, else two),
-// or one per tile where there can be no more tiles. Three a CU, where the registers allow
-// it (dims to 64): 36 x 20 heads x 1101 keys 61.6 -> 57.0 us, but 8 x 16 x 4096 52.4 -> 55.1
-// and 64 x 8 x 100 11.3 -> 13.3.
+// Runs of a launch: as many blocks as work best on a CU, or one per tile where there can be
+// no more tiles.
+// 16 rows: two. Three, where the registers allow it (dims to 64): 36 x 20 heads x 1101 keys
+// 61.6 -> 57.0 us, but 8 x 16 x 4096 52.4 -> 55.1 and 64 x 8 x 100 11.3 -> 13.3.
+// On parts one, which overlaps its own work; but two of 32 rows and dims to 64, which the
+// registers allow, where units are short and mostly begin and end: 19 nodes x 50 x 16 heads
+// over 119 keys of 40 42.0 -> 32.4, 28 nodes x 5 x 28 heads over at most 1391 of 18 35.0 ->
+// 24.7, but 30 nodes x 2 x 8 heads over at most 5000 of 33 24.4 -> 26.4.
 uint32_t runs_of(const RaggedShape &s) {
     const uint64_t tiles = ragged_tiles(s);
-    const uint32_t most = on_parts(s) ? kCus : 2 * kCus;
+    const bool two = !on_parts(s) || (block_rows(s) == 32 && s.dim <= 64 && unit_tiles(s) <= 16);
+    const uint32_t most = two ? 2 * kCus : kCus;
     return tiles >= most ? most : uint32_t((tiles + 7) / 8 * 8);
 }
 

@@ -8,7 +8,7 @@
 // Q, which the four waves share. A last chunk that is not whole reads into the next row (or
 // nothing past the tile): Q's parts are zeros there, and V's dims past the last are dropped.
 //
-// One wave a SIMD, so it overlaps its own work: an MFMA every 32 cycles, and between
+// One wave a SIMD (but for 32 rows of few dims), so it overlaps its own work: an MFMA every 32 cycles, and between
 // two of them two of the twelve pieces in which the next eight values of K or V are
 // split; a chunk is loaded again, for the next tile, as soon as it is split. For 64
 // rows and 32 keys of 128 dims that is 192 MFMAs (6144 cycles of a SIMD; FP32 MFMAs
@@ -86,6 +86,7 @@ struct Shape {
     // Where K and V of a tile are loaded: each chunk as soon as the last tile's is split,
     // or, where two row groups leave no registers for all of both, V before the scores
     // and K before and amid the outputs.
+    static constexpr int kWavesASimd = QG == 1 && DP <= 64 ? 2 : 1;  // what the registers hold
     static constexpr bool kEarly = QG == 1 || DP <= 96;
     static constexpr int kEarlyK = kEarly ? kSteps : 0;
     static_assert(QG * kSteps * kParts * 1024 <= kWaves * kRows * kPitch * 4, "Q's parts fit the sums' space");
@@ -93,7 +94,8 @@ struct Shape {
 
 // QG: groups of 32 rows, all of them every wave's.
 template <int DP, int QG, bool VEC>
-__global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(1, 1))) void
+__global__ __launch_bounds__(kThreads)
+__attribute__((amdgpu_waves_per_eu(Shape<DP, QG>::kWavesASimd, Shape<DP, QG>::kWavesASimd))) void
 attention_ragged_parts(RaggedArgs a) {
     using S = Shape<DP, QG>;
     constexpr int KS = S::kSteps, NB = S::kOut, RB = S::kRows;
