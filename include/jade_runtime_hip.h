@@ -77,7 +77,10 @@ int jr_execute(void *ctx, const jr_job *jobs, size_t job_count, uint32_t repeats
  * format of src/runtime/ir.rs:6-84), validates it under the HIP rules and
  * writes a JSON description: canonical spec, name, bindings (ir.rs:269-339),
  * the HIP launch shape, whether the reference's own rules (ir.rs:193-268)
- * accept it, and whether this backend runs it. */
+ * accept it, and whether this backend runs it. Besides the reference's
+ * operations these are those of a decoder's step: rotary, qk_norm_rotary,
+ * attention_tree, cache_append and attention_cross, FP32 like the others, with
+ * lengths, parents and picks as FP32 whole numbers. */
 int jr_spec_describe(const char *spec_json, size_t len, char *out, size_t out_cap, char *err, size_t cap);
 
 /* KernelSpec::validate_bindings, src/runtime/ir.rs:340-367, context-free:
