@@ -611,3 +611,18 @@ def test_attention_cross_not_finite_among_many_rows(runtime, heads, dim):
     kept = [d for d in range(dim) if d != 3]
     within(got[1][..., kept], want[1][..., kept], off[1][..., kept])
     assert np.isneginf(got[1, :, 0, 3]).all()
+
+
+@pytest.mark.parametrize("queries,dim", [(1, 8), (20, 8), (40, 12)])
+def test_thousands_of_sequences(runtime, queries, dim):
+    # Forty-seven scans of 64 sequences, most of them empty, so that runs begin far from each other.
+    batch = 3000
+    rng = np.random.default_rng(44)
+    spec = cross_spec(batch, 1, 1, queries, 150, dim)
+    lengths = np.where(rng.random(batch) < 0.7, 0, rng.integers(0, 151, batch))
+    x = cross_inputs(rng, spec, lengths)
+    got = run(runtime, spec, x)["out"].reshape(x["q"].shape)
+    assert (got[lengths == 0] == 0).all() and np.isfinite(got).all()
+    some = [0, 63, 64, 1500, 2999] + list(np.flatnonzero(lengths)[::90])
+    want, off = dec.cross(dict(spec, batch=len(some)), *(x[n][some] for n in "qkv"), lengths[some])
+    within(got[some], want, off)
