@@ -75,61 +75,82 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2, 2))
             voff[j][i] = d < a.dim ? uint32_t(16 * wave + 4 * g + i) * row_bytes + uint32_t(d) * 4u : kDeadOffset;
         }
 
+    // The part of a (sequence, kv head, row block) that tile t of the launch begins in this
+    // run; nothing where the run is over.
+    struct Unit {
+        uint32_t b, before, kv, rb, begin, end, tiles, len, cached;
+    };
+    auto unit_at = [&](uint32_t t, uint32_t b, uint32_t before) {
+        Unit u{};
+        if (t >= t_stop) return u;
+        for (u.b = b, u.before = before;; ++u.b) {  // the run ends with a sequence that has tiles
+            u.len = spread.length(u.b);
+            u.cached = (u.len + kTile - 1) / kTile;
+            u.tiles = u.cached + spread.draft_tiles;
+            if (u.tiles) break;
+        }
+        const uint32_t in = t - before * units, unit = in / u.tiles;
+        u.begin = in - unit * u.tiles;
+        u.kv = unit / a.row_blocks;
+        u.rb = unit - u.kv * a.row_blocks;
+        u.end = min(u.tiles, u.begin + (t_stop - t));
+        return u;
+    };
+    // Tile x of a unit's keys or values: its own descriptor (no offset passes 2^31, however
+    // long the cache), which ends with its last key's row; past `end` it holds nothing.
+    auto tile_of = [&](const float *caches, const float *drafts, const Unit &u, uint32_t x) {
+        const bool drafted = x >= u.cached;
+        const uint32_t at = drafted ? x - u.cached : x, left = (drafted ? a.nodes : u.len) - at * kTile;
+        const float *from = (drafted ? drafts + (u.b * a.d_batch + u.kv * a.d_head) : caches + (u.b * a.k_batch + u.kv * a.k_head)) +
+                            size_t(at) * kTile * a.k_row;
+        const uint32_t bytes = x < u.end ? (min(left, uint32_t(kTile)) - 1) * row_bytes + uint32_t(a.dim) * 4u : 0u;
+        return __builtin_amdgcn_make_buffer_rsrc(const_cast<float *>(from), 0, int(bytes), int(kRawBuffer));
+    };
+    // A last chunk that is not whole reads into the next row, or nothing past the tile.
+    auto load = [&](__amdgpu_buffer_rsrc_t from, uint32_t at) {
+        return __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(from, int(at), 0, 0));
+    };
+    f32x4 kf[KJ], vf[NJ][4], qf[KJ];
+    auto load_k = [&](const Unit &u, uint32_t x) {
+        const auto from = tile_of(a.k, a.kd, u, x);
+#pragma unroll
+        for (int j = 0; j < KJ; ++j) kf[j] = load(from, koff[j]);
+    };
+    auto load_v = [&](const Unit &u, uint32_t x) {
+        const auto from = tile_of(a.v, a.vd, u, x);
+#pragma unroll
+        for (int j = 0; j < NJ; ++j)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) vf[j][i] = load(from, voff[j][i]);
+    };
     uint32_t tree = ~0u;  // the sequence whose tree is in LDS
-    while (t < t_stop) {
-        const uint32_t len = spread.length(b);
-        const uint32_t cached = (len + kTile - 1) / kTile, tiles = cached + spread.draft_tiles;
-        if (!tiles) {
-            ++b;
-            continue;
-        }
-        const uint32_t in = t - before * units, unit = in / tiles, begin = in - unit * tiles;
-        const uint32_t kv = unit / a.row_blocks, rb = unit - kv * a.row_blocks;
-        const uint32_t end = min(tiles, begin + (t_stop - t));
-        const bool whole = begin == 0 && end == tiles;
-        float above_me = 0.f;
-        if (end > cached && tree != b && tid < int(a.nodes)) above_me = a.parents[size_t(b) * a.nodes + tid];
-
-        const float *kb = a.k + size_t(b) * a.k_batch + size_t(kv) * a.k_head;
-        const float *vb = a.v + size_t(b) * a.k_batch + size_t(kv) * a.k_head;
-        const float *kd = a.kd + size_t(b) * a.d_batch + size_t(kv) * a.d_head;
-        const float *vd = a.vd + size_t(b) * a.d_batch + size_t(kv) * a.d_head;
-        // Tile x of a tensor: its own descriptor (no offset passes 2^31, however long
-        // the cache), which ends with its last key's row; past `end` it holds nothing.
-        auto tile_of = [&](const float *cache, const float *draft, uint32_t x) {
-            const bool drafted = x >= cached;
-            const uint32_t at = drafted ? x - cached : x, left = (drafted ? a.nodes : len) - at * kTile;
-            const float *from = (drafted ? draft : cache) + size_t(at) * kTile * a.k_row;
-            const uint32_t bytes = x < end ? (min(left, uint32_t(kTile)) - 1) * row_bytes + uint32_t(a.dim) * 4u : 0u;
-            return __builtin_amdgcn_make_buffer_rsrc(const_cast<float *>(from), 0, int(bytes), int(kRawBuffer));
-        };
-        // A last chunk that is not whole reads into the next row, or nothing past the tile.
-        auto load = [&](__amdgpu_buffer_rsrc_t from, uint32_t at) {
-            return __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(from, int(at), 0, 0));
-        };
-        f32x4 kf[KJ], vf[NJ][4];
-        auto load_k = [&](uint32_t x) {
-            const auto from = tile_of(kb, kd, x);
+    float above_me = 0.f;
+    // Q^T operand: row m of the block, dims 16 j + 4 g + e; and what the tree is made of.
+    auto load_rows = [&](const Unit &u) {
+        if (u.begin == u.end) return;
+        if (u.end > u.cached && tree != u.b && tid < int(a.nodes)) above_me = a.parents[size_t(u.b) * a.nodes + tid];
+        const uint32_t r = u.rb * RB + m, head = r / a.queries, query = r - head * a.queries;
+        const float *row = a.q + size_t(u.b) * a.q_batch + (size_t(u.kv) * a.group + head) * a.q_head + size_t(query) * a.q_row;
 #pragma unroll
-            for (int j = 0; j < KJ; ++j) kf[j] = load(from, koff[j]);
-        };
-        auto load_v = [&](uint32_t x) {
-            const auto from = tile_of(vb, vd, x);
+        for (int j = 0; j < KJ; ++j) qf[j] = load_dims<VEC>(head < a.group ? row : nullptr, 16 * j + 4 * g, a.dim);
+    };
+    Unit u = unit_at(t, b, before);
+    load_k(u, u.begin);
+    load_v(u, u.begin);
+    load_rows(u);
+    while (u.begin < u.end) {
+        const uint32_t begin = u.begin, end = u.end, cached = u.cached, len = u.len;
+        const bool whole = begin == 0 && end == u.tiles;
+        // The unit after this one, whose first loads go beside this one's last products (64 x 32
+        // heads (8 of keys) over at most 512 keys of 128, 4 nodes: 53.7 -> 51.9 us; 1024 x 4
+        // heads over 64 keys of 64 72.0 -> 68.7; a launch of a tile a run 8.8 -> 8.9).
+        t += end - begin;
+        const bool over = t >= (u.before + u.tiles) * units;
+        const Unit next = unit_at(t, u.b + over, over ? u.before + u.tiles : u.before);
+        auto next_k = [&](uint32_t x) { x + 1 < end ? load_k(u, x + 1) : load_k(next, next.begin); };
+        auto next_v = [&](uint32_t x) { x + 1 < end ? load_v(u, x + 1) : load_v(next, next.begin); };
 #pragma unroll
-            for (int j = 0; j < NJ; ++j)
-#pragma unroll
-                for (int i = 0; i < 4; ++i) vf[j][i] = load(from, voff[j][i]);
-        };
-        load_k(begin);
-        load_v(begin);
-        // Q^T operand in log2 units: row m of the block, dims 16 j + 4 g + e.
-        const uint32_t r = rb * RB + m, head = r / a.queries, query = r - head * a.queries;
-        f32x4 qf[KJ];
-        {
-            const float *row = a.q + size_t(b) * a.q_batch + (size_t(kv) * a.group + head) * a.q_head + size_t(query) * a.q_row;
-#pragma unroll
-            for (int j = 0; j < KJ; ++j) qf[j] = load_dims<VEC>(head < a.group ? row : nullptr, 16 * j + 4 * g, a.dim) * a.qscale;
-        }
+        for (int j = 0; j < KJ; ++j) qf[j] *= a.qscale;  // log2 units
 
         f32x4 acc[NJ][4];
         float top = -INFINITY, sum = 0.f;
@@ -182,7 +203,7 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2, 2))
         uint32_t x = begin;
         for (; x < min(end, cached); ++x) {
             score();
-            load_k(x + 1);
+            next_k(x);
             if ((x + 1) * kTile > len) {
                 const int first = int(x) * kTile + 16 * wave + 4 * g;
 #pragma unroll
@@ -191,16 +212,17 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2, 2))
             }
             weigh();
             add();
-            load_v(x + 1);
+            next_v(x);
         }
 
         if (end > cached) {
-            if (tree != b) see_ancestors(a.nodes, above_me, sees, above);
-            tree = b;
+            if (tree != u.b) see_ancestors(a.nodes, above_me, sees, above);
+            tree = u.b;
+            const uint32_t query = (u.rb * RB + m) % a.queries;  // queries == nodes; rows past the last see as others do
             for (; x < end; ++x) {
                 score();
-                load_k(x + 1);
-                const uint64_t seen = sees[query][x - cached];  // queries == nodes; rows past the last see as others do
+                next_k(x);
+                const uint64_t seen = sees[query][x - cached];
 #pragma unroll
                 for (int i = 0; i < 4; ++i)
                     if (!(seen >> (16 * wave + 4 * g + i) & 1)) p[i] = -INFINITY;
@@ -238,9 +260,10 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2, 2))
                                         if (sums[i] > 0.f) acc[j][e][i] += special(k);
                             }
                 }
-                load_v(x + 1);
+                next_v(x);
             }
         }
+        load_rows(next);
 
         // The four waves' sums joined: row m, dims 64 j + 16 g + 4 i + e.
         __syncthreads();
@@ -253,12 +276,8 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2, 2))
                 *reinterpret_cast<f32x4 *>(&part[wave][m][64 * j + 16 * g + 4 * i]) =
                     f32x4{acc[j][0][i], acc[j][1][i], acc[j][2][i], acc[j][3][i]};
         __syncthreads();
-        finish<DP, RB, VEC>(a, run, b, kv, rb, whole, begin == 0, part, ml, plans, sees, 0.f);
-        t += end - begin;
-        if (t >= (before + tiles) * units) {
-            before += tiles;
-            ++b;
-        }
+        finish<DP, RB, VEC>(a, run, u.b, u.kv, u.rb, whole, begin == 0, part, ml, plans, sees, 0.f);
+        u = next;
     }
 }
 
