@@ -23,7 +23,7 @@
 //
 // This kernel takes up to 16 rows and is bound by reading K and V: 4 nodes x 32 heads (8 of
 // keys) over 131072 keys of 128, 1.07 GB in 187 us, 5.7 TB/s; 16 x 24 heads of one query
-// over at most 1531 keys of 80, 59 us, 4.9 TB/s; one query over 1024 keys 8.7 us, which is
+// over at most 1531 keys of 80, 59 us, 4.9 TB/s; one query over 1024 keys 8.9 us, which is
 // two launches and loads that wait for one another (lengths, Q, K, the partial sums). More
 // rows go to the kernel on bf16 parts (attention_ragged_parts.hip): 64 nodes over 4
 // sequences took 169 us with FP32 MFMAs, 64 rows a block, and take 116.
@@ -101,8 +101,8 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2, 2))
     auto tile_of = [&](const float *caches, const float *drafts, const Unit &u, uint32_t x) {
         const bool drafted = x >= u.cached;
         const uint32_t at = drafted ? x - u.cached : x, left = (drafted ? a.nodes : u.len) - at * kTile;
-        const float *from = (drafted ? drafts + (u.b * a.d_batch + u.kv * a.d_head) : caches + (u.b * a.k_batch + u.kv * a.k_head)) +
-                            size_t(at) * kTile * a.k_row;
+        const size_t head = drafted ? u.b * a.d_batch + u.kv * a.d_head : u.b * a.k_batch + u.kv * a.k_head;
+        const float *from = (drafted ? drafts : caches) + head + size_t(at) * kTile * a.k_row;
         const uint32_t bytes = x < u.end ? (min(left, uint32_t(kTile)) - 1) * row_bytes + uint32_t(a.dim) * 4u : 0u;
         return __builtin_amdgcn_make_buffer_rsrc(const_cast<float *>(from), 0, int(bytes), int(kRawBuffer));
     };
@@ -130,7 +130,7 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2, 2))
         if (u.begin == u.end) return;
         if (u.end > u.cached && tree != u.b && tid < int(a.nodes)) above_me = a.parents[size_t(u.b) * a.nodes + tid];
         const uint32_t r = u.rb * RB + m, head = r / a.queries, query = r - head * a.queries;
-        const float *row = a.q + size_t(u.b) * a.q_batch + (size_t(u.kv) * a.group + head) * a.q_head + size_t(query) * a.q_row;
+        const float *row = a.q + u.b * a.q_batch + (size_t(u.kv) * a.group + head) * a.q_head + size_t(query) * a.q_row;
 #pragma unroll
         for (int j = 0; j < KJ; ++j) qf[j] = load_dims<VEC>(head < a.group ? row : nullptr, 16 * j + 4 * g, a.dim);
     };
@@ -386,9 +386,11 @@ uint64_t ragged_tiles(const RaggedShape &s) { return uint64_t(s.batch) * s.kv_he
 // 16 x 3000 x 1500 of 96 160 and 178; 4 x 8 x 256 x 1024 of 128 131 and 40.
 bool on_flash(const RaggedShape &s) {
     const uint64_t d = s.dim, heads = uint64_t(s.batch) * s.kv_heads, rows = rows_of(s), fb = flash_ragged_rows(s.dim);
-    const uint64_t q_span = s.token_major ? d * s.heads * s.queries : d * rows, k_span = (s.token_major ? d * s.kv_heads : d) * (s.keys + 128ull);
+    const uint64_t q_span = s.token_major ? d * s.heads * s.queries : d * rows;
+    const uint64_t k_span = (s.token_major ? d * s.kv_heads : d) * (s.keys + 128ull);
     // Offsets of a head's rows in 31 bits, tiles past the last one in 32; grid.y.
-    if (!on_parts(s) || s.dim % 4 || s.nodes || q_span >= 1u << 29 || k_span >= 1u << 29 || (rows + fb - 1) / fb > 65535) return false;
+    if (!on_parts(s) || s.dim % 4 || s.nodes || q_span >= 1u << 29 || k_span >= 1u << 29) return false;
+    if ((rows + fb - 1) / fb > 65535) return false;
     const uint64_t blocks = heads * ((rows + fb - 1) / fb), units = heads * row_blocks(s);
     const double full = double(rows) / double((rows + fb - 1) / fb * fb);
     const double flash = 8.0 + double((blocks + kCus - 1) / kCus) * double((s.keys + 31) / 32) *

@@ -483,7 +483,8 @@ attention_ragged_parts(RaggedArgs a) {
 #pragma unroll
                             for (int v = 0; v < 16; ++v) {
                                 const uint32_t key = 8 * (v >> 2) + 4 * h + (v & 3);
-                                const float z = NB * c + e < a.dim && key0 + key < keys ? vrow[size_t(key) * a.k_row + NB * c + e] : 0.f;
+                                const int d = NB * c + e;
+                                const float z = d < a.dim && key0 + key < keys ? vrow[size_t(key) * a.k_row + d] : 0.f;
                                 const float y = k >= 0 ? is(k, z) : finite(z) || !drafted ? z : 0.f;
                                 sums = __builtin_amdgcn_mfma_f32_32x32x2f32(y, st[r][v], sums, 0, 0, 0);
                             }

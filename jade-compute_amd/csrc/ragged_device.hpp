@@ -125,7 +125,9 @@ __device__ inline bool is_node(float parent, int n) {
 // Run of block `id`: the runs of one XCD are neighbours.
 __device__ inline uint32_t run_of(uint32_t id, uint32_t runs) { return id % 8 * (runs / 8) + id / 8; }
 
-__device__ inline float across_keys_max(float x) { return fmaxf(fmaxf(x, __shfl_xor(x, 16)), fmaxf(__shfl_xor(x, 32), __shfl_xor(x, 48))); }
+__device__ inline float across_keys_max(float x) {
+    return fmaxf(fmaxf(x, __shfl_xor(x, 16)), fmaxf(__shfl_xor(x, 32), __shfl_xor(x, 48)));
+}
 __device__ inline float across_keys_sum(float x) {
     x += __shfl_xor(x, 16);
     return x + __shfl_xor(x, 32);
