@@ -146,6 +146,9 @@ attention_flash(const float *__restrict__ Q, const float *__restrict__ K, const 
         base = qbase = size_t(head) * size_t(seq) * size_t(dim);
         head_bytes = q_bytes = uint32_t(seq) * row_bytes;
     }
+    // Row qi of q and out from qbase, in elements; of `seq` rows of dims it is made anew where
+    // it is needed, so that no register keeps it across the main loop.
+    auto row_at = [&]() __attribute__((always_inline)) { return kRagged ? size_t(qoff / 4u) : size_t(qi) * dim; };
     const int t_end = ((CAUSAL ? min(seq, qb * kBQ + kBQ) : keys) + kKeys - 1) / kKeys;
 
     // Q^T operand: step s holds dims 16s + 8h + e of query qi, in log2 units.
@@ -649,8 +652,8 @@ attention_flash(const float *__restrict__ Q, const float *__restrict__ K, const 
 #pragma unroll
         for (int b = 0; b < NB; ++b) acc[b] = f32x16{};
         const bool mine = qi < seq;
-        const float *qrow = reinterpret_cast<const float *>(reinterpret_cast<const char *>(Q + qbase) + (mine ? qoff : 0u));
-        const size_t pitch = row_bytes / 4u;
+        const float *qrow = Q + qbase + (mine ? row_at() : 0);
+        const size_t pitch = kRagged ? row_bytes / 4u : uint32_t(dim);
         for (int t = 0; t < t_end && live(t); ++t) {
             const int key = t * kKeys + c;
             const float *krow = K + base + size_t(min(key, keys - 1)) * pitch;
@@ -700,7 +703,7 @@ attention_flash(const float *__restrict__ Q, const float *__restrict__ K, const 
     row_sum = halves_sum(row_sum);
     if (qi < seq) {
         const float inv = unscale / row_sum;
-        float *orow = reinterpret_cast<float *>(reinterpret_cast<char *>(O + qbase) + qoff);
+        float *orow = O + qbase + row_at();
         // LDS row r of V is dim 2r (r < DP / 2) or 2 (r - DP / 2) + 1, and a
         // lane holds rows 32b + 8 (v >> 2) + 4h + (v & 3): r, r + 1 and their
         // odd partners are four adjacent dims.
