@@ -18,9 +18,12 @@
 // nodes over 8 sequences: 71 us, 3.0 TB/s of K and V. A run's unit costs 8 to 11 us besides
 // its tiles: Q's loads and parts, the first tile's loads, the waves' sums joined.
 //
-// Q is scaled up before it is split (the scores are scaled back where their maximum is
-// taken off), so every finite Q is carried exactly; parts of K below 2^-109 lose bits
-// below 2^-134, which move no score: a query is at most 2^64. What the parts do not carry
+// Q is scaled up and K down before they are split, so every finite Q is carried exactly and
+// scores are in FP32's own range (with K as it is, they passed it from 2^104 on, and one at
+// -inf weighs nothing without a trace in the sums); a K below 2^-86 loses less than 2^-110,
+// which moves no score by more than 2^-46 a dim: a query is at most 2^64. The scaling is
+// beside the MFMAs (64 nodes as above 119 -> 118 us, 13 nodes 67.3 -> 68.2; a look at the
+// scores of each tile instead cost 1-2%). What the parts do not carry
 // (sums that are not finite, queries past 2^64, outputs so small that bits of V below
 // 2^-134 count) the block notices when it joins its sums, and does them again with FP32
 // MFMAs.
@@ -38,7 +41,7 @@ using namespace split;
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 
 constexpr int kTile = 128;  // keys per tile, 32 for each wave by keys
-constexpr float kMostQ = 0x1p64f * kScaleQ, kUnscaleS = 1.f / kScaleQ;
+constexpr float kMostQ = 0x1p64f * kScaleQ;
 // Sums of V times weights of at least 2^-8 (the lazy maximum) in all: below this an error
 // of 2^-134 a key is more than 2^-40 of them.
 constexpr float kLeastOut = 0x1p-70f;
@@ -274,8 +277,7 @@ attention_ragged_parts(RaggedArgs a) {
         };
         // The running maximum of the rows past this tile's scores; what was summed so far
         // is scaled to it.
-        // The scores come `unit` times as large as they are.
-        auto raise = [&](float unit) __attribute__((always_inline)) {
+        auto raise = [&]() __attribute__((always_inline)) {
 #pragma unroll
             for (int r = 0; r < QG; ++r) {
                 top[r] = state[r][lane].x;
@@ -283,8 +285,8 @@ attention_ragged_parts(RaggedArgs a) {
                 float most = st[r][0];
 #pragma unroll
                 for (int v = 1; v < 16; ++v) most = fmaxf(most, st[r][v]);
-                if (__any(most * unit > top[r] + kLazyMax)) {
-                    const float reached = fmaxf(top[r], halves_max(most) * unit);
+                if (__any(most > top[r] + kLazyMax)) {
+                    const float reached = fmaxf(top[r], halves_max(most));
                     const float keep = reached == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(top[r] - reached);
                     top[r] = reached;
                     sum[r] *= keep;
@@ -298,8 +300,8 @@ attention_ragged_parts(RaggedArgs a) {
             for (int r = 0; r < QG; ++r) state[r][lane] = float2{top[r], sum[r]};
         };
         // Score v of row group r to its weight.
-        auto weigh = [&](int r, int v, float unit) __attribute__((always_inline)) {
-            const float weight = __builtin_amdgcn_exp2f(fmaf(st[r][v], unit, top[r] == -INFINITY ? 0.f : -top[r]));
+        auto weigh = [&](int r, int v) __attribute__((always_inline)) {
+            const float weight = __builtin_amdgcn_exp2f(st[r][v] - (top[r] == -INFINITY ? 0.f : top[r]));
             sum[r] += weight;
             return weight;
         };
@@ -321,7 +323,7 @@ attention_ragged_parts(RaggedArgs a) {
         auto values = [&](int q, int pair) __attribute__((always_inline)) {
             const int s = (q + 1) % (KS + 2 * NB), o = s - KS;
             if (s < KS) {
-                const f32x4 k = kf[s][pair / 2];
+                const f32x4 k = kf[s][pair / 2] * kScaleK;
                 return pair % 2 ? f32x2{k.z, k.w} : f32x2{k.x, k.y};
             }
             return f32x2{vf[o / NB][2 * pair][o % NB], vf[o / NB][2 * pair + 1][o % NB]};
@@ -368,13 +370,13 @@ attention_ragged_parts(RaggedArgs a) {
             });
             __builtin_amdgcn_sched_barrier(0);
             mask(x);
-            raise(kUnscaleS);
+            raise();
             // Weights and their parts, of keys 0 .. 15 here, of 16 .. 31 beside the first outputs.
             uint32_t pp[QG][2][kParts][4];
             f32x2 prest[2];
             auto split_p = [&](int r, int s, int n) __attribute__((always_inline)) {
                 const int v = 8 * s + 2 * pair_of(n);
-                if (n % 6 < 2) prest[n % 2] = f32x2{weigh(r, v, kUnscaleS), weigh(r, v + 1, kUnscaleS)};
+                if (n % 6 < 2) prest[n % 2] = f32x2{weigh(r, v), weigh(r, v + 1)};
                 split_piece(n, prest, pp[r][s]);
             };
 #pragma unroll
@@ -467,11 +469,11 @@ attention_ragged_parts(RaggedArgs a) {
                     }
                 }
                 mask(x);
-                raise(1.f);
+                raise();
 #pragma unroll
                 for (int r = 0; r < QG; ++r)
 #pragma unroll
-                    for (int v = 0; v < 16; ++v) st[r][v] = weigh(r, v, 1.f);
+                    for (int v = 0; v < 16; ++v) st[r][v] = weigh(r, v);
                 keep_state();
                 // Drafted values that are not finite, which not every row may see: the finite
                 // ones, then the weight that each row gives to each special one.

@@ -1,0 +1,69 @@
+"""Operands at the ends of FP32's range in the attention of a decoder's step, on every kernel: bf16 parts have to carry
+them as FP32 does, or what they do not carry has to be noticed and done in FP32. The operands are chosen so that FP32 sums
+are exact or one key takes all, so the tolerances are a few roundings."""
+import numpy as np
+import pytest
+
+import decoder_oracle as dec
+import jade_hip
+import test_gpu_decoder as base
+
+pytestmark = pytest.mark.gpu
+
+KERNELS = base.KERNELS
+
+
+def query_of(dim):
+    """A query element that is eight bits after the kernels' scaling, log2(e) / sqrt(dim)."""
+    scale = np.float32(1) / np.sqrt(np.float32(dim)) * np.float32(1.44269504088896340736)
+    for bits in range(128, 256):
+        want = np.float32(bits * 2.0 ** 51)
+        for q in (want / scale, np.nextafter(want / scale, np.float32(0)), np.nextafter(want / scale, np.float32(np.inf))):
+            if q * scale == want:
+                return q
+    raise AssertionError(dim)
+
+
+@pytest.mark.parametrize("kernel", KERNELS)
+@pytest.mark.parametrize("single", [True, False])
+def test_scores_of_minus_ten_to_the_36(runtime, kernel, single):
+    # Scores that FP32 holds, but not times 2^24 (the scale of Q's parts), all their products of one sign. One key has
+    # the least of them by a factor of two, or is the only one: its weight is 1, all others are 0, the output is its
+    # value. Off by the division: 2.
+    spec = base.cross_spec(*KERNELS[kernel])
+    assert jade_hip.spec_describe(spec)["launch"]["kernel"] == kernel
+    rng = np.random.default_rng(50)
+    b, n = spec["batch"], spec["keys"]
+    lengths = [1] * b if single else [n, n - 1, max(2, n // 2)] + [n] * (b - 3)
+    x = base.cross_inputs(rng, spec, lengths)
+    wins = [int(rng.integers(0, length)) for length in lengths]
+    x["q"][:] = query_of(spec["dim"])
+    x["k"][:] = -(2.0 ** 58)
+    for i, win in enumerate(wins):
+        x["k"][i, :, win] = -(2.0 ** 57)
+    got = base.run(runtime, spec, x)["out"].reshape(x["q"].shape)
+    group = spec["heads"] // spec["kv_heads"]
+    for i, win in enumerate(wins):
+        want = np.repeat(x["v"][i, :, win], group, axis=0)[:, None, :].astype(np.float64)
+        want = np.broadcast_to(want, got[i].shape)
+        base.within(got[i], want, 2 * dec.U * np.abs(want))
+
+
+@pytest.mark.parametrize("heads", [5, 20, 40, 300])
+@pytest.mark.parametrize("dim", [64, 96, 100, 128])
+@pytest.mark.parametrize("keys", [7, 300])
+def test_scores_whose_dims_cancel(runtime, heads, dim, keys):
+    # The first key's score is -2a + a + a = 0 like all others', in exact steps, but -2a times 2^24 is past FP32's
+    # range. So all weights are 1 and the output is the mean, which the first key's value dominates.
+    rng = np.random.default_rng(51)
+    spec = base.cross_spec(1, heads, 1, 1, keys, dim)
+    x = base.cross_inputs(rng, spec, [keys])
+    x["q"][:] = query_of(dim)
+    x["k"][:] = 0
+    x["k"][0, 0, 0, [0, 16, 32]] = [-(2.0 ** 46), 2.0 ** 45, 2.0 ** 45]
+    x["v"][0, 0, 0] += np.float32(keys)
+    values = x["v"][0, 0].astype(np.float64)
+    want = np.broadcast_to(values.mean(axis=0), (heads, 1, dim))
+    # One rounding a key, and as in attend() 16 for joining and dividing.
+    off = dec.U * (keys + 16) * np.broadcast_to(np.abs(values).mean(axis=0), want.shape)
+    base.within(base.run(runtime, spec, x)["out"], want[None], off[None])
