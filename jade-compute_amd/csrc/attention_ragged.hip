@@ -276,7 +276,7 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2, 2))
                 *reinterpret_cast<f32x4 *>(&part[wave][m][64 * j + 16 * g + 4 * i]) =
                     f32x4{acc[j][0][i], acc[j][1][i], acc[j][2][i], acc[j][3][i]};
         __syncthreads();
-        finish<DP, RB, VEC>(a, run, u.b, u.kv, u.rb, whole, begin == 0, part, ml, plans, sees, 0.f);
+        finish<DP, RB, VEC>(a, run, u.b, u.kv, u.rb, whole, begin == 0, part, ml, plans, sees, 1.f);
         u = next;
     }
 }

@@ -18,15 +18,15 @@
 // nodes over 8 sequences: 71 us, 3.0 TB/s of K and V. A run's unit costs 8 to 11 us besides
 // its tiles: Q's loads and parts, the first tile's loads, the waves' sums joined.
 //
-// Q is scaled up and K down before they are split, so every finite Q is carried exactly and
-// scores are in FP32's own range (with K as it is, they passed it from 2^104 on, and one at
-// -inf weighs nothing without a trace in the sums); a K below 2^-86 loses less than 2^-110,
-// which moves no score by more than 2^-46 a dim: a query is at most 2^64. The scaling is
-// beside the MFMAs (64 nodes as above 119 -> 118 us, 13 nodes 67.3 -> 68.2; a look at the
-// scores of each tile instead cost 1-2%). What the parts do not carry
-// (sums that are not finite, queries past 2^64, outputs so small that bits of V below
-// 2^-134 count) the block notices when it joins its sums, and does them again with FP32
-// MFMAs.
+// Q and V are scaled up and K down before they are split. So every finite Q and V is
+// carried exactly (V as it is left nothing of values below 2^-134), and scores are in FP32's
+// own range (with K as it is they passed it from 2^104 on, and a score of -inf weighs
+// nothing without a trace in the sums). A K below 2^-86 loses less than 2^-110, which moves
+// no score by more than 2^-46 a dim: a query is at most 2^64. The scaling is beside the
+// MFMAs: in one run 13 nodes as above took 67.3 us without it and with it, 64 nodes 119.1
+// and 115.4 (a look at the scores of each tile instead cost 1-2%). What the parts do not
+// carry (sums that are not finite, queries past 2^64) the block notices when it joins its
+// sums, and does them again with FP32 MFMAs.
 #include "kernels.hpp"
 #include "ragged_device.hpp"
 #include "split_bf16.hpp"
@@ -42,9 +42,6 @@ typedef float f32x16 __attribute__((ext_vector_type(16)));
 
 constexpr int kTile = 128;  // keys per tile, 32 for each wave by keys
 constexpr float kMostQ = 0x1p64f * kScaleQ;
-// Sums of V times weights of at least 2^-8 (the lazy maximum) in all: below this an error
-// of 2^-134 a key is more than 2^-40 of them.
-constexpr float kLeastOut = 0x1p-70f;
 
 __device__ inline float halves_max(float x) {
     const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
@@ -326,7 +323,7 @@ attention_ragged_parts(RaggedArgs a) {
                 const f32x4 k = kf[s][pair / 2] * kScaleK;
                 return pair % 2 ? f32x2{k.z, k.w} : f32x2{k.x, k.y};
             }
-            return f32x2{vf[o / NB][2 * pair][o % NB], vf[o / NB][2 * pair + 1][o % NB]};
+            return f32x2{vf[o / NB][2 * pair][o % NB], vf[o / NB][2 * pair + 1][o % NB]} * kScaleV;
         };
         auto split = [&](int q, int n) __attribute__((always_inline)) {
             const int s = (q + 1) % (KS + 2 * NB), o = s - KS;
@@ -445,7 +442,7 @@ attention_ragged_parts(RaggedArgs a) {
             __syncthreads();
         };
         hand_over();
-        if (finish<DP, RB, VEC>(a, run, b, kv, rb, whole, begin == 0, part, ml, plans, sees, kLeastOut)) far = 1;
+        if (finish<DP, RB, VEC>(a, run, b, kv, rb, whole, begin == 0, part, ml, plans, sees, kUnscaleV)) far = 1;
         __syncthreads();
         if (far) {  // what the parts do not carry: see the file's head
             clear();
@@ -500,7 +497,7 @@ attention_ragged_parts(RaggedArgs a) {
                         }
             }
             hand_over();
-            finish<DP, RB, VEC>(a, run, b, kv, rb, whole, begin == 0, part, ml, plans, sees, kLeastOut);
+            finish<DP, RB, VEC>(a, run, b, kv, rb, whole, begin == 0, part, ml, plans, sees, 1.f);
         }
         t += end - begin;
         if (t >= (before + tiles) * units) {

@@ -183,12 +183,12 @@ struct RowPlan {
 // A unit's sums as its four waves by keys left them in LDS, joined: outputs where the
 // run holds the `whole` unit, else sums, maximum and weight to the run's slot (a unit's
 // first run had it last, the others first). The block's threads do it together; `plans`
-// is LDS. True for a thread that met a sum that is not finite, or one that is not zero but
-// below `least`.
+// is LDS. The sums in LDS are to be multiplied by `unscale`. True for a thread that met one
+// that is not finite.
 template <int DP, int RB, bool VEC>
 __device__ inline bool finish(const RaggedArgs &a, uint32_t run, uint32_t b, uint32_t kv, uint32_t rb, bool whole,
                               bool starts, const float (&part)[kWaves][RB][DP + 4], const float2 (&ml)[kWaves][RB],
-                              RowPlan (&plans)[RB], const uint64_t (&sees)[kMaxTreeNodes][kWords], float least) {
+                              RowPlan (&plans)[RB], const uint64_t (&sees)[kMaxTreeNodes][kWords], float unscale) {
     const uint32_t rows = min(uint32_t(RB), a.group * a.queries - rb * RB);
     uint32_t tid = threadIdx.x;
     asm volatile("" : "+v"(tid));  // nothing below is computed ahead of a caller's main loop
@@ -209,12 +209,12 @@ __device__ inline bool finish(const RaggedArgs &a, uint32_t run, uint32_t b, uin
             const uint32_t r = rb * RB + tid, head = r / a.queries, query = r - head * a.queries;
             p.at = size_t(b) * a.q_batch + (size_t(kv) * a.group + head) * a.q_head + size_t(query) * a.q_row;
             // A whole unit has the tree's tiles, and with them who sees whom.
-            p.top_sum.y = a.nodes && !(sees[query][query / 64] >> (query & 63) & 1) ? 0.f : 1.0f / l;
+            p.top_sum.y = a.nodes && !(sees[query][query / 64] >> (query & 63) & 1) ? 0.f : unscale / l;
         } else {
             const size_t slot = (2 * size_t(run) + starts) * RB + tid;
             p.at = slot * kSlotRow<DP>;
             reinterpret_cast<float2 *>(a.partial + 2 * size_t(a.runs) * RB * kSlotRow<DP>)[slot] = p.top_sum;
-            p.top_sum.y = 1.f;
+            p.top_sum.y = unscale;
         }
         plans[tid] = p;
     }
@@ -230,7 +230,7 @@ __device__ inline bool finish(const RaggedArgs &a, uint32_t run, uint32_t b, uin
         if (p.top_sum.y != 0.f && d < uint32_t(a.dim))
 #pragma unroll
             for (int e = 0; e < 4; ++e)
-                odd |= (VEC || d + e < uint32_t(a.dim)) && (!finite(o[e]) || (fabsf(o[e]) < least && o[e] != 0.f));
+                odd |= (VEC || d + e < uint32_t(a.dim)) && !finite(o[e]);
         // A slot without a node is zeros whatever its sums are.
         o = p.top_sum.y == 0.f ? f32x4{0.f, 0.f, 0.f, 0.f} : o * p.top_sum.y;
         if (VEC || !whole) {

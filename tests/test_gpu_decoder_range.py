@@ -67,3 +67,50 @@ def test_scores_whose_dims_cancel(runtime, heads, dim, keys):
     # One rounding a key, and as in attend() 16 for joining and dividing.
     off = dec.U * (keys + 16) * np.broadcast_to(np.abs(values).mean(axis=0), want.shape)
     base.within(base.run(runtime, spec, x)["out"], want[None], off[None])
+
+
+@pytest.mark.parametrize("kernel", KERNELS)
+@pytest.mark.parametrize("every", [1, 4])
+def test_values_below_bf16s_least(runtime, kernel, every):
+    # Values of 2^-138, in all dims or in every fourth: bf16's smallest number is 2^-133. Queries of zeros weigh all
+    # keys 1, and sums of subnormal numbers are exact, so an output is off by the division and its own rounding.
+    spec = base.cross_spec(*KERNELS[kernel])
+    rng = np.random.default_rng(52)
+    b, n = spec["batch"], spec["keys"]
+    lengths = [n, n - 1, 1] + [n] * (b - 3)
+    x = base.cross_inputs(rng, spec, lengths)
+    x["q"][:] = 0
+    x["v"][..., ::every] = (1 + np.abs(x["v"][..., ::every])) * np.float32(2.0 ** -138)
+    got = base.run(runtime, spec, x)["out"].reshape(x["q"].shape)
+    group = spec["heads"] // spec["kv_heads"]
+    for i, length in enumerate(lengths):
+        values = np.repeat(x["v"][i, :, :length].astype(np.float64), group, axis=0)
+        want = np.broadcast_to(values.mean(axis=1, keepdims=True), got[i].shape)[..., ::every]
+        base.within(got[i][..., ::every], want, 4 * dec.U * want + 2.0 ** -149)
+
+
+@pytest.mark.parametrize("nodes,dim", [(7, 64), (20, 64), (20, 96), (40, 128), (100, 80), (33, 50)])
+def test_drafted_values_below_bf16s_least(runtime, nodes, dim):
+    # A chain over an empty cache: node n's output is the mean of the values up to it.
+    rng = np.random.default_rng(53)
+    spec = base.tree_spec(2, 2, 2, nodes, 64, dim)
+    x = base.tree_inputs(rng, spec, [0, 0], [[n - 1 for n in range(nodes)]] * 2)
+    x["q"][:] = 0
+    x["v_draft"] = ((1 + np.abs(x["v_draft"])) * np.float32(2.0 ** -138)).astype(np.float32)
+    want = np.cumsum(x["v_draft"].astype(np.float64), axis=2) / np.arange(1, nodes + 1)[:, None]
+    base.within(base.run(runtime, spec, x)["out"], want, 4 * dec.U * want + 2.0 ** -149)
+
+
+@pytest.mark.parametrize("kernel", KERNELS)
+def test_values_of_zero(runtime, kernel):
+    # Not to be taken for values that the parts lost: plain zeros, some dims of them or all.
+    spec = base.cross_spec(*KERNELS[kernel])
+    rng = np.random.default_rng(54)
+    lengths = [spec["keys"]] * spec["batch"]
+    x = base.cross_inputs(rng, spec, lengths)
+    x["v"][..., 1::2] = 0
+    got = base.run(runtime, spec, x)["out"].reshape(x["q"].shape)
+    part = dict(spec, batch=2)
+    want, off = dec.cross(part, x["q"][:2], x["k"][:2], x["v"][:2], lengths)
+    base.within(got[:2], want, off)
+    assert (got[..., 1::2] == 0).all()
