@@ -388,9 +388,10 @@ bool on_flash(const RaggedShape &s) {
     const uint64_t d = s.dim, heads = uint64_t(s.batch) * s.kv_heads, rows = rows_of(s), fb = flash_ragged_rows(s.dim);
     const uint64_t q_span = s.token_major ? d * s.heads * s.queries : d * rows;
     const uint64_t k_span = (s.token_major ? d * s.kv_heads : d) * (s.keys + 128ull);
-    // Offsets of a head's rows in 31 bits, tiles past the last one in 32; grid.y.
+    // Offsets of a head's rows in 31 bits, tiles past the last one in 32; grid.y, and the
+    // threads along grid.x (2 fb a block).
     if (!on_parts(s) || s.dim % 4 || s.nodes || q_span >= 1u << 29 || k_span >= 1u << 29) return false;
-    if ((rows + fb - 1) / fb > 65535) return false;
+    if ((rows + fb - 1) / fb > 65535 || heads * 2 * fb > 0xffffffffull) return false;
     const uint64_t blocks = heads * ((rows + fb - 1) / fb), units = heads * row_blocks(s);
     const double full = double(rows) / double((rows + fb - 1) / fb * fb);
     const double flash = 8.0 + double((blocks + kCus - 1) / kCus) * double((s.keys + 31) / 32) *
