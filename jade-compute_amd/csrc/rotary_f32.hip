@@ -10,7 +10,7 @@
 //
 // The angle: position * rate in 64 bits, in turns, reduced there to within an
 // eighth of a turn of a multiple of a quarter; only that remainder goes to FP32
-// (off by at most 2^-25 of itself), into Taylor series (FP32 angles are off by
+// (off by at most 2^-24 of itself), into Taylor series (FP32 angles are off by
 // 2^-24 of the whole angle: 0.06 at position 10^6).
 #include "kernels.hpp"
 
