@@ -26,7 +26,7 @@
 // over at most 1531 keys of 80, 59 us, 4.9 TB/s; one query over 1024 keys 8.9 us, which is
 // two launches and loads that wait for one another (lengths, Q, K, the partial sums). More
 // rows go to the kernel on bf16 parts (attention_ragged_parts.hip): 64 nodes over 4
-// sequences took 169 us with FP32 MFMAs, 64 rows a block, and take 116.
+// sequences took 169 us with FP32 MFMAs, 64 rows a block, and take 115 to 125.
 #include <cmath>
 
 #include "attention_flash.hpp"

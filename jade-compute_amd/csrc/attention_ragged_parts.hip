@@ -12,11 +12,15 @@
 // two of them two of the twelve pieces in which the next eight values of K or V are
 // split; a chunk is loaded again, for the next tile, as soon as it is split. For 64
 // rows and 32 keys of 128 dims that is 192 MFMAs (6144 cycles of a SIMD; FP32 MFMAs
-// take 16384) and 1150 other vector instructions, most of them beside the MFMAs; masks,
+// take 16384) and 1300 other vector instructions, most of them beside the MFMAs; masks,
 // maxima and the first weights are between the two products and beside none. 64 nodes x 32
-// heads (8 of keys) over 4 sequences of at most 4096 keys of 128: 116 us, 117 TFLOP/s; 13
-// nodes over 8 sequences: 71 us, 3.0 TB/s of K and V. A run's unit costs 8 to 11 us besides
-// its tiles: Q's loads and parts, the first tile's loads, the waves' sums joined.
+// heads (8 of keys) over 4 sequences of at most 4096 keys of 128: 115 to 125 us by card, 109
+// to 118 TFLOP/s; 13 nodes over 8 sequences: 67 to 74 us, 3.0 to 3.2 TB/s of K and V. No unit
+// bounds them: of a wave's time MFMAs take 47 and 38%, vector instructions, most of them
+// beside MFMAs, 56 and 49%, waits for memory 16 and 20%, waits to issue 20 and 22%; 23 and
+// 30% of the SIMDs' cycles have no wave (unequal runs, the launch's ends). A run's unit costs
+// 8 to 11 us besides its tiles: Q's loads and parts, the first tile's loads, the waves' sums
+// joined.
 //
 // Q and V are scaled up and K down before they are split. So every finite Q and V is
 // carried exactly (V as it is left nothing of values below 2^-134), and scores are in FP32's
