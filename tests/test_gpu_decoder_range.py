@@ -114,3 +114,31 @@ def test_values_of_zero(runtime, kernel):
     want, off = dec.cross(part, x["q"][:2], x["k"][:2], x["v"][:2], lengths)
     base.within(got[:2], want, off)
     assert (got[..., 1::2] == 0).all()
+
+
+@pytest.mark.parametrize("kernel", KERNELS)
+@pytest.mark.parametrize("scale", [2.0 ** 90, 2.0 ** 108])
+def test_values_whose_scaled_sums_overflow(runtime, kernel, scale):
+    # V's parts carry values times 2^24: these, or sums of them, pass FP32's range there, but not as they are.
+    spec = base.cross_spec(*KERNELS[kernel])
+    rng = np.random.default_rng(55)
+    lengths = [spec["keys"]] * spec["batch"]
+    x = base.cross_inputs(rng, spec, lengths)
+    x["v"] = (x["v"] * np.float32(scale)).astype(np.float32)
+    want, off = dec.cross(dict(spec, batch=3), x["q"][:3], x["k"][:3], x["v"][:3], lengths)
+    got = base.run(runtime, spec, x)["out"].reshape(x["q"].shape)
+    base.within(got[:3], want, off)
+    assert np.isfinite(got).all()
+
+
+@pytest.mark.parametrize("nodes,dim", [(5, 64), (20, 128), (40, 64), (30, 90), (70, 128), (130, 50)])
+def test_large_drafted_values_stay_with_those_who_see_them(runtime, nodes, dim):
+    # Two branches; the second's values and keys are 2^108 and its queries as small, the first's are ordinary.
+    rng = np.random.default_rng(56)
+    half = nodes // 2
+    spec = base.tree_spec(1, 2, 1, nodes, 90, dim)
+    x = base.tree_inputs(rng, spec, [77], [[n - 1 for n in range(half)] + [-1] + list(range(half, nodes - 1))])
+    for name, scale in (("v_draft", 2.0 ** 108), ("k_draft", 2.0 ** 60), ("q", 2.0 ** -60)):
+        x[name][:, :, half:] *= np.float32(scale)
+    want, off = base.tree_want(spec, x)
+    base.within(base.run(runtime, spec, x)["out"], want, off)
