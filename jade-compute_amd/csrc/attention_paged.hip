@@ -1,0 +1,403 @@
+// Attention of a chunk of new tokens of every sequence over its pages
+// (attention_paged); one new token is ordinary decoding. Token j of sequence b is row
+// j % page of page tables[b, j / page]; query i < counts[b] is token
+// lengths[b] - counts[b] + i and sees the tokens up to itself:
+//   out_i = sum_j exp(s_ij - m_i) v_j / sum_j exp(s_ij - m_i), s_ij = q_i k_j / sqrt(dim).
+// Queries past a sequence's count, and those that see no key, are zeros. An entry of a table
+// that names no page is 16 or more tokens that nobody sees.
+//
+// The kernel of attention_ragged.hip over pages: one pass with a running maximum and sum,
+// FP32 MFMAs (16x16x4) in the transposed form, K, V and P in registers, four waves that take
+// 16 keys each of a tile of 64. Pages hold multiples of 16 tokens, so that a wave's 16 keys
+// lie in one page, whose row of the table it looks up a tile ahead; each has a descriptor of
+// its own, which ends with the sequence's last token, so no offset passes 2^31 however large
+// the pool, and what lies past the last token or in no page reads as zeros.
+//
+// All tiles of all (sequence, kv head, row block)s in a row are cut into equal runs, one a
+// block; a launch of its own joins what a cut went through.
+#include <cmath>
+
+#include "attention_paged.hpp"
+#include "kernels.hpp"
+
+namespace jade {
+namespace hipk {
+namespace {
+
+using namespace paged;
+
+constexpr int kTile = 64, kRows = 16;  // keys of a tile, rows of a block
+
+// DP: head dim padded (64, 128).
+template <int DP, bool VEC>
+__global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2, 2))) void attention_paged(PagedArgs a) {
+    constexpr int KJ = DP / 16, NJ = DP / 64, RB = kRows;
+    __shared__ __attribute__((aligned(16))) float part[kWaves][RB][DP + 4];
+    __shared__ float2 ml[kWaves][RB];
+    __shared__ RowPlan plans[RB];
+    const int tid = threadIdx.x, lane = tid & 63;
+    const uint32_t wave = uniform(tid >> 6);
+    const int m = lane & 15, g = lane >> 4;
+    const Work<kTile, RB> work(a);
+    const uint32_t chunk = (work.total + a.runs - 1) / a.runs;
+    const uint32_t run = run_of(blockIdx.x, a.runs);
+    uint32_t b, before;
+    const uint32_t t_stop = work.start(run + 1, chunk, b, before);
+    uint32_t t = work.start(run, chunk, b, before);
+
+    const uint32_t row_bytes = a.p_row * 4u;
+    uint32_t koff[KJ], voff[NJ][4];
+#pragma unroll
+    for (int j = 0; j < KJ; ++j) {
+        const uint32_t d = 16 * j + 4 * g;
+        koff[j] = d < a.dim ? uint32_t(m) * row_bytes + d * 4u : kDeadOffset;
+    }
+#pragma unroll
+    for (int j = 0; j < NJ; ++j)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const uint32_t d = 64 * j + 4 * m;
+            voff[j][i] = d < a.dim ? uint32_t(4 * g + i) * row_bytes + d * 4u : kDeadOffset;
+        }
+
+    // The part of a (sequence, kv head, row block) that tile t of the launch begins in this
+    // run; nothing where the run is over. Tiles from `stop` on are past what its rows see.
+    struct Unit {
+        uint32_t b, before, kv, rb, begin, end, stop, tiles, all;
+        Sequence s;
+    };
+    auto unit_at = [&](uint32_t t, uint32_t b, uint32_t before) {
+        Unit u{};
+        if (t >= t_stop) return u;
+        for (u.b = b, u.before = before;; ++u.b) {  // the run ends with a sequence that has tiles
+            u.s = work.at(u.b);
+            u.tiles = work.tiles(u.s);
+            if (u.tiles) break;
+        }
+        const uint32_t blocks = work.blocks(u.s), in = t - u.before, unit = in / u.tiles;
+        u.all = u.tiles * blocks * a.kv_heads;
+        u.begin = in - unit * u.tiles;
+        u.kv = unit / blocks;
+        u.rb = unit - u.kv * blocks;
+        u.end = min(u.tiles, u.begin + (t_stop - t));
+        const int last = int(u.s.length) - int(u.s.count) + int(min(u.s.count - 1, (u.rb * RB + RB - 1) / a.group));
+        u.stop = last < 0 ? 0u : min(u.end, uint32_t(last) / kTile + 1);
+        return u;
+    };
+    // The table's entry for this wave's keys of tile x, -1 past `stop`.
+    auto entry_of = [&](const Unit &u, uint32_t x) {
+        const uint32_t n = x * (kTile / 16) + wave;
+        return x < u.stop && n * 16 < u.s.length ? a.tables[size_t(u.b) * a.table + place_of(a, n).entry] : -1.f;
+    };
+    // Those keys or values: zeros where they have no page.
+    auto tile_of = [&](const float *pool, const Unit &u, uint32_t x, uint32_t page) {
+        const uint32_t n = x * (kTile / 16) + wave;
+        const bool some = page != kNoPage;
+        const float *from = pool + (some ? page * a.p_page + u.kv * a.p_head + size_t(place_of(a, n).step) * 16 * a.p_row : 0);
+        const uint32_t bytes = some ? (min(u.s.length - n * 16, 16u) - 1) * row_bytes + a.dim * 4u : 0u;
+        return __builtin_amdgcn_make_buffer_rsrc(const_cast<float *>(from), 0, int(bytes), int(kRawBuffer));
+    };
+    // A last chunk that is not whole reads into the next row, or nothing past the tile.
+    auto load = [&](__amdgpu_buffer_rsrc_t from, uint32_t at) {
+        return __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(from, int(at), 0, 0));
+    };
+    f32x4 kf[KJ], vf[NJ][4], qf[KJ];
+    auto load_k = [&](const Unit &u, uint32_t x, uint32_t page) {
+        const auto from = tile_of(a.k, u, x, page);
+#pragma unroll
+        for (int j = 0; j < KJ; ++j) kf[j] = load(from, koff[j]);
+    };
+    auto load_v = [&](const Unit &u, uint32_t x, uint32_t page) {
+        const auto from = tile_of(a.v, u, x, page);
+#pragma unroll
+        for (int j = 0; j < NJ; ++j)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) vf[j][i] = load(from, voff[j][i]);
+    };
+    auto rows_of = [&](const Unit &u) { return min(uint32_t(RB), u.s.count * a.group - u.rb * RB); };
+    // Q^T operand: row m of the block, dims 16 j + 4 g + e.
+    auto load_rows = [&](const Unit &u) {
+        if (u.begin == u.end) return;
+        const float *row = m < rows_of(u) ? a.q + row_at(a, u.b, u.kv, u.rb * RB + m) : nullptr;
+#pragma unroll
+        for (int j = 0; j < KJ; ++j) qf[j] = load_dims<VEC>(row, 16 * j + 4 * g, a.dim);
+    };
+    auto page_at = [&](float entry) { return uniform(page_of(a, entry)); };
+    Unit u = unit_at(t, b, before);
+    uint32_t page = page_at(entry_of(u, u.begin));  // of the tile at hand
+    float ahead = entry_of(u, u.begin + 1);         // of the one after
+    load_k(u, u.begin, page);
+    load_v(u, u.begin, page);
+    load_rows(u);
+    while (u.begin < u.end) {
+        const uint32_t begin = u.begin;
+        const bool whole = begin == 0 && u.end == u.tiles;
+        // The unit after this one, whose first loads go beside this one's last products.
+        t += u.end - begin;
+        const bool over = t >= u.before + u.all;
+        const Unit next = unit_at(t, u.b + over, over ? u.before + u.all : u.before);
+        const float first = entry_of(next, next.begin), second = entry_of(next, next.begin + 1);
+#pragma unroll
+        for (int j = 0; j < KJ; ++j) qf[j] *= a.qscale;  // log2 units
+
+        f32x4 acc[NJ][4];
+        float top = -INFINITY, sum = 0.f;
+#pragma unroll
+        for (int j = 0; j < NJ; ++j)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) acc[j][e] = f32x4{0.f, 0.f, 0.f, 0.f};
+        // Tokens of the block's first query and of row m.
+        const int old = int(u.s.length) - int(u.s.count), low = old + int(u.rb * RB / a.group);
+        const int mine = old + int((u.rb * RB + m) / a.group);
+        uint32_t page_next = page;
+        if (begin >= u.stop) {  // no tile of this unit's: the next one's
+            page_next = page_at(first);
+            load_k(next, next.begin, page_next);
+            load_v(next, next.begin, page_next);
+        }
+        for (uint32_t x = begin; x < u.stop; ++x) {
+            const bool last = x + 1 == u.stop;
+            if (!VEC)  // the next row's values may not be finite
+#pragma unroll
+                for (int j = 0; j < KJ; ++j)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        if (16 * j + 4 * g + e >= a.dim) kf[j][e] = 0.f;
+            f32x4 p = {0.f, 0.f, 0.f, 0.f};  // scores, then weights, of keys 16 wave + 4 g + i
+#pragma unroll
+            for (int j = 0; j < KJ; ++j)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) p = __builtin_amdgcn_mfma_f32_16x16x4f32(kf[j][e], qf[j][e], p, 0, 0, 0);
+            page_next = page_at(last ? first : ahead);
+            last ? load_k(next, next.begin, page_next) : load_k(u, x + 1, page_next);
+            ahead = entry_of(u, x + 2);
+            const bool masked = int(x * kTile + kTile) > low + 1;
+            if (masked || page == kNoPage) {
+                const int key = int(x) * kTile + 16 * int(wave) + 4 * g;
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    if (key + i > mine || page == kNoPage) p[i] = -INFINITY;
+            }
+            const float most = fmaxf(fmaxf(p.x, p.y), fmaxf(p.z, p.w));
+            if (__any(most > top + kLazyMax)) {
+                const float reached = fmaxf(top, across_keys_max(most));
+                const float keep = reached == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(top - reached);
+                top = reached;
+                sum *= keep;
+#pragma unroll
+                for (int j = 0; j < NJ; ++j)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) acc[j][e] *= keep;
+            }
+            const float from = top == -INFINITY ? 0.f : top;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                p[i] = __builtin_amdgcn_exp2f(p[i] - from);
+                sum += p[i];
+            }
+            bool odd = false;
+            if (masked && u.s.count > 1) {
+#pragma unroll
+                for (int j = 0; j < NJ; ++j)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) odd |= !finite(vf[j][i][e]);
+            }
+            if (!__any(odd)) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+#pragma unroll
+                    for (int j = 0; j < NJ; ++j)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e)
+                            acc[j][e] = __builtin_amdgcn_mfma_f32_16x16x4f32(vf[j][i][e], p[i], acc[j][e], 0, 0, 0);
+            } else {
+                // A value that is not finite, of a token that not every row may see: the
+                // finite ones, then the weight that each row gives to each special one.
+#pragma unroll
+                for (int j = 0; j < NJ; ++j)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+#pragma unroll
+                        for (int k = -1; k < 3; ++k) {
+                            __builtin_amdgcn_sched_barrier(0);  // one at a time: a rare path takes no registers
+                            f32x4 sums = k < 0 ? acc[j][e] : f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) {
+                                const float v = vf[j][i][e], y = k >= 0 ? is(k, v) : finite(v) ? v : 0.f;
+                                sums = __builtin_amdgcn_mfma_f32_16x16x4f32(y, p[i], sums, 0, 0, 0);
+                            }
+                            if (k < 0)
+                                acc[j][e] = sums;
+                            else
+#pragma unroll
+                                for (int i = 0; i < 4; ++i)
+                                    if (sums[i] > 0.f) acc[j][e][i] += special(k);
+                        }
+            }
+            last ? load_v(next, next.begin, page_next) : load_v(u, x + 1, page_next);
+            page = page_next;
+        }
+        page = page_next;
+        ahead = second;
+        const uint32_t rows = rows_of(u);
+        load_rows(next);
+
+        // The four waves' sums joined: row m, dims 64 j + 16 g + 4 i + e.
+        __syncthreads();
+        const float all = across_keys_sum(sum);
+        if (g == 0) ml[wave][m] = float2{top, all};
+#pragma unroll
+        for (int j = 0; j < NJ; ++j)
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                *reinterpret_cast<f32x4 *>(&part[wave][m][64 * j + 16 * g + 4 * i]) =
+                    f32x4{acc[j][0][i], acc[j][1][i], acc[j][2][i], acc[j][3][i]};
+        __syncthreads();
+        finish<DP, RB, VEC>(a, run, u.b, u.kv, u.rb, rows, whole, begin == 0, part, ml, plans, 1.f);
+        u = next;
+    }
+    clear_rows(a);
+}
+
+// What the runs left of a (sequence, kv head, row block) cut between them: block x has
+// the unit that the cut before run x is the first of. DP / 4 lanes have a row; ROWS rows of a
+// unit go to a block, each with all of its slots, or (ROWS 1) one, with the slots shared out
+// (a unit of many runs).
+template <int DP, int RB, int TILE, int ROWS, bool VEC>
+__global__ __launch_bounds__(kThreads) void attention_paged_join(PagedArgs a) {
+    constexpr int LANES = DP / 4, PARTS = kThreads / LANES / ROWS;
+    __shared__ __attribute__((aligned(16))) f32x4 sums[PARTS][LANES];
+    __shared__ float2 weights[PARTS];
+    const int tid = threadIdx.x, lane = tid % LANES, p = ROWS == 1 ? tid / LANES : 0;
+    const uint32_t row = blockIdx.y * ROWS + (ROWS == 1 ? 0 : tid / LANES), d = 4 * lane;
+    const Work<TILE, RB> work(a);
+    const uint32_t chunk = (work.total + a.runs - 1) / a.runs;
+    uint32_t b, before;
+    const uint32_t cut = work.start(blockIdx.x + 1, chunk, b, before);
+    if (cut == work.total) return;
+    const Sequence s = work.at(b);
+    const uint32_t tiles = work.tiles(s);
+    if (!tiles) return;  // at a sequence's start
+    const uint32_t unit = (cut - before) / tiles, start = before + unit * tiles;
+    if (start + chunk < cut || start == cut || Work<TILE, RB>::rounds(tiles, chunk)) return;  // not its first cut
+    const uint32_t blocks = work.blocks(s), kv = unit / blocks, rb = unit - kv * blocks;
+    const bool mine = row < min(uint32_t(RB), s.count * a.group - rb * RB);
+    const uint32_t first = start / chunk, last = (start + tiles - 1) / chunk;
+    const float2 *ml = reinterpret_cast<const float2 *>(a.partial + 2 * size_t(a.runs) * RB * DP);
+    // A unit's first run had it last, the others first.
+    auto slot = [&](uint32_t r) { return (2 * size_t(r) + (r == first)) * RB + row; };
+    float most = -INFINITY, l = 0.f;
+    f32x4 o = {0.f, 0.f, 0.f, 0.f};
+    auto join = [&](float top, float sum, f32x4 outs) {
+        const float next = fmaxf(most, top), from = next == -INFINITY ? 0.f : next;
+        const float old = __builtin_amdgcn_exp2f(most - from), weight = __builtin_amdgcn_exp2f(top - from);
+        most = next;
+        l = l * old + sum * weight;
+        o = o * old + outs * weight;
+    };
+    if (mine) {
+#pragma unroll 4
+        for (uint32_t r = first + p; r <= last; r += PARTS) {
+            const float2 x = ml[slot(r)];
+            join(x.x, x.y, *reinterpret_cast<const f32x4 *>(a.partial + slot(r) * DP + d));
+        }
+    }
+    if constexpr (PARTS > 1) {
+        sums[p][lane] = o;
+        if (lane == 0) weights[p] = float2{most, l};
+        __syncthreads();
+        if (p) return;
+#pragma unroll
+        for (int x = 1; x < PARTS; ++x) join(weights[x].x, weights[x].y, sums[x][lane]);
+    }
+    if (!mine) return;
+    o = l == 0.f ? f32x4{0.f, 0.f, 0.f, 0.f} : o * (1.0f / l);  // a row that sees no key is zeros
+    store_dims<VEC>(a.out + row_at(a, b, kv, rb * RB + row), int(d), int(a.dim), o);
+}
+
+uint64_t rows_of(const PagedShape &s) { return uint64_t(s.heads / s.kv_heads) * s.queries; }
+uint32_t block_rows(const PagedShape &) { return kRows; }
+uint32_t tile_of(const PagedShape &) { return kTile; }
+
+// Tiles of a (sequence, kv head, row block) of full length, and of a launch of such.
+uint64_t paged_tiles(const PagedShape &s) {
+    const uint32_t rb = block_rows(s), tile = tile_of(s);
+    return uint64_t(s.batch) * s.kv_heads * ((rows_of(s) + rb - 1) / rb) * ((uint64_t(s.table) * s.page + tile - 1) / tile);
+}
+
+// Runs of a launch: two blocks a CU, or one per tile where there can be no more tiles.
+uint32_t runs_of(const PagedShape &s) {
+    const uint64_t tiles = paged_tiles(s), most = 2 * kCus;
+    return tiles >= most ? uint32_t(most) : uint32_t((tiles + 7) / 8 * 8);
+}
+
+template <int DP, int RB, int TILE, bool VEC>
+void launch_join(hipStream_t stream, const PagedArgs &a, uint64_t units) {
+    if (a.runs < 2) return;
+    constexpr uint32_t kRowsOf = kThreads / (DP / 4);  // rows of a block
+    const uint64_t all = uint64_t(a.group) * a.queries;
+    const uint32_t rows = all < RB ? uint32_t(all) : RB;
+    // Units of 16 runs or more: their slots are shared out; else whole rows.
+    if (16 * units <= a.runs)
+        hipLaunchKernelGGL((attention_paged_join<DP, RB, TILE, 1, VEC>), dim3(a.runs - 1, rows), dim3(kThreads), 0, stream, a);
+    else
+        hipLaunchKernelGGL((attention_paged_join<DP, RB, TILE, kRowsOf, VEC>),
+                           dim3(a.runs - 1, (rows + kRowsOf - 1) / kRowsOf), dim3(kThreads), 0, stream, a);
+}
+
+template <int DP, bool VEC>
+hipError_t launch(hipStream_t stream, const PagedArgs &a, uint64_t units) {
+    hipLaunchKernelGGL((attention_paged<DP, VEC>), dim3(a.runs), dim3(kThreads), 0, stream, a);
+    launch_join<DP, kRows, kTile, VEC>(stream, a, units);
+    return hipGetLastError();
+}
+
+uint32_t paged_lds_bytes(uint32_t dim) {
+    const uint32_t pitch = (dim <= 64 ? 64 : 128) + 4;
+    return uint32_t(kWaves * kRows * (pitch * sizeof(float) + sizeof(float2)) + kRows * sizeof(RowPlan));
+}
+
+}  // namespace
+
+LaunchShape attention_paged_shape(const PagedShape &s) {
+    // Tiles are counted in 32 bits.
+    if (paged_tiles(s) > 0x7fffffffull) return {nullptr, {0, 0, 0}, {0, 0, 0}, 0};
+    return {s.dim <= 64 ? "attention_paged_d64" : "attention_paged_d128", {runs_of(s), 1, 1}, {kThreads, 1, 1},
+            paged_lds_bytes(s.dim)};
+}
+
+size_t attention_paged_workspace_bytes(const PagedShape &s) {
+    const size_t dp = s.dim > 64 ? 128 : 64;
+    return 2 * size_t(runs_of(s)) * block_rows(s) * (dp + 2) * sizeof(float);
+}
+
+hipError_t attention_paged_f32(hipStream_t stream, const PagedShape &s, const PagedBuffers &x, float *workspace) {
+    PagedArgs a{};
+    a.q = x.q; a.k = x.k; a.v = x.v; a.tables = x.tables; a.lengths = x.lengths; a.counts = x.counts;
+    a.out = x.out;
+    a.partial = workspace;
+    const size_t d = s.dim;
+    a.q_batch = d * s.heads * s.queries;
+    a.q_head = s.token_major ? d : d * s.queries;
+    a.q_row = uint32_t(s.token_major ? d * s.heads : d);
+    a.p_page = d * s.kv_heads * s.page;
+    a.p_head = s.pages_token_major ? d : d * s.page;
+    a.p_row = uint32_t(s.pages_token_major ? d * s.kv_heads : d);
+    a.batch = s.batch; a.kv_heads = s.kv_heads; a.group = s.heads / s.kv_heads; a.queries = s.queries;
+    a.pages = s.pages; a.table = s.table; a.page = s.page; a.dim = s.dim;
+    a.steps = s.page / 16;
+    a.inverse = uint32_t(((1ull << 31) + a.steps - 1) / a.steps);
+    a.runs = runs_of(s);
+    a.qscale = (1.0f / sqrtf(float(s.dim))) * kLog2e;
+    uintptr_t bits = 0;
+    for (const float *y : {x.q, x.k, x.v, const_cast<const float *>(x.out)}) bits |= reinterpret_cast<uintptr_t>(y);
+    if (!workspace || (s.dim % 4 == 0 && bits & 15u)) return hipErrorInvalidValue;  // the runtime's regions are aligned
+    const uint64_t units = uint64_t(s.batch) * s.kv_heads * ((rows_of(s) + kRows - 1) / kRows);
+    if (s.dim % 4) return s.dim <= 64 ? launch<64, false>(stream, a, units) : launch<128, false>(stream, a, units);
+    return s.dim <= 64 ? launch<64, true>(stream, a, units) : launch<128, true>(stream, a, units);
+}
+
+}  // namespace hipk
+}  // namespace jade

@@ -1,0 +1,276 @@
+// Attention over a paged cache: arguments, and the device parts that its kernels share:
+// where a run's tiles lie, and how a row's sums become outputs or go to the workspace.
+#pragma once
+
+#include <hip/hip_runtime.h>
+
+#include <cmath>
+#include <cstdint>
+
+#include "whole.hpp"
+
+namespace jade {
+namespace hipk {
+
+// Strides in elements. Rows of q and out are [batch, head, query]; a page's row of a head
+// is at page * p_page + kv head * p_head + row * p_row.
+struct PagedArgs {
+    const float *q, *k, *v, *tables, *lengths, *counts;
+    float *out, *partial;
+    size_t q_batch, q_head, p_page, p_head;
+    uint32_t q_row, p_row;
+    uint32_t batch, kv_heads, group, queries, pages, table, page, dim;
+    uint32_t steps, inverse;  // 16-token steps of a page; 2^31 / steps, rounded up
+    uint32_t runs;
+    float qscale;  // scale * log2(e)
+};
+
+namespace {
+namespace paged {
+
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+
+constexpr int kThreads = 256, kWaves = 4;
+constexpr uint32_t kCus = 256;
+constexpr float kLazyMax = 8.0f;   // log2 units: the running maximum moves only past this
+constexpr uint32_t kRawBuffer = 0x00020000;    // buffer descriptor word 3: raw buffer, 32-bit data format
+constexpr uint32_t kDeadOffset = 0x80000000u;  // past every descriptor's end: reads zero
+constexpr float kLog2e = 1.44269504088896340736f;
+constexpr uint32_t kNoPage = ~0u;
+
+__device__ inline uint32_t uniform(uint32_t x) { return __builtin_amdgcn_readfirstlane(x); }
+__device__ inline uint32_t of_lane(uint32_t x, int lane) { return __builtin_amdgcn_readlane(x, lane); }
+
+// Sum over the lanes up to and with this one: within the rows of 16 by shifts, then
+// each row's last lane into the rows after it.
+__device__ inline uint32_t scan_add(uint32_t x) {
+#define JADE_SCAN(control, rows) x += __builtin_amdgcn_update_dpp(0, x, control, rows, 0xf, false)
+    JADE_SCAN(0x111, 0xf);
+    JADE_SCAN(0x112, 0xf);
+    JADE_SCAN(0x114, 0xf);
+    JADE_SCAN(0x118, 0xf);
+    JADE_SCAN(0x142, 0xa);  // row_bcast:15 into rows 1 and 3
+    JADE_SCAN(0x143, 0xc);  // row_bcast:31 into rows 2 and 3
+#undef JADE_SCAN
+    return x;
+}
+
+__device__ inline float across_keys_max(float x) {
+    return fmaxf(fmaxf(x, __shfl_xor(x, 16)), fmaxf(__shfl_xor(x, 32), __shfl_xor(x, 48)));
+}
+__device__ inline float across_keys_sum(float x) {
+    x += __shfl_xor(x, 16);
+    return x + __shfl_xor(x, 32);
+}
+
+// Run of block `id`: the runs of one XCD are neighbours.
+__device__ inline uint32_t run_of(uint32_t id, uint32_t runs) { return id % 8 * (runs / 8) + id / 8; }
+
+// A sequence: its tokens, the new ones among them, and what they make of tiles of keys
+// and blocks of rows (for each kv head). Row r of a kv head is head r % group of the group
+// and query r / group, so that a block of rows has neighbouring queries, and sequences of
+// few new tokens have few blocks.
+struct Sequence {
+    uint32_t length, count;
+};
+template <int TILE, int RB>
+struct Work {
+    const PagedArgs &a;
+    const Sequence near;         // sequence (lane)
+    const uint32_t own, up_to;   // its tiles, of all kv heads and row blocks; those up to it
+    uint32_t total;
+
+    __device__ Sequence load(uint32_t b) const {
+        if (b >= a.batch) return {0, 0};
+        return {whole_below(a.lengths[b], a.table * a.page), whole_below(a.counts[b], a.queries)};
+    }
+    __device__ static uint32_t tiles(const Sequence &s) { return s.count ? (s.length + TILE - 1) / TILE : 0u; }
+    __device__ uint32_t blocks(const Sequence &s) const { return (s.count * a.group + RB - 1) / RB; }
+    __device__ uint32_t all_of(const Sequence &s) const { return tiles(s) * blocks(s) * a.kv_heads; }
+    // Of one sequence, for the whole wave.
+    __device__ Sequence at(uint32_t b) const {
+        if (b < 64) return {of_lane(near.length, int(b)), of_lane(near.count, int(b))};
+        const Sequence s = load(b);
+        return {uniform(s.length), uniform(s.count)};
+    }
+    __device__ explicit Work(const PagedArgs &args)
+        : a(args), near(load(threadIdx.x & 63)), own(all_of(near)), up_to(scan_add(own)), total(of_lane(up_to, 63)) {
+        for (uint32_t b0 = 64; b0 < a.batch; b0 += 64) total += of_lane(scan_add(lane_work(b0)), 63);
+    }
+    // This lane's work among the sequences from b0 on.
+    __device__ uint32_t lane_work(uint32_t b0) const { return all_of(load(b0 + (threadIdx.x & 63))); }
+    // The sequence that tile t < total belongs to, and the tiles before it.
+    __device__ void find(uint32_t t, uint32_t &b, uint32_t &before) const {
+        before = 0;
+        uint32_t sum = up_to, mine = own;
+        for (b = 0;; b += 64, mine = lane_work(b), sum = scan_add(mine)) {
+            const uint64_t past = __ballot(before + sum > t);
+            if (past) {
+                const int first = __builtin_ctzll(past);
+                b += first;
+                before += of_lane(sum - mine, first);
+                return;
+            }
+            before += of_lane(sum, 63);
+        }
+    }
+    // Where run `run` starts: tile run * chunk, but at the nearest end of a (kv head, row
+    // block) where a run has four or more whole ones of that sequence: then none of them
+    // needs joining. `b` and `before` as find() leaves them; at the last tile's end they say
+    // nothing.
+    __device__ uint32_t start(uint32_t run, uint32_t chunk, uint32_t &b, uint32_t &before) const {
+        const uint64_t at = uint64_t(run) * chunk;
+        if (at >= total) return total;
+        uint32_t t = uint32_t(at);
+        find(t, b, before);
+        const Sequence s = this->at(b);
+        const uint32_t n = tiles(s);
+        if (!rounds(n, chunk)) return t;
+        const uint32_t over = (t - before) % n;
+        t = 2 * over < n ? t - over : t - over + n;
+        const uint32_t all = all_of(s);
+        if (t == before + all) {
+            before += all;
+            ++b;
+        }
+        return t;
+    }
+    __device__ static bool rounds(uint32_t tiles, uint32_t chunk) { return 4 * tiles <= chunk; }
+};
+
+// Dims d .. d + 3 of a row, zeros from `dim` on and for no row. VEC: dim % 4 == 0 and
+// 16-byte rows.
+template <bool VEC>
+__device__ inline f32x4 load_dims(const float *row, int d, int dim) {
+    f32x4 x = {0.f, 0.f, 0.f, 0.f};
+    if (VEC) {
+        if (row && d < dim) x = *reinterpret_cast<const f32x4 *>(row + d);
+    } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            if (row && d + e < dim) x[e] = row[d + e];
+    }
+    return x;
+}
+template <bool VEC>
+__device__ inline void store_dims(float *row, int d, int dim, f32x4 x) {
+    if (VEC) {
+        if (d < dim) *reinterpret_cast<f32x4 *>(row + d) = x;
+    } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            if (d + e < dim) row[d + e] = x[e];
+    }
+}
+
+// Row r of (sequence b, kv head), from its first dim, in q and out.
+__device__ inline size_t row_at(const PagedArgs &a, uint32_t b, uint32_t kv, uint32_t r) {
+    const uint32_t query = r / a.group, head = r - query * a.group;
+    return size_t(b) * a.q_batch + (size_t(kv) * a.group + head) * a.q_head + size_t(query) * a.q_row;
+}
+
+// The 16 tokens from 16 n on of sequence b: their place in its table.
+struct Place {
+    uint32_t entry, step;  // of 16 tokens within the page
+};
+__device__ inline Place place_of(const PagedArgs &a, uint32_t n) {
+    const uint32_t entry = uint32_t(uint64_t(n) * a.inverse >> 31);
+    return {entry, n - entry * a.steps};
+}
+__device__ inline uint32_t page_of(const PagedArgs &a, float entry) {
+    return entry >= 0.f && entry < float(a.pages) && entry == truncf(entry) ? uint32_t(entry) : kNoPage;
+}
+
+// Zeros for the rows that no tile of keys reaches: those of queries past a sequence's
+// count, and all of one without tokens.
+__device__ inline void clear_rows(const PagedArgs &a) {
+    const uint32_t lane = threadIdx.x & 63, heads = a.kv_heads * a.group;
+    const uint64_t all = uint64_t(a.batch) * a.queries, step = uint64_t(a.runs) * kWaves;
+    for (uint64_t i = uint64_t(blockIdx.x) * kWaves + uniform(threadIdx.x >> 6); i < all; i += step) {
+        const uint32_t b = uint32_t(i / a.queries), query = uint32_t(i - uint64_t(b) * a.queries);
+        if (query < whole_below(a.counts[b], a.queries) && a.lengths[b] >= 1.f) continue;
+        float *const out = a.out + size_t(b) * a.q_batch + size_t(query) * a.q_row;
+        for (uint32_t e = lane; e < heads * a.dim; e += 64) {
+            const uint32_t h = e / a.dim;
+            out[h * a.q_head + (e - h * a.dim)] = 0.f;
+        }
+    }
+}
+
+__device__ inline bool finite(float x) { return fabsf(x) < INFINITY; }
+// The three values that a weight of zero does not cancel; is(k, x): x is the k-th.
+__device__ inline float special(int k) { return k == 0 ? INFINITY : k == 1 ? -INFINITY : NAN; }
+__device__ inline float is(int k, float x) { return (k == 2 ? x != x : x == special(k)) ? 1.f : 0.f; }
+
+// Floats of a row in a run's slots.
+template <int DP>
+constexpr int kSlotRow = DP <= 64 ? 64 : 128;
+
+// What joining the four waves' sums of a row takes.
+struct RowPlan {
+    f32x4 weights;  // of the waves
+    float2 top_sum;  // with `by` in place of the sum, once that is kept
+    size_t at;  // its first dim in the outputs, or in the run's slot
+};
+// The `rows` sums of row block rb of (sequence b, kv head) as the four waves by keys left
+// them in LDS, joined: outputs where the run holds the `whole` unit, else sums, maximum
+// and weight to the run's slot (a unit's first run had it last, the others first). The
+// block's threads do it together; `plans` is LDS. The sums in LDS are to be multiplied by
+// `unscale`. True for a thread that met one that is not finite.
+template <int DP, int RB, bool VEC>
+__device__ inline bool finish(const PagedArgs &a, uint32_t run, uint32_t b, uint32_t kv, uint32_t rb, uint32_t rows,
+                              bool whole, bool starts, const float (&part)[kWaves][RB][DP + 4],
+                              const float2 (&ml)[kWaves][RB], RowPlan (&plans)[RB], float unscale) {
+    uint32_t tid = threadIdx.x;
+    asm volatile("" : "+v"(tid));  // nothing below is computed ahead of a caller's main loop
+    if (tid < rows) {
+        float most = -INFINITY;
+#pragma unroll
+        for (int w = 0; w < kWaves; ++w) most = fmaxf(most, ml[w][tid].x);
+        const float from = most == -INFINITY ? 0.f : most;
+        RowPlan p;
+        float l = 0.f;
+#pragma unroll
+        for (int w = 0; w < kWaves; ++w) {
+            p.weights[w] = __builtin_amdgcn_exp2f(ml[w][tid].x - from);
+            l = fmaf(p.weights[w], ml[w][tid].y, l);
+        }
+        p.top_sum = float2{most, l};
+        if (whole) {
+            p.at = row_at(a, b, kv, rb * RB + tid);
+            p.top_sum.y = l == 0.f ? 0.f : unscale / l;  // a row that sees no key is zeros
+        } else {
+            const size_t slot = (2 * size_t(run) + starts) * RB + tid;
+            p.at = slot * kSlotRow<DP>;
+            reinterpret_cast<float2 *>(a.partial + 2 * size_t(a.runs) * RB * kSlotRow<DP>)[slot] = p.top_sum;
+            p.top_sum.y = unscale;
+        }
+        plans[tid] = p;
+    }
+    __syncthreads();
+    float *const to = whole ? a.out : a.partial;
+    bool odd = false;
+    for (uint32_t at = tid; at < rows * (DP / 4); at += kThreads) {
+        const uint32_t row = at / (DP / 4), d = at % (DP / 4) * 4;
+        const RowPlan &p = plans[row];
+        f32x4 o = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int w = 0; w < kWaves; ++w) o += p.weights[w] * *reinterpret_cast<const f32x4 *>(&part[w][row][d]);
+        if (d < a.dim)
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                odd |= (VEC || d + e < a.dim) && !finite(o[e]);
+        o = p.top_sum.y == 0.f ? f32x4{0.f, 0.f, 0.f, 0.f} : o * p.top_sum.y;
+        if (VEC || !whole) {
+            if (!whole || d < a.dim) *reinterpret_cast<f32x4 *>(to + p.at + d) = o;
+        } else {
+            store_dims<false>(to + p.at, int(d), int(a.dim), o);
+        }
+    }
+    return odd;
+}
+
+}  // namespace paged
+}  // namespace
+}  // namespace hipk
+}  // namespace jade

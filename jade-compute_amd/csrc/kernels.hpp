@@ -128,6 +128,67 @@ size_t attention_ragged_workspace_bytes(const RaggedShape &shape);
 hipError_t attention_ragged_f32(hipStream_t stream, const RaggedShape &shape, const RaggedBuffers &buffers,
                                 float *workspace);
 
+// Decoding over a paged cache. Token t of a sequence is row t % page of page
+// tables[b, t / page]; pages are [page, kv_heads, dim] (pages_token_major) or
+// [kv_heads, page, dim].
+
+// Rows i < counts[b] of k and v to the ends of their sequences.
+struct PagesAppendArgs {
+    const float *k, *v, *counts, *tables, *lengths;
+    float *k_pages, *v_pages, *new_lengths;
+    uint32_t batch, kv_heads, rows, pages, page, table, dim;
+    bool token_major, pages_token_major;
+};
+LaunchShape pages_append_shape(uint32_t batch, uint32_t kv_heads, uint32_t rows, uint32_t page, uint32_t dim,
+                               bool token_major);
+hipError_t pages_append_f32(hipStream_t stream, const PagesAppendArgs &args);
+
+// The first copy_rows[i] rows of page sources[i] to page targets[i].
+struct PagesCopyArgs {
+    const float *sources, *targets, *copy_rows;
+    float *k_pages, *v_pages;
+    uint32_t copies, kv_heads, pages, page, dim;
+    bool pages_token_major;
+};
+LaunchShape pages_copy_shape(uint32_t copies, uint32_t kv_heads, uint32_t page, uint32_t dim);
+hipError_t pages_copy_f32(hipStream_t stream, const PagesCopyArgs &args);
+
+// The tables of the sequences that go on from `parents`. The workspace is zeros before
+// the first call.
+struct PagesForkArgs {
+    const float *parents, *lengths, *tables, *reserve, *uses;
+    float *new_tables, *new_lengths, *new_uses, *sources, *targets, *copy_rows, *missing, *workspace;
+    uint32_t batch, pages, page, table;
+};
+LaunchShape pages_fork_shape(uint32_t batch);
+size_t pages_fork_workspace_bytes(uint32_t batch, uint32_t pages);
+hipError_t pages_fork_f32(hipStream_t stream, const PagesForkArgs &args);
+
+// The `picks` best continuations of `beams` beams each.
+struct BeamSelectArgs {
+    const float *logits, *scores, *finished;
+    float *parents, *tokens, *new_scores, *new_finished, *workspace;
+    uint32_t batch, beams, vocab, picks, end;
+};
+LaunchShape beam_select_shape(uint32_t batch, uint32_t beams, uint32_t vocab);
+size_t beam_select_workspace_bytes(uint32_t batch, uint32_t beams, uint32_t vocab, uint32_t picks);
+hipError_t beam_select_f32(hipStream_t stream, const BeamSelectArgs &args);
+
+// Attention of counts[b] new tokens a sequence, the last of its lengths[b], each over
+// the tokens up to its own.
+struct PagedShape {
+    uint32_t batch, heads, kv_heads, queries, pages, page, table, dim;
+    bool token_major, pages_token_major;
+};
+struct PagedBuffers {
+    const float *q, *k, *v, *tables, *lengths, *counts;
+    float *out;
+};
+LaunchShape attention_paged_shape(const PagedShape &shape);
+size_t attention_paged_workspace_bytes(const PagedShape &shape);
+hipError_t attention_paged_f32(hipStream_t stream, const PagedShape &shape, const PagedBuffers &buffers,
+                               float *workspace);
+
 // Streaming elementwise kernels.
 LaunchShape stream_shape(uint32_t len);
 hipError_t swiglu_f32(hipStream_t stream, const float *gate, const float *up, float *out, uint32_t len);

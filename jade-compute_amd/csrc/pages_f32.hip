@@ -1,0 +1,438 @@
+// The pages of a cache: rows appended to the pages of their sequences
+// (pages_append), tables forked, freed and made longer (pages_fork), and rows of
+// one page copied to another (pages_copy). Token t of a sequence is row t % page
+// of page table[t / page].
+//
+// pages_append and pages_copy move K and V in one launch, whole float4s where rows
+// allow it, with loads and stores past the L2.
+//
+// pages_fork is three launches, because what a page is used for is known only once
+// every sequence has said what it keeps, and which pages are free only after that:
+//   1. a block for each sequence: its parent's pages into its new table, and what its
+//      own old table's pages gain or lose into a sum for each page (integer atomics,
+//      so their order changes nothing);
+//   2. uses and sums into new uses, 1024 pages a block, which counts its free ones;
+//      one block more sums up what the sequences ask for;
+//   3. the free pages in order of their numbers to the sequences in theirs.
+// The sums are zeros before and after a call.
+#include "kernels.hpp"
+#include "whole.hpp"
+
+namespace jade {
+namespace hipk {
+namespace {
+
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+
+constexpr int kThreads = 256;
+constexpr uint32_t kBlockWords = 2 * kThreads;  // elements (float4s, or floats) of each tensor that a block moves
+constexpr uint32_t kMaxBlocks = 1u << 20;
+
+__device__ inline bool is_whole(float x, uint32_t most) { return x >= 0.f && x < float(most) && x == truncf(x); }
+
+template <typename T>
+__device__ inline void move(const float *k, const float *v, size_t from, float *k_to, float *v_to, size_t to) {
+    const T x = __builtin_nontemporal_load(reinterpret_cast<const T *>(k) + from);
+    const T y = __builtin_nontemporal_load(reinterpret_cast<const T *>(v) + from);
+    __builtin_nontemporal_store(x, reinterpret_cast<T *>(k_to) + to);
+    __builtin_nontemporal_store(y, reinterpret_cast<T *>(v_to) + to);
+}
+
+// ---- pages_append ------------------------------------------------------------------------
+
+// Rows of sequence b that can be appended, of its first `most`: those before the first
+// whose place has no page. For all threads of the block.
+__device__ inline uint32_t count_rows(const PagesAppendArgs &a, uint32_t b, uint32_t start, uint32_t most) {
+    __shared__ uint32_t least;
+    most = min(most, a.table * a.page - start);
+    if (!most) return 0;
+    if (threadIdx.x == 0) least = a.table;
+    __syncthreads();
+    const float *table = a.tables + size_t(b) * a.table;
+    const uint32_t last = (start + most - 1) / a.page;
+    uint32_t bad = a.table;
+    for (uint32_t e = start / a.page + threadIdx.x; e <= last; e += kThreads)
+        if (!is_whole(table[e], a.pages)) bad = min(bad, e);
+    if (bad < a.table) atomicMin(&least, bad);
+    __syncthreads();
+    const uint32_t got = least;
+    __syncthreads();
+    return got > last ? most : got * a.page > start ? got * a.page - start : 0u;
+}
+
+__device__ inline uint32_t start_of(const PagesAppendArgs &a, uint32_t b) {
+    return whole_below(a.lengths[b], a.table * a.page);
+}
+
+// Many rows: every sequence's new length by a launch of its own, so that the moving
+// blocks need not look at all the pages before theirs.
+__global__ __launch_bounds__(kThreads) void pages_count(PagesAppendArgs a) {
+    const uint32_t b = blockIdx.x, start = start_of(a, b);
+    const uint32_t count = count_rows(a, b, start, whole_below(a.counts[b], a.rows));
+    if (threadIdx.x == 0) a.new_lengths[b] = float(start + count);
+}
+
+// A block takes `span` rows of a sequence, of all heads where rows come by token (`heads`
+// is 1 then and `wide` all of a row), else of one head.
+template <typename T, bool COUNTED>
+__global__ __launch_bounds__(kThreads) void pages_append(PagesAppendArgs a, uint32_t heads, uint32_t wide, uint32_t span,
+                                                         uint32_t spans, uint32_t items) {
+    const uint32_t dim = a.dim * sizeof(float) / sizeof(T), row = a.kv_heads * dim;
+    for (uint32_t item = blockIdx.x; item < items; item += gridDim.x) {
+        const uint32_t at = item % spans, rest = item / spans, h = rest % heads, b = rest / heads;
+        const uint32_t first = at * span, start = start_of(a, b);
+        uint32_t count;
+        if (COUNTED) {
+            count = uint32_t(a.new_lengths[b]) - start;
+        } else {
+            // The first block of a sequence also writes its new length.
+            const bool whole = h == 0 && at == 0;
+            const uint32_t asked = whole_below(a.counts[b], a.rows);
+            count = count_rows(a, b, start, whole ? asked : min(asked, first + span));
+            if (whole && threadIdx.x == 0) a.new_lengths[b] = float(start + count);
+        }
+        if (count <= first) continue;
+        const uint32_t n = min(count - first, span) * wide;
+        const size_t from = (size_t(rest) * a.rows + first) * wide;
+        const float *table = a.tables + size_t(b) * a.table;
+#pragma unroll 2
+        for (uint32_t i = threadIdx.x; i < n; i += kThreads) {
+            const uint32_t r = i / wide, e = i - r * wide, t = start + first + r;
+            const uint32_t entry = t / a.page, in = t - entry * a.page;
+            const size_t page = uint32_t(table[entry]);
+            size_t to;
+            if (a.pages_token_major) {
+                to = (page * a.page + in) * row + (a.token_major ? e : h * dim + e);
+            } else {
+                const uint32_t head = a.token_major ? e / dim : h;
+                to = ((page * a.kv_heads + head) * a.page + in) * dim + (a.token_major ? e - head * dim : e);
+            }
+            move<T>(a.k, a.v, from + i, a.k_pages, a.v_pages, to);
+        }
+    }
+}
+
+// A block of the one-launch form looks at the entries of all the rows before its own.
+constexpr uint32_t kCountedEntries = 8192;
+
+struct Split {
+    uint32_t heads, wide, span, spans;
+    uint64_t items;
+};
+Split split_of(uint32_t batch, uint32_t kv_heads, uint32_t rows, uint32_t dim, bool token_major, bool vec) {
+    Split s;
+    s.heads = token_major ? 1 : kv_heads;
+    s.wide = (token_major ? kv_heads * dim : dim) / (vec ? 4 : 1);
+    s.span = s.wide < kBlockWords ? kBlockWords / s.wide : 1;
+    s.spans = (rows + s.span - 1) / s.span;
+    s.items = uint64_t(batch) * s.heads * s.spans;
+    return s;
+}
+
+template <typename T>
+hipError_t launch_append(hipStream_t stream, const PagesAppendArgs &a) {
+    const Split s = split_of(a.batch, a.kv_heads, a.rows, a.dim, a.token_major, sizeof(T) == 16);
+    const uint32_t items = uint32_t(s.items);
+    const dim3 grid(items < kMaxBlocks ? items : kMaxBlocks), block(kThreads);
+    if (a.rows / a.page > kCountedEntries) {
+        hipLaunchKernelGGL(pages_count, dim3(a.batch), block, 0, stream, a);
+        hipLaunchKernelGGL((pages_append<T, true>), grid, block, 0, stream, a, s.heads, s.wide, s.span, s.spans, items);
+    } else {
+        hipLaunchKernelGGL((pages_append<T, false>), grid, block, 0, stream, a, s.heads, s.wide, s.span, s.spans, items);
+    }
+    return hipGetLastError();
+}
+
+// ---- pages_copy --------------------------------------------------------------------------
+
+__device__ inline bool is_copy(const PagesCopyArgs &a, uint32_t i) {
+    return is_whole(a.sources[i], a.pages) && is_whole(a.targets[i], a.pages) && a.copy_rows[i] >= 1.f;
+}
+
+// `blocks` blocks for each copy. One whose target another reads, or an earlier one writes,
+// is not made, so that the order in which blocks run changes nothing.
+template <typename T>
+__global__ __launch_bounds__(kThreads) void pages_copy(PagesCopyArgs a, uint32_t blocks) {
+    const uint32_t c = blockIdx.x / blocks, part = blockIdx.x - c * blocks;
+    if (!is_copy(a, c)) return;
+    const float source = a.sources[c], target = a.targets[c];
+    bool clash = false;
+    for (uint32_t i = threadIdx.x; i < a.copies; i += kThreads)
+        if (a.sources[i] == target || (i < c && a.targets[i] == target)) clash |= is_copy(a, i);
+    if (__syncthreads_or(clash)) return;
+    const uint32_t rows = whole_below(a.copy_rows[c], a.page), dim = a.dim * sizeof(float) / sizeof(T);
+    // Runs of rows that lie together: all heads of a token, or one head's tokens.
+    const uint32_t run = a.pages_token_major ? rows * a.kv_heads * dim : rows * dim;
+    const uint32_t pitch = a.pages_token_major ? 0 : a.page * dim;
+    const uint64_t all = uint64_t(rows) * a.kv_heads * dim, page = uint64_t(a.page) * a.kv_heads * dim;
+    const size_t from = uint64_t(source) * page, to = uint64_t(target) * page;
+#pragma unroll 2
+    for (uint64_t i = uint64_t(part) * kThreads + threadIdx.x; i < all; i += uint64_t(blocks) * kThreads) {
+        const uint32_t h = uint32_t(i) / run;
+        const size_t at = size_t(h) * pitch + (uint32_t(i) - h * run);
+        move<T>(a.k_pages, a.v_pages, from + at, a.k_pages, a.v_pages, to + at);
+    }
+}
+
+// Blocks of a copy: two float4s of each tensor a thread where the copies are few, and
+// as many as fill the chip where they are many.
+constexpr uint32_t kCopyBlocks = 8192;
+uint32_t copy_blocks(uint32_t copies, uint32_t page, uint32_t kv_heads, uint32_t dim) {
+    const uint64_t words = uint64_t(page) * kv_heads * dim / (dim % 4 ? 1 : 4);
+    const uint64_t most = (words + kBlockWords - 1) / kBlockWords, share = (kCopyBlocks + copies - 1) / copies;
+    return uint32_t(most < share ? most : share);
+}
+
+// ---- pages_fork --------------------------------------------------------------------------
+
+constexpr uint32_t kForkPages = 4 * kThreads;  // pages of a block
+
+// The workspace, in 32-bit words.
+struct ForkSpace {
+    int *sums;                                // what each page's uses gain; zeros between calls
+    uint32_t *keep, *need, *before, *counts;  // of a sequence; needs before it (and in all); free pages of a block
+};
+__host__ __device__ inline uint32_t fork_blocks(uint32_t pages) { return (pages + kForkPages - 1) / kForkPages; }
+__host__ __device__ inline ForkSpace fork_space(float *workspace, uint32_t pages, uint32_t batch) {
+    uint32_t *const w = reinterpret_cast<uint32_t *>(workspace), *const per = w + pages;
+    return {reinterpret_cast<int *>(w), per, per + batch, per + 2 * size_t(batch), per + 3 * size_t(batch) + 1};
+}
+
+// A whole number of 0 .. batch - 1, or batch.
+__device__ inline uint32_t parent_of(const PagesForkArgs &a, uint32_t s) {
+    return is_whole(a.parents[s], a.batch) ? uint32_t(a.parents[s]) : a.batch;
+}
+
+// Pages of a table before its first entry that names none, for all threads of the block.
+__device__ inline uint32_t held_by(const PagesForkArgs &a, uint32_t s, uint32_t &least) {
+    if (threadIdx.x == 0) least = a.table;
+    __syncthreads();
+    const float *table = a.tables + size_t(s) * a.table;
+    uint32_t bad = a.table;
+#pragma unroll 4
+    for (uint32_t e = threadIdx.x; e < a.table; e += kThreads)
+        if (!is_whole(table[e], a.pages)) bad = min(bad, e);
+    if (bad < a.table) atomicMin(&least, bad);
+    __syncthreads();
+    const uint32_t got = least;
+    __syncthreads();
+    return got;
+}
+
+__global__ __launch_bounds__(kThreads) void pages_fork_tables(PagesForkArgs a) {
+    __shared__ uint32_t least, children, older;
+    const ForkSpace w = fork_space(a.workspace, a.pages, a.batch);
+    const uint32_t s = blockIdx.x, parent = parent_of(a, s);
+    if (threadIdx.x == 0) children = older = 0;
+    __syncthreads();
+    uint32_t mine = 0, before = 0;
+    for (uint32_t i = threadIdx.x; i < a.batch; i += kThreads) {
+        const uint32_t p = parent_of(a, i);
+        mine += p == s;
+        before += p == parent && i < s;
+    }
+    if (mine) atomicAdd(&children, mine);
+    if (before) atomicAdd(&older, before);
+    const uint32_t held = held_by(a, s, least);
+    {
+        // This sequence's pages: whole ones for each child, the others for its first.
+        const uint32_t length = min(whole_below(a.lengths[s], a.table * a.page), held * a.page), full = length / a.page;
+        const float *table = a.tables + size_t(s) * a.table;
+        const int n = int(children);
+        if (n != 1)
+            for (uint32_t e = threadIdx.x; e < held; e += kThreads) {
+                const int more = (e < full ? n : min(n, 1)) - 1;
+                if (more) atomicAdd(w.sums + uint32_t(table[e]), more);
+            }
+    }
+    float *const to = a.new_tables + size_t(s) * a.table;
+    uint32_t keep = 0, need = 0, length = 0, part = 0;
+    float source = -1.f;
+    if (parent < a.batch) {
+        const uint32_t theirs = parent == s ? held : held_by(a, parent, least);
+        length = min(whole_below(a.lengths[parent], a.table * a.page), theirs * a.page);
+        const uint32_t full = length / a.page;
+        const float *from = a.tables + size_t(parent) * a.table;
+        keep = older ? full : theirs;
+        if (older && full * a.page < length) {
+            part = length - full * a.page;
+            source = from[full];
+        }
+        const uint64_t end = uint64_t(length) + whole_below(a.reserve[s], a.table * a.page);
+        const uint32_t want = uint32_t(min(uint64_t(a.table), (end + a.page - 1) / a.page));
+        need = want > keep ? want - keep : 0;
+#pragma unroll 4
+        for (uint32_t e = threadIdx.x; e < a.table; e += kThreads) to[e] = e < keep ? from[e] : -1.f;
+    } else {
+        for (uint32_t e = threadIdx.x; e < a.table; e += kThreads) to[e] = -1.f;
+    }
+    if (threadIdx.x == 0) {
+        w.keep[s] = keep;
+        w.need[s] = need;
+        a.new_lengths[s] = float(length);
+        a.copy_rows[s] = float(part);
+        a.sources[s] = source;
+    }
+}
+
+// Sum over the block's threads up to and with this one; `total` of all.
+__device__ inline uint32_t block_scan(uint32_t x, uint32_t &total) {
+    __shared__ uint32_t waves[kThreads / 64];
+    const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x / 64;
+#pragma unroll
+    for (uint32_t d = 1; d < 64; d *= 2) {
+        const uint32_t y = __shfl_up(x, d);
+        if (lane >= d) x += y;
+    }
+    if (lane == 63) waves[wave] = x;
+    __syncthreads();
+    total = 0;
+#pragma unroll
+    for (uint32_t i = 0; i < kThreads / 64; ++i) {
+        if (i < wave) x += waves[i];
+        total += waves[i];
+    }
+    __syncthreads();
+    return x;
+}
+
+__global__ __launch_bounds__(kThreads) void pages_fork_count(PagesForkArgs a) {
+    const ForkSpace w = fork_space(a.workspace, a.pages, a.batch);
+    const uint32_t blocks = fork_blocks(a.pages);
+    uint32_t total;
+    if (blockIdx.x < blocks) {
+        uint32_t n = 0;
+#pragma unroll
+        for (uint32_t i = 0; i < 4; ++i) {
+            const uint32_t p = blockIdx.x * kForkPages + i * kThreads + threadIdx.x;
+            if (p >= a.pages) break;
+            const int more = w.sums[p];
+            const float uses = a.uses[p] + float(more);
+            a.new_uses[p] = uses;
+            if (more) w.sums[p] = 0;
+            n += uses == 0.f;
+        }
+        block_scan(n, total);
+        if (threadIdx.x == 0) w.counts[blockIdx.x] = total;
+        return;
+    }
+    uint32_t before = 0;
+    for (uint32_t s0 = 0; s0 < a.batch; s0 += kThreads) {
+        const uint32_t s = s0 + threadIdx.x, mine = s < a.batch ? w.need[s] : 0u;
+        const uint32_t up_to = block_scan(mine, total);
+        // A pool has at most 2^24 pages; sums that pass it need not be told apart.
+        if (s < a.batch) w.before[s] = before + up_to - mine;
+        before = min(before + total, 1u << 30);
+    }
+    if (threadIdx.x == 0) w.before[a.batch] = before;
+}
+
+__global__ __launch_bounds__(kThreads) void pages_fork_allot(PagesForkArgs a) {
+    const ForkSpace w = fork_space(a.workspace, a.pages, a.batch);
+    const uint32_t blocks = fork_blocks(a.pages), asked = w.before[a.batch];
+    const bool pages = blockIdx.x < blocks;
+    if (pages && !asked) return;
+    // Free pages before this block's, or of the whole pool.
+    uint32_t free = 0, n = 0;
+    for (uint32_t i = threadIdx.x; i < (pages ? blockIdx.x : blocks); i += kThreads) n += w.counts[i];
+    block_scan(n, free);
+    if (!pages) {
+        const uint32_t s = (blockIdx.x - blocks) * kThreads + threadIdx.x;
+        if (s >= a.batch) return;
+        const uint32_t before = w.before[s], need = w.need[s], got = before < free ? min(need, free - before) : 0u;
+        a.missing[s] = float(need - got);
+        const bool copy = a.copy_rows[s] > 0.f;
+        if (!copy || !got) a.targets[s] = -1.f;
+        if (copy && !got) {  // without the page that its partial one would go to
+            a.new_lengths[s] = float(w.keep[s] * a.page);
+            a.copy_rows[s] = 0.f;
+            a.sources[s] = -1.f;
+        }
+        return;
+    }
+    if (free >= asked) return;
+    // Four neighbouring pages a thread.
+    const uint32_t first = blockIdx.x * kForkPages + 4 * threadIdx.x;
+    bool open[4];
+    n = 0;
+#pragma unroll
+    for (uint32_t i = 0; i < 4; ++i) {
+        open[i] = first + i < a.pages && a.new_uses[first + i] == 0.f;
+        n += open[i];
+    }
+    uint32_t total, rank = free + block_scan(n, total) - n;
+    for (uint32_t i = 0; i < 4; ++i) {
+        if (!open[i]) continue;
+        if (rank >= asked) return;
+        // The last sequence with `before` at most rank has a need past it.
+        uint32_t lo = 0, hi = a.batch - 1;
+        while (lo < hi) {
+            const uint32_t mid = (lo + hi + 1) / 2;
+            if (w.before[mid] <= rank)
+                lo = mid;
+            else
+                hi = mid - 1;
+        }
+        const uint32_t place = w.keep[lo] + rank - w.before[lo];
+        a.new_tables[size_t(lo) * a.table + place] = float(first + i);
+        a.new_uses[first + i] = 1.f;
+        if (rank == w.before[lo] && a.copy_rows[lo] > 0.f) a.targets[lo] = float(first + i);
+        ++rank;
+    }
+}
+
+}  // namespace
+
+LaunchShape pages_append_shape(uint32_t batch, uint32_t kv_heads, uint32_t rows, uint32_t page, uint32_t dim,
+                               bool token_major) {
+    const uint64_t items = split_of(batch, kv_heads, rows, dim, token_major, dim % 4 == 0).items;
+    if (items > 0xfffffffeull - kMaxBlocks) return {nullptr, {0, 0, 0}, {0, 0, 0}, 0};
+    return {rows / page > kCountedEntries ? "pages_append_counted" : "pages_append",
+            {uint32_t(items < kMaxBlocks ? items : kMaxBlocks), 1, 1}, {kThreads, 1, 1}, uint32_t(sizeof(uint32_t))};
+}
+
+hipError_t pages_append_f32(hipStream_t stream, const PagesAppendArgs &a) {
+    const uintptr_t bits = reinterpret_cast<uintptr_t>(a.k) | reinterpret_cast<uintptr_t>(a.v) |
+                           reinterpret_cast<uintptr_t>(a.k_pages) | reinterpret_cast<uintptr_t>(a.v_pages);
+    if (a.dim % 4 == 0 && bits & 15u) return hipErrorInvalidValue;  // the runtime's regions are aligned
+    return a.dim % 4 == 0 ? launch_append<f32x4>(stream, a) : launch_append<float>(stream, a);
+}
+
+LaunchShape pages_copy_shape(uint32_t copies, uint32_t kv_heads, uint32_t page, uint32_t dim) {
+    const uint64_t blocks = uint64_t(copies) * copy_blocks(copies, page, kv_heads, dim);
+    // A page is counted in 32 bits.
+    if (uint64_t(page) * kv_heads * dim > 0x7fffffffull) return {nullptr, {0, 0, 0}, {0, 0, 0}, 0};
+    return {"pages_copy", {uint32_t(blocks), 1, 1}, {kThreads, 1, 1}, 0};
+}
+
+hipError_t pages_copy_f32(hipStream_t stream, const PagesCopyArgs &a) {
+    const uintptr_t bits = reinterpret_cast<uintptr_t>(a.k_pages) | reinterpret_cast<uintptr_t>(a.v_pages);
+    if (a.dim % 4 == 0 && bits & 15u) return hipErrorInvalidValue;
+    const uint32_t blocks = copy_blocks(a.copies, a.page, a.kv_heads, a.dim);
+    const dim3 grid(a.copies * blocks);
+    if (a.dim % 4 == 0)
+        hipLaunchKernelGGL(pages_copy<f32x4>, grid, dim3(kThreads), 0, stream, a, blocks);
+    else
+        hipLaunchKernelGGL(pages_copy<float>, grid, dim3(kThreads), 0, stream, a, blocks);
+    return hipGetLastError();
+}
+
+LaunchShape pages_fork_shape(uint32_t batch) {
+    return {"pages_fork", {batch, 1, 1}, {kThreads, 1, 1}, uint32_t(3 * sizeof(uint32_t))};
+}
+
+size_t pages_fork_workspace_bytes(uint32_t batch, uint32_t pages) {
+    return (size_t(pages) + 3 * size_t(batch) + 1 + fork_blocks(pages)) * sizeof(uint32_t);
+}
+
+hipError_t pages_fork_f32(hipStream_t stream, const PagesForkArgs &a) {
+    if (!a.workspace) return hipErrorInvalidValue;
+    const uint32_t blocks = fork_blocks(a.pages);
+    hipLaunchKernelGGL(pages_fork_tables, dim3(a.batch), dim3(kThreads), 0, stream, a);
+    hipLaunchKernelGGL(pages_fork_count, dim3(blocks + 1), dim3(kThreads), 0, stream, a);
+    hipLaunchKernelGGL(pages_fork_allot, dim3(blocks + (a.batch + kThreads - 1) / kThreads), dim3(kThreads), 0, stream, a);
+    return hipGetLastError();
+}
+
+}  // namespace hipk
+}  // namespace jade

@@ -18,6 +18,10 @@ hipk::RaggedShape ragged_shape(const KernelSpec &s) {
             s.dim, s.token_major};
 }
 
+hipk::PagedShape paged_shape(const KernelSpec &s) {
+    return {s.batch, s.heads, s.kv_heads, s.queries, s.pages, s.page, s.table, s.dim, s.token_major, s.pages_token_major};
+}
+
 hipk::LaunchShape launch_shape(const KernelSpec &s) {
     using namespace hipk;
     switch (s.op) {
@@ -45,6 +49,11 @@ hipk::LaunchShape launch_shape(const KernelSpec &s) {
         case Op::CacheAppend: return cache_append_shape(s.batch, s.kv_heads, s.picks, s.dim, s.token_major);
         case Op::AttentionTree:
         case Op::AttentionCross: return attention_ragged_shape(ragged_shape(s));
+        case Op::AttentionPaged: return attention_paged_shape(paged_shape(s));
+        case Op::PagesAppend: return pages_append_shape(s.batch, s.kv_heads, s.rows, s.page, s.dim, s.token_major);
+        case Op::PagesFork: return pages_fork_shape(s.batch);
+        case Op::PagesCopy: return pages_copy_shape(s.copies, s.kv_heads, s.page, s.dim);
+        case Op::BeamSelect: return beam_select_shape(s.batch, s.beams, s.vocab);
         case Op::GemmMps: break;
     }
     return {nullptr, {0, 0, 0}, {0, 0, 0}, 0};
@@ -75,6 +84,10 @@ size_t workspace_bytes_of(const KernelSpec &spec) {
         return hipk::attention_online_workspace_bytes(spec.heads, spec.seq, spec.dim, spec.causal);
     if (spec.op == Op::AttentionTree || spec.op == Op::AttentionCross)
         return hipk::attention_ragged_workspace_bytes(ragged_shape(spec));
+    if (spec.op == Op::AttentionPaged) return hipk::attention_paged_workspace_bytes(paged_shape(spec));
+    if (spec.op == Op::PagesFork) return hipk::pages_fork_workspace_bytes(spec.batch, spec.pages);
+    if (spec.op == Op::BeamSelect)
+        return hipk::beam_select_workspace_bytes(spec.batch, spec.beams, spec.vocab, spec.picks);
     return 0;
 }
 
@@ -149,6 +162,21 @@ hipError_t enqueue(const Pipeline &p, hipStream_t st, void *const *b) {
         case Op::AttentionCross:
             return attention_ragged_f32(st, ragged_shape(s),
                                         {in(0), in(1), in(2), in(3), nullptr, nullptr, nullptr, out(4)}, p.workspace);
+        case Op::AttentionPaged:
+            return attention_paged_f32(st, paged_shape(s), {in(0), in(1), in(2), in(3), in(4), in(5), out(6)},
+                                       p.workspace);
+        case Op::PagesAppend:
+            return pages_append_f32(st, {in(0), in(1), in(2), in(3), in(4), out(5), out(6), out(7), s.batch, s.kv_heads,
+                                         s.rows, s.pages, s.page, s.table, s.dim, s.token_major, s.pages_token_major});
+        case Op::PagesFork:
+            return pages_fork_f32(st, {in(0), in(1), in(2), in(3), in(4), out(5), out(6), out(7), out(8), out(9),
+                                       out(10), out(11), p.workspace, s.batch, s.pages, s.page, s.table});
+        case Op::PagesCopy:
+            return pages_copy_f32(st, {in(0), in(1), in(2), out(3), out(4), s.copies, s.kv_heads, s.pages, s.page, s.dim,
+                                       s.pages_token_major});
+        case Op::BeamSelect:
+            return beam_select_f32(st, {in(0), in(1), in(2), out(3), out(4), out(5), out(6), p.workspace, s.batch,
+                                        s.beams, s.vocab, s.picks, s.end});
         case Op::GemmMps: break;
     }
     return hipErrorInvalidValue;
@@ -220,10 +248,16 @@ Pipeline *PipelineCache::obtain(const KernelSpec &spec) {
                        text_of("%s needs %zu bytes of device workspace: %s", spec_name(spec), p->workspace_bytes,
                                hipGetErrorString(status)));
             }
+            if (spec.op == Op::PagesFork) {  // its sums start, and every call leaves them, at zero
+                dev::expect(hipMemsetAsync(p->workspace, 0, p->workspace_bytes, session_.queue()),
+                            "clearing the workspace");
+                session_.drain();
+            }
         }
     } catch (...) {
         if (p->program) (void)hipFree(p->program);
         if (p->rates) (void)hipFree(p->rates);
+        if (p->workspace) (void)hipFree(p->workspace);
         delete p;
         throw;
     }

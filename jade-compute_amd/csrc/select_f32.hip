@@ -1,0 +1,405 @@
+// A beam search's selection (beam_select): of every token of every beam, its score
+// plus the token's log-probability,
+//   score_b + logit_bt - log sum_u exp(logit_bu),
+// the `picks` best of a search, best first, ties to the lower beam, then token. A
+// finished beam goes on with its `end` token alone and keeps its score.
+//
+// One pass over the logits. A block takes a chunk of one beam's into registers, and from
+// there its maximum, its sum of exponentials and its best tokens, by value and token as
+// one 64-bit key: the picks-th largest of a wave's lane maxima is a lower bound of what can
+// be among the best, the few values from there on go to LDS and are ranked by counting
+// those above each. A second launch joins the chunks of a search in the same way: sums,
+// then scores in 64 bits, ranked likewise. Values that all but tie with their bound (equal
+// logits) do not fit the list in LDS: then the best are found one after the other.
+//
+// Beams are compared with one another by their sums of exponentials, so those are summed
+// in 64 bits, of terms that are off by one rounding each (their argument's own rounding
+// is carried along).
+#include <cmath>
+
+#include "kernels.hpp"
+
+namespace jade {
+namespace hipk {
+namespace {
+
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+
+constexpr int kThreads = 256, kWaves = 4;
+constexpr uint32_t kListed = 1024;       // values that a block ranks at once
+constexpr uint32_t kMaxBlocks = 1u << 20;
+constexpr float kLog2e = 1.44269504088896340736f;
+constexpr float kLog2eRest = 1.92596299112661746887e-8f;  // log2(e) less the float above
+constexpr float kLn2 = 0.693147180559945309417f;
+
+// Keys in the order of their values; NaN does not occur.
+__device__ inline uint32_t ordered(float x) {
+    const uint32_t b = __float_as_uint(x);
+    return b ^ (b >> 31 ? 0xffffffffu : 0x80000000u);
+}
+__device__ inline float value_of(uint32_t key) {
+    return __uint_as_float(key ^ (key >> 31 ? 0x80000000u : 0xffffffffu));
+}
+__device__ inline uint64_t ordered(double x) {
+    const uint64_t b = uint64_t(__double_as_longlong(x));
+    return b ^ (b >> 63 ? ~0ull : 1ull << 63);
+}
+__device__ inline double value_of(uint64_t key) {
+    return __longlong_as_double(int64_t(key ^ (key >> 63 ? 1ull << 63 : ~0ull)));
+}
+constexpr uint32_t kNone = 0x007fffffu;        // ordered(-INFINITY)
+constexpr uint64_t kNone64 = 0x000fffffffffffffull;
+
+// A chunk's best tokens, and the maximum and the sum of exp(logit - maximum) of all of them.
+struct Space {
+    float *value;     // [chunk of all][list]; -inf past the last
+    uint32_t *token;
+    double *sum;
+    float *top;
+};
+__host__ __device__ inline Space space_of(float *workspace, uint64_t items, uint32_t list) {
+    double *const sum = reinterpret_cast<double *>(workspace);
+    float *const value = reinterpret_cast<float *>(sum + items);
+    uint32_t *const token = reinterpret_cast<uint32_t *>(value + items * list);
+    return {value, token, sum, reinterpret_cast<float *>(token + items * list)};
+}
+
+// exp(x - top), x <= top, off by a rounding of exp2: the argument's rounding, d times
+// log2(e) in two parts, is put back to first order.
+__device__ inline float exp_below(float x, float top) {
+    if (x == top) return 1.f;
+    const float d = x - top, back = d + top, lost = x - back;  // x = top + d + lost, where all are finite
+    const float hi = d * kLog2e, lo = fmaf(d, kLog2e, -hi) + fmaf(d, kLog2eRest, lost * kLog2e);
+    const float e = __builtin_amdgcn_exp2f(hi);
+    return hi > -150.f ? fmaf(e, lo * kLn2, e) : 0.f;
+}
+
+__device__ inline float wave_max(float x) {
+#pragma unroll
+    for (int d = 32; d; d /= 2) x = fmaxf(x, __shfl_xor(x, d));
+    return x;
+}
+__device__ inline double wave_sum(double x) {
+#pragma unroll
+    for (int d = 32; d; d /= 2) x += __shfl_xor(x, d);
+    return x;
+}
+__device__ inline uint64_t wave_max(uint64_t x) {
+#pragma unroll
+    for (int d = 32; d; d /= 2) {
+        const uint64_t y = __shfl_xor(static_cast<unsigned long long>(x), d);
+        x = x > y ? x : y;
+    }
+    return x;
+}
+
+// A lower bound of the n-th largest of the wave's 64 keys, n at most 64: its 20 high bits.
+__device__ inline uint32_t nth_bound(uint32_t key, uint32_t n) {
+    uint32_t bound = 0;
+#pragma unroll
+    for (int bit = 31; bit >= 12; --bit) {
+        const uint32_t more = bound | 1u << bit;
+        if (uint32_t(__popcll(__ballot(key >= more))) >= n) bound = more;
+    }
+    return bound;
+}
+
+// V: float4s, or four floats, a thread. VEC: rows of whole float4s.
+template <int V, bool VEC>
+__global__ __launch_bounds__(kThreads) void beam_chunks(BeamSelectArgs a, uint32_t chunks, uint32_t items) {
+    __shared__ float tops[kWaves];
+    __shared__ double sums[kWaves];
+    __shared__ uint32_t bounds[kWaves], count;
+    __shared__ uint64_t keys[kListed];
+    constexpr uint32_t kChunk = 4 * V * kThreads;
+    const uint32_t tid = threadIdx.x, lane = tid & 63, wave = tid / 64, list = min(a.picks, a.vocab);
+    const Space w = space_of(a.workspace, items, list);
+    for (uint32_t item = blockIdx.x; item < items; item += gridDim.x) {
+        const uint32_t beam = item / chunks, first = (item - beam * chunks) * kChunk;
+        // Nothing of a beam that is finished, or cannot go on, is asked for.
+        if (a.finished[beam] > 0.f || !(a.scores[beam] > -INFINITY)) continue;
+        const float *const row = a.logits + size_t(beam) * a.vocab;
+        auto token_of = [&](int i, int e) { return first + (VEC ? (i * kThreads + tid) * 4 + e : (4 * i + e) * kThreads + tid); };
+        float x[V][4];
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+            if (VEC) {
+                f32x4 v = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+                if (token_of(i, 0) < a.vocab)
+                    v = __builtin_nontemporal_load(reinterpret_cast<const f32x4 *>(row + token_of(i, 0)));
+#pragma unroll
+                for (int e = 0; e < 4; ++e) x[i][e] = v[e];
+            } else {
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    x[i][e] = token_of(i, e) < a.vocab ? __builtin_nontemporal_load(row + token_of(i, e)) : -INFINITY;
+            }
+        }
+        float most = -INFINITY;
+#pragma unroll
+        for (int i = 0; i < V; ++i)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                if (x[i][e] != x[i][e]) x[i][e] = -INFINITY;  // NaN is not chosen
+                most = fmaxf(most, x[i][e]);
+            }
+        const uint32_t bound = nth_bound(ordered(most), list < 64 ? list : 64);
+        float top = wave_max(most);
+        if (lane == 0) {
+            tops[wave] = top;
+            bounds[wave] = bound;
+        }
+        if (tid == 0) count = 0;
+        __syncthreads();
+        top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
+        const uint32_t from = max(max(max(bounds[0], bounds[1]), max(bounds[2], bounds[3])), kNone + 1);
+        double sum = 0;
+#pragma unroll
+        for (int i = 0; i < V; ++i)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                sum += double(exp_below(x[i][e], top));
+                if (ordered(x[i][e]) >= from) {
+                    const uint32_t at = atomicAdd(&count, 1u);
+                    if (at < kListed) keys[at] = uint64_t(ordered(x[i][e])) << 32 | ~token_of(i, e);
+                }
+            }
+        sum = wave_sum(sum);
+        if (lane == 0) sums[wave] = sum;
+        __syncthreads();
+        const uint32_t n = count;
+        const size_t to = size_t(item) * list;
+        if (tid == 0) {
+            w.sum[item] = sums[0] + sums[1] + sums[2] + sums[3];
+            w.top[item] = top;
+        }
+        if (n <= kListed) {
+            for (uint32_t c = tid; c < n; c += kThreads) {
+                const uint64_t mine = keys[c];
+                uint32_t rank = 0;
+                for (uint32_t i = 0; i < n; ++i) rank += keys[i] > mine;
+                if (rank < list) {
+                    w.value[to + rank] = value_of(uint32_t(mine >> 32));
+                    w.token[to + rank] = ~uint32_t(mine);
+                }
+            }
+            for (uint32_t i = n + tid; i < list; i += kThreads) w.value[to + i] = -INFINITY;
+        } else {
+            uint64_t last = ~0ull;
+            for (uint32_t r = 0; r < list; ++r) {
+                uint64_t best = 0;
+#pragma unroll
+                for (int i = 0; i < V; ++i)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const uint64_t key = uint64_t(ordered(x[i][e])) << 32 | ~token_of(i, e);
+                        if (key < last && key > best) best = key;
+                    }
+                best = wave_max(best);
+                __syncthreads();
+                if (lane == 0) keys[wave] = best;
+                __syncthreads();
+                last = max(max(keys[0], keys[1]), max(keys[2], keys[3]));
+                if (tid == 0) {
+                    w.value[to + r] = value_of(uint32_t(last >> 32));
+                    w.token[to + r] = ~uint32_t(last);
+                }
+            }
+        }
+        __syncthreads();
+    }
+}
+
+// A candidate's place among the best: by score, then by number (beam * vocab + token).
+struct Ranked {
+    uint64_t key;
+    uint32_t number, unused;
+};
+__device__ inline bool above(uint64_t key, uint32_t number, uint64_t other, uint32_t others) {
+    return key > other || (key == other && number < others);
+}
+
+__global__ __launch_bounds__(kThreads) void beam_join(BeamSelectArgs a, uint32_t chunks, uint32_t items) {
+    __shared__ float tops[kMaxBeams];
+    __shared__ double logs[kMaxBeams];
+    __shared__ uint32_t bounds[kWaves], count;
+    __shared__ Ranked ranked[kListed];
+    const uint32_t tid = threadIdx.x, lane = tid & 63, wave = tid / 64, list = min(a.picks, a.vocab);
+    const uint32_t b = blockIdx.x, first = b * a.beams;
+    const Space w = space_of(a.workspace, items, list);
+    for (uint32_t beam = wave; beam < a.beams; beam += kWaves) {
+        const size_t at = size_t(first + beam) * chunks;
+        float top = -INFINITY;
+        double sum = 0;
+        if (!(a.finished[first + beam] > 0.f) && a.scores[first + beam] > -INFINITY) {
+            for (uint32_t i = lane; i < chunks; i += 64) top = fmaxf(top, w.top[at + i]);
+            top = wave_max(top);
+            for (uint32_t i = lane; i < chunks; i += 64) {
+                const float x = w.top[at + i];
+                if (x > -INFINITY) sum += w.sum[at + i] * (x == top ? 1.0 : exp(double(x) - double(top)));
+            }
+            sum = wave_sum(sum);
+        }
+        if (lane == 0) {
+            tops[beam] = top;
+            logs[beam] = log(sum);
+        }
+    }
+    if (tid == 0) count = 0;
+    __syncthreads();
+    const uint32_t per_beam = chunks * list, all = a.beams * per_beam;
+    // Candidate c of the search; a finished beam has one, in the place of its first.
+    auto candidate = [&](uint32_t c, uint64_t &key, uint32_t &number) {
+        const uint32_t beam = c / per_beam;
+        const float score = a.scores[first + beam];
+        key = kNone64;
+        number = 0;
+        if (!(score > -INFINITY)) return;
+        if (a.finished[first + beam] > 0.f) {
+            if (c == beam * per_beam && a.end < a.vocab) {
+                key = ordered(double(score));
+                number = beam * a.vocab + a.end;
+            }
+            return;
+        }
+        const size_t at = size_t(first) * per_beam + c;
+        const float x = w.value[at];
+        if (!(x > -INFINITY)) return;
+        // Infinite logits share what there is.
+        const double below = x == tops[beam] ? 0.0 : double(x) - double(tops[beam]);
+        if (!(below > -INFINITY)) return;
+        key = ordered(below - logs[beam] + double(score));
+        number = beam * a.vocab + w.token[at];
+    };
+    uint32_t most = 0;
+    for (uint32_t c = tid; c < all; c += kThreads) {
+        uint64_t key;
+        uint32_t number;
+        candidate(c, key, number);
+        most = max(most, uint32_t(key >> 32));
+    }
+    const uint32_t bound = nth_bound(most, a.picks);
+    if (lane == 0) bounds[wave] = bound;
+    __syncthreads();
+    const uint32_t from = max(max(bounds[0], bounds[1]), max(bounds[2], bounds[3]));
+    for (uint32_t c = tid; c < all; c += kThreads) {
+        uint64_t key;
+        uint32_t number;
+        candidate(c, key, number);
+        if (key > kNone64 && uint32_t(key >> 32) >= from) {
+            const uint32_t at = atomicAdd(&count, 1u);
+            if (at < kListed) ranked[at] = {key, number, 0};
+        }
+    }
+    __syncthreads();
+    const uint32_t n = count;
+    const size_t to = size_t(b) * a.picks;
+    auto pick = [&](uint32_t rank, uint64_t key, uint32_t number) {
+        const uint32_t beam = number / a.vocab, token = number - beam * a.vocab;
+        a.parents[to + rank] = float(first + beam);
+        a.tokens[to + rank] = float(token);
+        a.new_scores[to + rank] = float(value_of(key));
+        a.new_finished[to + rank] = token == a.end || a.finished[first + beam] > 0.f ? 1.f : 0.f;
+    };
+    uint32_t got = min(n, a.picks);
+    if (n <= kListed) {
+        for (uint32_t c = tid; c < n; c += kThreads) {
+            const Ranked mine = ranked[c];
+            uint32_t rank = 0;
+            for (uint32_t i = 0; i < n; ++i) rank += above(ranked[i].key, ranked[i].number, mine.key, mine.number);
+            if (rank < a.picks) pick(rank, mine.key, mine.number);
+        }
+    } else {
+        uint64_t last = ~0ull;
+        uint32_t last_number = 0;
+        for (got = 0; got < a.picks; ++got) {
+            uint64_t best = kNone64;
+            uint32_t number = ~0u;
+            for (uint32_t c = tid; c < all; c += kThreads) {
+                uint64_t key;
+                uint32_t mine;
+                candidate(c, key, mine);
+                if (key > kNone64 && above(last, last_number, key, mine) && above(key, mine, best, number)) {
+                    best = key;
+                    number = mine;
+                }
+            }
+#pragma unroll
+            for (int d = 32; d; d /= 2) {
+                const uint64_t key = __shfl_xor(static_cast<unsigned long long>(best), d);
+                const uint32_t other = __shfl_xor(number, d);
+                if (above(key, other, best, number)) {
+                    best = key;
+                    number = other;
+                }
+            }
+            __syncthreads();
+            if (lane == 0) ranked[wave] = {best, number, 0};
+            __syncthreads();
+            for (int i = 0; i < kWaves; ++i)
+                if (above(ranked[i].key, ranked[i].number, best, number)) {
+                    best = ranked[i].key;
+                    number = ranked[i].number;
+                }
+            if (best == kNone64) break;
+            last = best;
+            last_number = number;
+            if (tid == 0) pick(got, best, number);
+        }
+    }
+    for (uint32_t i = got + tid; i < a.picks; i += kThreads) {
+        a.parents[to + i] = a.tokens[to + i] = -1.f;
+        a.new_scores[to + i] = -INFINITY;
+        a.new_finished[to + i] = 0.f;
+    }
+}
+
+// float4s a thread: the most that leave two blocks a CU.
+uint32_t words_of(uint32_t batch, uint32_t beams, uint32_t vocab) {
+    uint32_t v = 8;
+    while (v > 1 && uint64_t(batch) * beams * ((vocab + 4 * v * kThreads - 1) / (4 * v * kThreads)) < 512) v /= 2;
+    return v;
+}
+uint32_t chunks_of(uint32_t batch, uint32_t beams, uint32_t vocab) {
+    const uint32_t chunk = 4 * words_of(batch, beams, vocab) * kThreads;
+    return (vocab + chunk - 1) / chunk;
+}
+
+template <int V>
+void launch_chunks(hipStream_t stream, const BeamSelectArgs &a, uint32_t chunks, uint32_t items) {
+    const dim3 grid(items < kMaxBlocks ? items : kMaxBlocks);
+    if (a.vocab % 4)
+        hipLaunchKernelGGL((beam_chunks<V, false>), grid, dim3(kThreads), 0, stream, a, chunks, items);
+    else
+        hipLaunchKernelGGL((beam_chunks<V, true>), grid, dim3(kThreads), 0, stream, a, chunks, items);
+}
+
+}  // namespace
+
+LaunchShape beam_select_shape(uint32_t batch, uint32_t beams, uint32_t vocab) {
+    const uint32_t items = batch * beams * chunks_of(batch, beams, vocab);  // at most the logits' number
+    return {"beam_select", {items < kMaxBlocks ? items : kMaxBlocks, 1, 1}, {kThreads, 1, 1},
+            uint32_t(kListed * sizeof(uint64_t) + kWaves * (sizeof(float) + sizeof(double) + sizeof(uint32_t)) + sizeof(uint32_t))};
+}
+
+size_t beam_select_workspace_bytes(uint32_t batch, uint32_t beams, uint32_t vocab, uint32_t picks) {
+    const uint64_t items = uint64_t(batch) * beams * chunks_of(batch, beams, vocab);
+    const uint64_t list = picks < vocab ? picks : vocab;
+    return items * (sizeof(double) + sizeof(float) + list * (sizeof(float) + sizeof(uint32_t)));
+}
+
+hipError_t beam_select_f32(hipStream_t stream, const BeamSelectArgs &a) {
+    if (!a.workspace || (a.vocab % 4 == 0 && reinterpret_cast<uintptr_t>(a.logits) & 15u)) return hipErrorInvalidValue;
+    const uint32_t chunks = chunks_of(a.batch, a.beams, a.vocab), items = a.batch * a.beams * chunks;
+    switch (words_of(a.batch, a.beams, a.vocab)) {
+        case 8: launch_chunks<8>(stream, a, chunks, items); break;
+        case 4: launch_chunks<4>(stream, a, chunks, items); break;
+        case 2: launch_chunks<2>(stream, a, chunks, items); break;
+        default: launch_chunks<1>(stream, a, chunks, items); break;
+    }
+    hipLaunchKernelGGL(beam_join, dim3(a.batch), dim3(kThreads), 0, stream, a, chunks, items);
+    return hipGetLastError();
+}
+
+}  // namespace hipk
+}  // namespace jade

@@ -39,6 +39,11 @@ constexpr OpName kOps[] = {
     {"attention_tree", Op::AttentionTree},
     {"cache_append", Op::CacheAppend},
     {"attention_cross", Op::AttentionCross},
+    {"attention_paged", Op::AttentionPaged},
+    {"pages_append", Op::PagesAppend},
+    {"pages_fork", Op::PagesFork},
+    {"pages_copy", Op::PagesCopy},
+    {"beam_select", Op::BeamSelect},
 };
 
 const char *tag_of(Op op) {
@@ -80,6 +85,12 @@ bool get_rotation(const Value &obj, KernelSpec &s, std::string &error) {
            maybe_f32(obj, "factor", s.factor, error) && maybe_f32(obj, "context", s.context, error) &&
            maybe_f32(obj, "low_turns", s.low_turns, error) && maybe_f32(obj, "high_turns", s.high_turns, error) &&
            maybe_f32(obj, "magnitude", s.magnitude, error);
+}
+
+bool get_pool(const Value &obj, KernelSpec &s, std::string &error) {
+    return get_u32(obj, "kv_heads", s.kv_heads, error) && get_u32(obj, "pages", s.pages, error) &&
+           get_u32(obj, "page", s.page, error) && get_u32(obj, "dim", s.dim, error) &&
+           get_bool(obj, "pages_token_major", s.pages_token_major, error);
 }
 
 bool parse_expr(const Value &v, Expr &out, std::string &error, int depth) {
@@ -196,6 +207,28 @@ bool grouped_ok(const KernelSpec &s, std::string &error) {
 }
 bool whole_ok(uint32_t v, const char *name, std::string &error) {
     if (!(v >= 1 && v <= kMaxWhole)) { error = std::string(name) + " must be 1..=16777216"; return false; }
+    return true;
+}
+
+// The pages and, where there are any, the tables that name them.
+bool pages_ok(const KernelSpec &s, bool tables, std::string &error) {
+    if (!(s.page >= kPageStep && s.page <= kMaxPage && s.page % kPageStep == 0)) {
+        error = "page must be a multiple of 16 in 16..=1024";
+        return false;
+    }
+    if (!whole_ok(s.pages, "pages", error)) return false;
+    if (!tables) return true;
+    if (!(s.table >= 1 && s.table <= kMaxWhole / s.page)) {
+        error = "table must be 1 or more, and table * page at most 16777216";
+        return false;
+    }
+    if (!(s.batch >= 1 && s.batch <= kHipMaxHeads)) { error = "batch must be 1..=65535"; return false; }
+    return matrix_ok(s.batch, s.table, error);
+}
+bool pool_ok(const KernelSpec &s, std::string &error) {
+    if (!(s.kv_heads >= 1 && s.kv_heads <= kHipMaxHeads)) { error = "heads and kv_heads must be 1..=65535"; return false; }
+    const uint64_t tokens = uint64_t(s.pages) * s.page;  // below 2^35
+    if (tokens * s.kv_heads > kMaxCacheElements / s.dim) { error = "cache exceeds 2^40 elements"; return false; }
     return true;
 }
 
@@ -323,6 +356,23 @@ bool parse_spec(const std::string &text, KernelSpec &out, std::string &error) {
                    get_u32(root, "kv_heads", out.kv_heads, error) && get_u32(root, "queries", out.queries, error) &&
                    get_u32(root, "keys", out.keys, error) && get_u32(root, "dim", out.dim, error) &&
                    get_bool(root, "token_major", out.token_major, error);
+        case Op::AttentionPaged:
+            return get_u32(root, "batch", out.batch, error) && get_u32(root, "heads", out.heads, error) &&
+                   get_u32(root, "queries", out.queries, error) && get_pool(root, out, error) &&
+                   get_u32(root, "table", out.table, error) && get_bool(root, "token_major", out.token_major, error);
+        case Op::PagesAppend:
+            return get_u32(root, "batch", out.batch, error) && get_u32(root, "rows", out.rows, error) &&
+                   get_pool(root, out, error) && get_u32(root, "table", out.table, error) &&
+                   get_bool(root, "token_major", out.token_major, error);
+        case Op::PagesFork:
+            return get_u32(root, "batch", out.batch, error) && get_u32(root, "pages", out.pages, error) &&
+                   get_u32(root, "page", out.page, error) && get_u32(root, "table", out.table, error);
+        case Op::PagesCopy:
+            return get_u32(root, "copies", out.copies, error) && get_pool(root, out, error);
+        case Op::BeamSelect:
+            return get_u32(root, "batch", out.batch, error) && get_u32(root, "beams", out.beams, error) &&
+                   get_u32(root, "vocab", out.vocab, error) && get_u32(root, "picks", out.picks, error) &&
+                   get_u32(root, "end", out.end, error);
     }
     return false;
 }
@@ -346,6 +396,11 @@ const char *spec_name(const KernelSpec &spec) {
         case Op::AttentionTree: return "attention_tree";
         case Op::CacheAppend: return "cache_append";
         case Op::AttentionCross: return "attention_cross";
+        case Op::AttentionPaged: return "attention_paged";
+        case Op::PagesAppend: return "pages_append";
+        case Op::PagesFork: return "pages_fork";
+        case Op::PagesCopy: return "pages_copy";
+        case Op::BeamSelect: return "beam_select";
     }
     return "?";
 }
@@ -434,6 +489,26 @@ bool validate(const KernelSpec &s, Rules rules, std::string &error) {
             return grouped_ok(s, error) && whole_ok(s.keys, "keys", error) &&
                    heads_ok(s.batch, s.heads, s.queries, s.dim, kIntMax, error) &&
                    heads_ok(s.batch, s.kv_heads, s.keys, s.dim, kMaxCacheElements, error);
+        case Op::AttentionPaged:
+            return grouped_ok(s, error) && pages_ok(s, true, error) && pool_ok(s, error) &&
+                   heads_ok(s.batch, s.heads, s.queries, s.dim, kIntMax, error) && whole_ok(s.queries, "queries", error);
+        case Op::PagesAppend:
+            if (!(s.dim >= 1 && s.dim <= kMaxRotaryDim)) { error = "head dimension must be 1..=512"; return false; }
+            return pages_ok(s, true, error) && pool_ok(s, error) && whole_ok(s.rows, "rows", error) &&
+                   heads_ok(s.batch, s.kv_heads, s.rows, s.dim, kIntMax, error);
+        case Op::PagesFork:
+            return pages_ok(s, true, error);
+        case Op::PagesCopy:
+            if (!(s.dim >= 1 && s.dim <= kMaxRotaryDim)) { error = "head dimension must be 1..=512"; return false; }
+            if (!(s.copies >= 1 && s.copies <= kHipMaxHeads)) { error = "copies must be 1..=65535"; return false; }
+            return pages_ok(s, false, error) && pool_ok(s, error);
+        case Op::BeamSelect:
+            if (!(s.beams >= 1 && s.beams <= kMaxBeams)) { error = "beams must be 1..=256"; return false; }
+            if (!(s.picks >= 1 && s.picks <= kMaxBeamPicks)) { error = "picks must be 1..=64"; return false; }
+            if (!(s.batch >= 1 && s.batch <= kHipMaxHeads)) { error = "batch must be 1..=65535"; return false; }
+            // Tokens, and numbers of sequences, are whole numbers in FP32.
+            if (uint64_t(s.batch) * s.beams > kMaxWhole) { error = "batch * beams must be at most 16777216"; return false; }
+            return whole_ok(s.vocab, "vocab", error) && matrix_ok(uint64_t(s.batch) * s.beams, s.vocab, error);
     }
     error = "unknown op";
     return false;
@@ -453,6 +528,7 @@ std::vector<Binding> bindings(const KernelSpec &s) {
     const uint64_t hsd = uint64_t(s.heads) * s.seq * s.dim;
     const uint64_t hss = uint64_t(s.heads) * s.seq * s.seq;
     const uint64_t b = s.batch, d = s.dim, kv = b * s.kv_heads * d;
+    const uint64_t pool = uint64_t(s.pages) * s.page * s.kv_heads * d;
     switch (s.op) {
         case Op::Elementwise: {
             std::vector<Binding> out;
@@ -503,6 +579,26 @@ std::vector<Binding> bindings(const KernelSpec &s) {
         case Op::AttentionCross:
             return {{"q", b * s.heads * s.queries * d, false}, {"k", kv * s.keys, false}, {"v", kv * s.keys, false},
                     {"lengths", b, false}, {"out", b * s.heads * s.queries * d, true}};
+        case Op::AttentionPaged:
+            return {{"q", b * s.heads * s.queries * d, false}, {"k_pages", pool, false}, {"v_pages", pool, false},
+                    {"tables", b * s.table, false}, {"lengths", b, false}, {"counts", b, false},
+                    {"out", b * s.heads * s.queries * d, true}};
+        case Op::PagesAppend:
+            return {{"k", kv * s.rows, false}, {"v", kv * s.rows, false}, {"counts", b, false},
+                    {"tables", b * s.table, false}, {"lengths", b, false}, {"k_pages", pool, true},
+                    {"v_pages", pool, true}, {"new_lengths", b, true}};
+        case Op::PagesFork:
+            return {{"parents", b, false}, {"lengths", b, false}, {"tables", b * s.table, false}, {"reserve", b, false},
+                    {"uses", s.pages, false}, {"new_tables", b * s.table, true}, {"new_lengths", b, true},
+                    {"new_uses", s.pages, true}, {"sources", b, true}, {"targets", b, true}, {"copy_rows", b, true},
+                    {"missing", b, true}};
+        case Op::PagesCopy:
+            return {{"sources", s.copies, false}, {"targets", s.copies, false}, {"copy_rows", s.copies, false},
+                    {"k_pages", pool, true}, {"v_pages", pool, true}};
+        case Op::BeamSelect:
+            return {{"logits", b * s.beams * s.vocab, false}, {"scores", b * s.beams, false},
+                    {"finished", b * s.beams, false}, {"parents", b * s.picks, true}, {"tokens", b * s.picks, true},
+                    {"new_scores", b * s.picks, true}, {"new_finished", b * s.picks, true}};
     }
     return {};
 }
@@ -537,6 +633,10 @@ std::string canonical_json(const KernelSpec &s) {
     auto u = [&](const char *k, uint32_t v) { out += std::string(",\"") + k + "\":" + std::to_string(v); };
     auto b = [&](const char *k, bool v) { out += std::string(",\"") + k + "\":" + (v ? "true" : "false"); };
     auto f = [&](const char *k, float v) { out += std::string(",\"") + k + "\":" + json::format_f32(v); };
+    auto pool = [&] {
+        u("kv_heads", s.kv_heads); u("pages", s.pages); u("page", s.page); u("dim", s.dim);
+        b("pages_token_major", s.pages_token_major);
+    };
     switch (s.op) {
         case Op::Elementwise:
             u("len", s.len);
@@ -578,6 +678,21 @@ std::string canonical_json(const KernelSpec &s) {
         case Op::AttentionCross:
             u("batch", s.batch); u("heads", s.heads); u("kv_heads", s.kv_heads); u("queries", s.queries);
             u("keys", s.keys); u("dim", s.dim); b("token_major", s.token_major);
+            break;
+        case Op::AttentionPaged:
+        case Op::PagesAppend:
+            u("batch", s.batch);
+            if (s.op == Op::AttentionPaged) { u("heads", s.heads); u("queries", s.queries); }
+            else u("rows", s.rows);
+            pool();
+            u("table", s.table); b("token_major", s.token_major);
+            break;
+        case Op::PagesFork:
+            u("batch", s.batch); u("pages", s.pages); u("page", s.page); u("table", s.table);
+            break;
+        case Op::PagesCopy: u("copies", s.copies); pool(); break;
+        case Op::BeamSelect:
+            u("batch", s.batch); u("beams", s.beams); u("vocab", s.vocab); u("picks", s.picks); u("end", s.end);
             break;
     }
     return out + "}";

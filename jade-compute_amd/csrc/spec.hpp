@@ -33,6 +33,12 @@ enum class Op {
     AttentionTree,
     CacheAppend,
     AttentionCross,
+    // Decoding over a paged cache, which it does not have either.
+    AttentionPaged,
+    PagesAppend,
+    PagesFork,
+    PagesCopy,
+    BeamSelect,
 };
 
 // Expression tree, ir.rs:74-84.
@@ -67,12 +73,17 @@ struct KernelSpec {
     uint32_t batch = 0, kv_heads = 0, rotary_dim = 0, queries = 0, keys = 0, nodes = 0, capacity = 0, picks = 0;
     bool interleaved = false, inverse = false, token_major = false, out_token_major = false;
     float base = 0.0f, factor = 1.0f, context = 0.0f, low_turns = 0.0f, high_turns = 0.0f, magnitude = 1.0f;
+    // Decoding over a paged cache.
+    uint32_t pages = 0, page = 0, table = 0, copies = 0, beams = 0, vocab = 0, end = 0;
+    bool pages_token_major = false;
 };
 
 constexpr uint32_t kMaxRotaryDim = 512;        // head dim: a head in one wavefront's registers
 constexpr uint32_t kMaxTreeNodes = 256;        // drafted nodes of a sequence
 constexpr uint32_t kMaxWhole = 1u << 24;       // whole numbers are FP32 values: all up to here are exact
 constexpr uint64_t kMaxCacheElements = 1ull << 40;
+constexpr uint32_t kPageStep = 16, kMaxPage = 1024;  // tokens of a page: a multiple of the one, at most the other
+constexpr uint32_t kMaxBeams = 256, kMaxBeamPicks = 64;
 
 // ir.rs:146-151. Elements are f32 counts.
 struct Binding {
