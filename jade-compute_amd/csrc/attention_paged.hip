@@ -318,23 +318,41 @@ __global__ __launch_bounds__(kThreads) void attention_paged_join(PagedArgs a) {
 }
 
 uint64_t rows_of(const PagedShape &s) { return uint64_t(s.heads / s.kv_heads) * s.queries; }
-uint32_t block_rows(const PagedShape &) { return kRows; }
-uint32_t tile_of(const PagedShape &) { return kTile; }
 
-// Tiles of a (sequence, kv head, row block) of full length, and of a launch of such.
-uint64_t paged_tiles(const PagedShape &s) {
-    const uint32_t rb = block_rows(s), tile = tile_of(s);
-    return uint64_t(s.batch) * s.kv_heads * ((rows_of(s) + rb - 1) / rb) * ((uint64_t(s.table) * s.page + tile - 1) / tile);
+// Sequences of more rows than this, for each kv head, go to the kernel on bf16 parts
+// (attention_paged_flash.hip), by a launch of its own.
+uint32_t few_rows(const PagedShape &s) { return s.dim <= 64 ? 64 : 96; }
+bool has_many(const PagedShape &s) {
+    // Offsets of a sequence's rows in 31 bits.
+    return s.dim % 4 == 0 && rows_of(s) > few_rows(s) && uint64_t(s.heads) * s.queries * s.dim < 1u << 29;
 }
 
-// Runs of a launch: two blocks a CU, or one per tile where there can be no more tiles.
-uint32_t runs_of(const PagedShape &s) {
-    const uint64_t tiles = paged_tiles(s), most = 2 * kCus;
-    return tiles >= most ? uint32_t(most) : uint32_t((tiles + 7) / 8 * 8);
+// One of the two launches: its rows a block and keys a tile; tiles of a launch of full lengths.
+struct Half {
+    uint32_t rows, tile, dims;  // dims of a row in a run's slots
+    uint64_t units, tiles;
+    uint32_t runs;
+};
+Half half_of(const PagedShape &s, uint64_t rows, uint32_t rb, uint32_t tile, uint32_t blocks) {
+    Half x{rb, tile, s.dim > 64 ? 128u : 64u, 0, 0, 0};
+    x.units = uint64_t(s.batch) * s.kv_heads * ((rows + rb - 1) / rb);
+    x.tiles = x.units * ((uint64_t(s.table) * s.page + tile - 1) / tile);
+    // As many blocks as work on the chip at once, or one per tile where there can be no more.
+    x.runs = x.tiles >= blocks ? blocks : uint32_t((x.tiles + 7) / 8 * 8);
+    return x;
 }
+Half few_of(const PagedShape &s) {
+    const uint64_t rows = rows_of(s);
+    return half_of(s, has_many(s) && rows > few_rows(s) ? few_rows(s) : rows, kRows, kTile, 2 * kCus);
+}
+Half many_of(const PagedShape &s) {
+    return half_of(s, rows_of(s), paged_flash_rows(s.dim), kPagedFlashTile, s.dim <= 64 ? 2 * kCus : kCus);
+}
+size_t bytes_of(const Half &x) { return 2 * size_t(x.runs) * x.rows * (x.dims + 2) * sizeof(float); }
 
 template <int DP, int RB, int TILE, bool VEC>
 void launch_join(hipStream_t stream, const PagedArgs &a, uint64_t units) {
+    static_assert(DP == kSlotRow<DP>, "slots are of 64 or 128 dims");
     if (a.runs < 2) return;
     constexpr uint32_t kRowsOf = kThreads / (DP / 4);  // rows of a block
     const uint64_t all = uint64_t(a.group) * a.queries;
@@ -348,9 +366,22 @@ void launch_join(hipStream_t stream, const PagedArgs &a, uint64_t units) {
 }
 
 template <int DP, bool VEC>
-hipError_t launch(hipStream_t stream, const PagedArgs &a, uint64_t units) {
+hipError_t launch(hipStream_t stream, const PagedShape &s, PagedArgs a) {
+    const Half few = few_of(s);
+    a.least_rows = 1;
+    a.most_rows = has_many(s) ? few_rows(s) : ~0u;
+    a.runs = few.runs;
     hipLaunchKernelGGL((attention_paged<DP, VEC>), dim3(a.runs), dim3(kThreads), 0, stream, a);
-    launch_join<DP, kRows, kTile, VEC>(stream, a, units);
+    launch_join<DP, kRows, kTile, VEC>(stream, a, few.units);
+    if constexpr (VEC)
+        if (has_many(s)) {
+            const Half many = many_of(s);
+            a.least_rows = a.most_rows + 1;
+            a.most_rows = ~0u;
+            a.runs = many.runs;
+            launch_paged_flash(stream, a);
+            launch_join<DP, DP == 64 ? 128 : 256, int(kPagedFlashTile), true>(stream, a, many.units);
+        }
     return hipGetLastError();
 }
 
@@ -362,15 +393,21 @@ uint32_t paged_lds_bytes(uint32_t dim) {
 }  // namespace
 
 LaunchShape attention_paged_shape(const PagedShape &s) {
+    const Half few = few_of(s), many = many_of(s);
     // Tiles are counted in 32 bits.
-    if (paged_tiles(s) > 0x7fffffffull) return {nullptr, {0, 0, 0}, {0, 0, 0}, 0};
-    return {s.dim <= 64 ? "attention_paged_d64" : "attention_paged_d128", {runs_of(s), 1, 1}, {kThreads, 1, 1},
+    if (few.tiles > 0x7fffffffull || (has_many(s) && many.tiles > 0x7fffffffull)) return {nullptr, {0, 0, 0}, {0, 0, 0}, 0};
+    if (has_many(s)) {
+        static const char *const names[4] = {"attention_paged_flash_d32", "attention_paged_flash_d64",
+                                             "attention_paged_flash_d96", "attention_paged_flash_d128"};
+        return {names[(s.dim - 1) / 32], {many.runs, 1, 1}, {2 * many.rows, 1, 1}, paged_flash_lds_bytes(s.dim)};
+    }
+    return {s.dim <= 64 ? "attention_paged_d64" : "attention_paged_d128", {few.runs, 1, 1}, {kThreads, 1, 1},
             paged_lds_bytes(s.dim)};
 }
 
 size_t attention_paged_workspace_bytes(const PagedShape &s) {
-    const size_t dp = s.dim > 64 ? 128 : 64;
-    return 2 * size_t(runs_of(s)) * block_rows(s) * (dp + 2) * sizeof(float);
+    const size_t few = bytes_of(few_of(s)), many = has_many(s) ? bytes_of(many_of(s)) : 0;
+    return few > many ? few : many;  // the launches follow each other
 }
 
 hipError_t attention_paged_f32(hipStream_t stream, const PagedShape &s, const PagedBuffers &x, float *workspace) {
@@ -389,14 +426,12 @@ hipError_t attention_paged_f32(hipStream_t stream, const PagedShape &s, const Pa
     a.pages = s.pages; a.table = s.table; a.page = s.page; a.dim = s.dim;
     a.steps = s.page / 16;
     a.inverse = uint32_t(((1ull << 31) + a.steps - 1) / a.steps);
-    a.runs = runs_of(s);
     a.qscale = (1.0f / sqrtf(float(s.dim))) * kLog2e;
     uintptr_t bits = 0;
     for (const float *y : {x.q, x.k, x.v, const_cast<const float *>(x.out)}) bits |= reinterpret_cast<uintptr_t>(y);
     if (!workspace || (s.dim % 4 == 0 && bits & 15u)) return hipErrorInvalidValue;  // the runtime's regions are aligned
-    const uint64_t units = uint64_t(s.batch) * s.kv_heads * ((rows_of(s) + kRows - 1) / kRows);
-    if (s.dim % 4) return s.dim <= 64 ? launch<64, false>(stream, a, units) : launch<128, false>(stream, a, units);
-    return s.dim <= 64 ? launch<64, true>(stream, a, units) : launch<128, true>(stream, a, units);
+    if (s.dim % 4) return s.dim <= 64 ? launch<64, false>(stream, s, a) : launch<128, false>(stream, s, a);
+    return s.dim <= 64 ? launch<64, true>(stream, s, a) : launch<128, true>(stream, s, a);
 }
 
 }  // namespace hipk

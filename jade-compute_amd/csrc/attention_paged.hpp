@@ -21,9 +21,17 @@ struct PagedArgs {
     uint32_t q_row, p_row;
     uint32_t batch, kv_heads, group, queries, pages, table, page, dim;
     uint32_t steps, inverse;  // 16-token steps of a page; 2^31 / steps, rounded up
+    uint32_t least_rows, most_rows;  // of a kv head, of the sequences that a launch takes
     uint32_t runs;
     float qscale;  // scale * log2(e)
 };
+
+// The kernel on bf16 parts (attention_paged_flash.hip). Needs dim % 4 == 0 and at most 128,
+// 16-byte aligned tensors and a sequence's rows of q below 2 GiB.
+constexpr uint32_t kPagedFlashTile = 32;
+inline uint32_t paged_flash_rows(uint32_t dim) { return dim <= 64 ? 128 : 256; }
+void launch_paged_flash(hipStream_t stream, const PagedArgs &args);
+uint32_t paged_flash_lds_bytes(uint32_t dim);
 
 namespace {
 namespace paged {
@@ -84,12 +92,18 @@ struct Work {
         if (b >= a.batch) return {0, 0};
         return {whole_below(a.lengths[b], a.table * a.page), whole_below(a.counts[b], a.queries)};
     }
-    __device__ static uint32_t tiles(const Sequence &s) { return s.count ? (s.length + TILE - 1) / TILE : 0u; }
+    __device__ uint32_t tiles(const Sequence &s) const {
+        const uint32_t rows = s.count * a.group;
+        return rows >= a.least_rows && rows <= a.most_rows ? (s.length + TILE - 1) / TILE : 0u;
+    }
     __device__ uint32_t blocks(const Sequence &s) const { return (s.count * a.group + RB - 1) / RB; }
     __device__ uint32_t all_of(const Sequence &s) const { return tiles(s) * blocks(s) * a.kv_heads; }
     // Of one sequence, for the whole wave.
     __device__ Sequence at(uint32_t b) const {
-        if (b < 64) return {of_lane(near.length, int(b)), of_lane(near.count, int(b))};
+        return b < 64 ? Sequence{of_lane(near.length, int(b)), of_lane(near.count, int(b))} : anew(b);
+    }
+    // The same from memory: no register keeps the near ones for it.
+    __device__ Sequence anew(uint32_t b) const {
         const Sequence s = load(b);
         return {uniform(s.length), uniform(s.count)};
     }
@@ -163,6 +177,14 @@ __device__ inline void store_dims(float *row, int d, int dim, f32x4 x) {
     }
 }
 
+// The lane's number, made anew: what is computed from it is not kept in registers from
+// outside a main loop.
+__device__ inline int lane_now() {
+    int l = __builtin_amdgcn_mbcnt_hi(~0u, __builtin_amdgcn_mbcnt_lo(~0u, 0u));
+    asm volatile("" : "+v"(l));
+    return l;
+}
+
 // Row r of (sequence b, kv head), from its first dim, in q and out.
 __device__ inline size_t row_at(const PagedArgs &a, uint32_t b, uint32_t kv, uint32_t r) {
     const uint32_t query = r / a.group, head = r - query * a.group;
@@ -173,11 +195,13 @@ __device__ inline size_t row_at(const PagedArgs &a, uint32_t b, uint32_t kv, uin
 struct Place {
     uint32_t entry, step;  // of 16 tokens within the page
 };
-__device__ inline Place place_of(const PagedArgs &a, uint32_t n) {
+template <class Args>
+__device__ inline Place place_of(const Args &a, uint32_t n) {
     const uint32_t entry = uint32_t(uint64_t(n) * a.inverse >> 31);
     return {entry, n - entry * a.steps};
 }
-__device__ inline uint32_t page_of(const PagedArgs &a, float entry) {
+template <class Args>
+__device__ inline uint32_t page_of(const Args &a, float entry) {
     return entry >= 0.f && entry < float(a.pages) && entry == truncf(entry) ? uint32_t(entry) : kNoPage;
 }
 

@@ -104,7 +104,7 @@ def test_attention_paged_odd_lengths_and_counts(runtime, heads, kv_heads, querie
     assert (got[none] == 0).all()
 
 
-@pytest.mark.parametrize("queries,dim", [(1, 64), (5, 80), (24, 128)])
+@pytest.mark.parametrize("queries,dim", [(1, 64), (5, 80), (24, 128), (48, 64), (48, 32), (48, 96), (48, 128), (48, 37)])
 def test_attention_paged_entries_that_name_no_page(runtime, queries, dim):
     rng = np.random.default_rng(8)
     spec = paged_spec(4, 4, 2, queries, 48, 4, dim)
@@ -115,7 +115,8 @@ def test_attention_paged_entries_that_name_no_page(runtime, queries, dim):
     assert (got[3] == 0).all()
 
 
-@pytest.mark.parametrize("queries,dim", [(3, 64), (9, 128), (30, 64), (40, 128), (25, 80), (5, 37), (21, 30)])
+@pytest.mark.parametrize("queries,dim", [(3, 64), (9, 128), (30, 64), (40, 128), (25, 80), (5, 37), (21, 30), (70, 64), (90, 128),
+                                         (120, 32), (140, 80), (100, 37)])
 def test_attention_paged_later_tokens_that_are_not_finite(runtime, queries, dim):
     # A chunk's own keys and values that are not finite reach the queries from that token on and no others.
     rng = np.random.default_rng(9)
@@ -137,7 +138,7 @@ def test_attention_paged_later_tokens_that_are_not_finite(runtime, queries, dim)
     assert not np.isfinite(got[:, first:]).any()
 
 
-@pytest.mark.parametrize("queries,dim", [(1, 64), (1, 128), (3, 80), (20, 128), (40, 64)])
+@pytest.mark.parametrize("queries,dim", [(1, 64), (1, 128), (3, 80), (20, 128), (40, 64), (60, 128), (200, 64), (70, 32), (90, 80)])
 @pytest.mark.parametrize("layout", LAYOUTS)
 def test_attention_paged_long_contexts_are_cut_and_joined(runtime, queries, dim, layout):
     rng = np.random.default_rng(10)
@@ -145,18 +146,47 @@ def test_attention_paged_long_contexts_are_cut_and_joined(runtime, queries, dim,
     check_paged(runtime, spec, paged_inputs(rng, spec, [3840, 1777], [queries, 1]))
 
 
-@pytest.mark.parametrize("queries", [1, 12, 24])
+@pytest.mark.parametrize("queries", [1, 12, 24, 64])
 def test_attention_paged_many_sequences_most_of_them_idle(runtime, queries):
     # More than a wave's lanes of sequences, most of them without tokens or without new ones.
     rng = np.random.default_rng(11)
     batch = 333
-    spec = paged_spec(batch, 2, 2, queries, 16, 4, 32)
+    spec = paged_spec(batch, 4, 2, queries, 16, 4, 32)
     lengths = [int(rng.integers(1, 65)) if b % 3 == 0 else 0 for b in range(batch)]
     counts = [0 if b % 5 == 0 else min(max(n, 1), int(rng.integers(1, queries + 1))) for b, n in enumerate(lengths)]
     check_paged(runtime, spec, paged_inputs(rng, spec, lengths, counts))
 
 
-@pytest.mark.parametrize("queries", [1, 24])
+# Whole prompts without a past, whose blocks of rows end at keys of their own; many short units a run.
+@pytest.mark.parametrize("batch,heads,kv_heads,length,dim", [(1, 4, 1, 700, 64), (2, 2, 2, 600, 128), (3, 24, 24, 300, 32), (40, 8, 8, 150, 64)])
+def test_attention_paged_whole_prompts(runtime, batch, heads, kv_heads, length, dim):
+    rng = np.random.default_rng(16)
+    spec = paged_spec(batch, heads, kv_heads, length, 32, -(-length // 32), dim)
+    lengths = [length - 7 * b for b in range(batch)]
+    x = paged_inputs(rng, spec, [max(1, n) for n in lengths], [max(1, n) for n in lengths])
+    if batch * heads * length * length < 4e6:
+        check_paged(runtime, spec, x)
+        return
+    # The same from a sequence's own prompt by itself, which the small cases check.
+    got = po.rows_by_token(spec, run(runtime, spec, x)["out"], heads, length)
+    for b in (0, batch // 2, batch - 1):
+        one = dict(spec, batch=1)
+        y = dict(x, tables=x["tables"][b:b + 1], lengths=x["lengths"][b:b + 1], counts=x["counts"][b:b + 1],
+                 q=x["q"].reshape(batch, -1)[b])
+        n = int(x["lengths"][b])
+        rows = [0, n // 2, n - 1]
+        pools = [po.pool_by_token(spec, x[name].astype(np.float64)) for name in ("k_pages", "v_pages")]
+        places = po.places(spec, x["tables"][b], range(n))
+        keys, values = ([pool[p] for p in places] for pool in pools)
+        keys, values = np.array(keys), np.array(values)
+        q = po.rows_by_token(one, y["q"].astype(np.float64), heads, length)[0]
+        for i in rows:
+            for h in (0, heads - 1):
+                want, off = po.attend(q[i, h], keys[:, h * kv_heads // heads], values[:, h * kv_heads // heads], range(i + 1))
+                assert (np.abs(got[b, i, h] - want) <= off).all()
+
+
+@pytest.mark.parametrize("queries", [1, 24, 70])
 def test_attention_paged_sequences_that_share_pages(runtime, queries):
     rng = np.random.default_rng(12)
     spec = paged_spec(3, 4, 4, queries, 16, 8, 64)
@@ -165,7 +195,7 @@ def test_attention_paged_sequences_that_share_pages(runtime, queries):
     check_paged(runtime, spec, x)
 
 
-@pytest.mark.parametrize("queries,dim", [(1, 64), (24, 128), (24, 80)])
+@pytest.mark.parametrize("queries,dim", [(1, 64), (24, 128), (24, 80), (40, 64), (60, 128), (60, 96)])
 def test_attention_paged_large_and_tiny_operands(runtime, queries, dim):
     rng = np.random.default_rng(13)
     spec = paged_spec(1, 2, 1, queries, 16, 6, dim)
@@ -182,7 +212,7 @@ def test_attention_paged_large_and_tiny_operands(runtime, queries, dim):
 
 def test_attention_paged_runs_the_same_twice(runtime):
     rng = np.random.default_rng(14)
-    for queries in (1, 24):
+    for queries in (1, 24, 100):
         spec = paged_spec(3, 8, 2, queries, 16, 40, 128)
         x = paged_inputs(rng, spec, [640, 333, 500], [queries, 1, queries])
         first, again = (run(runtime, spec, x, repeats)["out"] for repeats in (1, 3))
