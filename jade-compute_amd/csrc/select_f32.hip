@@ -28,6 +28,7 @@ typedef float f32x4 __attribute__((ext_vector_type(4)));
 constexpr int kThreads = 256, kWaves = 4;
 constexpr uint32_t kListed = 1024;       // values that a block ranks at once
 constexpr uint32_t kMaxBlocks = 1u << 20;
+constexpr uint32_t kRawBuffer = 0x00020000;  // buffer descriptor word 3: raw buffer, 32-bit data format
 constexpr float kLog2e = 1.44269504088896340736f;
 constexpr float kLog2eRest = 1.92596299112661746887e-8f;  // log2(e) less the float above
 constexpr float kLn2 = 0.693147180559945309417f;
@@ -47,6 +48,9 @@ __device__ inline uint64_t ordered(double x) {
 __device__ inline double value_of(uint64_t key) {
     return __longlong_as_double(int64_t(key ^ (key >> 63 ? 1ull << 63 : ~0ull)));
 }
+// A logit and its token as one key: larger logits first, then lower tokens; no zero is
+// below another.
+__device__ inline uint64_t key_of(float x, uint32_t token) { return uint64_t(ordered(x + 0.f)) << 32 | ~token; }
 constexpr uint32_t kNone = 0x007fffffu;        // ordered(-INFINITY)
 constexpr uint64_t kNone64 = 0x000fffffffffffffull;
 
@@ -64,14 +68,14 @@ __host__ __device__ inline Space space_of(float *workspace, uint64_t items, uint
     return {value, token, sum, reinterpret_cast<float *>(token + items * list)};
 }
 
-// exp(x - top), x <= top, off by a rounding of exp2: the argument's rounding, d times
-// log2(e) in two parts, is put back to first order.
+// exp(x - top), x <= top and top finite, off by a rounding of exp2 and one more: the
+// argument's roundings are put back to first order. Nothing of 2^-126 or less counts.
 __device__ inline float exp_below(float x, float top) {
-    if (x == top) return 1.f;
-    const float d = x - top, back = d + top, lost = x - back;  // x = top + d + lost, where all are finite
-    const float hi = d * kLog2e, lo = fmaf(d, kLog2e, -hi) + fmaf(d, kLog2eRest, lost * kLog2e);
+    const float d = fmaxf(x - top, -100.f);
+    const float lost = __builtin_amdgcn_fmed3f(x - (d + top), -1.f, 1.f);  // x = top + d + lost, but for those
+    const float hi = d * kLog2e, lo = fmaf(lost, kLog2e, fmaf(d, kLog2eRest, fmaf(d, kLog2e, -hi)));
     const float e = __builtin_amdgcn_exp2f(hi);
-    return hi > -150.f ? fmaf(e, lo * kLn2, e) : 0.f;
+    return fmaf(e, lo * kLn2, e);
 }
 
 __device__ inline float wave_max(float x) {
@@ -104,8 +108,8 @@ __device__ inline uint32_t nth_bound(uint32_t key, uint32_t n) {
     return bound;
 }
 
-// V: float4s, or four floats, a thread. VEC: rows of whole float4s.
-template <int V, bool VEC>
+// V: float4s a thread.
+template <int V>
 __global__ __launch_bounds__(kThreads) void beam_chunks(BeamSelectArgs a, uint32_t chunks, uint32_t items) {
     __shared__ float tops[kWaves];
     __shared__ double sums[kWaves];
@@ -118,32 +122,31 @@ __global__ __launch_bounds__(kThreads) void beam_chunks(BeamSelectArgs a, uint32
         const uint32_t beam = item / chunks, first = (item - beam * chunks) * kChunk;
         // Nothing of a beam that is finished, or cannot go on, is asked for.
         if (a.finished[beam] > 0.f || !(a.scores[beam] > -INFINITY)) continue;
-        const float *const row = a.logits + size_t(beam) * a.vocab;
-        auto token_of = [&](int i, int e) { return first + (VEC ? (i * kThreads + tid) * 4 + e : (4 * i + e) * kThreads + tid); };
-        float x[V][4];
-#pragma unroll
-        for (int i = 0; i < V; ++i) {
-            if (VEC) {
-                f32x4 v = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-                if (token_of(i, 0) < a.vocab)
-                    v = __builtin_nontemporal_load(reinterpret_cast<const f32x4 *>(row + token_of(i, 0)));
-#pragma unroll
-                for (int e = 0; e < 4; ++e) x[i][e] = v[e];
-            } else {
-#pragma unroll
-                for (int e = 0; e < 4; ++e)
-                    x[i][e] = token_of(i, e) < a.vocab ? __builtin_nontemporal_load(row + token_of(i, e)) : -INFINITY;
-            }
-        }
-        float most = -INFINITY;
+        // The row's own descriptor: what lies past its end is never read, and vectors need no
+        // more than 4-byte alignment.
+        const __amdgpu_buffer_rsrc_t row = __builtin_amdgcn_make_buffer_rsrc(
+            const_cast<float *>(a.logits + size_t(beam) * a.vocab), 0, int(a.vocab * 4u), int(kRawBuffer));
+        auto token_of = [&](int i, int e) { return first + (i * kThreads + tid) * 4 + e; };
+        f32x4 x[V];
 #pragma unroll
         for (int i = 0; i < V; ++i)
+            x[i] = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(row, int(token_of(i, 0) * 4u), 0, 0));
+        if (first + kChunk > a.vocab)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                if (x[i][e] != x[i][e]) x[i][e] = -INFINITY;  // NaN is not chosen
-                most = fmaxf(most, x[i][e]);
-            }
-        const uint32_t bound = nth_bound(ordered(most), list < 64 ? list : 64);
+            for (int i = 0; i < V; ++i)
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    if (token_of(i, e) >= a.vocab) x[i][e] = -INFINITY;
+        float best[V];  // of four tokens
+        float most = -INFINITY;
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) x[i][e] = fmaxf(x[i][e], -INFINITY);  // NaN is not chosen
+            best[i] = fmaxf(fmaxf(x[i][0], x[i][1]), fmaxf(x[i][2], x[i][3]));
+            most = fmaxf(most, best[i]);
+        }
+        const uint32_t bound = nth_bound(ordered(most + 0.f), list < 64 ? list : 64);
         float top = wave_max(most);
         if (lane == 0) {
             tops[wave] = top;
@@ -152,18 +155,30 @@ __global__ __launch_bounds__(kThreads) void beam_chunks(BeamSelectArgs a, uint32
         if (tid == 0) count = 0;
         __syncthreads();
         top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
-        const uint32_t from = max(max(max(bounds[0], bounds[1]), max(bounds[2], bounds[3])), kNone + 1);
+        const float from = value_of(max(max(max(bounds[0], bounds[1]), max(bounds[2], bounds[3])), kNone + 1));
         double sum = 0;
+        if (fabsf(top) < INFINITY) {
 #pragma unroll
-        for (int i = 0; i < V; ++i)
+            for (int i = 0; i < V; ++i)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                sum += double(exp_below(x[i][e], top));
-                if (ordered(x[i][e]) >= from) {
+                for (int e = 0; e < 4; e += 2)
+                    sum += double(exp_below(x[i][e], top) + exp_below(x[i][e + 1], top));
+        } else {  // infinite logits share what there is
+#pragma unroll
+            for (int i = 0; i < V; ++i)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) sum += x[i][e] == top ? 1.0 : 0.0;
+        }
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+            if (best[i] < from) continue;
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                if (x[i][e] >= from) {
                     const uint32_t at = atomicAdd(&count, 1u);
-                    if (at < kListed) keys[at] = uint64_t(ordered(x[i][e])) << 32 | ~token_of(i, e);
+                    if (at < kListed) keys[at] = key_of(x[i][e], token_of(i, e));
                 }
-            }
+        }
         sum = wave_sum(sum);
         if (lane == 0) sums[wave] = sum;
         __syncthreads();
@@ -177,6 +192,7 @@ __global__ __launch_bounds__(kThreads) void beam_chunks(BeamSelectArgs a, uint32
             for (uint32_t c = tid; c < n; c += kThreads) {
                 const uint64_t mine = keys[c];
                 uint32_t rank = 0;
+#pragma unroll 8
                 for (uint32_t i = 0; i < n; ++i) rank += keys[i] > mine;
                 if (rank < list) {
                     w.value[to + rank] = value_of(uint32_t(mine >> 32));
@@ -192,7 +208,7 @@ __global__ __launch_bounds__(kThreads) void beam_chunks(BeamSelectArgs a, uint32
                 for (int i = 0; i < V; ++i)
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
-                        const uint64_t key = uint64_t(ordered(x[i][e])) << 32 | ~token_of(i, e);
+                        const uint64_t key = key_of(x[i][e], token_of(i, e));
                         if (key < last && key > best) best = key;
                     }
                 best = wave_max(best);
@@ -219,60 +235,86 @@ __device__ inline bool above(uint64_t key, uint32_t number, uint64_t other, uint
     return key > other || (key == other && number < others);
 }
 
+constexpr uint32_t kNear = 8;  // candidates that a thread keeps in registers
+
 __global__ __launch_bounds__(kThreads) void beam_join(BeamSelectArgs a, uint32_t chunks, uint32_t items) {
-    __shared__ float tops[kMaxBeams];
+    __shared__ float tops[kMaxBeams], scores[kMaxBeams], ended[kMaxBeams];
     __shared__ double logs[kMaxBeams];
     __shared__ uint32_t bounds[kWaves], count;
     __shared__ Ranked ranked[kListed];
     const uint32_t tid = threadIdx.x, lane = tid & 63, wave = tid / 64, list = min(a.picks, a.vocab);
     const uint32_t b = blockIdx.x, first = b * a.beams;
     const Space w = space_of(a.workspace, items, list);
+    const uint32_t per_beam = chunks * list, all = a.beams * per_beam;
+    // The first candidates are on their way while the beams' sums are joined.
+    const size_t from_first = size_t(first) * per_beam;
+    float near_x[kNear];
+    uint32_t near_token[kNear];
+#pragma unroll
+    for (uint32_t i = 0; i < kNear; ++i) {
+        const uint32_t c = tid + i * kThreads;
+        near_x[i] = c < all ? w.value[from_first + c] : 0.f;
+        near_token[i] = c < all ? w.token[from_first + c] : 0u;
+    }
     for (uint32_t beam = wave; beam < a.beams; beam += kWaves) {
         const size_t at = size_t(first + beam) * chunks;
-        float top = -INFINITY;
-        double sum = 0;
-        if (!(a.finished[first + beam] > 0.f) && a.scores[first + beam] > -INFINITY) {
-            for (uint32_t i = lane; i < chunks; i += 64) top = fmaxf(top, w.top[at + i]);
+        const float score = a.scores[first + beam], end = a.finished[first + beam];
+        // The first 64 chunks' maxima and sums together; of a beam that does not go on they
+        // are nothing.
+        float top = lane < chunks ? w.top[at + lane] : -INFINITY, x = top;
+        const double near_sum = lane < chunks ? w.sum[at + lane] : 0.0;
+        if (!(end > 0.f) && score > -INFINITY) {
+            for (uint32_t i = 64 + lane; i < chunks; i += 64) top = fmaxf(top, w.top[at + i]);
             top = wave_max(top);
+            double sum = 0;
             for (uint32_t i = lane; i < chunks; i += 64) {
-                const float x = w.top[at + i];
-                if (x > -INFINITY) sum += w.sum[at + i] * (x == top ? 1.0 : exp(double(x) - double(top)));
+                if (i >= 64) x = w.top[at + i];
+                if (x > -INFINITY) sum += (i >= 64 ? w.sum[at + i] : near_sum) * (x == top ? 1.0 : exp(double(x) - double(top)));
             }
             sum = wave_sum(sum);
+            if (lane == 0) logs[beam] = log(sum);
         }
         if (lane == 0) {
             tops[beam] = top;
-            logs[beam] = log(sum);
+            scores[beam] = score;
+            ended[beam] = end;
         }
     }
     if (tid == 0) count = 0;
     __syncthreads();
-    const uint32_t per_beam = chunks * list, all = a.beams * per_beam;
-    // Candidate c of the search; a finished beam has one, in the place of its first.
-    auto candidate = [&](uint32_t c, uint64_t &key, uint32_t &number) {
+    // Candidate c of the search, of a logit and token as its chunk left them; a finished beam
+    // has one, in the place of its first.
+    auto rate = [&](uint32_t c, float x, uint32_t token, uint64_t &key, uint32_t &number) __attribute__((always_inline)) {
         const uint32_t beam = c / per_beam;
-        const float score = a.scores[first + beam];
+        const double score = double(scores[beam]);
         key = kNone64;
         number = 0;
         if (!(score > -INFINITY)) return;
-        if (a.finished[first + beam] > 0.f) {
+        if (ended[beam] > 0.f) {
             if (c == beam * per_beam && a.end < a.vocab) {
-                key = ordered(double(score));
+                key = ordered(score + 0.0);
                 number = beam * a.vocab + a.end;
             }
             return;
         }
-        const size_t at = size_t(first) * per_beam + c;
-        const float x = w.value[at];
-        if (!(x > -INFINITY)) return;
         // Infinite logits share what there is.
         const double below = x == tops[beam] ? 0.0 : double(x) - double(tops[beam]);
-        if (!(below > -INFINITY)) return;
-        key = ordered(below - logs[beam] + double(score));
-        number = beam * a.vocab + w.token[at];
+        if (!(x > -INFINITY) || !(below > -INFINITY)) return;
+        key = ordered(below - logs[beam] + score + 0.0);
+        number = beam * a.vocab + token;
     };
+    auto candidate = [&](uint32_t c, uint64_t &key, uint32_t &number) {
+        rate(c, w.value[from_first + c], w.token[from_first + c], key, number);
+    };
+    uint64_t near[kNear];
     uint32_t most = 0;
-    for (uint32_t c = tid; c < all; c += kThreads) {
+#pragma unroll
+    for (uint32_t i = 0; i < kNear; ++i) {
+        near[i] = kNone64;
+        if (tid + i * kThreads < all) rate(tid + i * kThreads, near_x[i], near_token[i], near[i], near_token[i]);
+        most = max(most, uint32_t(near[i] >> 32));
+    }
+    for (uint32_t c = tid + kNear * kThreads; c < all; c += kThreads) {
         uint64_t key;
         uint32_t number;
         candidate(c, key, number);
@@ -282,30 +324,36 @@ __global__ __launch_bounds__(kThreads) void beam_join(BeamSelectArgs a, uint32_t
     if (lane == 0) bounds[wave] = bound;
     __syncthreads();
     const uint32_t from = max(max(bounds[0], bounds[1]), max(bounds[2], bounds[3]));
-    for (uint32_t c = tid; c < all; c += kThreads) {
-        uint64_t key;
-        uint32_t number;
-        candidate(c, key, number);
+    auto list_it = [&](uint64_t key, uint32_t number) __attribute__((always_inline)) {
         if (key > kNone64 && uint32_t(key >> 32) >= from) {
             const uint32_t at = atomicAdd(&count, 1u);
             if (at < kListed) ranked[at] = {key, number, 0};
         }
+    };
+#pragma unroll
+    for (uint32_t i = 0; i < kNear; ++i) list_it(near[i], near_token[i]);
+    for (uint32_t c = tid + kNear * kThreads; c < all; c += kThreads) {
+        uint64_t key;
+        uint32_t number;
+        candidate(c, key, number);
+        list_it(key, number);
     }
     __syncthreads();
     const uint32_t n = count;
     const size_t to = size_t(b) * a.picks;
-    auto pick = [&](uint32_t rank, uint64_t key, uint32_t number) {
+    auto pick = [&](uint32_t rank, uint64_t key, uint32_t number) __attribute__((always_inline)) {
         const uint32_t beam = number / a.vocab, token = number - beam * a.vocab;
         a.parents[to + rank] = float(first + beam);
         a.tokens[to + rank] = float(token);
         a.new_scores[to + rank] = float(value_of(key));
-        a.new_finished[to + rank] = token == a.end || a.finished[first + beam] > 0.f ? 1.f : 0.f;
+        a.new_finished[to + rank] = token == a.end || ended[beam] > 0.f ? 1.f : 0.f;
     };
     uint32_t got = min(n, a.picks);
     if (n <= kListed) {
         for (uint32_t c = tid; c < n; c += kThreads) {
             const Ranked mine = ranked[c];
             uint32_t rank = 0;
+#pragma unroll 8
             for (uint32_t i = 0; i < n; ++i) rank += above(ranked[i].key, ranked[i].number, mine.key, mine.number);
             if (rank < a.picks) pick(rank, mine.key, mine.number);
         }
@@ -368,10 +416,7 @@ uint32_t chunks_of(uint32_t batch, uint32_t beams, uint32_t vocab) {
 template <int V>
 void launch_chunks(hipStream_t stream, const BeamSelectArgs &a, uint32_t chunks, uint32_t items) {
     const dim3 grid(items < kMaxBlocks ? items : kMaxBlocks);
-    if (a.vocab % 4)
-        hipLaunchKernelGGL((beam_chunks<V, false>), grid, dim3(kThreads), 0, stream, a, chunks, items);
-    else
-        hipLaunchKernelGGL((beam_chunks<V, true>), grid, dim3(kThreads), 0, stream, a, chunks, items);
+    hipLaunchKernelGGL(beam_chunks<V>, grid, dim3(kThreads), 0, stream, a, chunks, items);
 }
 
 }  // namespace
@@ -389,7 +434,7 @@ size_t beam_select_workspace_bytes(uint32_t batch, uint32_t beams, uint32_t voca
 }
 
 hipError_t beam_select_f32(hipStream_t stream, const BeamSelectArgs &a) {
-    if (!a.workspace || (a.vocab % 4 == 0 && reinterpret_cast<uintptr_t>(a.logits) & 15u)) return hipErrorInvalidValue;
+    if (!a.workspace) return hipErrorInvalidValue;
     const uint32_t chunks = chunks_of(a.batch, a.beams, a.vocab), items = a.batch * a.beams * chunks;
     switch (words_of(a.batch, a.beams, a.vocab)) {
         case 8: launch_chunks<8>(stream, a, chunks, items); break;
