@@ -203,75 +203,99 @@ __device__ inline uint32_t parent_of(const PagesForkArgs &a, uint32_t s) {
     return is_whole(a.parents[s], a.batch) ? uint32_t(a.parents[s]) : a.batch;
 }
 
-// Pages of a table before its first entry that names none, for all threads of the block.
-__device__ inline uint32_t held_by(const PagesForkArgs &a, uint32_t s, uint32_t &least) {
-    if (threadIdx.x == 0) least = a.table;
-    __syncthreads();
-    const float *table = a.tables + size_t(s) * a.table;
+// A table's entries that a thread keeps in registers (of kThreads at a time); -1 past the
+// table, or where it names no page.
+constexpr uint32_t kNearEntries = 8;
+struct Entries {
+    float x[kNearEntries];
+};
+__device__ inline Entries near_entries(const PagesForkArgs &a, const float *table) {
+    Entries e;
+#pragma unroll
+    for (uint32_t i = 0; i < kNearEntries; ++i) {
+        const uint32_t at = threadIdx.x + i * kThreads;
+        e.x[i] = at < a.table ? table[at] : -1.f;
+    }
+    return e;
+}
+// The first of this thread's entries that names no page, or the table's end.
+__device__ inline uint32_t first_gap(const PagesForkArgs &a, const float *table, const Entries &e) {
     uint32_t bad = a.table;
-#pragma unroll 4
-    for (uint32_t e = threadIdx.x; e < a.table; e += kThreads)
-        if (!is_whole(table[e], a.pages)) bad = min(bad, e);
-    if (bad < a.table) atomicMin(&least, bad);
-    __syncthreads();
-    const uint32_t got = least;
-    __syncthreads();
-    return got;
+    for (uint32_t at = threadIdx.x + kNearEntries * kThreads; at < a.table; at += kThreads)
+        if (!is_whole(table[at], a.pages)) bad = min(bad, at);
+#pragma unroll
+    for (uint32_t i = 0; i < kNearEntries; ++i)
+        if (!is_whole(e.x[i], a.pages)) bad = min(bad, threadIdx.x + i * kThreads);
+    return bad;
 }
 
 __global__ __launch_bounds__(kThreads) void pages_fork_tables(PagesForkArgs a) {
-    __shared__ uint32_t least, children, older;
+    __shared__ uint32_t children, older, held, theirs;
     const ForkSpace w = fork_space(a.workspace, a.pages, a.batch);
-    const uint32_t s = blockIdx.x, parent = parent_of(a, s);
-    if (threadIdx.x == 0) children = older = 0;
-    __syncthreads();
-    uint32_t mine = 0, before = 0;
-    for (uint32_t i = threadIdx.x; i < a.batch; i += kThreads) {
+    const uint32_t s = blockIdx.x, parent = parent_of(a, s), tid = threadIdx.x;
+    const bool alive = parent < a.batch;
+    const float *const table = a.tables + size_t(s) * a.table;
+    const float *const from = a.tables + size_t(alive ? parent : s) * a.table;
+    // Everything that is read, at once: both tables and who goes on from whom.
+    const Entries mine = near_entries(a, table), yours = near_entries(a, from);
+    const float my_length = a.lengths[s], your_length = a.lengths[alive ? parent : s], reserve = a.reserve[s];
+    uint32_t going = 0, before = 0;
+    for (uint32_t i = tid; i < a.batch; i += kThreads) {
         const uint32_t p = parent_of(a, i);
-        mine += p == s;
+        going += p == s;
         before += p == parent && i < s;
     }
-    if (mine) atomicAdd(&children, mine);
+    if (tid == 0) {
+        children = older = 0;
+        held = theirs = a.table;
+    }
+    __syncthreads();
+    // Pages of a table: those before its first entry that names none.
+    const uint32_t gap = first_gap(a, table, mine), your_gap = first_gap(a, from, yours);
+    if (gap < a.table) atomicMin(&held, gap);
+    if (your_gap < a.table) atomicMin(&theirs, your_gap);
+    if (going) atomicAdd(&children, going);
     if (before) atomicAdd(&older, before);
-    const uint32_t held = held_by(a, s, least);
+    __syncthreads();
     {
         // This sequence's pages: whole ones for each child, the others for its first.
-        const uint32_t length = min(whole_below(a.lengths[s], a.table * a.page), held * a.page), full = length / a.page;
-        const float *table = a.tables + size_t(s) * a.table;
+        const uint32_t length = min(whole_below(my_length, a.table * a.page), held * a.page), full = length / a.page;
         const int n = int(children);
-        if (n != 1)
-            for (uint32_t e = threadIdx.x; e < held; e += kThreads) {
-                const int more = (e < full ? n : min(n, 1)) - 1;
-                if (more) atomicAdd(w.sums + uint32_t(table[e]), more);
-            }
+        auto gain = [&](uint32_t e, float page) {
+            const int more = (e < full ? n : min(n, 1)) - 1;
+            if (e < held && more) atomicAdd(w.sums + uint32_t(page), more);
+        };
+        if (n != 1) {
+#pragma unroll
+            for (uint32_t i = 0; i < kNearEntries; ++i) gain(tid + i * kThreads, mine.x[i]);
+            for (uint32_t e = tid + kNearEntries * kThreads; e < held; e += kThreads) gain(e, table[e]);
+        }
     }
     float *const to = a.new_tables + size_t(s) * a.table;
-    uint32_t keep = 0, need = 0, length = 0, part = 0;
-    float source = -1.f;
-    if (parent < a.batch) {
-        const uint32_t theirs = parent == s ? held : held_by(a, parent, least);
-        length = min(whole_below(a.lengths[parent], a.table * a.page), theirs * a.page);
-        const uint32_t full = length / a.page;
-        const float *from = a.tables + size_t(parent) * a.table;
+    uint32_t keep = 0, need = 0, length = 0, part = 0, full = 0;
+    if (alive) {
+        length = min(whole_below(your_length, a.table * a.page), theirs * a.page);
+        full = length / a.page;
         keep = older ? full : theirs;
-        if (older && full * a.page < length) {
-            part = length - full * a.page;
-            source = from[full];
-        }
-        const uint64_t end = uint64_t(length) + whole_below(a.reserve[s], a.table * a.page);
+        if (older) part = length - full * a.page;
+        const uint64_t end = uint64_t(length) + whole_below(reserve, a.table * a.page);
         const uint32_t want = uint32_t(min(uint64_t(a.table), (end + a.page - 1) / a.page));
         need = want > keep ? want - keep : 0;
-#pragma unroll 4
-        for (uint32_t e = threadIdx.x; e < a.table; e += kThreads) to[e] = e < keep ? from[e] : -1.f;
-    } else {
-        for (uint32_t e = threadIdx.x; e < a.table; e += kThreads) to[e] = -1.f;
     }
-    if (threadIdx.x == 0) {
+    auto inherit = [&](uint32_t e, float page) {
+        to[e] = e < keep ? page : -1.f;
+        if (part && e == full) a.sources[s] = page;  // its partial page, which this sequence gets a copy of
+    };
+#pragma unroll
+    for (uint32_t i = 0; i < kNearEntries; ++i)
+        if (tid + i * kThreads < a.table) inherit(tid + i * kThreads, yours.x[i]);
+    for (uint32_t e = tid + kNearEntries * kThreads; e < a.table; e += kThreads) inherit(e, from[e]);
+    if (tid == 0) {
         w.keep[s] = keep;
         w.need[s] = need;
         a.new_lengths[s] = float(length);
         a.copy_rows[s] = float(part);
-        a.sources[s] = source;
+        if (!part) a.sources[s] = -1.f;
     }
 }
 
@@ -327,19 +351,35 @@ __global__ __launch_bounds__(kThreads) void pages_fork_count(PagesForkArgs a) {
     if (threadIdx.x == 0) w.before[a.batch] = before;
 }
 
+constexpr uint32_t kNearNeeds = 2048;
+
 __global__ __launch_bounds__(kThreads) void pages_fork_allot(PagesForkArgs a) {
+    __shared__ uint32_t needs[kNearNeeds];
     const ForkSpace w = fork_space(a.workspace, a.pages, a.batch);
     const uint32_t blocks = fork_blocks(a.pages), asked = w.before[a.batch];
     const bool pages = blockIdx.x < blocks;
-    if (pages && !asked) return;
-    // Free pages before this block's, or of the whole pool.
-    uint32_t free = 0, n = 0;
-    for (uint32_t i = threadIdx.x; i < (pages ? blockIdx.x : blocks); i += kThreads) n += w.counts[i];
-    block_scan(n, free);
+    // Everything that is read, at once: four neighbouring pages a thread, the free ones of the
+    // blocks before (of a block of sequences: of all), and for the search below the sums of
+    // needs, in LDS where they fit.
+    const uint32_t first = blockIdx.x * kForkPages + 4 * threadIdx.x;
+    const bool fits = a.batch <= kNearNeeds;
+    bool open[4];
+    uint32_t free = 0, before = 0, n = 0;
+    if (pages) {
+#pragma unroll
+        for (uint32_t i = 0; i < 4; ++i) {
+            open[i] = first + i < a.pages && a.new_uses[first + i] == 0.f;
+            n += open[i];
+        }
+        if (fits)
+            for (uint32_t s = threadIdx.x; s < a.batch; s += kThreads) needs[s] = w.before[s];
+    }
+    for (uint32_t i = threadIdx.x; i < (pages ? blockIdx.x : blocks); i += kThreads) before += w.counts[i];
+    block_scan(before, free);
     if (!pages) {
         const uint32_t s = (blockIdx.x - blocks) * kThreads + threadIdx.x;
         if (s >= a.batch) return;
-        const uint32_t before = w.before[s], need = w.need[s], got = before < free ? min(need, free - before) : 0u;
+        const uint32_t start = w.before[s], need = w.need[s], got = start < free ? min(need, free - start) : 0u;
         a.missing[s] = float(need - got);
         const bool copy = a.copy_rows[s] > 0.f;
         if (!copy || !got) a.targets[s] = -1.f;
@@ -351,15 +391,6 @@ __global__ __launch_bounds__(kThreads) void pages_fork_allot(PagesForkArgs a) {
         return;
     }
     if (free >= asked) return;
-    // Four neighbouring pages a thread.
-    const uint32_t first = blockIdx.x * kForkPages + 4 * threadIdx.x;
-    bool open[4];
-    n = 0;
-#pragma unroll
-    for (uint32_t i = 0; i < 4; ++i) {
-        open[i] = first + i < a.pages && a.new_uses[first + i] == 0.f;
-        n += open[i];
-    }
     uint32_t total, rank = free + block_scan(n, total) - n;
     for (uint32_t i = 0; i < 4; ++i) {
         if (!open[i]) continue;
@@ -368,7 +399,7 @@ __global__ __launch_bounds__(kThreads) void pages_fork_allot(PagesForkArgs a) {
         uint32_t lo = 0, hi = a.batch - 1;
         while (lo < hi) {
             const uint32_t mid = (lo + hi + 1) / 2;
-            if (w.before[mid] <= rank)
+            if ((fits ? needs[mid] : w.before[mid]) <= rank)
                 lo = mid;
             else
                 hi = mid - 1;
@@ -418,7 +449,7 @@ hipError_t pages_copy_f32(hipStream_t stream, const PagesCopyArgs &a) {
 }
 
 LaunchShape pages_fork_shape(uint32_t batch) {
-    return {"pages_fork", {batch, 1, 1}, {kThreads, 1, 1}, uint32_t(3 * sizeof(uint32_t))};
+    return {"pages_fork", {batch, 1, 1}, {kThreads, 1, 1}, uint32_t(4 * sizeof(uint32_t))};
 }
 
 size_t pages_fork_workspace_bytes(uint32_t batch, uint32_t pages) {
