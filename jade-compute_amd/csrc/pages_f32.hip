@@ -149,6 +149,9 @@ __device__ inline bool is_copy(const PagesCopyArgs &a, uint32_t i) {
     return is_whole(a.sources[i], a.pages) && is_whole(a.targets[i], a.pages) && a.copy_rows[i] >= 1.f;
 }
 
+// Float4s, or floats, of each tensor that a thread has on their way at once.
+constexpr uint32_t kCopyWords = 4;
+
 // `blocks` blocks for each copy. One whose target another reads, or an earlier one writes,
 // is not made, so that the order in which blocks run changes nothing.
 template <typename T>
@@ -162,21 +165,30 @@ __global__ __launch_bounds__(kThreads) void pages_copy(PagesCopyArgs a, uint32_t
     if (__syncthreads_or(clash)) return;
     const uint32_t rows = whole_below(a.copy_rows[c], a.page), dim = a.dim * sizeof(float) / sizeof(T);
     // Runs of rows that lie together: all heads of a token, or one head's tokens.
-    const uint32_t run = a.pages_token_major ? rows * a.kv_heads * dim : rows * dim;
-    const uint32_t pitch = a.pages_token_major ? 0 : a.page * dim;
-    const uint64_t all = uint64_t(rows) * a.kv_heads * dim, page = uint64_t(a.page) * a.kv_heads * dim;
-    const size_t from = uint64_t(source) * page, to = uint64_t(target) * page;
-#pragma unroll 2
-    for (uint64_t i = uint64_t(part) * kThreads + threadIdx.x; i < all; i += uint64_t(blocks) * kThreads) {
-        const uint32_t h = uint32_t(i) / run;
-        const size_t at = size_t(h) * pitch + (uint32_t(i) - h * run);
-        move<T>(a.k_pages, a.v_pages, from + at, a.k_pages, a.v_pages, to + at);
+    const uint32_t runs = a.pages_token_major ? 1 : a.kv_heads, run = rows * dim * (a.pages_token_major ? a.kv_heads : 1);
+    const size_t page = size_t(a.page) * a.kv_heads * dim, pitch = size_t(a.page) * dim;
+    const uint32_t pieces = (run + kCopyWords * kThreads - 1) / (kCopyWords * kThreads);
+    for (uint32_t i = part; i < runs * pieces; i += blocks) {
+        const uint32_t h = i / pieces, at = (i - h * pieces) * kCopyWords * kThreads + threadIdx.x;
+        const size_t from = size_t(source) * page + h * pitch + at, to = size_t(target) * page + h * pitch + at;
+        T k[kCopyWords], v[kCopyWords];
+#pragma unroll
+        for (uint32_t x = 0; x < kCopyWords; ++x)
+            if (at + x * kThreads < run) {
+                k[x] = __builtin_nontemporal_load(reinterpret_cast<const T *>(a.k_pages) + from + x * kThreads);
+                v[x] = __builtin_nontemporal_load(reinterpret_cast<const T *>(a.v_pages) + from + x * kThreads);
+            }
+#pragma unroll
+        for (uint32_t x = 0; x < kCopyWords; ++x)
+            if (at + x * kThreads < run) {
+                __builtin_nontemporal_store(k[x], reinterpret_cast<T *>(a.k_pages) + to + x * kThreads);
+                __builtin_nontemporal_store(v[x], reinterpret_cast<T *>(a.v_pages) + to + x * kThreads);
+            }
     }
 }
 
-// Blocks of a copy: two float4s of each tensor a thread where the copies are few, and
-// as many as fill the chip where they are many.
-constexpr uint32_t kCopyBlocks = 8192;
+// Blocks of a copy: as many as there is work for, but no more than fill the chip.
+constexpr uint32_t kCopyBlocks = 16384;
 uint32_t copy_blocks(uint32_t copies, uint32_t page, uint32_t kv_heads, uint32_t dim) {
     const uint64_t words = uint64_t(page) * kv_heads * dim / (dim % 4 ? 1 : 4);
     const uint64_t most = (words + kBlockWords - 1) / kBlockWords, share = (kCopyBlocks + copies - 1) / copies;
