@@ -261,30 +261,42 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2, 2))
     clear_rows(a);
 }
 
-// What the runs left of a (sequence, kv head, row block) cut between them: block x has
-// the unit that the cut before run x is the first of. DP / 4 lanes have a row; ROWS rows of a
-// unit go to a block, each with all of its slots, or (ROWS 1) one, with the slots shared out
-// (a unit of many runs).
-template <int DP, int RB, int TILE, int ROWS, bool VEC>
-__global__ __launch_bounds__(kThreads) void attention_paged_join(PagedArgs a) {
+// How the launch that joins is laid out: blocks x rows, and which unit a block has.
+struct JoinGrid {
+    uint32_t x, y;
+    bool shared, by_unit;
+};
+
+// What the runs left of a (sequence, kv head, row block) cut between them: block x has unit
+// x (BY_UNIT), or the unit that the cut before run x + 1 is the first of. DP / 4 lanes have a
+// row; ROWS rows of a unit go to a block, each with all of its slots, or (ROWS 1) one, with
+// the slots shared out (a unit of many runs).
+template <int DP, int RB, int TILE, int ROWS, bool BY_UNIT, bool VEC>
+__device__ void join_unit(const PagedArgs &a, uint32_t block, uint32_t rows_from) {
     constexpr int LANES = DP / 4, PARTS = kThreads / LANES / ROWS;
     __shared__ __attribute__((aligned(16))) f32x4 sums[PARTS][LANES];
     __shared__ float2 weights[PARTS];
     const int tid = threadIdx.x, lane = tid % LANES, p = ROWS == 1 ? tid / LANES : 0;
-    const uint32_t row = blockIdx.y * ROWS + (ROWS == 1 ? 0 : tid / LANES), d = 4 * lane;
+    const uint32_t row = rows_from * ROWS + (ROWS == 1 ? 0 : tid / LANES), d = 4 * lane;
     const Work<TILE, RB> work(a);
     const uint32_t chunk = (work.total + a.runs - 1) / a.runs;
-    uint32_t b, before;
-    const uint32_t cut = work.start(blockIdx.x + 1, chunk, b, before);
-    if (cut == work.total) return;
+    uint32_t b, before, unit, cut = 0;
+    if (BY_UNIT) {
+        if (!work.find_unit(block, b, unit, before)) return;
+    } else {
+        cut = work.start(block + 1, chunk, b, before);
+        if (cut == work.total) return;
+    }
     const Sequence s = work.at(b);
     const uint32_t tiles = work.tiles(s);
-    if (!tiles) return;  // at a sequence's start
-    const uint32_t unit = (cut - before) / tiles, start = before + unit * tiles;
-    if (start + chunk < cut || start == cut || Work<TILE, RB>::rounds(tiles, chunk)) return;  // not its first cut
+    if (!tiles || Work<TILE, RB>::rounds(tiles, chunk)) return;  // at a sequence's start; whole units
+    if (!BY_UNIT) unit = (cut - before) / tiles;
+    const uint32_t start = before + unit * tiles;
+    if (!BY_UNIT && (start + chunk < cut || start == cut)) return;  // not its first cut
     const uint32_t blocks = work.blocks(s), kv = unit / blocks, rb = unit - kv * blocks;
     const bool mine = row < min(uint32_t(RB), s.count * a.group - rb * RB);
     const uint32_t first = start / chunk, last = (start + tiles - 1) / chunk;
+    if (first == last) return;
     const float2 *ml = reinterpret_cast<const float2 *>(a.partial + 2 * size_t(a.runs) * RB * DP);
     // A unit's first run had it last, the others first.
     auto slot = [&](uint32_t r) { return (2 * size_t(r) + (r == first)) * RB + row; };
@@ -316,12 +328,36 @@ __global__ __launch_bounds__(kThreads) void attention_paged_join(PagedArgs a) {
     o = l == 0.f ? f32x4{0.f, 0.f, 0.f, 0.f} : o * (1.0f / l);  // a row that sees no key is zeros
     store_dims<VEC>(a.out + row_at(a, b, kv, rb * RB + row), int(d), int(a.dim), o);
 }
+template <int DP, int RB, int TILE, bool VEC>
+__device__ void join(const PagedArgs &a, const JoinGrid &g, uint32_t block) {
+    constexpr int kRowsOf = kThreads / (DP / 4);  // rows of a block
+    const uint32_t y = block / g.x, x = block - y * g.x;
+    if (g.shared)
+        join_unit<DP, RB, TILE, 1, true, VEC>(a, x, y);
+    else if (g.by_unit)
+        join_unit<DP, RB, TILE, kRowsOf, true, VEC>(a, x, y);
+    else
+        join_unit<DP, RB, TILE, kRowsOf, false, VEC>(a, x, y);
+}
+// Both launches' units: of the one for few rows, then of the one for many.
+template <int DP, bool VEC>
+__global__ __launch_bounds__(kThreads) void attention_paged_join(PagedArgs few, JoinGrid few_grid, PagedArgs many,
+                                                                 JoinGrid many_grid) {
+    const uint32_t blocks = few_grid.x * few_grid.y;
+    if (blockIdx.x < blocks)
+        join<DP, kRows, kTile, VEC>(few, few_grid, blockIdx.x);
+    else if constexpr (VEC)
+        join<DP, DP == 64 ? 128 : 256, int(kPagedFlashTile), VEC>(many, many_grid, blockIdx.x - blocks);
+}
 
 uint64_t rows_of(const PagedShape &s) { return uint64_t(s.heads / s.kv_heads) * s.queries; }
 
 // Sequences of more rows than this, for each kv head, go to the kernel on bf16 parts
-// (attention_paged_flash.hip), by a launch of its own.
-uint32_t few_rows(const PagedShape &s) { return s.dim <= 64 ? 64 : 96; }
+// (attention_paged_flash.hip), by a launch of its own. Measured, this kernel and that one, 8
+// sequences of at most 4096 keys, 8 kv heads, 32, 48 and 64 rows: dims of 32 32.8, 42.7, 51.7
+// and 42.5, 48.1, 47.7 us; of 64 42.1, 60.1, 71.7 and 48.6, 57.7, 58.0; of 80 56.6, 78.6, 102.7
+// and 78.9, 83.1, 82.9; of 128 80.3, 110.7, 145.0 and 92.3, 96.8, 96.6.
+uint32_t few_rows(const PagedShape &s) { return s.dim <= 32 ? 48 : 32; }
 bool has_many(const PagedShape &s) {
     // Offsets of a sequence's rows in 31 bits.
     return s.dim % 4 == 0 && rows_of(s) > few_rows(s) && uint64_t(s.heads) * s.queries * s.dim < 1u << 29;
@@ -350,38 +386,39 @@ Half many_of(const PagedShape &s) {
 }
 size_t bytes_of(const Half &x) { return 2 * size_t(x.runs) * x.rows * (x.dims + 2) * sizeof(float); }
 
-template <int DP, int RB, int TILE, bool VEC>
-void launch_join(hipStream_t stream, const PagedArgs &a, uint64_t units) {
-    static_assert(DP == kSlotRow<DP>, "slots are of 64 or 128 dims");
-    if (a.runs < 2) return;
-    constexpr uint32_t kRowsOf = kThreads / (DP / 4);  // rows of a block
-    const uint64_t all = uint64_t(a.group) * a.queries;
-    const uint32_t rows = all < RB ? uint32_t(all) : RB;
+JoinGrid join_grid(const PagedShape &s, const Half &x) {
+    if (x.runs < 2) return {1, 0, false, false};  // nothing is cut
+    const uint64_t all = rows_of(s);
+    const uint32_t rows = all < x.rows ? uint32_t(all) : x.rows, rows_of_block = uint32_t(kThreads) / (x.dims / 4);
     // Units of 16 runs or more: their slots are shared out; else whole rows.
-    if (16 * units <= a.runs)
-        hipLaunchKernelGGL((attention_paged_join<DP, RB, TILE, 1, VEC>), dim3(a.runs - 1, rows), dim3(kThreads), 0, stream, a);
-    else
-        hipLaunchKernelGGL((attention_paged_join<DP, RB, TILE, kRowsOf, VEC>),
-                           dim3(a.runs - 1, (rows + kRowsOf - 1) / kRowsOf), dim3(kThreads), 0, stream, a);
+    const bool shared = 16 * x.units <= x.runs, by_unit = x.units < x.runs;
+    return {by_unit ? uint32_t(x.units) : x.runs - 1, shared ? rows : (rows + rows_of_block - 1) / rows_of_block, shared, by_unit};
 }
 
 template <int DP, bool VEC>
-hipError_t launch(hipStream_t stream, const PagedShape &s, PagedArgs a) {
-    const Half few = few_of(s);
-    a.least_rows = 1;
-    a.most_rows = has_many(s) ? few_rows(s) : ~0u;
-    a.runs = few.runs;
-    hipLaunchKernelGGL((attention_paged<DP, VEC>), dim3(a.runs), dim3(kThreads), 0, stream, a);
-    launch_join<DP, kRows, kTile, VEC>(stream, a, few.units);
-    if constexpr (VEC)
-        if (has_many(s)) {
-            const Half many = many_of(s);
-            a.least_rows = a.most_rows + 1;
-            a.most_rows = ~0u;
-            a.runs = many.runs;
-            launch_paged_flash(stream, a);
-            launch_join<DP, DP == 64 ? 128 : 256, int(kPagedFlashTile), true>(stream, a, many.units);
-        }
+hipError_t launch(hipStream_t stream, const PagedShape &s, PagedArgs few, float *workspace) {
+    static_assert(DP == kSlotRow<DP>, "slots are of 64 or 128 dims");
+    const bool both = VEC && has_many(s);
+    const Half half = few_of(s), other = many_of(s);
+    PagedArgs many = few;
+    few.least_rows = 1;
+    few.most_rows = both ? few_rows(s) : ~0u;
+    few.runs = half.runs;
+    few.partial = workspace;
+    const JoinGrid few_grid = join_grid(s, half);
+    JoinGrid many_grid{1, 0, false, false};
+    hipLaunchKernelGGL((attention_paged<DP, VEC>), dim3(few.runs), dim3(kThreads), 0, stream, few);
+    if (both) {
+        many.least_rows = few_rows(s) + 1;
+        many.most_rows = ~0u;
+        many.runs = other.runs;
+        many.partial = workspace + bytes_of(half) / sizeof(float);
+        many_grid = join_grid(s, other);
+        launch_paged_flash(stream, many);
+    }
+    const uint32_t blocks = few_grid.x * few_grid.y + many_grid.x * many_grid.y;
+    if (blocks)
+        hipLaunchKernelGGL((attention_paged_join<DP, VEC>), dim3(blocks), dim3(kThreads), 0, stream, few, few_grid, many, many_grid);
     return hipGetLastError();
 }
 
@@ -406,15 +443,13 @@ LaunchShape attention_paged_shape(const PagedShape &s) {
 }
 
 size_t attention_paged_workspace_bytes(const PagedShape &s) {
-    const size_t few = bytes_of(few_of(s)), many = has_many(s) ? bytes_of(many_of(s)) : 0;
-    return few > many ? few : many;  // the launches follow each other
+    return bytes_of(few_of(s)) + (has_many(s) ? bytes_of(many_of(s)) : 0);
 }
 
 hipError_t attention_paged_f32(hipStream_t stream, const PagedShape &s, const PagedBuffers &x, float *workspace) {
     PagedArgs a{};
     a.q = x.q; a.k = x.k; a.v = x.v; a.tables = x.tables; a.lengths = x.lengths; a.counts = x.counts;
     a.out = x.out;
-    a.partial = workspace;
     const size_t d = s.dim;
     a.q_batch = d * s.heads * s.queries;
     a.q_head = s.token_major ? d : d * s.queries;
@@ -430,8 +465,8 @@ hipError_t attention_paged_f32(hipStream_t stream, const PagedShape &s, const Pa
     uintptr_t bits = 0;
     for (const float *y : {x.q, x.k, x.v, const_cast<const float *>(x.out)}) bits |= reinterpret_cast<uintptr_t>(y);
     if (!workspace || (s.dim % 4 == 0 && bits & 15u)) return hipErrorInvalidValue;  // the runtime's regions are aligned
-    if (s.dim % 4) return s.dim <= 64 ? launch<64, false>(stream, s, a) : launch<128, false>(stream, s, a);
-    return s.dim <= 64 ? launch<64, true>(stream, s, a) : launch<128, true>(stream, s, a);
+    if (s.dim % 4) return s.dim <= 64 ? launch<64, false>(stream, s, a, workspace) : launch<128, false>(stream, s, a, workspace);
+    return s.dim <= 64 ? launch<64, true>(stream, s, a, workspace) : launch<128, true>(stream, s, a, workspace);
 }
 
 }  // namespace hipk

@@ -149,6 +149,33 @@ struct Work {
         }
         return t;
     }
+    // The (kv head, row block)s of all sequences: number n's sequence and its number there, and
+    // the tiles before that sequence; false past the last.
+    __device__ uint32_t units_of(const Sequence &s) const { return tiles(s) ? blocks(s) * a.kv_heads : 0u; }
+    __device__ bool find_unit(uint32_t n, uint32_t &b, uint32_t &unit, uint32_t &before) const {
+        before = 0;
+        uint32_t mine = units_of(near), tiles_up_to = up_to, tiles_mine = own;
+        for (b = 0; b < a.batch; b += 64) {
+            if (b) {
+                const Sequence s = load(b + (threadIdx.x & 63));
+                mine = units_of(s);
+                tiles_mine = all_of(s);
+                tiles_up_to = scan_add(tiles_mine);
+            }
+            const uint32_t sum = scan_add(mine);
+            const uint64_t past = __ballot(sum > n);
+            if (past) {
+                const int first = __builtin_ctzll(past);
+                b += first;
+                unit = n - of_lane(sum - mine, first);
+                before += of_lane(tiles_up_to - tiles_mine, first);
+                return true;
+            }
+            n -= of_lane(sum, 63);
+            before += of_lane(tiles_up_to, 63);
+        }
+        return false;
+    }
     __device__ static bool rounds(uint32_t tiles, uint32_t chunk) { return 4 * tiles <= chunk; }
 };
 
