@@ -145,10 +145,6 @@ hipError_t launch_append(hipStream_t stream, const PagesAppendArgs &a) {
 
 // ---- pages_copy --------------------------------------------------------------------------
 
-__device__ inline bool is_copy(const PagesCopyArgs &a, uint32_t i) {
-    return is_whole(a.sources[i], a.pages) && is_whole(a.targets[i], a.pages) && a.copy_rows[i] >= 1.f;
-}
-
 // Float4s, or floats, of each tensor that a thread has on their way at once.
 constexpr uint32_t kCopyWords = 4;
 
@@ -157,17 +153,14 @@ constexpr uint32_t kCopyWords = 4;
 template <typename T>
 __global__ __launch_bounds__(kThreads) void pages_copy(PagesCopyArgs a, uint32_t blocks) {
     const uint32_t c = blockIdx.x / blocks, part = blockIdx.x - c * blocks;
-    if (!is_copy(a, c)) return;
     const float source = a.sources[c], target = a.targets[c];
-    bool clash = false;
-    for (uint32_t i = threadIdx.x; i < a.copies; i += kThreads)
-        if (a.sources[i] == target || (i < c && a.targets[i] == target)) clash |= is_copy(a, i);
-    if (__syncthreads_or(clash)) return;
+    if (!is_whole(source, a.pages) || !is_whole(target, a.pages) || !(a.copy_rows[c] >= 1.f)) return;
     const uint32_t rows = whole_below(a.copy_rows[c], a.page), dim = a.dim * sizeof(float) / sizeof(T);
     // Runs of rows that lie together: all heads of a token, or one head's tokens.
     const uint32_t runs = a.pages_token_major ? 1 : a.kv_heads, run = rows * dim * (a.pages_token_major ? a.kv_heads : 1);
     const size_t page = size_t(a.page) * a.kv_heads * dim, pitch = size_t(a.page) * dim;
     const uint32_t pieces = (run + kCopyWords * kThreads - 1) / (kCopyWords * kThreads);
+    if (part >= runs * pieces) return;
     for (uint32_t i = part; i < runs * pieces; i += blocks) {
         const uint32_t h = i / pieces, at = (i - h * pieces) * kCopyWords * kThreads + threadIdx.x;
         const size_t from = size_t(source) * page + h * pitch + at, to = size_t(target) * page + h * pitch + at;
@@ -178,6 +171,15 @@ __global__ __launch_bounds__(kThreads) void pages_copy(PagesCopyArgs a, uint32_t
                 k[x] = __builtin_nontemporal_load(reinterpret_cast<const T *>(a.k_pages) + from + x * kThreads);
                 v[x] = __builtin_nontemporal_load(reinterpret_cast<const T *>(a.v_pages) + from + x * kThreads);
             }
+        if (i == part) {  // asked while the first rows are on their way
+            bool clash = false;
+#pragma unroll 4
+            for (uint32_t j = threadIdx.x; j < a.copies; j += kThreads) {
+                const float from = a.sources[j], to = a.targets[j], n = a.copy_rows[j];
+                clash |= ((from == target) | ((j < c) & (to == target))) & is_whole(from, a.pages) & is_whole(to, a.pages) & (n >= 1.f);
+            }
+            if (__syncthreads_or(clash)) return;
+        }
 #pragma unroll
         for (uint32_t x = 0; x < kCopyWords; ++x)
             if (at + x * kThreads < run) {
@@ -191,7 +193,8 @@ __global__ __launch_bounds__(kThreads) void pages_copy(PagesCopyArgs a, uint32_t
 constexpr uint32_t kCopyBlocks = 16384;
 uint32_t copy_blocks(uint32_t copies, uint32_t page, uint32_t kv_heads, uint32_t dim) {
     const uint64_t words = uint64_t(page) * kv_heads * dim / (dim % 4 ? 1 : 4);
-    const uint64_t most = (words + kBlockWords - 1) / kBlockWords, share = (kCopyBlocks + copies - 1) / copies;
+    const uint64_t piece = kCopyWords * kThreads, share = (kCopyBlocks + copies - 1) / copies;
+    const uint64_t most = (words + piece - 1) / piece;
     return uint32_t(most < share ? most : share);
 }
 
