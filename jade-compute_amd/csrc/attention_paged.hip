@@ -26,12 +26,15 @@ namespace {
 
 using namespace paged;
 
-constexpr int kTile = 64, kRows = 16;  // keys of a tile, rows of a block
+constexpr int kTile = 64;  // keys of a tile
 
-// DP: head dim padded (64, 128).
-template <int DP, bool VEC>
-__global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2, 2))) void attention_paged(PagedArgs a) {
-    constexpr int KJ = DP / 16, NJ = DP / 64, RB = kRows;
+// DP: head dim padded (64, 128). G: groups of 16 rows, all of them every wave's.
+template <int DP, int G>
+constexpr int kWavesASimd = DP == 128 && G == 2 ? 1 : 2;  // what the registers hold
+template <int DP, int G, bool VEC>
+__global__ __launch_bounds__(kThreads)
+__attribute__((amdgpu_waves_per_eu(kWavesASimd<DP, G>, kWavesASimd<DP, G>))) void attention_paged(PagedArgs a) {
+    constexpr int KJ = DP / 16, NJ = DP / 64, RB = 16 * G;
     __shared__ __attribute__((aligned(16))) float part[kWaves][RB][DP + 4];
     __shared__ float2 ml[kWaves][RB];
     __shared__ RowPlan plans[RB];
@@ -101,7 +104,7 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2, 2))
     auto load = [&](__amdgpu_buffer_rsrc_t from, uint32_t at) {
         return __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(from, int(at), 0, 0));
     };
-    f32x4 kf[KJ], vf[NJ][4], qf[KJ];
+    f32x4 kf[KJ], vf[NJ][4], qf[G][KJ];
     auto load_k = [&](const Unit &u, uint32_t x, uint32_t page) {
         const auto from = tile_of(a.k, u, x, page);
 #pragma unroll
@@ -115,12 +118,15 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2, 2))
             for (int i = 0; i < 4; ++i) vf[j][i] = load(from, voff[j][i]);
     };
     auto rows_of = [&](const Unit &u) { return min(uint32_t(RB), u.s.count * a.group - u.rb * RB); };
-    // Q^T operand: row m of the block, dims 16 j + 4 g + e.
+    // Q^T operand: row 16 r + m of the block, dims 16 j + 4 g + e.
     auto load_rows = [&](const Unit &u) {
         if (u.begin == u.end) return;
-        const float *row = m < rows_of(u) ? a.q + row_at(a, u.b, u.kv, u.rb * RB + m) : nullptr;
 #pragma unroll
-        for (int j = 0; j < KJ; ++j) qf[j] = load_dims<VEC>(row, 16 * j + 4 * g, a.dim);
+        for (int r = 0; r < G; ++r) {
+            const float *row = 16 * r + m < rows_of(u) ? a.q + row_at(a, u.b, u.kv, u.rb * RB + 16 * r + m) : nullptr;
+#pragma unroll
+            for (int j = 0; j < KJ; ++j) qf[r][j] = load_dims<VEC>(row, 16 * j + 4 * g, a.dim);
+        }
     };
     auto page_at = [&](float entry) { return uniform(page_of(a, entry)); };
     Unit u = unit_at(t, b, before);
@@ -138,17 +144,26 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2, 2))
         const Unit next = unit_at(t, u.b + over, over ? u.before + u.all : u.before);
         const float first = entry_of(next, next.begin), second = entry_of(next, next.begin + 1);
 #pragma unroll
-        for (int j = 0; j < KJ; ++j) qf[j] *= a.qscale;  // log2 units
+        for (int r = 0; r < G; ++r)
+#pragma unroll
+            for (int j = 0; j < KJ; ++j) qf[r][j] *= a.qscale;  // log2 units
 
-        f32x4 acc[NJ][4];
-        float top = -INFINITY, sum = 0.f;
+        f32x4 acc[G][NJ][4];
+        float top[G], sum[G];
 #pragma unroll
-        for (int j = 0; j < NJ; ++j)
+        for (int r = 0; r < G; ++r) {
+            top[r] = -INFINITY;
+            sum[r] = 0.f;
 #pragma unroll
-            for (int e = 0; e < 4; ++e) acc[j][e] = f32x4{0.f, 0.f, 0.f, 0.f};
-        // Tokens of the block's first query and of row m.
+            for (int j = 0; j < NJ; ++j)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) acc[r][j][e] = f32x4{0.f, 0.f, 0.f, 0.f};
+        }
+        // Tokens of the block's first query and of this lane's rows.
         const int old = int(u.s.length) - int(u.s.count), low = old + int(u.rb * RB / a.group);
-        const int mine = old + int((u.rb * RB + m) / a.group);
+        int mine[G];
+#pragma unroll
+        for (int r = 0; r < G; ++r) mine[r] = old + int((u.rb * RB + 16 * r + m) / a.group);
         uint32_t page_next = page;
         if (begin >= u.stop) {  // no tile of this unit's: the next one's
             page_next = page_at(first);
@@ -163,11 +178,14 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2, 2))
 #pragma unroll
                     for (int e = 0; e < 4; ++e)
                         if (16 * j + 4 * g + e >= a.dim) kf[j][e] = 0.f;
-            f32x4 p = {0.f, 0.f, 0.f, 0.f};  // scores, then weights, of keys 16 wave + 4 g + i
+            f32x4 p[G] = {};  // scores, then weights, of keys 16 wave + 4 g + i
 #pragma unroll
             for (int j = 0; j < KJ; ++j)
 #pragma unroll
-                for (int e = 0; e < 4; ++e) p = __builtin_amdgcn_mfma_f32_16x16x4f32(kf[j][e], qf[j][e], p, 0, 0, 0);
+                for (int e = 0; e < 4; ++e)
+#pragma unroll
+                    for (int r = 0; r < G; ++r)
+                        p[r] = __builtin_amdgcn_mfma_f32_16x16x4f32(kf[j][e], qf[r][j][e], p[r], 0, 0, 0);
             page_next = page_at(last ? first : ahead);
             last ? load_k(next, next.begin, page_next) : load_k(u, x + 1, page_next);
             ahead = entry_of(u, x + 2);
@@ -175,25 +193,30 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2, 2))
             if (masked || page == kNoPage) {
                 const int key = int(x) * kTile + 16 * int(wave) + 4 * g;
 #pragma unroll
-                for (int i = 0; i < 4; ++i)
-                    if (key + i > mine || page == kNoPage) p[i] = -INFINITY;
+                for (int r = 0; r < G; ++r)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        if (key + i > mine[r] || page == kNoPage) p[r][i] = -INFINITY;
             }
-            const float most = fmaxf(fmaxf(p.x, p.y), fmaxf(p.z, p.w));
-            if (__any(most > top + kLazyMax)) {
-                const float reached = fmaxf(top, across_keys_max(most));
-                const float keep = reached == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(top - reached);
-                top = reached;
-                sum *= keep;
 #pragma unroll
-                for (int j = 0; j < NJ; ++j)
+            for (int r = 0; r < G; ++r) {
+                const float most = fmaxf(fmaxf(p[r].x, p[r].y), fmaxf(p[r].z, p[r].w));
+                if (__any(most > top[r] + kLazyMax)) {
+                    const float reached = fmaxf(top[r], across_keys_max(most));
+                    const float keep = reached == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(top[r] - reached);
+                    top[r] = reached;
+                    sum[r] *= keep;
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) acc[j][e] *= keep;
-            }
-            const float from = top == -INFINITY ? 0.f : top;
+                    for (int j = 0; j < NJ; ++j)
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                p[i] = __builtin_amdgcn_exp2f(p[i] - from);
-                sum += p[i];
+                        for (int e = 0; e < 4; ++e) acc[r][j][e] *= keep;
+                }
+                const float from = top[r] == -INFINITY ? 0.f : top[r];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    p[r][i] = __builtin_amdgcn_exp2f(p[r][i] - from);
+                    sum[r] += p[r][i];
+                }
             }
             bool odd = false;
             if (masked && u.s.count > 1) {
@@ -211,30 +234,34 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2, 2))
                     for (int j = 0; j < NJ; ++j)
 #pragma unroll
                         for (int e = 0; e < 4; ++e)
-                            acc[j][e] = __builtin_amdgcn_mfma_f32_16x16x4f32(vf[j][i][e], p[i], acc[j][e], 0, 0, 0);
+#pragma unroll
+                            for (int r = 0; r < G; ++r)
+                                acc[r][j][e] = __builtin_amdgcn_mfma_f32_16x16x4f32(vf[j][i][e], p[r][i], acc[r][j][e], 0, 0, 0);
             } else {
                 // A value that is not finite, of a token that not every row may see: the
                 // finite ones, then the weight that each row gives to each special one.
 #pragma unroll
-                for (int j = 0; j < NJ; ++j)
+                for (int r = 0; r < G; ++r)
 #pragma unroll
-                    for (int e = 0; e < 4; ++e)
+                    for (int j = 0; j < NJ; ++j)
 #pragma unroll
-                        for (int k = -1; k < 3; ++k) {
-                            __builtin_amdgcn_sched_barrier(0);  // one at a time: a rare path takes no registers
-                            f32x4 sums = k < 0 ? acc[j][e] : f32x4{0.f, 0.f, 0.f, 0.f};
+                        for (int e = 0; e < 4; ++e)
 #pragma unroll
-                            for (int i = 0; i < 4; ++i) {
-                                const float v = vf[j][i][e], y = k >= 0 ? is(k, v) : finite(v) ? v : 0.f;
-                                sums = __builtin_amdgcn_mfma_f32_16x16x4f32(y, p[i], sums, 0, 0, 0);
+                            for (int k = -1; k < 3; ++k) {
+                                __builtin_amdgcn_sched_barrier(0);  // one at a time: a rare path takes no registers
+                                f32x4 sums = k < 0 ? acc[r][j][e] : f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                                for (int i = 0; i < 4; ++i) {
+                                    const float v = vf[j][i][e], y = k >= 0 ? is(k, v) : finite(v) ? v : 0.f;
+                                    sums = __builtin_amdgcn_mfma_f32_16x16x4f32(y, p[r][i], sums, 0, 0, 0);
+                                }
+                                if (k < 0)
+                                    acc[r][j][e] = sums;
+                                else
+#pragma unroll
+                                    for (int i = 0; i < 4; ++i)
+                                        if (sums[i] > 0.f) acc[r][j][e][i] += special(k);
                             }
-                            if (k < 0)
-                                acc[j][e] = sums;
-                            else
-#pragma unroll
-                                for (int i = 0; i < 4; ++i)
-                                    if (sums[i] > 0.f) acc[j][e][i] += special(k);
-                        }
             }
             last ? load_v(next, next.begin, page_next) : load_v(u, x + 1, page_next);
             page = page_next;
@@ -244,16 +271,19 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2, 2))
         const uint32_t rows = rows_of(u);
         load_rows(next);
 
-        // The four waves' sums joined: row m, dims 64 j + 16 g + 4 i + e.
+        // The four waves' sums joined: row 16 r + m, dims 64 j + 16 g + 4 i + e.
         __syncthreads();
-        const float all = across_keys_sum(sum);
-        if (g == 0) ml[wave][m] = float2{top, all};
 #pragma unroll
-        for (int j = 0; j < NJ; ++j)
+        for (int r = 0; r < G; ++r) {
+            const float all = across_keys_sum(sum[r]);
+            if (g == 0) ml[wave][16 * r + m] = float2{top[r], all};
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
-                *reinterpret_cast<f32x4 *>(&part[wave][m][64 * j + 16 * g + 4 * i]) =
-                    f32x4{acc[j][0][i], acc[j][1][i], acc[j][2][i], acc[j][3][i]};
+            for (int j = 0; j < NJ; ++j)
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    *reinterpret_cast<f32x4 *>(&part[wave][16 * r + m][64 * j + 16 * g + 4 * i]) =
+                        f32x4{acc[r][j][0][i], acc[r][j][1][i], acc[r][j][2][i], acc[r][j][3][i]};
+        }
         __syncthreads();
         finish<DP, RB, VEC>(a, run, u.b, u.kv, u.rb, rows, whole, begin == 0, part, ml, plans, 1.f);
         u = next;
@@ -340,13 +370,13 @@ __device__ void join(const PagedArgs &a, const JoinGrid &g, uint32_t block) {
         join_unit<DP, RB, TILE, kRowsOf, false, VEC>(a, x, y);
 }
 // Both launches' units: of the one for few rows, then of the one for many.
-template <int DP, bool VEC>
+template <int DP, int RB, bool VEC>
 __global__ __launch_bounds__(kThreads) void attention_paged_join(PagedArgs few, JoinGrid few_grid, PagedArgs many,
                                                                  JoinGrid many_grid) {
     const uint32_t blocks = few_grid.x * few_grid.y;
     if (blockIdx.x < blocks)
-        join<DP, kRows, kTile, VEC>(few, few_grid, blockIdx.x);
-    else if constexpr (VEC)
+        join<DP, RB, kTile, VEC>(few, few_grid, blockIdx.x);
+    else if constexpr (VEC && RB == 16)
         join<DP, DP == 64 ? 128 : 256, int(kPagedFlashTile), VEC>(many, many_grid, blockIdx.x - blocks);
 }
 
@@ -377,9 +407,15 @@ Half half_of(const PagedShape &s, uint64_t rows, uint32_t rb, uint32_t tile, uin
     x.runs = x.tiles >= blocks ? blocks : uint32_t((x.tiles + 7) / 8 * 8);
     return x;
 }
+// Two groups of rows a wave, which read K and V once for both, where a kv head has more than
+// one and none goes to the other launch (which leaves sequences of few new tokens to this
+// one). 32 rows, one group and two: 8 sequences of at most 4096 keys, 8 kv heads of 64 42.1
+// and 36.8 us, of 80 56.6 and 61.2, of 128 80.3 and 62.2; one sequence of 8192 23.0 and 20.1,
+// 29.2 and 25.6, 34.0 and 28.3.
+uint32_t groups_of(const PagedShape &s) { return rows_of(s) > 16 && !has_many(s) ? 2 : 1; }
 Half few_of(const PagedShape &s) {
-    const uint64_t rows = rows_of(s);
-    return half_of(s, has_many(s) && rows > few_rows(s) ? few_rows(s) : rows, kRows, kTile, 2 * kCus);
+    const uint32_t groups = groups_of(s);
+    return half_of(s, has_many(s) ? few_rows(s) : rows_of(s), 16 * groups, kTile, groups == 2 && s.dim > 64 ? kCus : 2 * kCus);
 }
 Half many_of(const PagedShape &s) {
     return half_of(s, rows_of(s), paged_flash_rows(s.dim), kPagedFlashTile, s.dim <= 64 ? 2 * kCus : kCus);
@@ -395,10 +431,10 @@ JoinGrid join_grid(const PagedShape &s, const Half &x) {
     return {by_unit ? uint32_t(x.units) : x.runs - 1, shared ? rows : (rows + rows_of_block - 1) / rows_of_block, shared, by_unit};
 }
 
-template <int DP, bool VEC>
+template <int DP, int G, bool VEC>
 hipError_t launch(hipStream_t stream, const PagedShape &s, PagedArgs few, float *workspace) {
     static_assert(DP == kSlotRow<DP>, "slots are of 64 or 128 dims");
-    const bool both = VEC && has_many(s);
+    const bool both = VEC && G == 1 && has_many(s);
     const Half half = few_of(s), other = many_of(s);
     PagedArgs many = few;
     few.least_rows = 1;
@@ -407,7 +443,7 @@ hipError_t launch(hipStream_t stream, const PagedShape &s, PagedArgs few, float 
     few.partial = workspace;
     const JoinGrid few_grid = join_grid(s, half);
     JoinGrid many_grid{1, 0, false, false};
-    hipLaunchKernelGGL((attention_paged<DP, VEC>), dim3(few.runs), dim3(kThreads), 0, stream, few);
+    hipLaunchKernelGGL((attention_paged<DP, G, VEC>), dim3(few.runs), dim3(kThreads), 0, stream, few);
     if (both) {
         many.least_rows = few_rows(s) + 1;
         many.most_rows = ~0u;
@@ -418,13 +454,18 @@ hipError_t launch(hipStream_t stream, const PagedShape &s, PagedArgs few, float 
     }
     const uint32_t blocks = few_grid.x * few_grid.y + many_grid.x * many_grid.y;
     if (blocks)
-        hipLaunchKernelGGL((attention_paged_join<DP, VEC>), dim3(blocks), dim3(kThreads), 0, stream, few, few_grid, many, many_grid);
+        hipLaunchKernelGGL((attention_paged_join<DP, 16 * G, VEC>), dim3(blocks), dim3(kThreads), 0, stream, few, few_grid, many, many_grid);
     return hipGetLastError();
 }
 
-uint32_t paged_lds_bytes(uint32_t dim) {
+template <int DP, bool VEC>
+hipError_t launch_groups(hipStream_t stream, const PagedShape &s, const PagedArgs &a, float *workspace) {
+    return groups_of(s) == 2 ? launch<DP, 2, VEC>(stream, s, a, workspace) : launch<DP, 1, VEC>(stream, s, a, workspace);
+}
+
+uint32_t paged_lds_bytes(uint32_t dim, uint32_t rows) {
     const uint32_t pitch = (dim <= 64 ? 64 : 128) + 4;
-    return uint32_t(kWaves * kRows * (pitch * sizeof(float) + sizeof(float2)) + kRows * sizeof(RowPlan));
+    return uint32_t(kWaves * rows * (pitch * sizeof(float) + sizeof(float2)) + rows * sizeof(RowPlan));
 }
 
 }  // namespace
@@ -438,8 +479,9 @@ LaunchShape attention_paged_shape(const PagedShape &s) {
                                              "attention_paged_flash_d96", "attention_paged_flash_d128"};
         return {names[(s.dim - 1) / 32], {many.runs, 1, 1}, {2 * many.rows, 1, 1}, paged_flash_lds_bytes(s.dim)};
     }
-    return {s.dim <= 64 ? "attention_paged_d64" : "attention_paged_d128", {few.runs, 1, 1}, {kThreads, 1, 1},
-            paged_lds_bytes(s.dim)};
+    static const char *const names[2][2] = {{"attention_paged_d64_r16", "attention_paged_d64_r32"},
+                                            {"attention_paged_d128_r16", "attention_paged_d128_r32"}};
+    return {names[s.dim > 64][groups_of(s) - 1], {few.runs, 1, 1}, {kThreads, 1, 1}, paged_lds_bytes(s.dim, few.rows)};
 }
 
 size_t attention_paged_workspace_bytes(const PagedShape &s) {
@@ -465,8 +507,9 @@ hipError_t attention_paged_f32(hipStream_t stream, const PagedShape &s, const Pa
     uintptr_t bits = 0;
     for (const float *y : {x.q, x.k, x.v, const_cast<const float *>(x.out)}) bits |= reinterpret_cast<uintptr_t>(y);
     if (!workspace || (s.dim % 4 == 0 && bits & 15u)) return hipErrorInvalidValue;  // the runtime's regions are aligned
-    if (s.dim % 4) return s.dim <= 64 ? launch<64, false>(stream, s, a, workspace) : launch<128, false>(stream, s, a, workspace);
-    return s.dim <= 64 ? launch<64, true>(stream, s, a, workspace) : launch<128, true>(stream, s, a, workspace);
+    if (s.dim % 4)
+        return s.dim <= 64 ? launch_groups<64, false>(stream, s, a, workspace) : launch_groups<128, false>(stream, s, a, workspace);
+    return s.dim <= 64 ? launch_groups<64, true>(stream, s, a, workspace) : launch_groups<128, true>(stream, s, a, workspace);
 }
 
 }  // namespace hipk
