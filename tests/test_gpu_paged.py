@@ -210,6 +210,66 @@ def test_attention_paged_large_and_tiny_operands(runtime, queries, dim):
         within(got, want, off + 96 * 2.0 ** -149)
 
 
+@pytest.mark.parametrize("queries,dim", [(1, 64), (6, 128), (10, 64), (40, 64), (40, 128), (9, 37)])
+def test_attention_paged_queries_that_are_not_finite(runtime, queries, dim):
+    # They spoil their own row and no other, whichever rows share their wave.
+    rng = np.random.default_rng(17)
+    spec = paged_spec(2, 8, 2, queries, 16, 8, dim)
+    x = paged_inputs(rng, spec, [128, 100], [queries, queries])
+    clean = x["q"].copy()
+    q = po.rows_by_token(spec, x["q"], 8, queries)
+    bad = [(0, 0, 1, 0, np.nan), (0, queries - 1, 6, dim - 1, np.inf), (1, queries // 2, 3, dim // 2, -np.inf)]
+    for b, i, h, d, value in bad:
+        q[b, i, h, d] = value
+    want, off = po.paged(spec, clean, x["k_pages"], x["v_pages"], x["tables"], x["lengths"], x["counts"])
+    got = po.rows_by_token(spec, run(runtime, spec, x)["out"], 8, queries)
+    spoilt = np.zeros(got.shape[:3], bool)
+    for b, i, h, *_ in bad:
+        spoilt[b, i, h] = True
+    assert np.isnan(got[spoilt]).any(axis=1).all()
+    within(got[~spoilt], want[~spoilt], off[~spoilt])
+
+
+@pytest.mark.parametrize("by_token", [True, False])
+def test_pages_past_32_bits_of_elements(runtime, by_token):
+    # Two pools of 20 GB, which only the kernels write: rows appended to their last pages, copied to the first, read by both
+    # attention kernels. Without a copy on the host the first pages' content is what attention says it is.
+    rng = np.random.default_rng(18)
+    pool = dict(kv_heads=8, pages=300000, page=16, dim=128, pages_token_major=by_token)
+    assert pool["pages"] * 16 * 8 * 128 > 2 ** 32
+    k_pages, v_pages = (runtime.alloc(pool["pages"] * 16 * 8 * 128) for _ in range(2))
+    append = runtime.compile({"op": "pages_append", "batch": 1, "rows": 100, **pool, "table": 7, "token_major": True})
+    copy = runtime.compile({"op": "pages_copy", "copies": 7, **pool})
+    far = np.array([299999, 262144, 262143, 299000, 280001, 299998, 270000], np.float32)
+    near = np.array([0, 5, 1, 9, 2, 7, 3], np.float32)
+    k, v = normal(rng, 1, 100, 8, 128), normal(rng, 1, 100, 8, 128)
+    named = {n: runtime.resident(x) for n, x in dict(k=k, v=v, counts=[100], far=far, near=near, lengths=[0], ends=[100],
+                                                     rows=[16] * 6 + [4]).items()}
+    new_lengths = runtime.alloc(1)
+    runtime.execute([(append, [named["k"], named["v"], named["counts"], named["far"], named["lengths"], k_pages, v_pages, new_lengths]),
+                     (copy, [named["far"], named["near"], named["rows"], k_pages, v_pages])], 1)
+    assert runtime.download(new_lengths) == [100]
+    # The oracle's small pool: the pages in order.
+    small = dict(pool, pages=7, pages_token_major=True)
+    pools = [np.zeros((7, 16, 8, 128), np.float32) for _ in range(2)]
+    for x, y in zip(pools, (k, v)):
+        x.reshape(112, 8, 128)[:100] = y[0]
+    for queries, count in ((1, 1), (40, 40)):
+        spec = {"op": "attention_paged", "batch": 1, "heads": 16, "queries": queries, **pool, "table": 7, "token_major": True}
+        attend = runtime.compile(spec)
+        q = normal(rng, 1, queries, 16, 128)
+        bq, bc, out = runtime.resident(q), runtime.resident([count]), runtime.alloc(q.size)
+        want, off = po.paged(dict(spec, **small), q, *pools, np.arange(7.0)[None], [100], [count])
+        for table in ("far", "near"):
+            runtime.execute([(attend, [bq, k_pages, v_pages, named[table], named["ends"], bc, out])], 1)
+            within(runtime.download(out), want, off)
+        for x in (bq, bc, out):
+            x.free()
+        attend.release()
+    for x in (*named.values(), k_pages, v_pages, new_lengths):
+        x.free()
+
+
 def test_attention_paged_runs_the_same_twice(runtime):
     rng = np.random.default_rng(14)
     for queries in (1, 24, 100):
