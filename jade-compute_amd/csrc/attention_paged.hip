@@ -64,7 +64,7 @@ __attribute__((amdgpu_waves_per_eu(kWavesASimd<DP, G>, kWavesASimd<DP, G>))) voi
         }
 
     // The part of a (sequence, kv head, row block) that tile t of the launch begins in this
-    // run; nothing where the run is over. Tiles from `stop` on are past what its rows see.
+    // run; nothing where the run is over. Tiles from `stop` on show its rows nothing.
     struct Unit {
         uint32_t b, before, kv, rb, begin, end, stop, tiles, all;
         Sequence s;
@@ -74,17 +74,17 @@ __attribute__((amdgpu_waves_per_eu(kWavesASimd<DP, G>, kWavesASimd<DP, G>))) voi
         if (t >= t_stop) return u;
         for (u.b = b, u.before = before;; ++u.b) {  // the run ends with a sequence that has tiles
             u.s = work.at(u.b);
-            u.tiles = work.tiles(u.s);
-            if (u.tiles) break;
+            if (work.active(u.s)) break;
         }
-        const uint32_t blocks = work.blocks(u.s), in = t - u.before, unit = in / u.tiles;
-        u.all = u.tiles * blocks * a.kv_heads;
-        u.begin = in - unit * u.tiles;
-        u.kv = unit / blocks;
-        u.rb = unit - u.kv * blocks;
+        u.all = work.all_at(u.b, u.s);
+        const Spot p = work.spot(u.s, u.all, t - u.before);
+        u.kv = p.kv;
+        u.rb = p.rb;
+        u.begin = p.tile;
+        u.tiles = p.tiles;
         u.end = min(u.tiles, u.begin + (t_stop - t));
         const int last = int(u.s.length) - int(u.s.count) + int(min(u.s.count - 1, (u.rb * RB + RB - 1) / a.group));
-        u.stop = last < 0 ? 0u : min(u.end, uint32_t(last) / kTile + 1);
+        u.stop = last < 0 ? 0u : u.end;
         return u;
     };
     // The table's entry for this wave's keys of tile x, -1 past `stop`.
@@ -318,12 +318,21 @@ __device__ void join_unit(const PagedArgs &a, uint32_t block, uint32_t rows_from
         if (cut == work.total) return;
     }
     const Sequence s = work.at(b);
-    const uint32_t tiles = work.tiles(s);
-    if (!tiles || Work<TILE, RB>::rounds(tiles, chunk)) return;  // at a sequence's start; whole units
-    if (!BY_UNIT) unit = (cut - before) / tiles;
-    const uint32_t start = before + unit * tiles;
-    if (!BY_UNIT && (start + chunk < cut || start == cut)) return;  // not its first cut
-    const uint32_t blocks = work.blocks(s), kv = unit / blocks, rb = unit - kv * blocks;
+    if (!work.active(s) || work.rounds(s, chunk)) return;  // at a sequence's start; whole units
+    Spot at;
+    uint32_t start;
+    if (BY_UNIT) {
+        const uint32_t blocks = work.blocks(s), head = work.all_at(b, s) / a.kv_heads;
+        at.kv = unit / blocks;
+        at.rb = unit - at.kv * blocks;
+        at.tiles = work.tiles(s, at.rb);
+        start = before + at.kv * head + work.tiles_before(s, at.rb);
+    } else {
+        at = work.spot(s, work.all_at(b, s), cut - before);
+        start = cut - at.tile;
+        if (start + chunk < cut || start == cut) return;  // not its first cut
+    }
+    const uint32_t kv = at.kv, rb = at.rb, tiles = at.tiles;
     const bool mine = row < min(uint32_t(RB), s.count * a.group - rb * RB);
     const uint32_t first = start / chunk, last = (start + tiles - 1) / chunk;
     if (first == last) return;

@@ -74,12 +74,16 @@ __device__ inline float across_keys_sum(float x) {
 // Run of block `id`: the runs of one XCD are neighbours.
 __device__ inline uint32_t run_of(uint32_t id, uint32_t runs) { return id % 8 * (runs / 8) + id / 8; }
 
-// A sequence: its tokens, the new ones among them, and what they make of tiles of keys
-// and blocks of rows (for each kv head). Row r of a kv head is head r % group of the group
-// and query r / group, so that a block of rows has neighbouring queries, and sequences of
-// few new tokens have few blocks.
+// A sequence: its tokens, the new ones among them, and what they make of blocks of rows (for
+// each kv head) and tiles of keys (for each block, as many as its last query sees). Row r of
+// a kv head is head r % group of the group and query r / group, so that a block of rows has
+// neighbouring queries, and sequences of few new tokens have few blocks.
 struct Sequence {
     uint32_t length, count;
+};
+// A (kv head, row block) of a sequence, a place among its tiles and how many those are.
+struct Spot {
+    uint32_t kv, rb, tile, tiles;
 };
 template <int TILE, int RB>
 struct Work {
@@ -92,12 +96,61 @@ struct Work {
         if (b >= a.batch) return {0, 0};
         return {whole_below(a.lengths[b], a.table * a.page), whole_below(a.counts[b], a.queries)};
     }
-    __device__ uint32_t tiles(const Sequence &s) const {
+    // Whether there is anything to do, by this launch.
+    __device__ bool active(const Sequence &s) const {
         const uint32_t rows = s.count * a.group;
-        return rows >= a.least_rows && rows <= a.most_rows ? (s.length + TILE - 1) / TILE : 0u;
+        return s.length && rows >= a.least_rows && rows <= a.most_rows;
     }
-    __device__ uint32_t blocks(const Sequence &s) const { return (s.count * a.group + RB - 1) / RB; }
-    __device__ uint32_t all_of(const Sequence &s) const { return tiles(s) * blocks(s) * a.kv_heads; }
+    __device__ uint32_t blocks(const Sequence &s) const { return active(s) ? (s.count * a.group + RB - 1) / RB : 0u; }
+    // Tiles that row block rb sees any key of; one where there is none, for the rows' zeros.
+    __device__ uint32_t tiles(const Sequence &s, uint32_t rb) const {
+        const int seen = int(s.length) - int(s.count) + int(min(s.count, (rb * RB + RB - 1) / a.group + 1));
+        return seen > TILE ? uint32_t(seen + TILE - 1) / TILE : 1u;
+    }
+    __device__ uint32_t tiles_a_head(const Sequence &s) const {
+        const uint32_t n = blocks(s);
+        if (n <= 1) return n ? (s.length + TILE - 1) / TILE : 0u;
+        uint32_t sum = 0;
+        for (uint32_t rb = 0; rb < n; ++rb) sum += tiles(s, rb);
+        return sum;
+    }
+    __device__ uint32_t all_of(const Sequence &s) const { return tiles_a_head(s) * a.kv_heads; }
+    // Place `in` of a sequence's tiles, `all` of them.
+    __device__ Spot spot(const Sequence &s, uint32_t all, uint32_t in) const {
+        const uint32_t head = all / a.kv_heads, n = blocks(s);
+        Spot p;
+        p.kv = in / head;
+        p.rb = 0;
+        p.tile = in - p.kv * head;
+        p.tiles = head;
+        if (n > 1)
+            for (;; p.rb += 64) {
+                const uint32_t rb = p.rb + (threadIdx.x & 63), mine = rb < n ? tiles(s, rb) : 0u, sum = scan_add(mine);
+                const uint64_t past = __ballot(sum > p.tile);
+                if (past) {
+                    const int first = __builtin_ctzll(past);
+                    p.rb += first;
+                    p.tile -= of_lane(sum - mine, first);
+                    p.tiles = of_lane(mine, first);
+                    break;
+                }
+                p.tile -= of_lane(sum, 63);
+            }
+        return p;
+    }
+    // The tiles of one kv head before row block rb.
+    __device__ uint32_t tiles_before(const Sequence &s, uint32_t rb) const {
+        uint32_t sum = 0;
+        for (uint32_t first = 0; first < rb; first += 64) {
+            const uint32_t x = first + (threadIdx.x & 63);
+            sum += of_lane(scan_add(x < rb ? tiles(s, x) : 0u), 63);
+        }
+        return sum;
+    }
+    // All tiles of sequence b, s.
+    __device__ uint32_t all_at(uint32_t b, const Sequence &s) const {
+        return b < 64 ? of_lane(own, int(b)) : uniform(all_of(s));
+    }
     // Of one sequence, for the whole wave.
     __device__ Sequence at(uint32_t b) const {
         return b < 64 ? Sequence{of_lane(near.length, int(b)), of_lane(near.count, int(b))} : anew(b);
@@ -138,11 +191,10 @@ struct Work {
         uint32_t t = uint32_t(at);
         find(t, b, before);
         const Sequence s = this->at(b);
-        const uint32_t n = tiles(s);
-        if (!rounds(n, chunk)) return t;
-        const uint32_t over = (t - before) % n;
-        t = 2 * over < n ? t - over : t - over + n;
-        const uint32_t all = all_of(s);
+        if (!rounds(s, chunk)) return t;
+        const uint32_t all = all_at(b, s);
+        const Spot p = spot(s, all, t - before);
+        t = 2 * p.tile < p.tiles ? t - p.tile : t - p.tile + p.tiles;
         if (t == before + all) {
             before += all;
             ++b;
@@ -151,7 +203,7 @@ struct Work {
     }
     // The (kv head, row block)s of all sequences: number n's sequence and its number there, and
     // the tiles before that sequence; false past the last.
-    __device__ uint32_t units_of(const Sequence &s) const { return tiles(s) ? blocks(s) * a.kv_heads : 0u; }
+    __device__ uint32_t units_of(const Sequence &s) const { return blocks(s) * a.kv_heads; }
     __device__ bool find_unit(uint32_t n, uint32_t &b, uint32_t &unit, uint32_t &before) const {
         before = 0;
         uint32_t mine = units_of(near), tiles_up_to = up_to, tiles_mine = own;
@@ -176,7 +228,9 @@ struct Work {
         }
         return false;
     }
-    __device__ static bool rounds(uint32_t tiles, uint32_t chunk) { return 4 * tiles <= chunk; }
+    // A run has four or more whole blocks of the sequence: by its longest, so that all are cut
+    // alike.
+    __device__ bool rounds(const Sequence &s, uint32_t chunk) const { return 4 * ((s.length + TILE - 1) / TILE) <= chunk; }
 };
 
 // Dims d .. d + 3 of a row, zeros from `dim` on and for no row. VEC: dim % 4 == 0 and

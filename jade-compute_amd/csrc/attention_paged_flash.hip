@@ -10,7 +10,7 @@
 // descriptor of its own, looked up three tiles ahead. What lies past the last token or in no
 // page reads as zeros and is masked. All tiles of all (sequence, kv head, row block)s in a
 // row are cut into equal runs, one a block, so that few long sequences fill the chip, too;
-// rows come by query, so a block's tiles end where its last query does.
+// rows come by query, and a block's tiles end where its last query does.
 //
 // V is scaled before it is split and the sums are scaled back, Q is scaled up and K down, so
 // every finite V and Q is carried exactly. What the parts do not carry is noticed and done
@@ -168,14 +168,14 @@ attention_paged_flash(PagedArgs a) {
     uint32_t at = work.start(run, chunk, b, before);
     while (at < t_stop) {
         const Sequence seq = work.anew(b);
-        const uint32_t tiles = work.tiles(seq);
-        if (!tiles) {
+        if (!work.active(seq)) {
             ++b;
             continue;
         }
-        const uint32_t blocks = work.blocks(seq), in = at - before, unit = in / tiles, begin = in - unit * tiles;
-        const uint32_t kv = unit / blocks, rb = unit - kv * blocks, end = min(tiles, begin + (t_stop - at));
-        const bool whole = begin == 0 && end == tiles;
+        const uint32_t all = uniform(work.all_of(seq));
+        const Spot spot = work.spot(seq, all, at - before);
+        const uint32_t kv = spot.kv, rb = spot.rb, begin = spot.tile, end = min(spot.tiles, begin + (t_stop - at));
+        const bool whole = begin == 0 && end == spot.tiles;
         const uint32_t rows = min(uint32_t(RB), seq.count * a.group - rb * RB);
         // Tokens of the block's last query, of this wave's first and last, and of row c's.
         const int old = int(seq.length) - int(seq.count), newest = int(seq.length) - 1;
@@ -184,7 +184,7 @@ attention_paged_flash(PagedArgs a) {
         const int low = old + int(r0 / a.group), high = min(newest, old + int((r0 + 31) / a.group));
         const int token = old + int((r0 + uint32_t(c)) / a.group);
         const bool some = uint32_t(wave) * 32u < rows;
-        const int t0 = int(begin), t_end = last < 0 ? 0 : int(min(end, uint32_t(last) / kKeys + 1));
+        const int t0 = int(begin), t_end = last < 0 ? 0 : int(end);
 
         // The table's entries for both halves of tile t, -1 past the last; and the keys or
         // values that this wave stages: zeros where they have no page.
@@ -552,8 +552,8 @@ attention_paged_flash(PagedArgs a) {
             }
         }
         at += end - begin;
-        if (at >= before + tiles * blocks * a.kv_heads) {
-            before += tiles * blocks * a.kv_heads;
+        if (at >= before + all) {
+            before += all;
             ++b;
         }
     }
