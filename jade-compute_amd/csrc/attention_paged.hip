@@ -288,7 +288,7 @@ __attribute__((amdgpu_waves_per_eu(kWavesASimd<DP, G>, kWavesASimd<DP, G>))) voi
         finish<DP, RB, VEC>(a, run, u.b, u.kv, u.rb, rows, whole, begin == 0, part, ml, plans, 1.f);
         u = next;
     }
-    clear_rows(a);
+    clear_rows(work);
 }
 
 // How the launch that joins is laid out: blocks x rows, and which unit a block has.

@@ -93,8 +93,9 @@ struct Work {
     uint32_t total;
 
     __device__ Sequence load(uint32_t b) const {
-        if (b >= a.batch) return {0, 0};
-        return {whole_below(a.lengths[b], a.table * a.page), whole_below(a.counts[b], a.queries)};
+        const uint32_t i = min(b, a.batch - 1);  // no branch, so that loads of several are on their way at once
+        const uint32_t length = whole_below(a.lengths[i], a.table * a.page), count = whole_below(a.counts[i], a.queries);
+        return b < a.batch ? Sequence{length, count} : Sequence{0, 0};
     }
     // Whether there is anything to do, by this launch.
     __device__ bool active(const Sequence &s) const {
@@ -162,6 +163,7 @@ struct Work {
     }
     __device__ explicit Work(const PagedArgs &args)
         : a(args), near(load(threadIdx.x & 63)), own(all_of(near)), up_to(scan_add(own)), total(of_lane(up_to, 63)) {
+#pragma unroll 4
         for (uint32_t b0 = 64; b0 < a.batch; b0 += 64) total += of_lane(scan_add(lane_work(b0)), 63);
     }
     // This lane's work among the sequences from b0 on.
@@ -170,7 +172,9 @@ struct Work {
     __device__ void find(uint32_t t, uint32_t &b, uint32_t &before) const {
         before = 0;
         uint32_t sum = up_to, mine = own;
-        for (b = 0;; b += 64, mine = lane_work(b), sum = scan_add(mine)) {
+        Sequence next{0, 0};
+        if (a.batch > 64) next = load(64 + (threadIdx.x & 63));
+        for (b = 0;; b += 64, mine = all_of(next), sum = scan_add(mine), next = load(b + 64 + (threadIdx.x & 63))) {
             const uint64_t past = __ballot(before + sum > t);
             if (past) {
                 const int first = __builtin_ctzll(past);
@@ -286,18 +290,24 @@ __device__ inline uint32_t page_of(const Args &a, float entry) {
     return entry >= 0.f && entry < float(a.pages) && entry == truncf(entry) ? uint32_t(entry) : kNoPage;
 }
 
-// Zeros for the rows that no tile of keys reaches: those of queries past a sequence's
-// count, and all of one without tokens.
-__device__ inline void clear_rows(const PagedArgs &a) {
-    const uint32_t lane = threadIdx.x & 63, heads = a.kv_heads * a.group;
-    const uint64_t all = uint64_t(a.batch) * a.queries, step = uint64_t(a.runs) * kWaves;
-    for (uint64_t i = uint64_t(blockIdx.x) * kWaves + uniform(threadIdx.x >> 6); i < all; i += step) {
-        const uint32_t b = uint32_t(i / a.queries), query = uint32_t(i - uint64_t(b) * a.queries);
-        if (query < whole_below(a.counts[b], a.queries) && a.lengths[b] >= 1.f) continue;
-        float *const out = a.out + size_t(b) * a.q_batch + size_t(query) * a.q_row;
-        for (uint32_t e = lane; e < heads * a.dim; e += 64) {
-            const uint32_t h = e / a.dim;
-            out[h * a.q_head + (e - h * a.dim)] = 0.f;
+// Zeros for the rows that no launch has tiles for: those of queries past a sequence's count,
+// and all of one without tokens. Row by row over the grid's waves.
+template <int TILE, int RB>
+__device__ inline void clear_rows(const Work<TILE, RB> &work) {
+    const PagedArgs &a = work.a;
+    const uint32_t lane = threadIdx.x & 63, wide = a.kv_heads * a.group * a.dim, waves = a.runs * kWaves;
+    for (uint32_t b0 = 0; b0 < a.batch; b0 += 64) {
+        const Sequence s = b0 ? work.load(b0 + lane) : work.near;
+        const uint32_t kept = s.length ? s.count : 0u, rows = b0 + lane < a.batch ? a.queries - kept : 0u;
+        const uint32_t sum = scan_add(rows), all = of_lane(sum, 63);
+        for (uint32_t i = blockIdx.x * kWaves + uniform(threadIdx.x >> 6); i < all; i += waves) {
+            const int at = __builtin_ctzll(__ballot(sum > i));
+            const uint32_t query = of_lane(kept, at) + (i - of_lane(sum - rows, at));
+            float *const out = a.out + size_t(b0 + at) * a.q_batch + size_t(query) * a.q_row;
+            for (uint32_t e = lane; e < wide; e += 64) {
+                const uint32_t h = e / a.dim;
+                out[h * a.q_head + (e - h * a.dim)] = 0.f;
+            }
         }
     }
 }

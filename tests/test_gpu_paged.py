@@ -70,6 +70,7 @@ def test_attention_paged_few_rows(runtime, batch, heads, kv_heads, queries, page
 
 
 @pytest.mark.parametrize("batch,heads,kv_heads,queries,page,table,dim", [
+    (2, 40, 1, 1, 16, 9, 64), (1, 40, 1, 2, 16, 9, 37), (1, 300, 1, 1, 16, 5, 128), (1, 300, 1, 3, 32, 3, 30), (2, 20, 1, 2, 48, 4, 32),
     (1, 2, 2, 17, 16, 4, 64), (2, 8, 2, 8, 16, 10, 128), (1, 6, 3, 40, 48, 4, 80), (2, 4, 1, 33, 32, 9, 96), (1, 1, 1, 200, 16, 15, 32),
     (2, 3, 3, 70, 80, 3, 37), (1, 5, 1, 61, 64, 7, 128), (2, 2, 1, 100, 256, 1, 30), (1, 7, 7, 129, 16, 9, 126), (2, 4, 2, 64, 16, 8, 64)])
 @pytest.mark.parametrize("layout", LAYOUTS)
@@ -85,7 +86,8 @@ def test_attention_paged_chunks(runtime, batch, heads, kv_heads, queries, page, 
 @pytest.mark.parametrize("heads,kv_heads,queries,dim", [(4, 2, 1, 64), (4, 2, 3, 30), (4, 2, 20, 128), (4, 1, 70, 64)])
 def test_attention_paged_odd_lengths_and_counts(runtime, heads, kv_heads, queries, dim, layout):
     # Lengths zero, one, fractions, NaN, past the table; counts zero, NaN, past the queries and past the length. Keys and
-    # values past the lengths, and all of the pages that no table names, are NaN and infinite; rows without a key are zeros.
+    # values past the lengths, and all of the pages that no table names, are NaN and infinite, and so are queries past the
+    # counts; tables go on past the lengths with pages that are others', or with anything. Rows without a key are zeros.
     rng = np.random.default_rng(7)
     lengths = [0.0, 1.0, 16.0, 17.9, np.nan, -4.0, 1e30, 33.0, 5.0, 64.0, 40.0, np.inf]
     counts = [1.0, 1.0, 2.5, 1e9, 1.0, 1.0, 2.0, 0.0, 64.0, np.nan, 3.0, 1.0]
@@ -99,6 +101,11 @@ def test_attention_paged_odd_lengths_and_counts(runtime, heads, kv_heads, querie
     for name, value in (("k_pages", np.nan), ("v_pages", np.inf)):
         po.pool_by_token(spec, x[name])[~seen] = value
         po.pool_by_token(spec, clean[name])[~seen] = 0
+    q = po.rows_by_token(spec, x["q"], heads, queries)
+    for b, (n, c) in enumerate(zip(lengths, counts)):
+        held = -(-po.length_of(n, 80) // 16)
+        x["tables"][b, held:] = rng.choice([0, 3, spec["pages"] - 1, np.nan, -1, 1e9, np.inf, 0.5], 5 - held)
+        q[b, po.length_of(c, queries):] = np.nan
     got, want = check_paged(runtime, spec, x, clean)
     none = want == 0
     assert (got[none] == 0).all()
@@ -509,6 +516,23 @@ def test_beam_select(runtime, batch, beams, vocab, picks):
     rng = np.random.default_rng(vocab + picks)
     check_select(runtime, select_spec(batch, beams, vocab, picks), 3 * normal(rng, batch, beams, vocab),
                  (-10 * rng.random((batch, beams))).astype(np.float32), (rng.random((batch, beams)) < 0.2).astype(np.float32))
+
+
+def test_beam_select_more_chunks_than_a_grid_has_blocks(runtime):
+    rng = np.random.default_rng(54)
+    batch, beams, picks = 65535, 17, 3
+    logits, scores = normal(rng, batch, beams, 2), normal(rng, batch, beams)
+    got = run(runtime, select_spec(batch, beams, 2, picks, 1), {"logits": logits, "scores": scores, "finished": np.zeros((batch, beams))})
+    x = logits.astype(np.float64)
+    every = (x - np.log(np.exp(x).sum(-1, keepdims=True)) + scores[..., None].astype(np.float64)).reshape(batch, -1)
+    order = np.argsort(-every, axis=1, kind="stable")[:, :picks + 1]
+    best = np.take_along_axis(every, order, 1)
+    clear = (best[:, :-1] - best[:, 1:] > 2 * po.score_bound(10)).all(axis=1)
+    assert clear.mean() > 0.99
+    order = order[:, :picks]
+    np.testing.assert_array_equal(got["parents"].reshape(batch, picks)[clear], (order // 2 + np.arange(batch)[:, None] * beams)[clear])
+    np.testing.assert_array_equal(got["tokens"].reshape(batch, picks)[clear], (order % 2)[clear])
+    assert (np.abs(got["new_scores"].reshape(batch, picks) - best[:, :picks]) <= po.score_bound(best[:, :picks])).all()
 
 
 def test_beam_select_first_step_and_finished_beams(runtime):
