@@ -160,8 +160,8 @@ struct PagesForkArgs {
     float *new_tables, *new_lengths, *new_uses, *sources, *targets, *copy_rows, *missing, *workspace;
     uint32_t batch, pages, page, table;
 };
-LaunchShape pages_fork_shape(uint32_t batch);
-size_t pages_fork_workspace_bytes(uint32_t batch, uint32_t pages);
+LaunchShape pages_fork_shape(uint32_t batch, uint32_t pages, uint32_t table);
+size_t pages_fork_workspace_bytes(uint32_t batch, uint32_t pages, uint32_t table);
 hipError_t pages_fork_f32(hipStream_t stream, const PagesForkArgs &args);
 
 // The `picks` best continuations of `beams` beams each.

@@ -51,7 +51,7 @@ hipk::LaunchShape launch_shape(const KernelSpec &s) {
         case Op::AttentionCross: return attention_ragged_shape(ragged_shape(s));
         case Op::AttentionPaged: return attention_paged_shape(paged_shape(s));
         case Op::PagesAppend: return pages_append_shape(s.batch, s.kv_heads, s.rows, s.page, s.dim, s.token_major);
-        case Op::PagesFork: return pages_fork_shape(s.batch);
+        case Op::PagesFork: return pages_fork_shape(s.batch, s.pages, s.table);
         case Op::PagesCopy: return pages_copy_shape(s.copies, s.kv_heads, s.page, s.dim);
         case Op::BeamSelect: return beam_select_shape(s.batch, s.beams, s.vocab);
         case Op::GemmMps: break;
@@ -85,7 +85,7 @@ size_t workspace_bytes_of(const KernelSpec &spec) {
     if (spec.op == Op::AttentionTree || spec.op == Op::AttentionCross)
         return hipk::attention_ragged_workspace_bytes(ragged_shape(spec));
     if (spec.op == Op::AttentionPaged) return hipk::attention_paged_workspace_bytes(paged_shape(spec));
-    if (spec.op == Op::PagesFork) return hipk::pages_fork_workspace_bytes(spec.batch, spec.pages);
+    if (spec.op == Op::PagesFork) return hipk::pages_fork_workspace_bytes(spec.batch, spec.pages, spec.table);
     if (spec.op == Op::BeamSelect)
         return hipk::beam_select_workspace_bytes(spec.batch, spec.beams, spec.vocab, spec.picks);
     return 0;
@@ -248,7 +248,7 @@ Pipeline *PipelineCache::obtain(const KernelSpec &spec) {
                        text_of("%s needs %zu bytes of device workspace: %s", spec_name(spec), p->workspace_bytes,
                                hipGetErrorString(status)));
             }
-            if (spec.op == Op::PagesFork) {  // its sums start, and every call leaves them, at zero
+            if (spec.op == Op::PagesFork && p->workspace) {  // its sums start, and every call leaves them, at zero
                 dev::expect(hipMemsetAsync(p->workspace, 0, p->workspace_bytes, session_.queue()),
                             "clearing the workspace");
                 session_.drain();

@@ -443,7 +443,8 @@ def fork_state(rng, batch, page, table, pages, spare_pages=True):
 
 
 @pytest.mark.parametrize("batch,page,table,pages", [(1, 16, 1, 1), (4, 16, 8, 40), (16, 48, 5, 60), (7, 16, 30, 150), (300, 16, 9, 3000),
-                                                    (33, 1024, 3, 80), (5, 16, 300, 5000), (64, 32, 40, 1500)])
+                                                    (33, 1024, 3, 80), (5, 16, 300, 5000), (64, 32, 40, 1500),
+                                                    (64, 16, 64, 8192), (64, 16, 65, 3000), (65, 16, 5, 300), (5, 16, 8, 8193), (3, 48, 2000, 5000)])
 @pytest.mark.parametrize("reserve", [0, 1, 40])
 def test_pages_fork(runtime, batch, page, table, pages, reserve):
     rng = np.random.default_rng(batch + pages + reserve)
@@ -453,26 +454,30 @@ def test_pages_fork(runtime, batch, page, table, pages, reserve):
                    {**state, "parents": rng.integers(-1, batch, batch), "reserve": np.full(batch, reserve)}, repeats=2)
 
 
-def test_pages_fork_odd_parents_lengths_tables_and_pinned_pages(runtime):
+@pytest.mark.parametrize("pages,kernel", [(64, "pages_fork_small"), (9000, "pages_fork")])
+def test_pages_fork_odd_parents_lengths_tables_and_pinned_pages(runtime, pages, kernel):
     rng = np.random.default_rng(41)
-    spec = {"op": "pages_fork", "batch": 8, "pages": 64, "page": 16, "table": 6}
-    state = fork_state(rng, 8, 16, 6, 64)
+    spec = {"op": "pages_fork", "batch": 8, "pages": pages, "page": 16, "table": 6}
+    assert runtime.compile(spec).launch["kernel"] == kernel
+    state = fork_state(rng, 8, 16, 6, pages)
     state["lengths"] = state["lengths"].astype(np.float32)
-    state["uses"][:] += rng.integers(0, 2, 64)  # held by others too
+    state["uses"][:] += rng.integers(0, 2, pages)  # held by others too
     state["uses"][5] = np.nan
     for parents in ([0, 0, 0, 0, 0, 0, 0, 0], [-1, 8, np.nan, 0.5, np.inf, -0.0, 7, 1e9], [7, 6, 5, 4, 3, 2, 1, 0], [-1] * 8):
         check_fork(runtime, spec, {**state, "parents": np.array(parents, np.float32), "reserve": np.ones(8)})
     state["lengths"][:4] = [np.nan, 1e9, -1.0, 33.7]
-    state["tables"][1, 1], state["tables"][2, 0], state["tables"][4, 2] = np.nan, 64, 1.5  # the pages after them are not held
+    state["tables"][1, 1], state["tables"][2, 0], state["tables"][4, 2] = np.nan, pages, 1.5  # the pages after them are not held
     check_fork(runtime, spec, {**state, "parents": np.array([0, 1, 1, 2, 4, 4, 3, 3], np.float32),
                                "reserve": np.array([0, 1, np.nan, 1e9, 16, 17, -3, 2.5], np.float32)})
 
 
-def test_pages_fork_without_free_pages(runtime):
+@pytest.mark.parametrize("pages", [4, 9000])
+def test_pages_fork_without_free_pages(runtime, pages):
     # Three children of a sequence with a partial page, and one page to spare: the second child gets it, the third is cut
     # to its whole pages.
-    spec = {"op": "pages_fork", "batch": 3, "pages": 4, "page": 16, "table": 4}
-    want = check_fork(runtime, spec, {"parents": [0, 0, 0], "lengths": [40, 0, 0], "reserve": [1, 1, 1], "uses": [1, 1, 1, 0],
+    spec = {"op": "pages_fork", "batch": 3, "pages": pages, "page": 16, "table": 4}
+    want = check_fork(runtime, spec, {"parents": [0, 0, 0], "lengths": [40, 0, 0], "reserve": [1, 1, 1],
+                                      "uses": [1, 1, 1, 0] + [1] * (pages - 4),
                                       "tables": [[2, 0, 1, -1], [-1] * 4, [-1] * 4]})
     assert want["new_lengths"].tolist() == [40, 40, 32] and want["missing"].tolist() == [0, 0, 1]
     assert want["targets"].tolist() == [-1, 3, -1] and want["sources"].tolist() == [-1, 1, -1]
