@@ -163,7 +163,6 @@ struct Work {
     }
     __device__ explicit Work(const PagedArgs &args)
         : a(args), near(load(threadIdx.x & 63)), own(all_of(near)), up_to(scan_add(own)), total(of_lane(up_to, 63)) {
-#pragma unroll 4
         for (uint32_t b0 = 64; b0 < a.batch; b0 += 64) total += of_lane(scan_add(lane_work(b0)), 63);
     }
     // This lane's work among the sequences from b0 on.

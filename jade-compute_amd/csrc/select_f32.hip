@@ -12,6 +12,11 @@
 // then scores in 64 bits, ranked likewise. Values that all but tie with their bound (equal
 // logits) do not fit the list in LDS: then the best are found one after the other.
 //
+// 64 searches of 8 beams over 131071 tokens, 16 picks: 62 us for the chunks, 4.3 TB/s,
+// bound by vector instructions (24 a logit, 72% of the SIMDs' cycles; chunks of 4096 logits
+// took 73, a chunk loaded ahead 94, 6 waves a SIMD in fewer registers 76), and 10.5 for the
+// join. One search of 4 beams over 32000: 5 and 6 us.
+//
 // Beams are compared with one another by their sums of exponentials, so those are summed
 // in 64 bits, of terms that are off by one rounding each (their argument's own rounding
 // is carried along).
