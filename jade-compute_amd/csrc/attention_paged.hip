@@ -35,14 +35,14 @@ using namespace paged;
 
 constexpr int kTile = 64;  // keys of a tile
 
-// DP: head dim padded (64, 128). G: groups of 16 rows, all of them every wave's.
+// DP: head dim padded (64, 96, 128). G: groups of 16 rows, all of them every wave's.
 template <int DP, int G>
-constexpr int kWavesASimd = DP == 128 && G == 2 ? 1 : 2;  // what the registers hold
+constexpr int kWavesASimd = DP > 64 && G == 2 ? 1 : 2;  // what the registers hold
 template <int DP, int G, bool VEC>
 __global__ __launch_bounds__(kThreads)
 __attribute__((amdgpu_waves_per_eu(kWavesASimd<DP, G>, kWavesASimd<DP, G>))) void attention_paged(PagedArgs a) {
-    constexpr int KJ = DP / 16, NJ = DP / 64, RB = 16 * G;
-    __shared__ __attribute__((aligned(16))) float part[kWaves][RB][DP + 4];
+    constexpr int KJ = DP / 16, NJ = (DP + 63) / 64, RB = 16 * G, OUT = 64 * NJ;
+    __shared__ __attribute__((aligned(16))) float part[kWaves][RB][OUT + 4];
     __shared__ float2 ml[kWaves][RB];
     __shared__ RowPlan plans[RB];
     const int tid = threadIdx.x, lane = tid & 63;
@@ -292,7 +292,7 @@ __attribute__((amdgpu_waves_per_eu(kWavesASimd<DP, G>, kWavesASimd<DP, G>))) voi
                         f32x4{acc[r][j][0][i], acc[r][j][1][i], acc[r][j][2][i], acc[r][j][3][i]};
         }
         __syncthreads();
-        finish<DP, RB, VEC>(a, run, u.b, u.kv, u.rb, rows, whole, begin == 0, part, ml, plans, 1.f);
+        finish<OUT, RB, VEC>(a, run, u.b, u.kv, u.rb, rows, whole, begin == 0, part, ml, plans, 1.f);
         u = next;
     }
     clear_rows(work);
@@ -427,8 +427,8 @@ Half half_of(const PagedShape &s, uint64_t rows, uint32_t rb, uint32_t tile, uin
 // Two groups of rows a wave, which read K and V once for both, where a kv head has more than
 // one and none goes to the other launch (which leaves sequences of few new tokens to this
 // one). 32 rows, one group and two: 8 sequences of at most 4096 keys, 8 kv heads of 64 42.1
-// and 36.8 us, of 80 56.6 and 61.2, of 128 80.3 and 62.2; one sequence of 8192 23.0 and 20.1,
-// 29.2 and 25.6, 34.0 and 28.3.
+// and 36.8 us, of 80 56.6 and 61.2 (57 since), of 128 80.3 and 62.2; one sequence of 8192 23.0
+// and 20.1, 29.2 and 25.6, 34.0 and 28.3.
 uint32_t groups_of(const PagedShape &s) { return rows_of(s) > 16 && !has_many(s) ? 2 : 1; }
 Half few_of(const PagedShape &s) {
     const uint32_t groups = groups_of(s);
@@ -459,7 +459,12 @@ hipError_t launch(hipStream_t stream, const PagedShape &s, PagedArgs few, float 
     few.partial = workspace;
     const JoinGrid few_grid = join_grid(s, half);
     JoinGrid many_grid{1, 0, false, false};
-    hipLaunchKernelGGL((attention_paged<DP, G, VEC>), dim3(few.runs), dim3(kThreads), 0, stream, few);
+    // Scores of 96 dims rather than 128: 32 rows over 8 sequences of at most 4096 keys, 8 kv
+    // heads of 80, 56.8 -> 51.7 us; 16 x 24 heads, one row, at most 1531 keys 65.6 -> 63.4.
+    if (DP == 128 && s.dim <= 96)
+        hipLaunchKernelGGL((attention_paged<96, G, VEC>), dim3(few.runs), dim3(kThreads), 0, stream, few);
+    else
+        hipLaunchKernelGGL((attention_paged<DP, G, VEC>), dim3(few.runs), dim3(kThreads), 0, stream, few);
     if (both) {
         many.least_rows = few_rows(s) + 1;
         many.most_rows = ~0u;
@@ -494,9 +499,10 @@ LaunchShape attention_paged_shape(const PagedShape &s) {
                                              "attention_paged_flash_d96", "attention_paged_flash_d128"};
         return {names[(s.dim - 1) / 32], {many.runs, 1, 1}, {2 * many.rows, 1, 1}, paged_flash_lds_bytes(s.dim)};
     }
-    static const char *const names[2][2] = {{"attention_paged_d64_r16", "attention_paged_d64_r32"},
+    static const char *const names[3][2] = {{"attention_paged_d64_r16", "attention_paged_d64_r32"},
+                                            {"attention_paged_d96_r16", "attention_paged_d96_r32"},
                                             {"attention_paged_d128_r16", "attention_paged_d128_r32"}};
-    return {names[s.dim > 64][groups_of(s) - 1], {few.runs, 1, 1}, {kThreads, 1, 1}, paged_lds_bytes(s.dim, few.rows)};
+    return {names[s.dim <= 64 ? 0 : s.dim <= 96 ? 1 : 2][groups_of(s) - 1], {few.runs, 1, 1}, {kThreads, 1, 1}, paged_lds_bytes(s.dim, few.rows)};
 }
 
 size_t attention_paged_workspace_bytes(const PagedShape &s) {

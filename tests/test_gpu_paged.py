@@ -71,6 +71,7 @@ def test_attention_paged_few_rows(runtime, batch, heads, kv_heads, queries, page
 
 @pytest.mark.parametrize("batch,heads,kv_heads,queries,page,table,dim", [
     (2, 40, 1, 1, 16, 9, 64), (1, 40, 1, 2, 16, 9, 37), (1, 300, 1, 1, 16, 5, 128), (1, 300, 1, 3, 32, 3, 30), (2, 20, 1, 2, 48, 4, 32),
+    (2, 20, 1, 1, 16, 9, 80), (1, 12, 1, 2, 16, 20, 96), (1, 20, 1, 1, 32, 5, 90), (2, 3, 1, 9, 16, 9, 67),
     (1, 2, 2, 17, 16, 4, 64), (2, 8, 2, 8, 16, 10, 128), (1, 6, 3, 40, 48, 4, 80), (2, 4, 1, 33, 32, 9, 96), (1, 1, 1, 200, 16, 15, 32),
     (2, 3, 3, 70, 80, 3, 37), (1, 5, 1, 61, 64, 7, 128), (2, 2, 1, 100, 256, 1, 30), (1, 7, 7, 129, 16, 9, 126), (2, 4, 2, 64, 16, 8, 64)])
 @pytest.mark.parametrize("layout", LAYOUTS)
