@@ -437,6 +437,18 @@ Half few_of(const PagedShape &s) {
 Half many_of(const PagedShape &s) {
     return half_of(s, rows_of(s), paged_flash_rows(s.dim), kPagedFlashTile, s.dim <= 64 ? 2 * kCus : kCus);
 }
+// Short caches: whole (sequence, kv head, row block)s to every run, and no launch that joins.
+// Where none is longer than two tiles, or there are as many as runs and none is longer than
+// four (eight on parts). Cut and joined, and whole: 8 heads of 64, one query, at most 64 keys
+// 8.3 and 6.4 us, 128 9.2 and 7.3; 64 x 8 kv heads of 128, at most 128 17.8 and 15.8, 256 28.0 and
+// 25.4; but 16 x 8, 256 keys 14.9 and 18.2; on parts 8 units of four tiles 13.7 and 15.5.
+bool uncut(const PagedShape &s) {
+    auto whole = [&](const Half &x, uint32_t most) {
+        return x.tiles <= 2 * x.units || (x.units >= x.runs && x.tiles <= most * x.units);
+    };
+    return whole(few_of(s), 4) && (!has_many(s) || whole(many_of(s), 8));
+}
+
 size_t bytes_of(const Half &x) { return 2 * size_t(x.runs) * x.rows * (x.dims + 2) * sizeof(float); }
 
 JoinGrid join_grid(const PagedShape &s, const Half &x) {
@@ -456,6 +468,7 @@ hipError_t launch(hipStream_t stream, const PagedShape &s, PagedArgs few, float 
     few.least_rows = 1;
     few.most_rows = both ? few_rows(s) : ~0u;
     few.runs = half.runs;
+    few.uncut = many.uncut = uncut(s);
     few.partial = workspace;
     const JoinGrid few_grid = join_grid(s, half);
     JoinGrid many_grid{1, 0, false, false};
@@ -469,11 +482,12 @@ hipError_t launch(hipStream_t stream, const PagedShape &s, PagedArgs few, float 
         many.least_rows = few_rows(s) + 1;
         many.most_rows = ~0u;
         many.runs = other.runs;
-        many.partial = workspace + bytes_of(half) / sizeof(float);
+        if (workspace) many.partial = workspace + bytes_of(half) / sizeof(float);
         many_grid = join_grid(s, other);
         launch_paged_flash(stream, many);
     }
-    hipLaunchKernelGGL((attention_paged_join<DP, 16 * G, VEC>), dim3(few_grid.x * few_grid.y + many_grid.x * many_grid.y),
+    if (!few.uncut)
+        hipLaunchKernelGGL((attention_paged_join<DP, 16 * G, VEC>), dim3(few_grid.x * few_grid.y + many_grid.x * many_grid.y),
                        dim3(kThreads), 0, stream, few, few_grid, many, many_grid);
     return hipGetLastError();
 }
@@ -506,7 +520,7 @@ LaunchShape attention_paged_shape(const PagedShape &s) {
 }
 
 size_t attention_paged_workspace_bytes(const PagedShape &s) {
-    return bytes_of(few_of(s)) + (has_many(s) ? bytes_of(many_of(s)) : 0);
+    return uncut(s) ? 0 : bytes_of(few_of(s)) + (has_many(s) ? bytes_of(many_of(s)) : 0);
 }
 
 hipError_t attention_paged_f32(hipStream_t stream, const PagedShape &s, const PagedBuffers &x, float *workspace) {
@@ -527,7 +541,7 @@ hipError_t attention_paged_f32(hipStream_t stream, const PagedShape &s, const Pa
     a.qscale = (1.0f / sqrtf(float(s.dim))) * kLog2e;
     uintptr_t bits = 0;
     for (const float *y : {x.q, x.k, x.v, const_cast<const float *>(x.out)}) bits |= reinterpret_cast<uintptr_t>(y);
-    if (!workspace || (s.dim % 4 == 0 && bits & 15u)) return hipErrorInvalidValue;  // the runtime's regions are aligned
+    if ((!workspace && !uncut(s)) || (s.dim % 4 == 0 && bits & 15u)) return hipErrorInvalidValue;  // the runtime's regions are aligned
     if (s.dim % 4)
         return s.dim <= 64 ? launch_groups<64, false>(stream, s, a, workspace) : launch_groups<128, false>(stream, s, a, workspace);
     return s.dim <= 64 ? launch_groups<64, true>(stream, s, a, workspace) : launch_groups<128, true>(stream, s, a, workspace);

@@ -154,13 +154,13 @@ def test_attention_paged_long_contexts_are_cut_and_joined(runtime, queries, dim,
     check_paged(runtime, spec, paged_inputs(rng, spec, [3840, 1777], [queries, 1]))
 
 
-@pytest.mark.parametrize("queries", [1, 12, 24, 64])
-def test_attention_paged_many_sequences_most_of_them_idle(runtime, queries):
+@pytest.mark.parametrize("queries,batch,table", [(1, 333, 4), (12, 333, 4), (24, 333, 4), (64, 333, 4), (1, 100, 13), (5, 70, 40), (24, 150, 9),
+                                                 (64, 90, 21)])
+def test_attention_paged_many_sequences_most_of_them_idle(runtime, queries, batch, table):
     # More than a wave's lanes of sequences, most of them without tokens or without new ones.
     rng = np.random.default_rng(11)
-    batch = 333
-    spec = paged_spec(batch, 4, 2, queries, 16, 4, 32)
-    lengths = [int(rng.integers(1, 65)) if b % 3 == 0 else 0 for b in range(batch)]
+    spec = paged_spec(batch, 4, 2, queries, 16, table, 32)
+    lengths = [int(rng.integers(1, 16 * table + 1)) if b % 3 == 0 else 0 for b in range(batch)]
     counts = [0 if b % 5 == 0 else min(max(n, 1), int(rng.integers(1, queries + 1))) for b, n in enumerate(lengths)]
     check_paged(runtime, spec, paged_inputs(rng, spec, lengths, counts))
 
