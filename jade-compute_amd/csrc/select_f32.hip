@@ -6,16 +6,19 @@
 //
 // One pass over the logits. A block takes a chunk of one beam's into registers, and from
 // there its maximum, its sum of exponentials and its best tokens, by value and token as
-// one 64-bit key: the picks-th largest of a wave's lane maxima is a lower bound of what can
-// be among the best, the few values from there on go to LDS and are ranked by counting
-// those above each. A second launch joins the chunks of a search in the same way: sums,
-// then scores in 64 bits, ranked likewise. Values that all but tie with their bound (equal
-// logits) do not fit the list in LDS: then the best are found one after the other.
+// one 64-bit key: from the least of the four waves' own bounds on every wave has a quarter
+// of the picks, so nothing below it is among the best; the few values from there on go to
+// LDS and are ranked by counting those above each. A second launch joins the chunks of a
+// search in the same way: sums, then the sorted lists' first scores in 64 bits, then the
+// entries of those lists whose first one counts. Values that all but tie with their bound
+// (equal logits) do not fit the list in LDS: then the best are found one after the other.
 //
-// 64 searches of 8 beams over 131071 tokens, 16 picks: 62 us for the chunks, 4.3 TB/s,
-// bound by vector instructions (24 a logit, 72% of the SIMDs' cycles; chunks of 4096 logits
-// took 73, a chunk loaded ahead 94, 6 waves a SIMD in fewer registers 76), and 10.5 for the
-// join. One search of 4 beams over 32000: 5 and 6 us.
+// 64 searches of 8 beams over 131071 tokens, 16 picks: 55 us for the chunks, 4.8 TB/s,
+// bound by vector instructions (chunks of 4096 logits took 73, a chunk loaded ahead 94, 6
+// waves a SIMD in fewer registers 76; the greatest bound of a wave that has all of the picks,
+// which lets more values through, 62), and 9 for the join. One search of 4 beams over
+// 32000: 5 and 6 us; 64 such of 64 picks: 14 and 16 (152 together with one wave's bound and
+// every entry looked at); 3 of 16 beams over 50257, 32 picks: 8 and 11 (56).
 //
 // Beams are compared with one another by their sums of exponentials, so those are summed
 // in 64 bits, of terms that are off by one rounding each (their argument's own rounding
@@ -151,7 +154,10 @@ __global__ __launch_bounds__(kThreads) void beam_chunks(BeamSelectArgs a, uint32
             best[i] = fmaxf(fmaxf(x[i][0], x[i][1]), fmaxf(x[i][2], x[i][3]));
             most = fmaxf(most, best[i]);
         }
-        const uint32_t bound = nth_bound(ordered(most + 0.f), list < 64 ? list : 64);
+        // Every wave has its share of the list from the least of the waves' bounds on; of a
+        // row's short end, where waves have nothing, a wave that has all of it counts.
+        const bool shared = a.vocab - first >= 4 * kThreads;
+        const uint32_t bound = nth_bound(ordered(most + 0.f), shared ? (list + kWaves - 1) / kWaves : list);
         float top = wave_max(most);
         if (lane == 0) {
             tops[wave] = top;
@@ -160,7 +166,9 @@ __global__ __launch_bounds__(kThreads) void beam_chunks(BeamSelectArgs a, uint32
         if (tid == 0) count = 0;
         __syncthreads();
         top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
-        const float from = value_of(max(max(max(bounds[0], bounds[1]), max(bounds[2], bounds[3])), kNone + 1));
+        const uint32_t least = shared ? min(min(bounds[0], bounds[1]), min(bounds[2], bounds[3]))
+                                      : max(max(bounds[0], bounds[1]), max(bounds[2], bounds[3]));
+        const float from = value_of(max(least, kNone + 1));
         double sum = 0;
         if (fabsf(top) < INFINITY) {
 #pragma unroll
@@ -240,28 +248,27 @@ __device__ inline bool above(uint64_t key, uint32_t number, uint64_t other, uint
     return key > other || (key == other && number < others);
 }
 
-constexpr uint32_t kNear = 8;  // candidates that a thread keeps in registers
-
-__global__ __launch_bounds__(kThreads) void beam_join(BeamSelectArgs a, uint32_t chunks, uint32_t items) {
+// One block for each search. The chunks' lists are sorted, so a bound of the picks-th largest
+// of their first scores bounds what can be among the best, and only lists whose first reaches
+// it are looked at further.
+template <int THREADS>
+__global__ __launch_bounds__(THREADS) void beam_join(BeamSelectArgs a, uint32_t chunks, uint32_t items) {
+    constexpr int WAVES = THREADS / 64;
+    constexpr uint32_t kLists = 512;  // that are looked at further, at once
+    constexpr uint32_t kFew = 256;    // entries that are ranked without another bound
     __shared__ float tops[kMaxBeams], scores[kMaxBeams], ended[kMaxBeams];
     __shared__ double logs[kMaxBeams];
-    __shared__ uint32_t bounds[kWaves], count;
+    __shared__ uint64_t counts[2][WAVES];
+    __shared__ uint32_t bounds[WAVES], chosen[kLists], count, list_count;
     __shared__ Ranked ranked[kListed];
     const uint32_t tid = threadIdx.x, lane = tid & 63, wave = tid / 64, list = min(a.picks, a.vocab);
-    const uint32_t b = blockIdx.x, first = b * a.beams;
+    const uint32_t b = blockIdx.x, first = b * a.beams, lists = a.beams * chunks;
+    const uint32_t spread = lane * WAVES + wave;  // neighbours, often of one beam, go to different waves
     const Space w = space_of(a.workspace, items, list);
-    const uint32_t per_beam = chunks * list, all = a.beams * per_beam;
-    // The first candidates are on their way while the beams' sums are joined.
-    const size_t from_first = size_t(first) * per_beam;
-    float near_x[kNear];
-    uint32_t near_token[kNear];
-#pragma unroll
-    for (uint32_t i = 0; i < kNear; ++i) {
-        const uint32_t c = tid + i * kThreads;
-        near_x[i] = c < all ? w.value[from_first + c] : 0.f;
-        near_token[i] = c < all ? w.token[from_first + c] : 0u;
-    }
-    for (uint32_t beam = wave; beam < a.beams; beam += kWaves) {
+    const size_t from_first = size_t(first) * chunks;
+    // The first lists' first logits are on their way while the beams' sums are joined.
+    const float near = spread < lists ? w.value[(from_first + spread) * list] : 0.f;
+    for (uint32_t beam = wave; beam < a.beams; beam += WAVES) {
         const size_t at = size_t(first + beam) * chunks;
         const float score = a.scores[first + beam], end = a.finished[first + beam];
         // The first 64 chunks' maxima and sums together; of a beam that does not go on they
@@ -285,66 +292,94 @@ __global__ __launch_bounds__(kThreads) void beam_join(BeamSelectArgs a, uint32_t
             ended[beam] = end;
         }
     }
-    if (tid == 0) count = 0;
+    if (tid == 0) count = list_count = 0;
     __syncthreads();
-    // Candidate c of the search, of a logit and token as its chunk left them; a finished beam
-    // has one, in the place of its first.
-    auto rate = [&](uint32_t c, float x, uint32_t token, uint64_t &key, uint32_t &number) __attribute__((always_inline)) {
-        const uint32_t beam = c / per_beam;
+    // The score of entry e, a logit x, of list l; a finished beam has one, in the place of its
+    // first.
+    auto rate = [&](uint32_t l, uint32_t e, float x) __attribute__((always_inline)) {
+        const uint32_t beam = l / chunks;
         const double score = double(scores[beam]);
-        key = kNone64;
-        number = 0;
-        if (!(score > -INFINITY)) return;
-        if (ended[beam] > 0.f) {
-            if (c == beam * per_beam && a.end < a.vocab) {
-                key = ordered(score + 0.0);
-                number = beam * a.vocab + a.end;
-            }
-            return;
-        }
+        if (!(score > -INFINITY)) return kNone64;
+        if (ended[beam] > 0.f) return l == beam * chunks && e == 0 && a.end < a.vocab ? ordered(score + 0.0) : kNone64;
         // Infinite logits share what there is.
         const double below = x == tops[beam] ? 0.0 : double(x) - double(tops[beam]);
-        if (!(x > -INFINITY) || !(below > -INFINITY)) return;
-        key = ordered(below - logs[beam] + score + 0.0);
-        number = beam * a.vocab + token;
+        if (!(x > -INFINITY) || !(below > -INFINITY)) return kNone64;
+        return ordered(below - logs[beam] + score + 0.0);
     };
-    auto candidate = [&](uint32_t c, uint64_t &key, uint32_t &number) {
-        rate(c, w.value[from_first + c], w.token[from_first + c], key, number);
+    auto number_of = [&](uint32_t l, uint32_t e) {
+        const uint32_t beam = l / chunks;
+        return beam * a.vocab + (ended[beam] > 0.f ? a.end : w.token[(from_first + l) * list + e]);
     };
-    uint64_t near[kNear];
-    uint32_t most = 0;
+    // A lower bound of the picks-th largest of the threads' keys: every wave has its share of
+    // picks from the least of the waves' bounds on.
+    auto bound_of = [&](uint32_t most) {
+        const uint32_t bound = nth_bound(most, (a.picks + WAVES - 1) / WAVES);
+        if (lane == 0) bounds[wave] = bound;
+        __syncthreads();
+        uint32_t least = bounds[0];
 #pragma unroll
-    for (uint32_t i = 0; i < kNear; ++i) {
-        near[i] = kNone64;
-        if (tid + i * kThreads < all) rate(tid + i * kThreads, near_x[i], near_token[i], near[i], near_token[i]);
-        most = max(most, uint32_t(near[i] >> 32));
-    }
-    for (uint32_t c = tid + kNear * kThreads; c < all; c += kThreads) {
-        uint64_t key;
-        uint32_t number;
-        candidate(c, key, number);
-        most = max(most, uint32_t(key >> 32));
-    }
-    const uint32_t bound = nth_bound(most, a.picks);
-    if (lane == 0) bounds[wave] = bound;
-    __syncthreads();
-    const uint32_t from = max(max(bounds[0], bounds[1]), max(bounds[2], bounds[3]));
-    auto list_it = [&](uint64_t key, uint32_t number) __attribute__((always_inline)) {
-        if (key > kNone64 && uint32_t(key >> 32) >= from) {
-            const uint32_t at = atomicAdd(&count, 1u);
-            if (at < kListed) ranked[at] = {key, number, 0};
+        for (int i = 1; i < WAVES; ++i) least = min(least, bounds[i]);
+        return least;
+    };
+    // The same to 20 bits, by two bits at a time: where waves differ, some of them with a bad
+    // beam's alone.
+    auto close_bound_of = [&](uint32_t most) {
+        uint32_t bound = 0;
+        for (int bit = 30, turn = 0; bit >= 12; bit -= 2, turn ^= 1) {
+            const uint32_t one = 1u << bit;
+            const uint64_t mine = uint64_t(__popcll(__ballot(most >= (bound | one)))) |
+                                  uint64_t(__popcll(__ballot(most >= (bound | 2 * one)))) << 20 |
+                                  uint64_t(__popcll(__ballot(most >= (bound | 3 * one)))) << 40;
+            if (lane == 0) counts[turn][wave] = mine;
+            __syncthreads();
+            uint64_t sum = 0;
+#pragma unroll
+            for (int i = 0; i < WAVES; ++i) sum += counts[turn][i];
+            bound += (uint32_t(sum & 0xfffff) >= a.picks) * one + (uint32_t(sum >> 20 & 0xfffff) >= a.picks) * one +
+                     (uint32_t(sum >> 40) >= a.picks) * one;
         }
+        return bound;
     };
-#pragma unroll
-    for (uint32_t i = 0; i < kNear; ++i) list_it(near[i], near_token[i]);
-    for (uint32_t c = tid + kNear * kThreads; c < all; c += kThreads) {
-        uint64_t key;
-        uint32_t number;
-        candidate(c, key, number);
-        list_it(key, number);
+    uint32_t most = spread < lists ? uint32_t(rate(spread, 0, near) >> 32) : 0u;
+    for (uint32_t l = spread + THREADS; l < lists; l += THREADS)
+        most = max(most, uint32_t(rate(l, 0, w.value[(from_first + l) * list]) >> 32));
+    uint32_t from = bound_of(most);
+    for (uint32_t l = spread; l < lists; l += THREADS) {
+        const uint64_t key = rate(l, 0, l == spread ? near : w.value[(from_first + l) * list]);
+        if (key > kNone64 && uint32_t(key >> 32) >= from) {
+            const uint32_t at = atomicAdd(&list_count, 1u);
+            if (at < kLists) chosen[at] = l;
+        }
     }
     __syncthreads();
-    const uint32_t n = count;
+    // The entries of those lists, all their first ones before their second ones, bounded in
+    // the same way where they are many.
+    const uint32_t looked = list_count, entries = looked <= kLists ? looked * list : 0;
+    auto entry = [&](uint32_t i, uint32_t &l, uint32_t &e) {
+        e = i / looked;
+        l = chosen[i - e * looked];
+        return rate(l, e, w.value[(from_first + l) * list + e]);
+    };
+    most = 0;
+    if (entries > kFew) {
+        for (uint32_t i = spread, l, e; i < entries; i += THREADS) most = max(most, uint32_t(entry(i, l, e) >> 32));
+        from = max(from, bound_of(most));
+    }
+    for (int turn = 0;; ++turn) {
+        for (uint32_t i = spread, l, e; i < entries; i += THREADS) {
+            const uint64_t key = entry(i, l, e);
+            if (key > kNone64 && uint32_t(key >> 32) >= from) {
+                const uint32_t place = atomicAdd(&count, 1u);
+                if (place < kListed) ranked[place] = {key, number_of(l, e), 0};
+            }
+        }
+        __syncthreads();
+        if (turn || count <= kFew || entries <= kFew) break;
+        from = max(from, close_bound_of(most));
+        if (tid == 0) count = 0;
+        __syncthreads();
+    }
+    const uint32_t n = looked <= kLists ? count : kListed + 1;
     const size_t to = size_t(b) * a.picks;
     auto pick = [&](uint32_t rank, uint64_t key, uint32_t number) __attribute__((always_inline)) {
         const uint32_t beam = number / a.vocab, token = number - beam * a.vocab;
@@ -355,24 +390,29 @@ __global__ __launch_bounds__(kThreads) void beam_join(BeamSelectArgs a, uint32_t
     };
     uint32_t got = min(n, a.picks);
     if (n <= kListed) {
-        for (uint32_t c = tid; c < n; c += kThreads) {
+        // Four threads for each, of one wave.
+        for (uint32_t c = tid / 4; c < n; c += THREADS / 4) {
             const Ranked mine = ranked[c];
             uint32_t rank = 0;
-#pragma unroll 8
-            for (uint32_t i = 0; i < n; ++i) rank += above(ranked[i].key, ranked[i].number, mine.key, mine.number);
-            if (rank < a.picks) pick(rank, mine.key, mine.number);
+#pragma unroll 4
+            for (uint32_t i = tid % 4; i < n; i += 4) rank += above(ranked[i].key, ranked[i].number, mine.key, mine.number);
+            rank += __shfl_xor(rank, 1);
+            rank += __shfl_xor(rank, 2);
+            if (tid % 4 == 0 && rank < a.picks) pick(rank, mine.key, mine.number);
         }
     } else {
+        // Scores that all but tie: the best one after the other.
         uint64_t last = ~0ull;
         uint32_t last_number = 0;
         for (got = 0; got < a.picks; ++got) {
             uint64_t best = kNone64;
             uint32_t number = ~0u;
-            for (uint32_t c = tid; c < all; c += kThreads) {
-                uint64_t key;
-                uint32_t mine;
-                candidate(c, key, mine);
-                if (key > kNone64 && above(last, last_number, key, mine) && above(key, mine, best, number)) {
+            for (uint32_t c = tid; c < lists * list; c += THREADS) {
+                const uint32_t l = c / list, e = c - l * list;
+                const uint64_t key = rate(l, e, w.value[from_first * list + c]);
+                if (key <= kNone64 || key < best) continue;
+                const uint32_t mine = number_of(l, e);
+                if (above(last, last_number, key, mine) && above(key, mine, best, number)) {
                     best = key;
                     number = mine;
                 }
@@ -389,7 +429,7 @@ __global__ __launch_bounds__(kThreads) void beam_join(BeamSelectArgs a, uint32_t
             __syncthreads();
             if (lane == 0) ranked[wave] = {best, number, 0};
             __syncthreads();
-            for (int i = 0; i < kWaves; ++i)
+            for (int i = 0; i < WAVES; ++i)
                 if (above(ranked[i].key, ranked[i].number, best, number)) {
                     best = ranked[i].key;
                     number = ranked[i].number;
@@ -400,17 +440,19 @@ __global__ __launch_bounds__(kThreads) void beam_join(BeamSelectArgs a, uint32_t
             if (tid == 0) pick(got, best, number);
         }
     }
-    for (uint32_t i = got + tid; i < a.picks; i += kThreads) {
+    for (uint32_t i = got + tid; i < a.picks; i += THREADS) {
         a.parents[to + i] = a.tokens[to + i] = -1.f;
         a.new_scores[to + i] = -INFINITY;
         a.new_finished[to + i] = 0.f;
     }
 }
 
-// float4s a thread: the most that leave two blocks a CU.
+// float4s a thread: the most that leave two blocks a CU and are not more than a row has.
 uint32_t words_of(uint32_t batch, uint32_t beams, uint32_t vocab) {
     uint32_t v = 8;
-    while (v > 1 && uint64_t(batch) * beams * ((vocab + 4 * v * kThreads - 1) / (4 * v * kThreads)) < 512) v /= 2;
+    while (v > 1 && (2 * v * kThreads >= vocab ||
+                     uint64_t(batch) * beams * ((vocab + 4 * v * kThreads - 1) / (4 * v * kThreads)) < 512))
+        v /= 2;
     return v;
 }
 uint32_t chunks_of(uint32_t batch, uint32_t beams, uint32_t vocab) {
@@ -447,7 +489,13 @@ hipError_t beam_select_f32(hipStream_t stream, const BeamSelectArgs &a) {
         case 2: launch_chunks<2>(stream, a, chunks, items); break;
         default: launch_chunks<1>(stream, a, chunks, items); break;
     }
-    hipLaunchKernelGGL(beam_join, dim3(a.batch), dim3(kThreads), 0, stream, a, chunks, items);
+    // Sixteen waves where four would take several beams' sums in turn or several lists a
+    // thread: 8.8 us against 9.6 for 64 searches of 8 beams, 10 against 18 for 31 of 16, but
+    // 7.9 against 6.4 for one of 4 and 38 against 12 for 2000 of 4.
+    if (a.beams > 4 || a.beams * chunks > 256)
+        hipLaunchKernelGGL(beam_join<1024>, dim3(a.batch), dim3(1024), 0, stream, a, chunks, items);
+    else
+        hipLaunchKernelGGL(beam_join<kThreads>, dim3(a.batch), dim3(kThreads), 0, stream, a, chunks, items);
     return hipGetLastError();
 }
 

@@ -583,3 +583,30 @@ def test_beam_select_flat_and_peaked_logits(runtime, scale):
     logits = (scale * rng.standard_normal((4, 3, 20000))).astype(np.float32)
     logits[3] += np.float32(1e4)
     check_select(runtime, select_spec(4, 3, 20000, 6), logits, (-5 * rng.random((4, 3))).astype(np.float32), np.zeros((4, 3), np.float32))
+
+
+@pytest.mark.parametrize("batch,beams,vocab,picks", [(5, 4, 32000, 64), (2, 16, 20000, 32), (3, 16, 64, 64), (300, 2, 9100, 64), (1, 200, 4500, 64)])
+def test_beam_select_one_beam_far_ahead(runtime, batch, beams, vocab, picks):
+    # All that is chosen comes from one beam's lists, of fewer threads than are asked; sorted logits besides, where one
+    # chunk has them all.
+    rng = np.random.default_rng(55 + beams)
+    logits = 3 * normal(rng, batch, beams, vocab)
+    logits[0] = np.sort(logits[0], axis=-1)
+    scores = np.full((batch, beams), -60.0, np.float32)
+    scores[np.arange(batch), rng.integers(0, beams, batch)] = -1
+    check_select(runtime, select_spec(batch, beams, vocab, picks), logits, scores, np.zeros((batch, beams), np.float32))
+
+
+def test_beam_select_more_equal_lists_than_are_looked_at_at_once(runtime):
+    spec = select_spec(1, 256, 5000, 64)
+    logits, scores = np.zeros((1, 256, 5000), np.float32), np.full((1, 256), -2.0, np.float32)
+    logits[0, 200:, 1::7] = 0.5
+    want, _ = po.select(spec, logits, scores, np.zeros((1, 256)))
+    got = run(runtime, spec, {"logits": logits, "scores": scores, "finished": np.zeros((1, 256))})
+    for name in ("parents", "tokens"):
+        same(got[name], want[name])
+    logits[:] = 0
+    want, _ = po.select(spec, logits, scores, np.zeros((1, 256)))
+    got = run(runtime, spec, {"logits": logits, "scores": scores, "finished": np.zeros((1, 256))})
+    for name in ("parents", "tokens"):
+        same(got[name], want[name])
