@@ -34,6 +34,9 @@ namespace {
 using namespace paged;
 
 constexpr int kTile = 64;  // keys of a tile
+// Tiles after which a wave's sums are put aside and begun anew: FP32 sums of 65536 equal
+// weights each were off by up to 2.9e-3 (512 sequences of 2^20 tokens, one run each).
+constexpr uint32_t kPiece = 64;
 
 // DP: head dim padded (64, 96, 128). G: groups of 16 rows, all of them every wave's.
 template <int DP, int G>
@@ -177,8 +180,40 @@ __attribute__((amdgpu_waves_per_eu(kWavesASimd<DP, G>, kWavesASimd<DP, G>))) voi
             load_k(next, next.begin, page_next);
             load_v(next, next.begin, page_next);
         }
+        // This wave's sums since the last time, on top of those, in LDS: row 16 r + m, dims
+        // 64 j + 16 g + 4 i + e.
+        auto put_aside = [&](bool first) __attribute__((always_inline)) {
+#pragma unroll
+            for (int r = 0; r < G; ++r) {
+                float2 &kept = ml[wave][16 * r + m];
+                const float2 old = first ? float2{-INFINITY, 0.f} : kept;
+                const float all = across_keys_sum(sum[r]), from = top[r] == -INFINITY ? 0.f : top[r];
+                const float weight = __builtin_amdgcn_exp2f(old.x - from);
+                if (g == 0) kept = float2{top[r], fmaf(weight, old.y, all)};
+#pragma unroll
+                for (int j = 0; j < NJ; ++j)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        f32x4 &to = *reinterpret_cast<f32x4 *>(&part[wave][16 * r + m][64 * j + 16 * g + 4 * i]);
+                        const f32x4 x = {acc[r][j][0][i], acc[r][j][1][i], acc[r][j][2][i], acc[r][j][3][i]};
+                        to = first ? x : x + weight * to;
+                    }
+            }
+        };
         for (uint32_t x = begin; x < u.stop; ++x) {
             const bool last = x + 1 == u.stop;
+            if (x != begin && (x - begin) % kPiece == 0) {
+                if (x - begin == kPiece) __syncthreads();  // the last unit's sums are read
+                put_aside(x - begin == kPiece);
+#pragma unroll
+                for (int r = 0; r < G; ++r) {
+                    sum[r] = 0.f;
+#pragma unroll
+                    for (int j = 0; j < NJ; ++j)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) acc[r][j][e] = f32x4{0.f, 0.f, 0.f, 0.f};
+                }
+            }
             if (!VEC)  // the next row's values may not be finite
 #pragma unroll
                 for (int j = 0; j < KJ; ++j)
@@ -278,19 +313,9 @@ __attribute__((amdgpu_waves_per_eu(kWavesASimd<DP, G>, kWavesASimd<DP, G>))) voi
         const uint32_t rows = rows_of(u);
         load_rows(next);
 
-        // The four waves' sums joined: row 16 r + m, dims 64 j + 16 g + 4 i + e.
+        // The four waves' sums joined.
         __syncthreads();
-#pragma unroll
-        for (int r = 0; r < G; ++r) {
-            const float all = across_keys_sum(sum[r]);
-            if (g == 0) ml[wave][16 * r + m] = float2{top[r], all};
-#pragma unroll
-            for (int j = 0; j < NJ; ++j)
-#pragma unroll
-                for (int i = 0; i < 4; ++i)
-                    *reinterpret_cast<f32x4 *>(&part[wave][16 * r + m][64 * j + 16 * g + 4 * i]) =
-                        f32x4{acc[r][j][0][i], acc[r][j][1][i], acc[r][j][2][i], acc[r][j][3][i]};
-        }
+        put_aside(u.stop <= begin + kPiece);
         __syncthreads();
         finish<OUT, RB, VEC>(a, run, u.b, u.kv, u.rb, rows, whole, begin == 0, part, ml, plans, 1.f);
         u = next;

@@ -37,6 +37,9 @@ using namespace split;
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 
 constexpr int kKeys = int(kPagedFlashTile);
+// Tiles after which a wave's sums are put aside and begun anew: FP32 sums of 2^22 equal
+// weights were off by up to 2.9e-3.
+constexpr int kPiece = 128;
 // Scaled Q past this takes the FP32 path: then no product of a part of Q with a part of a
 // tiny K loses more than an FP32 score's rounding.
 constexpr float kMostQ = 0x1p64f * kScaleQ;
@@ -240,6 +243,56 @@ attention_paged_flash(PagedArgs a) {
             return Row{mine, query, mine - query * a.group, mine - rb * RB < rows};
         };
         const size_t q_base = size_t(b) * a.q_batch + size_t(kv) * a.group * a.q_head;
+        // This lane's outputs by four neighbouring dims, first_dim + d and on, each become
+        // f(d, x). LDS row r of V is dim 2r (r < DP / 2) or 2 (r - DP / 2) + 1, and
+        // a lane holds rows 32x + 8 (v >> 2) + 4h + (v & 3): r, r + 1 and their odd partners are four
+        // adjacent dims.
+        auto each_four = [&](auto &&f) __attribute__((always_inline)) {
+#pragma unroll
+            for (int y = 0; y < NB * 16; y += 2) {
+                const int x = y / 16, v = y % 16, r = 32 * x + 8 * (v >> 2) + (v & 3);
+                if (r >= DP / 2) continue;
+                const int r2 = r + DP / 2, x2 = r2 / 32, v2 = 4 * (r2 % 32 / 8) + r2 % 4;
+                const f32x4 four = f(2 * r, f32x4{acc[x][v], acc[x2][v2], acc[x][v + 1], acc[x2][v2 + 1]});
+                acc[x][v] = four.x, acc[x2][v2] = four.y, acc[x][v + 1] = four.z, acc[x2][v2 + 1] = four.w;
+            }
+        };
+        // The sums so far of a long unit, in its slot; `later`: on top of what is there already. Then
+        // they begin anew. Or (`back`) what is there on top of the sums.
+        auto put_aside = [&](bool later, bool back) __attribute__((always_inline)) {
+            const Row row = row_now();
+            const uint32_t dim = dim_now(a), first_dim = 8u * uint32_t(lane_now() >> 5);
+            Args *const now = args_now();
+            const size_t slot = (2 * size_t(run) + (begin == 0)) * RB + (row.mine - rb * RB);
+            float2 &kept = reinterpret_cast<float2 *>(now->partial + 2 * size_t(now->runs) * RB * kSlotRow<DP>)[slot];
+            const float2 old = row.me && later ? kept : float2{-INFINITY, 0.f};
+            const float sum = halves_sum(row_sum), from = row_max == -INFINITY ? 0.f : row_max;
+            const float weight = __builtin_amdgcn_exp2f(old.x - from);
+            if (row.me) {
+                float *const to = now->partial + slot * kSlotRow<DP> + first_dim;
+                each_four([&](int d, f32x4 x) __attribute__((always_inline)) {
+                    __builtin_amdgcn_sched_barrier(0);  // one at a time: the main loop has no registers to spare
+                    if (first_dim + d >= dim) return x;
+                    f32x4 &there = *reinterpret_cast<f32x4 *>(to + d);
+                    if (later) x += weight * there;
+                    if (!back) there = x;
+                    return x;
+                });
+            }
+            row_sum = fmaf(weight, old.y, sum);
+            if (!back) {
+                if (row.me && lane_now() < 32) kept = float2{row_max, row_sum};
+                __threadfence_block();  // read by the other half of the wave
+                row_sum = 0.f;
+#pragma unroll
+                for (int x = 0; x < NB; ++x) acc[x] = f32x16{};
+            } else if (lane_now() >= 32) {
+                row_sum = 0.f;  // halves are added up again
+            }
+        };
+        auto new_piece = [&](int t) __attribute__((always_inline)) {
+            if (t != t0 && (t - t0) % kPiece == 0) put_aside(t - t0 != kPiece, false);
+        };
 
         if (t0 < t_end) {
             // Q^T operand: step s holds dims 16s + 8h + e of row c, in log2 units. Rows past the
@@ -447,12 +500,14 @@ attention_paged_flash(PagedArgs a) {
                 gaps >>= 2;
             };
             for (int t = t0; t < t_end - 1; ++t) {
+                new_piece(t);
                 if (live(t))
                     tile(t, std::true_type{}, std::true_type{});
                 else
                     tile(t, std::false_type{}, std::true_type{});
             }
             if (live(t_end - 1)) tile(t_end - 1, std::true_type{}, std::false_type{});
+            if (t_end - 1 - t0 > kPiece) put_aside(true, true);
         }
 
         // What the parts do not carry: see the file's head.
@@ -472,7 +527,9 @@ attention_paged_flash(PagedArgs a) {
             const uint32_t dim = dim_now(a);
             const int l = lane_now(), c = l & 31, h = l >> 5;
             const float *const qrow = row.me ? a.q + q_base + row.member * a.q_head + size_t(row.query) * a.q_row : nullptr;
-            for (int t = t0; t < t_end && t * kKeys <= high; ++t) {
+            const int t_last = high < 0 ? -1 : min(t_end - 1, high / kKeys);
+            for (int t = t0; t <= t_last; ++t) {
+                new_piece(t);
                 const Entries e = entries_of(t);
                 const uint32_t p0 = uniform(page_of(a, e.x[0])), p1 = uniform(page_of(a, e.x[1]));
                 // Key x of the tile: its first dim's place in the pools; 0, which is one, and false
@@ -533,6 +590,7 @@ attention_paged_flash(PagedArgs a) {
                     }
                 }
             }
+            if (t_last - t0 >= kPiece) put_aside(true, true);
         }
 
         row_sum = halves_sum(row_sum);
@@ -545,18 +603,10 @@ attention_paged_flash(PagedArgs a) {
             float *const to = whole ? a.out + row_at(a, b, kv, row.mine) : a.partial + slot * kSlotRow<DP>;
             if (!whole && h == 0)
                 reinterpret_cast<float2 *>(a.partial + 2 * size_t(a.runs) * RB * kSlotRow<DP>)[slot] = float2{row_max, row_sum};
-            // LDS row r of V is dim 2r (r < DP / 2) or 2 (r - DP / 2) + 1, and a lane holds rows
-            // 32x + 8 (v >> 2) + 4h + (v & 3): r, r + 1 and their odd partners are four adjacent dims.
-#pragma unroll
-            for (int y = 0; y < NB * 16; y += 2) {
-                const int x = y / 16, v = y % 16, r = 32 * x + 8 * (v >> 2) + (v & 3);
-                if (r >= DP / 2) continue;
-                const int r2 = r + DP / 2, x2 = r2 / 32, v2 = 4 * (r2 % 32 / 8) + r2 % 4;
-                const uint32_t d = first_dim + 2 * r;
-                if (d < dim)
-                    *reinterpret_cast<f32x4 *>(to + d) =
-                        f32x4{acc[x][v] * by, acc[x2][v2] * by, acc[x][v + 1] * by, acc[x2][v2 + 1] * by};
-            }
+            each_four([&](int d, f32x4 x) __attribute__((always_inline)) {
+                if (first_dim + d < dim) *reinterpret_cast<f32x4 *>(to + first_dim + d) = x * by;
+                return x;
+            });
         }
         at += end - begin;
         if (at >= before + all) {

@@ -1,0 +1,96 @@
+"""Paged attention over long caches: sums of many weights, tables of many entries. References in 64 bits for a few rows;
+bounds count roundings (U is half an ulp), as paged_oracle.py's do."""
+import numpy as np
+import pytest
+
+from decoder_oracle import U
+from test_gpu_decoder import normal
+
+pytestmark = pytest.mark.gpu
+
+
+def compile_paged(runtime, batch, heads, queries, page, tokens, dim, pages):
+    return runtime.compile({"op": "attention_paged", "batch": batch, "heads": heads, "kv_heads": 1, "queries": queries,
+                            "pages": pages, "page": page, "table": -(-tokens // page), "dim": dim,
+                            "token_major": True, "pages_token_major": True})
+
+
+def attend_on(runtime, kernel, *inputs):
+    buffers = [runtime.resident(x) for x in inputs]
+    out = runtime.alloc(inputs[0].size)
+    runtime.execute([(kernel, buffers + [out])], 1)
+    got = runtime.download(out).astype(np.float64)
+    for b in (*buffers, out):
+        b.free()
+    kernel.release()
+    return got
+
+
+# Roundings of sums over keys, of terms alike: a running sum is half of its last value in the mean. A sum is put aside
+# and begun anew after 64 tiles of a wave's 16 keys (FP32 MFMAs: an addition for each key, a lane's weights a quarter of
+# them) or 128 tiles of 32 (parts: six products a key). The matrix cores do not round to nearest, 2 U for each addition.
+# Then an addition for each such piece, and 512 for the runs that are joined. Numerator and denominator; last, both
+# weights' and their scores' own roundings: 4 for exp2 and its argument, dim + 2 for the score.
+def mean_bound(parts, tokens, dim):
+    pieces = tokens / (4096 if parts else 1024) + 512
+    products, weights = (128 * 32 * 6, 128 * 16) if parts else (64 * 16, 64 * 4)
+    return U * ((2 * products + pieces) / 2 + (weights + pieces) / 2 + 2 * (4 + 2 * (dim + 2)) + 16)
+
+
+@pytest.mark.parametrize("queries,dim,tokens", [(1, 8, 2 ** 21 + 777), (20, 8, 2 ** 20 + 1), (1, 80, 2 ** 18 + 99), (64, 8, 2 ** 22 + 33),
+                                                (64, 128, 2 ** 19 + 5)])
+@pytest.mark.parametrize("batch", [1, 300, 512])
+def test_attention_paged_sums_of_a_million_equal_weights(runtime, queries, dim, tokens, batch):
+    # The first token's score is the greatest; all others weigh 0.502 beside it, which takes two bf16 parts. Many
+    # sequences over the same pages, so that one run has all of a sequence's tokens; and one, cut between all runs.
+    rng = np.random.default_rng(60)
+    page = 1024
+    table = -(-tokens // page)
+    q = np.zeros((batch, queries, 1, dim), np.float32)
+    q[..., 0] = 1
+    k, v = np.zeros((2, table * page, dim), np.float32)
+    k[1:, 0] = np.log(0.501953125) * np.sqrt(dim)
+    # Values: everywhere 1; the first half of the tokens; every other one; one wave's; random ones; far ones.
+    at = np.arange(table * page)
+    v[:, 0], v[:, 1], v[:, 2], v[:, 3] = 1, at < tokens // 2, at % 2, at % 64 < 16
+    v[:, 4], v[:, 5], v[:, 6] = rng.random(at.size), at >= tokens - 5000, 1 + (at % 3 == 0)
+    v[:, 7:] = v[:, :1]
+    tables = np.tile(np.arange(table, dtype=np.float32), (batch, 1))
+    kernel = compile_paged(runtime, batch, 1, queries, page, tokens, dim, table)
+    parts = kernel.launch["kernel"].startswith("attention_paged_flash")
+    assert parts == (queries == 64)
+    got = attend_on(runtime, kernel, q, k, v, tables, np.full(batch, tokens, np.float32), np.full(batch, queries, np.float32))
+    weights = np.ones(tokens)
+    weights[1:] = np.exp(float(k[1, 0]) / np.sqrt(dim))
+    sums = np.cumsum(weights[:, None] * v[:tokens, :8].astype(np.float64), axis=0)[-queries:]
+    want = sums / np.cumsum(weights)[-queries:, None]
+    error = np.abs(got.reshape(batch, queries, dim)[..., :8] - want) / want
+    assert error.max() <= mean_bound(parts, tokens, dim), (error.max(axis=(0, 1)), mean_bound(parts, tokens, dim))
+
+
+@pytest.mark.parametrize("page,queries,dim", [(16, 1, 32), (48, 1, 31), (1008, 1, 32), (1024, 1, 32), (16, 64, 32), (48, 64, 32),
+                                              (1008, 64, 32), (1024, 64, 32), (48, 20, 32)])
+def test_attention_paged_tables_of_many_entries(runtime, page, queries, dim):
+    # Pages in no order; scores so far apart that a few dozen of the keys make up a row, wherever they lie.
+    rng = np.random.default_rng(page + queries)
+    tokens = 300000 + page // 2 + 5
+    table = -(-tokens // page)
+    q = 3 * normal(rng, 1, queries, 1, dim)
+    k, v = normal(rng, 2, table * page, dim)
+    tables = rng.permutation(table + 7)[:table].astype(np.float32)
+    pools = np.full((2, table + 7, page, dim), np.nan, np.float32)
+    for pool, x in zip(pools, (k, v)):
+        pool[tables.astype(int)] = x.reshape(table, page, dim)
+    kernel = compile_paged(runtime, 1, 1, queries, page, tokens, dim, table + 7)
+    parts = kernel.launch["kernel"].startswith("attention_paged_flash")
+    got = attend_on(runtime, kernel, q, *pools, tables, [tokens], [queries]).reshape(queries, dim)
+    k, v = k.astype(np.float64), v.astype(np.float64)
+    for i in sorted({0, queries // 2, queries - 1}):
+        seen = tokens - queries + 1 + i
+        row = q[0, i, 0].astype(np.float64) / np.sqrt(dim)
+        scores, sizes = k[:seen] @ row, np.abs(k[:seen]) @ np.abs(row)
+        p = np.exp(scores - scores.max())
+        p /= p.sum()
+        # Terms of any order: every addition's rounding in full, twice what mean_bound says; scores' by their sizes.
+        off = 2 * mean_bound(parts, tokens, dim) + U * 4 * (dim + 2) * sizes.max()
+        assert (np.abs(got[i] - p @ v[:seen]) <= off * (p @ np.abs(v[:seen]))).all()
