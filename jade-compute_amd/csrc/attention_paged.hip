@@ -317,7 +317,7 @@ __attribute__((amdgpu_waves_per_eu(kWavesASimd<DP, G>, kWavesASimd<DP, G>))) voi
         __syncthreads();
         put_aside(u.stop <= begin + kPiece);
         __syncthreads();
-        finish<OUT, RB, VEC>(a, run, u.b, u.kv, u.rb, rows, whole, begin == 0, part, ml, plans, 1.f);
+        finish<OUT, RB, VEC>(a, run, u.b, u.kv, u.rb, rows, whole, begin == 0, part, ml, plans);
         u = next;
     }
     clear_rows(work);

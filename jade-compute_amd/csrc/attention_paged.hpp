@@ -335,12 +335,11 @@ struct RowPlan {
 // The `rows` sums of row block rb of (sequence b, kv head) as the four waves by keys left
 // them in LDS, joined: outputs where the run holds the `whole` unit, else sums, maximum
 // and weight to the run's slot (a unit's first run had it last, the others first). The
-// block's threads do it together; `plans` is LDS. The sums in LDS are to be multiplied by
-// `unscale`. True for a thread that met one that is not finite.
+// block's threads do it together; `plans` is LDS.
 template <int DP, int RB, bool VEC>
-__device__ inline bool finish(const PagedArgs &a, uint32_t run, uint32_t b, uint32_t kv, uint32_t rb, uint32_t rows,
+__device__ inline void finish(const PagedArgs &a, uint32_t run, uint32_t b, uint32_t kv, uint32_t rb, uint32_t rows,
                               bool whole, bool starts, const float (&part)[kWaves][RB][DP + 4],
-                              const float2 (&ml)[kWaves][RB], RowPlan (&plans)[RB], float unscale) {
+                              const float2 (&ml)[kWaves][RB], RowPlan (&plans)[RB]) {
     uint32_t tid = threadIdx.x;
     asm volatile("" : "+v"(tid));  // nothing below is computed ahead of a caller's main loop
     if (tid < rows) {
@@ -358,28 +357,23 @@ __device__ inline bool finish(const PagedArgs &a, uint32_t run, uint32_t b, uint
         p.top_sum = float2{most, l};
         if (whole) {
             p.at = row_at(a, b, kv, rb * RB + tid);
-            p.top_sum.y = l == 0.f ? 0.f : unscale / l;  // a row that sees no key is zeros
+            p.top_sum.y = l == 0.f ? 0.f : 1.f / l;  // a row that sees no key is zeros
         } else {
             const size_t slot = (2 * size_t(run) + starts) * RB + tid;
             p.at = slot * kSlotRow<DP>;
             reinterpret_cast<float2 *>(a.partial + 2 * size_t(a.runs) * RB * kSlotRow<DP>)[slot] = p.top_sum;
-            p.top_sum.y = unscale;
+            p.top_sum.y = 1.f;
         }
         plans[tid] = p;
     }
     __syncthreads();
     float *const to = whole ? a.out : a.partial;
-    bool odd = false;
     for (uint32_t at = tid; at < rows * (DP / 4); at += kThreads) {
         const uint32_t row = at / (DP / 4), d = at % (DP / 4) * 4;
         const RowPlan &p = plans[row];
         f32x4 o = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int w = 0; w < kWaves; ++w) o += p.weights[w] * *reinterpret_cast<const f32x4 *>(&part[w][row][d]);
-        if (d < a.dim)
-#pragma unroll
-            for (int e = 0; e < 4; ++e)
-                odd |= (VEC || d + e < a.dim) && !finite(o[e]);
         o = p.top_sum.y == 0.f ? f32x4{0.f, 0.f, 0.f, 0.f} : o * p.top_sum.y;
         if (VEC || !whole) {
             if (!whole || d < a.dim) *reinterpret_cast<f32x4 *>(to + p.at + d) = o;
@@ -387,7 +381,6 @@ __device__ inline bool finish(const PagedArgs &a, uint32_t run, uint32_t b, uint
             store_dims<false>(to + p.at, int(d), int(a.dim), o);
         }
     }
-    return odd;
 }
 
 }  // namespace paged
