@@ -48,8 +48,10 @@ __attribute__((amdgpu_waves_per_eu(kWavesASimd<DP, G>, kWavesASimd<DP, G>))) voi
     __shared__ __attribute__((aligned(16))) float part[kWaves][RB][OUT + 4];
     __shared__ float2 ml[kWaves][RB];
     __shared__ RowPlan plans[RB];
+    __shared__ uint32_t odd[kWaves];  // whether a wave met an output that is not finite
     const int tid = threadIdx.x, lane = tid & 63;
     const uint32_t wave = uniform(tid >> 6);
+    odd[wave] = 0;
     const int m = lane & 15, g = lane >> 4;
     const Work<kTile, RB> work(a);
     const uint32_t chunk = (work.total + a.runs - 1) / a.runs;
@@ -317,10 +319,11 @@ __attribute__((amdgpu_waves_per_eu(kWavesASimd<DP, G>, kWavesASimd<DP, G>))) voi
         __syncthreads();
         put_aside(u.stop <= begin + kPiece);
         __syncthreads();
-        finish<OUT, RB, VEC>(a, run, u.b, u.kv, u.rb, rows, whole, begin == 0, part, ml, plans);
+        finish<OUT, RB, VEC>(a, run, u.b, u.kv, u.rb, rows, whole, begin == 0, part, ml, plans, odd);
         u = next;
     }
     clear_rows(work);
+    if (__builtin_expect(uniform(odd[wave]), 0)) sum_again<kTile, RB, OUT, kThreads / OUT, VEC>();
 }
 
 // How the launch that joins is laid out: blocks x rows, and which unit a block has.
@@ -371,14 +374,24 @@ __device__ void join_unit(const PagedArgs &a, uint32_t block, uint32_t rows_from
     const float2 *ml = reinterpret_cast<const float2 *>(a.partial + 2 * size_t(a.runs) * RB * DP);
     // A unit's first run had it last, the others first.
     auto slot = [&](uint32_t r) { return (2 * size_t(r) + (r == first)) * RB + row; };
+    // Sums of the slots' means, by their weights; and 2^-40 of them, for where those pass FP32's
+    // largest (a slot weighs 2^8 for each of its keys at most).
     float most = -INFINITY, l = 0.f;
-    f32x4 o = {0.f, 0.f, 0.f, 0.f};
-    auto join = [&](float top, float sum, f32x4 outs) {
+    f32x4 o = {0.f, 0.f, 0.f, 0.f}, small = o;
+    auto join = [&](float top, float sum, f32x4 mean) {
         const float next = fmaxf(most, top), from = next == -INFINITY ? 0.f : next;
-        const float old = __builtin_amdgcn_exp2f(most - from), weight = __builtin_amdgcn_exp2f(top - from);
+        const float old = __builtin_amdgcn_exp2f(most - from), weight = sum * __builtin_amdgcn_exp2f(top - from);
         most = next;
-        l = l * old + sum * weight;
-        o = o * old + outs * weight;
+        l = l * old + weight;
+        o = o * old + mean * weight;
+        small = small * old + mean * (weight * 0x1p-40f);
+    };
+    auto mean = [&] {
+        const float by = 1.0f / l;
+        f32x4 x;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) x[e] = l == 0.f ? 0.f : finite(o[e]) ? o[e] * by : small[e] * (0x1p40f * by);
+        return x;  // a row that sees no key is zeros
     };
     if (mine) {
 #pragma unroll 4
@@ -387,16 +400,25 @@ __device__ void join_unit(const PagedArgs &a, uint32_t block, uint32_t rows_from
             join(x.x, x.y, *reinterpret_cast<const f32x4 *>(a.partial + slot(r) * DP + d));
         }
     }
+    o = mean();
     if constexpr (PARTS > 1) {
         sums[p][lane] = o;
         if (lane == 0) weights[p] = float2{most, l};
         __syncthreads();
         if (p) return;
 #pragma unroll
-        for (int x = 1; x < PARTS; ++x) join(weights[x].x, weights[x].y, sums[x][lane]);
+        for (int x = 1; x < PARTS; ++x) most = fmaxf(most, weights[x].x);
+        const float from = most == -INFINITY ? 0.f : most;
+        float shares[PARTS];
+        l = 0.f;
+#pragma unroll
+        for (int x = 0; x < PARTS; ++x) l += shares[x] = weights[x].y * __builtin_amdgcn_exp2f(weights[x].x - from);
+        const float by = l == 0.f ? 0.f : 1.0f / l;  // a row that sees no key is zeros
+        o = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int x = 0; x < PARTS; ++x) o += sums[x][lane] * (shares[x] * by);
     }
     if (!mine) return;
-    o = l == 0.f ? f32x4{0.f, 0.f, 0.f, 0.f} : o * (1.0f / l);  // a row that sees no key is zeros
     store_dims<VEC>(a.out + row_at(a, b, kv, rb * RB + row), int(d), int(a.dim), o);
 }
 template <int DP, int RB, int TILE, bool VEC>
@@ -524,7 +546,7 @@ hipError_t launch_groups(hipStream_t stream, const PagedShape &s, const PagedArg
 
 uint32_t paged_lds_bytes(uint32_t dim, uint32_t rows) {
     const uint32_t pitch = (dim <= 64 ? 64 : 128) + 4;
-    return uint32_t(kWaves * rows * (pitch * sizeof(float) + sizeof(float2)) + rows * sizeof(RowPlan));
+    return uint32_t(kWaves * rows * (pitch * sizeof(float) + sizeof(float2)) + rows * sizeof(RowPlan) + kWaves * sizeof(uint32_t));
 }
 
 }  // namespace

@@ -275,6 +275,16 @@ __device__ inline int lane_now() {
     return l;
 }
 
+// The kernel's arguments where they were passed, read anew: nothing made of them is kept in
+// registers across a main loop that has none to spare. Only in a kernel itself: a function
+// that is called has no such place, and reads at 0.
+typedef const __attribute__((address_space(4))) PagedArgs Args;
+__device__ __attribute__((always_inline)) inline Args *args_now() {
+    Args *p = reinterpret_cast<Args *>(reinterpret_cast<uintptr_t>(__builtin_amdgcn_kernarg_segment_ptr()));
+    asm volatile("" : "+s"(p));
+    return p;
+}
+
 // Row r of (sequence b, kv head), from its first dim, in q and out.
 __device__ inline size_t row_at(const PagedArgs &a, uint32_t b, uint32_t kv, uint32_t r) {
     const uint32_t query = r / a.group, head = r - query * a.group;
@@ -329,17 +339,20 @@ constexpr int kSlotRow = DP <= 64 ? 64 : 128;
 // What joining the four waves' sums of a row takes.
 struct RowPlan {
     f32x4 weights;  // of the waves
-    float2 top_sum;  // with `by` in place of the sum, once that is kept
-    size_t at;  // its first dim in the outputs, or in the run's slot
+    size_t at;      // its first dim in the outputs, or in the run's slot
+    bool sees;      // any key
+    bool sound;     // its weights are numbers
 };
 // The `rows` sums of row block rb of (sequence b, kv head) as the four waves by keys left
-// them in LDS, joined: outputs where the run holds the `whole` unit, else sums, maximum
-// and weight to the run's slot (a unit's first run had it last, the others first). The
-// block's threads do it together; `plans` is LDS.
+// them in LDS, joined: outputs where the run holds the `whole` unit, else means, maximum
+// and weight to the run's slot (a unit's first run had it last, the others first). Sums meet
+// weights that are divided already, so that FP32 holds what it holds of each wave's. The
+// block's threads do it together; `plans` is LDS. odd[wave] becomes 1 where the wave met an
+// output that is not finite, of weights that are numbers.
 template <int DP, int RB, bool VEC>
 __device__ inline void finish(const PagedArgs &a, uint32_t run, uint32_t b, uint32_t kv, uint32_t rb, uint32_t rows,
                               bool whole, bool starts, const float (&part)[kWaves][RB][DP + 4],
-                              const float2 (&ml)[kWaves][RB], RowPlan (&plans)[RB]) {
+                              const float2 (&ml)[kWaves][RB], RowPlan (&plans)[RB], uint32_t (&odd)[kWaves]) {
     uint32_t tid = threadIdx.x;
     asm volatile("" : "+v"(tid));  // nothing below is computed ahead of a caller's main loop
     if (tid < rows) {
@@ -354,31 +367,161 @@ __device__ inline void finish(const PagedArgs &a, uint32_t run, uint32_t b, uint
             p.weights[w] = __builtin_amdgcn_exp2f(ml[w][tid].x - from);
             l = fmaf(p.weights[w], ml[w][tid].y, l);
         }
-        p.top_sum = float2{most, l};
+        p.sees = l != 0.f;
+        p.sound = finite(l);
+        p.weights *= 1.f / l;
         if (whole) {
             p.at = row_at(a, b, kv, rb * RB + tid);
-            p.top_sum.y = l == 0.f ? 0.f : 1.f / l;  // a row that sees no key is zeros
         } else {
             const size_t slot = (2 * size_t(run) + starts) * RB + tid;
             p.at = slot * kSlotRow<DP>;
-            reinterpret_cast<float2 *>(a.partial + 2 * size_t(a.runs) * RB * kSlotRow<DP>)[slot] = p.top_sum;
-            p.top_sum.y = 1.f;
+            reinterpret_cast<float2 *>(a.partial + 2 * size_t(a.runs) * RB * kSlotRow<DP>)[slot] = float2{most, l};
         }
         plans[tid] = p;
     }
     __syncthreads();
     float *const to = whole ? a.out : a.partial;
+    float met = 0.f;  // NaN from an output on that is not finite
     for (uint32_t at = tid; at < rows * (DP / 4); at += kThreads) {
         const uint32_t row = at / (DP / 4), d = at % (DP / 4) * 4;
         const RowPlan &p = plans[row];
         f32x4 o = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int w = 0; w < kWaves; ++w) o += p.weights[w] * *reinterpret_cast<const f32x4 *>(&part[w][row][d]);
-        o = p.top_sum.y == 0.f ? f32x4{0.f, 0.f, 0.f, 0.f} : o * p.top_sum.y;
+        if (!p.sees) o = f32x4{0.f, 0.f, 0.f, 0.f};  // a row that sees no key
+        float all = 0.f;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) all = VEC || d + e < a.dim ? fmaf(o[e], 0.f, all) : all;
+        if (p.sound) met += all;
         if (VEC || !whole) {
             if (!whole || d < a.dim) *reinterpret_cast<f32x4 *>(to + p.at + d) = o;
         } else {
             store_dims<false>(to + p.at, int(d), int(a.dim), o);
+        }
+    }
+    if (met != 0.f) odd[tid / 64] = 1;
+}
+
+// The outputs, or means in slots, of the block's run that this wave left and that are not
+// finite, once more: those whose sums alone passed FP32's largest (values of 1e37 over a hundred
+// equal keys) are finite then. A wave leaves OWN neighbouring rows of a unit, then its next.
+// Weights are 2^-32 as large, which 2^24 keys of 1 each leave room for, and a row's
+// values are summed by themselves: 64 keys' scores, a lane each, then their values, a lane for two
+// dims. Not made to be fast, nor called where all is finite; and where the values themselves are
+// not, that is found by one look at them (512 queries over 16384 keys of 128 dims, every 1024th
+// value infinite: 5.5 ms, 3.5 without this). Inlined, as args_now() asks.
+template <int TILE, int RB, int ROW, int OWN, bool VEC>
+__device__ __attribute__((always_inline)) inline void sum_again() {
+    constexpr uint32_t kPiece = 4096;  // keys whose sums are put aside
+    __threadfence_block();  // other lanes left what this one looks at
+    const PagedArgs &a = *(const PagedArgs *)args_now();  // no register keeps them for this across a main loop
+    const Work<TILE, RB> work(a);
+    const uint32_t run = run_of(blockIdx.x, a.runs);
+    const uint32_t lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6), waves = blockDim.x / 64;
+    const uint32_t chunk = (work.total + a.runs - 1) / a.runs;
+    uint32_t b, before;
+    const uint32_t t_stop = work.start(run + 1, chunk, b, before);
+    uint32_t t = work.start(run, chunk, b, before);
+    while (t < t_stop) {
+        const Sequence s = work.anew(b);
+        if (!work.active(s)) {
+            ++b;
+            continue;
+        }
+        const uint32_t all = uniform(work.all_of(s));
+        const Spot p = work.spot(s, all, t - before);
+        const uint32_t begin = p.tile, end = min(p.tiles, begin + (t_stop - t));
+        const bool whole = begin == 0 && end == p.tiles;
+        const uint32_t rows = min(uint32_t(RB), s.count * a.group - p.rb * RB);
+        const bool near = lane < a.dim, far = lane + 64 < a.dim;
+        // The first token whose value is not finite, of this lane's dims; looked for where a row asks.
+        uint32_t near_first = 0, far_first = 0;
+        bool looked = false;
+        for (uint32_t r = 0; r < rows; ++r) {
+            if (r / OWN % waves != wave) continue;
+            const uint32_t row = p.rb * RB + r;
+            const size_t q_at = row_at(a, b, p.kv, row), slot = (2 * size_t(run) + (begin == 0)) * RB + r;
+            float *const to = whole ? a.out + q_at : a.partial + slot * ROW;
+            bool near_odd = near && !finite(to[lane]), far_odd = far && !finite(to[lane + 64]);
+            if (!__any(near_odd || far_odd)) continue;
+            if (!looked) {
+                looked = true;
+                near_first = far_first = ~0u;
+                const uint32_t tokens = min(end * TILE, s.length);
+                for (uint32_t key = begin * TILE; key < tokens; key += 16) {
+                    const Place of = place_of(a, key / 16);
+                    const uint32_t page = uniform(page_of(a, a.tables[size_t(b) * a.table + of.entry]));
+                    if (page == kNoPage) continue;
+                    const float *const v = a.v + page * a.p_page + p.kv * a.p_head + size_t(of.step) * 16 * a.p_row;
+#pragma unroll 4
+                    for (uint32_t i = 0; i < 16; ++i) {
+                        const bool there = key + i < tokens;
+                        const float x = there && near ? v[i * a.p_row + lane] : 0.f, y = there && far ? v[i * a.p_row + lane + 64] : 0.f;
+                        if (!finite(x)) near_first = min(near_first, key + i);
+                        if (!finite(y)) far_first = min(far_first, key + i);
+                    }
+                }
+            }
+            const int token = int(s.length) - int(s.count) + int(row / a.group);
+            const uint32_t stop = token < 0 ? 0u : min(min(end * TILE, s.length), uint32_t(token) + 1);
+            near_odd = near_odd && near_first >= stop;
+            far_odd = far_odd && far_first >= stop;
+            if (!__any(near_odd || far_odd)) continue;
+            // A key's score, -inf where there is none; and its place in the pools.
+            auto score_of = [&](uint32_t key, size_t &place) __attribute__((always_inline)) {
+                const Place of = place_of(a, key / 16);
+                const uint32_t page = key < stop ? page_of(a, a.tables[size_t(b) * a.table + of.entry]) : kNoPage;
+                if (page == kNoPage) return -INFINITY;
+                place = page * a.p_page + p.kv * a.p_head + (size_t(of.step) * 16 + key % 16) * a.p_row;
+                float x = 0.f;
+                for (uint32_t d = 0; d < a.dim; d += 4) {
+                    const f32x4 q = load_dims<VEC>(a.q + q_at, int(d), int(a.dim)) * a.qscale;
+                    const f32x4 k = load_dims<VEC>(a.k + place, int(d), int(a.dim));
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) x = fmaf(q[e], k[e], x);
+                }
+                return x;
+            };
+            size_t place = 0;
+            float top = -INFINITY;
+            bool nan = false;
+            for (uint32_t key = begin * TILE; key < stop; key += 64) {
+                const float score = score_of(key + lane, place);
+                top = fmaxf(top, score);
+                nan |= score != score;
+            }
+#pragma unroll
+            for (int d = 32; d; d /= 2) top = fmaxf(top, __shfl_xor(top, d));
+            if (!finite(top) || __any(nan)) continue;
+            float sum = 0.f, sum_now = 0.f;
+            float2 out = {0.f, 0.f}, now = out;
+            for (uint32_t key = begin * TILE; key < stop; key += 64) {
+                const float weight = __builtin_amdgcn_exp2f(score_of(key + lane, place) - top);
+                sum_now += weight;
+                for (uint32_t i = 0; i < min(64u, stop - key); ++i) {
+                    const float w = __uint_as_float(of_lane(__float_as_uint(weight), int(i)));
+                    if (w == 0.f) continue;
+                    const size_t at = size_t(of_lane(uint32_t(place >> 32), int(i))) << 32 | of_lane(uint32_t(place), int(i));
+                    if (near) now.x = fmaf(w * 0x1p-32f, a.v[at + lane], now.x);
+                    if (far) now.y = fmaf(w * 0x1p-32f, a.v[at + lane + 64], now.y);
+                }
+                if ((key / 64 + 1) % (kPiece / 64) == 0 || key + 64 >= stop) {
+                    sum += sum_now;
+                    out.x += now.x;
+                    out.y += now.y;
+                    sum_now = now.x = now.y = 0.f;
+                }
+            }
+#pragma unroll
+            for (int d = 32; d; d /= 2) sum += __shfl_xor(sum, d);
+            const float by = 0x1p32f / sum;
+            if (near_odd) to[lane] = out.x * by;
+            if (far_odd) to[lane + 64] = out.y * by;
+        }
+        t += end - begin;
+        if (t >= before + all) {
+            before += all;
+            ++b;
         }
     }
 }

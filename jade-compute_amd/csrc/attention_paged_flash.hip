@@ -22,7 +22,8 @@
 // V is scaled before it is split and the sums are scaled back, Q is scaled up and K down, so
 // every finite V and Q is carried exactly. What the parts do not carry is noticed and done
 // again from global memory with FP32 MFMAs, per wave: sums that are not finite (also where a
-// later token's value that is not finite met a weight of zero) and queries past 2^64.
+// later token's value that is not finite met a weight of zero) and queries past 2^64. Sums
+// of finite values that FP32 does not hold are taken once more at the end (sum_again).
 #include "attention_paged.hpp"
 #include "kernels.hpp"
 #include "split_bf16.hpp"
@@ -68,15 +69,6 @@ struct Shape {
     static_assert(kLdsBytes <= 160 * 1024, "LDS of a CU");
     static_assert(kKeys * kWide / 8 == 64 * kWaves, "a thread stages eight dims of K");
 };
-
-// The kernel's arguments where they were passed, read anew: nothing made of them is kept in
-// registers across a main loop that has none to spare.
-typedef const __attribute__((address_space(4))) PagedArgs Args;
-__device__ inline Args *args_now() {
-    Args *p = reinterpret_cast<Args *>(reinterpret_cast<uintptr_t>(__builtin_amdgcn_kernarg_segment_ptr()));
-    asm volatile("" : "+s"(p));
-    return p;
-}
 
 __device__ inline uint32_t dim_now(const PagedArgs &a) {
     uint32_t dim = a.dim;
@@ -176,6 +168,7 @@ attention_paged_flash(PagedArgs a) {
     uint32_t b, before;
     const uint32_t t_stop = work.start(run + 1, chunk, b, before);
     uint32_t at = work.start(run, chunk, b, before);
+    bool odd = false;  // met a sum that is not finite, of weights that are numbers
     while (at < t_stop) {
         const Sequence seq = work.anew(b);
         if (!work.active(seq)) {
@@ -591,20 +584,26 @@ attention_paged_flash(PagedArgs a) {
                 }
             }
             if (t_last - t0 >= kPiece) put_aside(true, true);
+            const bool sound = finite(halves_sum(row_sum));
+#pragma unroll
+            for (int x = 0; x < NB; ++x)
+#pragma unroll
+                for (int v = 0; v < 16; ++v) odd |= sound && !finite(acc[x][v]);
         }
 
         row_sum = halves_sum(row_sum);
         const Row row = row_now();
         if (row.me) {
             const uint32_t dim = dim_now(a), first_dim = 8u * uint32_t(lane_now() >> 5);
-            // A row that sees no key is zeros.
-            const float by = !whole ? unscale : row_sum == 0.f ? 0.f : unscale / row_sum;
+            const float by = unscale / row_sum;
             const size_t slot = (2 * size_t(run) + (begin == 0)) * RB + (row.mine - rb * RB);
             float *const to = whole ? a.out + row_at(a, b, kv, row.mine) : a.partial + slot * kSlotRow<DP>;
             if (!whole && h == 0)
                 reinterpret_cast<float2 *>(a.partial + 2 * size_t(a.runs) * RB * kSlotRow<DP>)[slot] = float2{row_max, row_sum};
             each_four([&](int d, f32x4 x) __attribute__((always_inline)) {
-                if (first_dim + d < dim) *reinterpret_cast<f32x4 *>(to + first_dim + d) = x * by;
+                // A row that sees no key is zeros.
+                if (first_dim + d < dim)
+                    *reinterpret_cast<f32x4 *>(to + first_dim + d) = row_sum == 0.f ? f32x4{0.f, 0.f, 0.f, 0.f} : x * by;
                 return x;
             });
         }
@@ -614,6 +613,7 @@ attention_paged_flash(PagedArgs a) {
             ++b;
         }
     }
+    if (__builtin_expect(__any(odd), 0)) sum_again<kKeys, RB, kSlotRow<DP>, 32, true>();
 }
 
 template <int DP>

@@ -1,10 +1,13 @@
-"""Paged attention over long caches: sums of many weights, tables of many entries. References in 64 bits for a few rows;
+"""Paged attention over long caches and large values: sums of many weights, tables of many entries, means of values
+whose sums no FP32 number holds. References in 64 bits for a few rows;
 bounds count roundings (U is half an ulp), as paged_oracle.py's do."""
 import numpy as np
 import pytest
 
+import paged_oracle as po
 from decoder_oracle import U
-from test_gpu_decoder import normal
+from test_gpu_decoder import normal, run, within
+from test_gpu_paged import paged_inputs, paged_spec
 
 pytestmark = pytest.mark.gpu
 
@@ -94,3 +97,50 @@ def test_attention_paged_tables_of_many_entries(runtime, page, queries, dim):
         # Terms of any order: every addition's rounding in full, twice what mean_bound says; scores' by their sizes.
         off = 2 * mean_bound(parts, tokens, dim) + U * 4 * (dim + 2) * sizes.max()
         assert (np.abs(got[i] - p @ v[:seen]) <= off * (p @ np.abs(v[:seen]))).all()
+
+
+@pytest.mark.parametrize("queries,dim", [(1, 64), (1, 37), (1, 128), (3, 80), (20, 64), (24, 128), (40, 64), (60, 96), (60, 128), (70, 30), (140, 128)])
+@pytest.mark.parametrize("tokens", [96, 3840])
+@pytest.mark.parametrize("scale", [0.0, 4.0])
+def test_attention_paged_values_near_the_largest(runtime, queries, dim, tokens, scale):
+    # Values whose weighted sum no FP32 number holds, though their mean is one: over equal keys, and where the maximum
+    # grows from tile to tile; subnormal and ordinary values in the same rows. Whole, and cut between runs.
+    rng = np.random.default_rng(61)
+    spec = paged_spec(1, 2, 1, queries, 48, tokens // 48, dim)
+    x = paged_inputs(rng, spec, [tokens], [queries])
+    x["q"] *= np.float32(scale)
+    v = po.pool_by_token(spec, x["v_pages"])
+    v[..., 0::5] = np.abs(v[..., 0::5]) * 1e37 + 2e38
+    v[..., 1::5] *= 5e37
+    v[..., 2::5] *= 1e-38
+    v[..., 4::5] *= 1e-43
+    np.clip(v, -3.2e38, 3.2e38, out=v)
+    want, off = po.paged(spec, x["q"], x["k_pages"], x["v_pages"], x["tables"], x["lengths"], x["counts"])
+    assert (np.abs(want) + off).max() < np.finfo(np.float32).max
+    got = po.rows_by_token(spec, run(runtime, spec, x)["out"], 2, queries)
+    # Subnormal values: a smallest subnormal for each one summed.
+    within(got, want, off + tokens * 2.0 ** -149)
+
+
+@pytest.mark.parametrize("queries,dim", [(1, 64), (20, 128), (40, 64), (60, 128)])
+def test_attention_paged_large_values_over_long_caches(runtime, queries, dim):
+    # So many of them that sums are put aside; infinities beside them, which reach their dims' rows and no others.
+    rng = np.random.default_rng(62)
+    tokens, page = 70000, 1024
+    table = -(-tokens // page)
+    batch = 300
+    q, k = np.zeros((batch, queries, 1, dim), np.float32), np.zeros((table * page, dim), np.float32)
+    v = np.full((table * page, dim), 2.5e38, np.float32)
+    v[:, 1], v[:, 2] = 1e-30, rng.random(table * page)
+    v[tokens - queries // 2:tokens, 3] = np.inf
+    v[::2, 4] = -2.5e38
+    kernel = compile_paged(runtime, batch, 1, queries, page, tokens, dim, table)
+    got = attend_on(runtime, kernel, q, k, v, np.tile(np.arange(table, dtype=np.float32), (batch, 1)),
+                    np.full(batch, tokens), np.full(batch, queries)).reshape(batch, queries, dim)
+    seen = tokens - queries + 1 + np.arange(queries)
+    sizes, sums = (np.cumsum(f(v.astype(np.float64)), axis=0)[seen - 1] / seen[:, None] for f in (np.abs, np.asarray))
+    reached = np.isinf(sums)
+    assert reached[:, 3].sum() == queries // 2 and not reached[:, 4:].any()
+    assert (got[:, reached] == np.inf).all()
+    off = 2 * mean_bound(queries >= 40, tokens, dim) * sizes
+    assert (np.abs(got[:, ~reached] - sums[~reached]) <= off[~reached]).all()
