@@ -13,7 +13,7 @@
 // entries of those lists whose first one counts. Values that all but tie with their bound
 // (equal logits) do not fit the list in LDS: then the best are found one after the other.
 //
-// 64 searches of 8 beams over 131071 tokens, 16 picks: 55 us for the chunks, 4.8 TB/s,
+// 64 searches of 8 beams over 131071 tokens, 16 picks: 56 us for the chunks, 4.8 TB/s,
 // bound by vector instructions (chunks of 4096 logits took 73, a chunk loaded ahead 94, 6
 // waves a SIMD in fewer registers 76; the greatest bound of a wave that has all of the picks,
 // which lets more values through, 62), and 9 for the join. One search of 4 beams over
@@ -21,8 +21,9 @@
 // every entry looked at); 3 of 16 beams over 50257, 32 picks: 8 and 11 (56).
 //
 // Beams are compared with one another by their sums of exponentials, so those are summed
-// in 64 bits, of terms that are off by one rounding each (their argument's own rounding
-// is carried along).
+// in 64 bits, term by term (adding neighbours in 32 first lost half a part in 2^24 for good where
+// one is tiny, and took 1-2% less). A term is off by an ulp of exp2 and two roundings; its
+// argument's own rounding is carried along.
 #include <cmath>
 
 #include "kernels.hpp"
@@ -76,7 +77,7 @@ __host__ __device__ inline Space space_of(float *workspace, uint64_t items, uint
     return {value, token, sum, reinterpret_cast<float *>(token + items * list)};
 }
 
-// exp(x - top), x <= top and top finite, off by a rounding of exp2 and one more: the
+// exp(x - top), x <= top and top finite, off by an ulp of exp2 and two roundings: the
 // argument's roundings are put back to first order. Nothing of 2^-126 or less counts.
 __device__ inline float exp_below(float x, float top) {
     const float d = fmaxf(x - top, -100.f);
@@ -174,8 +175,7 @@ __global__ __launch_bounds__(kThreads) void beam_chunks(BeamSelectArgs a, uint32
 #pragma unroll
             for (int i = 0; i < V; ++i)
 #pragma unroll
-                for (int e = 0; e < 4; e += 2)
-                    sum += double(exp_below(x[i][e], top) + exp_below(x[i][e + 1], top));
+                for (int e = 0; e < 4; ++e) sum += double(exp_below(x[i][e], top));
         } else {  // infinite logits share what there is
 #pragma unroll
             for (int i = 0; i < V; ++i)

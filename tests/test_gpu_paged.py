@@ -610,3 +610,16 @@ def test_beam_select_more_equal_lists_than_are_looked_at_at_once(runtime):
     got = run(runtime, spec, {"logits": logits, "scores": scores, "finished": np.zeros((1, 256))})
     for name in ("parents", "tokens"):
         same(got[name], want[name])
+
+
+@pytest.mark.parametrize("vocab", [2048, 40000])
+def test_beam_select_sums_of_tiny_terms_beside_large_ones(runtime, vocab):
+    # Two beams of the same logits, 0 and -17, in another order, the second ahead by 1e-8. exp(0) is exact and exp(-17), off
+    # by 4 U of its 4.1e-8, no matter; sums in 64 bits are good to 1e-12. Were neighbours added in 32 bits, the first beam's
+    # sum would be short by 4.1e-8 of itself, and it ahead.
+    logits = np.zeros((1, 2, vocab), np.float32)
+    logits[0, 0, 1::2] = -17
+    logits[0, 1, 2::4] = logits[0, 1, 3::4] = -17
+    got = run(runtime, select_spec(1, 2, vocab, 3), {"logits": logits, "scores": np.array([0, 1e-8]), "finished": np.zeros(2)})
+    same(got["parents"], np.array([1, 1, 1]))
+    same(got["tokens"], np.array([0, 1, 4]))
