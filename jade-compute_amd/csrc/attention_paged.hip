@@ -447,10 +447,13 @@ uint64_t rows_of(const PagedShape &s) { return uint64_t(s.heads / s.kv_heads) * 
 
 // Sequences of more rows than this, for each kv head, go to the kernel on bf16 parts
 // (attention_paged_flash.hip), by a launch of its own. Measured, this kernel and that one, 8
-// sequences of at most 4096 keys, 8 kv heads, 32, 48 and 64 rows: dims of 32 32.8, 42.7, 51.7
-// and 42.5, 48.1, 47.7 us; of 64 42.1, 60.1, 71.7 and 48.6, 57.7, 58.0; of 80 56.6, 78.6, 102.7
-// and 78.9, 83.1, 82.9; of 128 80.3, 110.7, 145.0 and 92.3, 96.8, 96.6.
-uint32_t few_rows(const PagedShape &s) { return s.dim <= 32 ? 48 : 32; }
+// sequences of at most 4096 keys, 8 kv heads, 48 rows. In calls that have no others, by two groups
+// here: dims of 32 55.0 and 51.5 us, of 40 55.8 and 60.0, of 64 57.4 and 60.9, of 80 96.8 and 87.5,
+// of 96 98.9 and 90.2, of 128 108 and 101. In calls whose spec has more, by one: 48.4 and 52.7,
+// 52.6 and 59.7, 64.2 and 62.4, 84.6 and 89.8, 87.8 and 92.4, 122 and 106. One sequence of 8192
+// keys, dims of 64: 26.1 and 30.0, 27.3 and 32.5. 64 rows of 64 dims in a call that has more:
+// 75.5 and 61.5.
+uint32_t few_rows(const PagedShape &s) { return s.dim <= 64 ? 48 : 32; }
 bool has_many(const PagedShape &s) {
     // Offsets of a sequence's rows in 31 bits.
     return s.dim % 4 == 0 && rows_of(s) > few_rows(s) && uint64_t(s.heads) * s.queries * s.dim < 1u << 29;

@@ -122,7 +122,7 @@ def test_attention_paged_values_near_the_largest(runtime, queries, dim, tokens, 
     within(got, want, off + tokens * 2.0 ** -149)
 
 
-@pytest.mark.parametrize("queries,dim", [(1, 64), (20, 128), (40, 64), (60, 128)])
+@pytest.mark.parametrize("queries,dim", [(1, 64), (20, 128), (40, 64), (60, 128), (60, 64)])
 def test_attention_paged_large_values_over_long_caches(runtime, queries, dim):
     # So many of them that sums are put aside; infinities beside them, which reach their dims' rows and no others.
     rng = np.random.default_rng(62)
