@@ -623,3 +623,37 @@ def test_beam_select_sums_of_tiny_terms_beside_large_ones(runtime, vocab):
     got = run(runtime, select_spec(1, 2, vocab, 3), {"logits": logits, "scores": np.array([0, 1e-8]), "finished": np.zeros(2)})
     same(got["parents"], np.array([1, 1, 1]))
     same(got["tokens"], np.array([0, 1, 4]))
+
+
+@pytest.mark.parametrize("batch,page,table,pages", [(6, 16, 2100, 7000), (5, 1024, 4097, 9000), (2049, 16, 3, 4000), (2500, 48, 4, 6500),
+                                                    (4097, 16, 2, 5500)])
+def test_pages_fork_of_long_tables_and_large_batches(runtime, batch, page, table, pages):
+    # Entries past those that a thread keeps in registers; needs past those that a block keeps in LDS.
+    rng = np.random.default_rng(43)
+    for reserve in (1, page * table):  # the second asks for whole tables
+        state = fork_state(rng, batch, page, table, pages)
+        check_fork(runtime, {"op": "pages_fork", "batch": batch, "pages": pages, "page": page, "table": table},
+                   {**state, "parents": rng.integers(-1, batch, batch), "reserve": np.full(batch, reserve)}, repeats=2)
+
+
+def test_pages_append_more_items_than_a_grid_has_blocks(runtime):
+    # A row of each of 17 heads of 65535 sequences: blocks take a second item, of another sequence, after one whose table
+    # has a page too few or none at all.
+    rng = np.random.default_rng(22)
+    spec = {"op": "pages_append", "batch": 65535, "kv_heads": 17, "rows": 1, "pages": 2 * 65535, "page": 16, "table": 2, "dim": 1,
+            "token_major": False, "pages_token_major": True}
+    assert 65535 * 17 > 2 ** 20
+    n = 65535 * 17
+    lengths = rng.integers(0, 33, 65535).astype(np.float32)
+    tables = rng.permutation(2 * 65535).reshape(65535, 2).astype(np.float32)
+    tables[::5, 0], tables[1::5, 1] = -1, np.nan
+    counts = rng.integers(0, 3, 65535).astype(np.float32)
+    x = {"k": normal(rng, n), "v": normal(rng, n), "counts": counts, "tables": tables, "lengths": lengths, **pools_for(rng, spec)}
+    got = run(runtime, spec, x, 2)
+    entry = np.take_along_axis(tables, np.minimum(lengths.astype(int)[:, None] // 16, 1), 1)[:, 0]
+    made = (counts >= 1) & (lengths < 32) & (entry >= 0)
+    same(got["new_lengths"], lengths + made)
+    for name in "kv":
+        want = x[name + "_pages"].reshape(-1, 16, 17).copy()
+        want[entry[made].astype(int), lengths[made].astype(int) % 16] = x[name].reshape(65535, 17)[made]
+        same(got[name + "_pages"], want)
