@@ -144,3 +144,23 @@ def test_attention_paged_large_values_over_long_caches(runtime, queries, dim):
     assert (got[:, reached] == np.inf).all()
     off = 2 * mean_bound(queries >= 40, tokens, dim) * sizes
     assert (np.abs(got[:, ~reached] - sums[~reached]) <= off[~reached]).all()
+
+
+@pytest.mark.parametrize("queries,dim", [(1, 64), (3, 37), (20, 128), (40, 64), (70, 32), (60, 96), (60, 128)])
+@pytest.mark.parametrize("tokens", [96, 3840])
+def test_attention_paged_scores_of_minus_infinity(runtime, queries, dim, tokens):
+    # They weigh nothing: rows that see no other score are zeros, those that see one other have its value.
+    rng = np.random.default_rng(63)
+    spec = paged_spec(1, 2, 1, queries, 48, tokens // 48, dim, spare=0)
+    x = paged_inputs(rng, spec, [tokens], [queries])
+    x["q"][:] = np.abs(x["q"])
+    place = po.places(spec, x["tables"][0], [tokens - (queries + 1) // 2])[0]
+    k = po.pool_by_token(spec, x["k_pages"])
+    other = k[place].copy()
+    k[..., dim // 2] = -np.inf
+    k[place] = other
+    got = po.rows_by_token(spec, run(runtime, spec, x)["out"], 2, queries)[0]
+    first = queries - (queries + 1) // 2
+    assert (got[:first] == 0).all()
+    value = po.pool_by_token(spec, x["v_pages"])[place][0]
+    assert (np.abs(got[first:] - value) <= 16 * U * np.abs(value)).all()
