@@ -17,11 +17,12 @@
 // block; a launch of its own joins what a cut went through.
 //
 // Up to 16 rows it is bound by reading K and V: 16 sequences of 4096 to 8192 keys, 32 heads (8
-// of keys) of 128, one query each, 834 MB in pages of 16 tokens: 143 us, 5.8 TB/s, and 4.4 us
-// for the join. One sequence of 1000 keys, 8 heads of 64: 6.4 and 3.3 us, each a chain of
+// of keys) of 128, one query each, 834 MB in pages of 16 tokens: 145 us, 5.7 TB/s, and 4.6 us
+// for the join. One sequence of 1000 keys, 8 heads of 64: 7.1 and 4.2 us, each a chain of
 // loads that wait for one another (lengths, table, keys; lengths, sums). Many sequences of few
 // keys are bound by what a unit takes from its first load to its outputs: 1024 of 50 to 100
-// keys, 8 kv heads of 128, 629 MB in 177 us.
+// keys, 8 kv heads of 128, 629 MB in 175 us. Besides, every wave walks the whole batch, 64
+// sequences at a time, before it knows its run.
 #include <cmath>
 
 #include "attention_paged.hpp"
@@ -374,33 +375,32 @@ __device__ void join_unit(const PagedArgs &a, uint32_t block, uint32_t rows_from
     const float2 *ml = reinterpret_cast<const float2 *>(a.partial + 2 * size_t(a.runs) * RB * DP);
     // A unit's first run had it last, the others first.
     auto slot = [&](uint32_t r) { return (2 * size_t(r) + (r == first)) * RB + row; };
-    // Sums of the slots' means, by their weights; and 2^-40 of them, for where those pass FP32's
-    // largest (a slot weighs 2^8 for each of its keys at most).
+    // The mean of the slots' means so far, weighed by their shares of the weight: no sum passes
+    // the values. Four slots at a time, on their way together.
+    constexpr int kAtOnce = 4;
     float most = -INFINITY, l = 0.f;
-    f32x4 o = {0.f, 0.f, 0.f, 0.f}, small = o;
-    auto join = [&](float top, float sum, f32x4 mean) {
-        const float next = fmaxf(most, top), from = next == -INFINITY ? 0.f : next;
-        const float old = __builtin_amdgcn_exp2f(most - from), weight = sum * __builtin_amdgcn_exp2f(top - from);
-        most = next;
-        l = l * old + weight;
-        o = o * old + mean * weight;
-        small = small * old + mean * (weight * 0x1p-40f);
-    };
-    auto mean = [&] {
-        const float by = 1.0f / l;
-        f32x4 x;
+    f32x4 o = {0.f, 0.f, 0.f, 0.f};  // zeros for a row that sees no key
+    for (uint32_t r0 = first + p; mine && r0 <= last; r0 += kAtOnce * PARTS) {
+        float2 x[kAtOnce];
+        f32x4 means[kAtOnce];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) x[e] = l == 0.f ? 0.f : finite(o[e]) ? o[e] * by : small[e] * (0x1p40f * by);
-        return x;  // a row that sees no key is zeros
-    };
-    if (mine) {
-#pragma unroll 4
-        for (uint32_t r = first + p; r <= last; r += PARTS) {
-            const float2 x = ml[slot(r)];
-            join(x.x, x.y, *reinterpret_cast<const f32x4 *>(a.partial + slot(r) * DP + d));
+        for (int i = 0; i < kAtOnce; ++i) {
+            const uint32_t r = r0 + i * PARTS;
+            x[i] = r <= last ? ml[slot(r)] : float2{-INFINITY, 0.f};
+            means[i] = r <= last ? *reinterpret_cast<const f32x4 *>(a.partial + slot(r) * DP + d) : f32x4{0.f, 0.f, 0.f, 0.f};
         }
+        const float was = most;
+#pragma unroll
+        for (int i = 0; i < kAtOnce; ++i) most = fmaxf(most, x[i].x);
+        const float from = most == -INFINITY ? 0.f : most, old = l * __builtin_amdgcn_exp2f(was - from);
+        l = old;
+#pragma unroll
+        for (int i = 0; i < kAtOnce; ++i) l += x[i].y *= __builtin_amdgcn_exp2f(x[i].x - from);
+        const float by = l == 0.f ? 0.f : 1.0f / l;
+        o *= old * by;
+#pragma unroll
+        for (int i = 0; i < kAtOnce; ++i) o += means[i] * (x[i].y * by);
     }
-    o = mean();
     if constexpr (PARTS > 1) {
         sums[p][lane] = o;
         if (lane == 0) weights[p] = float2{most, l};
