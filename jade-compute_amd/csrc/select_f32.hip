@@ -13,7 +13,7 @@
 // entries of those lists whose first one counts. Values that all but tie with their bound
 // (equal logits) do not fit the list in LDS: then the best are found one after the other.
 //
-// 64 searches of 8 beams over 131071 tokens, 16 picks: 56 us for the chunks, 4.8 TB/s,
+// 64 searches of 8 beams over 131071 tokens, 16 picks: 57 us for the chunks, 4.7 TB/s,
 // bound by vector instructions (chunks of 4096 logits took 73, a chunk loaded ahead 94, 6
 // waves a SIMD in fewer registers 76; the greatest bound of a wave that has all of the picks,
 // which lets more values through, 62), and 9 for the join. One search of 4 beams over
