@@ -49,10 +49,10 @@ __attribute__((amdgpu_waves_per_eu(kWavesASimd<DP, G>, kWavesASimd<DP, G>))) voi
     __shared__ __attribute__((aligned(16))) float part[kWaves][RB][OUT + 4];
     __shared__ float2 ml[kWaves][RB];
     __shared__ RowPlan plans[RB];
-    __shared__ uint32_t odd[kWaves];  // whether a wave met an output that is not finite
+    __shared__ uint32_t odd_outputs[kWaves];  // whether a wave met an output that is not finite
     const int tid = threadIdx.x, lane = tid & 63;
     const uint32_t wave = uniform(tid >> 6);
-    odd[wave] = 0;
+    odd_outputs[wave] = 0;
     const int m = lane & 15, g = lane >> 4;
     const Work<kTile, RB> work(a);
     const uint32_t chunk = (work.total + a.runs - 1) / a.runs;
@@ -320,11 +320,11 @@ __attribute__((amdgpu_waves_per_eu(kWavesASimd<DP, G>, kWavesASimd<DP, G>))) voi
         __syncthreads();
         put_aside(u.stop <= begin + kPiece);
         __syncthreads();
-        finish<OUT, RB, VEC>(a, run, u.b, u.kv, u.rb, rows, whole, begin == 0, part, ml, plans, odd);
+        finish<OUT, RB, VEC>(a, run, u.b, u.kv, u.rb, rows, whole, begin == 0, part, ml, plans, odd_outputs);
         u = next;
     }
     clear_rows(work);
-    if (__builtin_expect(uniform(odd[wave]), 0)) sum_again<kTile, RB, OUT, kThreads / OUT, VEC>();
+    if (__builtin_expect(uniform(odd_outputs[wave]), 0)) sum_again<kTile, RB, OUT, kThreads / OUT, VEC>();
 }
 
 // How the launch that joins is laid out: blocks x rows, and which unit a block has.
